@@ -60,7 +60,9 @@ EXPORTS = ["gnet_param_count", "gnet_graph_count", "gnet_graph_fill", "gnet_grap
            "gnet_forward", "gnet_loss", "gnet_match_prepare", "gnet_backward", "gnet_backward_prepare", "det_matching_workspace_bytes", "det_matching_f32",
            "roi_pool_fwd_f32", "roi_pool_bwd_f32", "roi_pool_bwd_atomic_f32", "gnet_version", "gnet_profiler_create", "gnet_profiler_read",
            "gnet_profiler_destroy", "gnet_profiler_set_stride", "gnet_profiler_begin", "gnet_profiler_end", "gnet_adam_step", "gnet_momentum_step", "gnet_clip_by_norm",
-           "gnet_fc_workspace_bytes", "gnet_fc_forward", "gnet_fc_backward", "gnet_box_iou", "gnet_debug_gemm", "gnet_abi_version", "gnet_abi_sizes"]
+           "gnet_fc_workspace_bytes", "gnet_fc_forward", "gnet_fc_backward", "gnet_box_iou", "gnet_debug_gemm", "gnet_abi_version", "gnet_abi_sizes",
+           "gnet_embed_forward", "gnet_embed_workspace_bytes", "gnet_embed_backward", "gnet_embed_scale_backward", "gnet_vocab_workspace_bytes",
+           "gnet_xent_forward", "gnet_xent_backward", "gnet_distill_forward", "gnet_distill_backward"]
 
 KCLASSES = ["graph", "pack", "pw_fwd", "node_fwd", "edge_fwd", "loss", "head_bwd", "winner_lists", "edge_bwd", "gather_winners",
             "node_bwd", "pw_bwd_main", "pw_w1_nodesums", "pw_w1_classrows", "reduce_partials", "edge_geometry"]
@@ -202,6 +204,24 @@ def _bind(lib):
     lib.gnet_box_iou.argtypes = [vp, i32, vp, i32, vp, vp, vp, i32, vp, vp]
     lib.gnet_debug_gemm.restype = C.c_int
     lib.gnet_debug_gemm.argtypes = [vp, vp, i64, i64, i64, C.c_int, vp, vp, vp]
+    lib.gnet_embed_forward.restype = C.c_int
+    lib.gnet_embed_forward.argtypes = [vp, i32, vp, i64, f32, vp, i64, i64, i64, i32, vp, vp]
+    lib.gnet_embed_workspace_bytes.restype = sz
+    lib.gnet_embed_workspace_bytes.argtypes = [i64, i64]
+    lib.gnet_embed_backward.restype = C.c_int
+    lib.gnet_embed_backward.argtypes = [vp, i32, vp, i64, f32, vp, i64, i64, i64, i32, vp, i32, vp, sz, vp]
+    lib.gnet_embed_scale_backward.restype = C.c_int
+    lib.gnet_embed_scale_backward.argtypes = [vp, i32, vp, i64, vp, i64, f32, i64, i64, i64, i32, vp, vp]
+    lib.gnet_vocab_workspace_bytes.restype = sz
+    lib.gnet_vocab_workspace_bytes.argtypes = [vp, i64, i64, i64, i64, i64, i32, i32]
+    lib.gnet_xent_forward.restype = C.c_int
+    lib.gnet_xent_forward.argtypes = [vp, i64, vp, i64, vp, i32, i64, i64, i64, i32, vp, vp, vp, vp, sz, vp]
+    lib.gnet_xent_backward.restype = C.c_int
+    lib.gnet_xent_backward.argtypes = [vp, i64, vp, i64, vp, i32, vp, vp, vp, i64, i64, i64, i32, vp, vp, vp, sz, vp]
+    lib.gnet_distill_forward.restype = C.c_int
+    lib.gnet_distill_forward.argtypes = [vp, i64, vp, i64, vp, i32, vp, f32, i64, i64, i64, i64, i32, vp, vp, vp, vp, sz, vp]
+    lib.gnet_distill_backward.restype = C.c_int
+    lib.gnet_distill_backward.argtypes = [vp, i64, vp, i64, vp, i32, vp, f32, vp, vp, vp, i64, i64, i64, i64, i32, vp, vp, vp, sz, vp]
     lib.gnet_version.restype = C.c_char_p
     lib.gnet_version.argtypes = []
     _lib = lib

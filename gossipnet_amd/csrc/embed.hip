@@ -1,0 +1,324 @@
+// Rows of a vocabulary table for token ids, scaled, and the table's gradient summed in token order.
+//   forward    y[m] = scale * s[m] * table[id[m]]                 (zero where the id is outside [0, V))
+//   backward   d table[v] = scale * sum over the tokens m with id[m] = v, ascending, of s[m] * dy[m]
+//              d s[m] = scale * dy[m] . table[id[m]]
+// Every kernel here moves bytes: M rows in, M rows out; the backward pass reads M rows of dy and writes the V rows of the table's
+// gradient once, the rows without a token included.
+//   embed_sort    keys (id << 32 | token), distinct, sorted in LDS per 4096 tokens; embed_merge joins 16 sorted runs at a time by
+//                 binary searches in the others (no atomics: the order of every sum is fixed)
+//   embed_rows    a workgroup owns a range of the table's rows and finds their tokens by binary search; a row with more than HOT
+//                 tokens is left to
+//   embed_hot     one partial sum per HOT consecutive sorted tokens and run, and embed_hot_rows, which adds a run's partial sums
+#include "vocab_gemm.hpp"
+
+namespace {
+
+typedef unsigned long long u64;
+constexpr int RUN = 4096;          // tokens sorted by one workgroup: 32 KB of keys
+constexpr int WAY = 16;            // runs joined by one merge pass
+constexpr int HOT = 64;            // tokens a row's own wave adds up
+
+template <int DT> struct Elem { typedef u16 type; };
+template <> struct Elem<GNET_F32> { typedef float type; };
+template <int DT> __device__ __forceinline__ float dec(typename Elem<DT>::type v) {
+  if constexpr (DT == GNET_F32) return v;
+  else if constexpr (DT == GNET_BF16) return Bf16T::dec(v);
+  else return F16T::dec(v);
+}
+template <int DT> __device__ __forceinline__ typename Elem<DT>::type enc(float v) {
+  if constexpr (DT == GNET_F32) return v;
+  else if constexpr (DT == GNET_BF16) return Bf16T::enc(v);
+  else return F16T::enc(v);
+}
+template <class E, int VEC> struct alignas(sizeof(E) * VEC) Pack { E v[VEC]; };
+
+__device__ __forceinline__ int64_t load_id(const void* p, int64_t i, int is64) {
+  return is64 ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
+}
+
+// ---- forward ------------------------------------------------------------------------------------------------------
+struct ForwardArgs {
+  const void* ids; int ids64; int64_t M, V, D;
+  const void* table; int64_t ld; float scale; const float* token_scale;
+  void* y; int blocks;                 // column blocks of 64 * VEC elements a row
+};
+template <int DT, int VEC> __global__ void __launch_bounds__(256) embed_rows_out(const ForwardArgs a) {
+  typedef typename Elem<DT>::type E;
+  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t m = w / a.blocks, d = ((w % a.blocks) * 64 + (threadIdx.x & 63)) * VEC;
+  if (m >= a.M || d >= a.D) return;
+  const int64_t id = load_id(a.ids, m, a.ids64);
+  Pack<E, VEC> o;
+  if (id >= 0 && id < a.V) {
+    const Pack<E, VEC> t = *reinterpret_cast<const Pack<E, VEC>*>((const E*)a.table + id * a.ld + d);
+    const float s = a.token_scale ? a.scale * a.token_scale[m] : a.scale;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) o.v[i] = enc<DT>(dec<DT>(t.v[i]) * s);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) o.v[i] = enc<DT>(0.f);
+  }
+  *reinterpret_cast<Pack<E, VEC>*>((E*)a.y + m * a.D + d) = o;
+}
+
+// ---- the order of the tokens ------------------------------------------------------------------------------------------
+// Bitonic sort of one run in LDS; keys are distinct, so the result is the stable order.
+__global__ void __launch_bounds__(1024) embed_sort(const void* ids, int ids64, int64_t M, int64_t V, int n, u64* __restrict__ keys) {
+  __shared__ u64 s[RUN];
+  const int64_t base = (int64_t)blockIdx.x * RUN;
+  for (int i = threadIdx.x; i < n; i += 1024) {
+    u64 key = ~0ull;                                   // behind the last token
+    if (base + i < M) {
+      const int64_t id = load_id(ids, base + i, ids64);
+      key = ((id >= 0 && id < V ? (u64)id : 0xffffffffull) << 32) | (u64)(base + i);
+    }
+    s[i] = key;
+  }
+  for (int k = 2; k <= n; k <<= 1)
+    for (int j = k >> 1; j; j >>= 1) {
+      __syncthreads();
+      for (int t = threadIdx.x; t < n / 2; t += 1024) {
+        const int i = ((t & ~(j - 1)) << 1) | (t & (j - 1));
+        const u64 x = s[i], y = s[i + j];
+        if ((x > y) == ((i & k) == 0)) { s[i] = y; s[i + j] = x; }
+      }
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += 1024) if (base + i < M) keys[base + i] = s[i];
+}
+
+// keys of [lo, hi) below `key`
+__device__ __forceinline__ int64_t lower_bound(const u64* __restrict__ keys, int64_t lo, int64_t hi, u64 key) {
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (keys[mid] < key) lo = mid + 1; else hi = mid;
+  }
+  return lo;
+}
+__global__ void __launch_bounds__(256) embed_merge(const u64* __restrict__ in, u64* __restrict__ out, int64_t M, int64_t run) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= M) return;
+  const u64 key = in[i];
+  const int64_t own = i / run, first = own / WAY * WAY;
+  int64_t at = first * run + (i - own * run);
+  for (int64_t r = first; r < first + WAY && r * run < M; ++r)
+    if (r != own) at += lower_bound(in, r * run, min(M, (r + 1) * run), key) - r * run;
+  out[at] = key;
+}
+
+// ---- backward ------------------------------------------------------------------------------------------------------
+struct BackwardArgs {
+  const u64* keys; int64_t M, V, D;
+  const void* dy; int64_t ld; float scale; const float* token_scale;
+  void* out; int64_t ld_out; int accumulate;
+  int rows;                            // table rows of a workgroup
+  float* part;                         // [segment][2][D]
+};
+
+template <int DT, int VEC> __device__ __forceinline__ void add_token(float (&sum)[VEC], const BackwardArgs& a, int64_t m, int64_t d) {
+  typedef typename Elem<DT>::type E;
+  const Pack<E, VEC> g = *reinterpret_cast<const Pack<E, VEC>*>((const E*)a.dy + m * a.ld + d);
+  const float s = a.token_scale ? a.token_scale[m] : 1.f;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) sum[i] = fmaf(dec<DT>(g.v[i]), s, sum[i]);
+}
+template <int DT, int VEC> __device__ __forceinline__ void store_row(const float (&sum)[VEC], const BackwardArgs& a, int64_t v, int64_t d) {
+  typedef typename Elem<DT>::type E;
+  Pack<E, VEC>* p = reinterpret_cast<Pack<E, VEC>*>((E*)a.out + v * a.ld_out + d);
+  Pack<E, VEC> o;
+  if (a.accumulate) o = *p;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) o.v[i] = enc<DT>(a.accumulate ? dec<DT>(o.v[i]) + sum[i] * a.scale : sum[i] * a.scale);
+  *p = o;
+}
+
+constexpr int MOST_ROWS = 64;
+template <int DT, int VEC> __global__ void __launch_bounds__(256) embed_rows(const BackwardArgs a) {
+  __shared__ int64_t start[MOST_ROWS + 1];
+  const int64_t v0 = (int64_t)blockIdx.x * a.rows;
+  const int lane = threadIdx.x & 63;
+  if (threadIdx.x <= a.rows) start[threadIdx.x] = lower_bound(a.keys, 0, a.M, (u64)(v0 + threadIdx.x) << 32);
+  __syncthreads();
+  for (int r = threadIdx.x >> 6; r < a.rows && v0 + r < a.V; r += 4) {
+    const int64_t lo = start[r], hi = start[r + 1];
+    if (hi - lo > HOT || (a.accumulate && lo == hi)) continue;
+    for (int64_t d = (int64_t)lane * VEC; d < a.D; d += 64 * VEC) {
+      float sum[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) sum[i] = 0.f;
+      for (int64_t j = lo; j < hi; ++j) add_token<DT, VEC>(sum, a, (int64_t)(a.keys[j] & 0xffffffffull), d);
+      store_row<DT, VEC>(sum, a, v0 + r, d);
+    }
+  }
+}
+
+// The runs of more than HOT equal ids: a segment of HOT sorted tokens meets at most two, one that comes in over its first token
+// (slot 0: also a run that starts right there) and one that leaves over its last (slot 1).
+constexpr unsigned NONE = 0xffffffffu;      // id of a token that is left out: sorted behind all others
+__device__ __forceinline__ unsigned id_at(const u64* keys, int64_t i) { return (unsigned)(keys[i] >> 32); }
+template <int DT, int VEC> __global__ void __launch_bounds__(256) embed_hot(const BackwardArgs a) {
+  const int64_t seg = blockIdx.x, lo = seg * HOT, hi = min(a.M, lo + HOT);
+  const unsigned first = id_at(a.keys, lo), last = id_at(a.keys, hi - 1);
+  const bool whole = first == last && hi < a.M && id_at(a.keys, hi) == first;
+  const bool in = first != NONE && (whole || (lo > 0 && id_at(a.keys, lo - 1) == first));
+  const bool out = first != last && last != NONE && hi < a.M && id_at(a.keys, hi) == last;
+  for (int slot = 0; slot < 2; ++slot) {
+    if (!(slot ? out : in)) continue;
+    const u64 id = slot ? last : first;
+    const int64_t run0 = lower_bound(a.keys, 0, hi, id << 32), run1 = lower_bound(a.keys, lo, a.M, (id + 1) << 32);
+    if (run1 - run0 <= HOT) continue;
+    const int64_t b = max(lo, run0), e = min(hi, run1);
+    for (int64_t d = (int64_t)threadIdx.x * VEC; d < a.D; d += 256 * VEC) {
+      float sum[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) sum[i] = 0.f;
+      for (int64_t j = b; j < e; ++j) add_token<DT, VEC>(sum, a, (int64_t)(a.keys[j] & 0xffffffffull), d);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) a.part[(seg * 2 + slot) * a.D + d + i] = sum[i];
+    }
+  }
+}
+template <int DT, int VEC> __global__ void __launch_bounds__(256) embed_hot_rows(const BackwardArgs a) {
+  // the segment in which a run of more than HOT tokens starts adds its partial sums, in order
+  const int64_t seg = blockIdx.x, lo = seg * HOT, hi = min(a.M, lo + HOT);
+  if (hi >= a.M) return;
+  const unsigned id = id_at(a.keys, hi - 1);
+  if (id == NONE || id_at(a.keys, hi) != id) return;              // no run leaves this segment
+  const bool whole = id_at(a.keys, lo) == id;
+  if (whole && lo > 0 && id_at(a.keys, lo - 1) == id) return;            // it started earlier
+  const int64_t b = whole ? lo : lower_bound(a.keys, lo, hi, (u64)id << 32);
+  const int64_t e = lower_bound(a.keys, hi, a.M, ((u64)id + 1) << 32);
+  if (e - b <= HOT) return;                                              // embed_rows has it
+  const int64_t last = (e - 1) / HOT;
+  for (int64_t d = (int64_t)threadIdx.x * VEC; d < a.D; d += 256 * VEC) {
+    float sum[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) sum[i] = a.part[(seg * 2 + (whole ? 0 : 1)) * a.D + d + i];
+    for (int64_t s = seg + 1; s <= last; ++s)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) sum[i] += a.part[s * 2 * a.D + d + i];
+    store_row<DT, VEC>(sum, a, id, d);
+  }
+}
+
+struct ScaleArgs {
+  const void* ids; int ids64; int64_t M, V, D;
+  const void* table; int64_t ld; const void* dy; int64_t ld_dy; float scale; float* dscale;
+};
+template <int DT, int VEC> __global__ void __launch_bounds__(256) embed_scale_grad(const ScaleArgs a) {
+  typedef typename Elem<DT>::type E;
+  const int64_t m = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (m >= a.M) return;
+  const int64_t id = load_id(a.ids, m, a.ids64);
+  float dot = 0.f;
+  if (id >= 0 && id < a.V) {
+    for (int64_t d = (int64_t)(threadIdx.x & 63) * VEC; d < a.D; d += 64 * VEC) {
+      const Pack<E, VEC> t = *reinterpret_cast<const Pack<E, VEC>*>((const E*)a.table + id * a.ld + d);
+      const Pack<E, VEC> g = *reinterpret_cast<const Pack<E, VEC>*>((const E*)a.dy + m * a.ld_dy + d);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) dot = fmaf(dec<DT>(t.v[i]), dec<DT>(g.v[i]), dot);
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) dot += __shfl_xor(dot, o);
+  }
+  if ((threadIdx.x & 63) == 0) a.dscale[m] = dot * a.scale;
+}
+
+// Elements a lane takes at once: the widest access that width, row strides and addresses allow (16 bytes at most) and that still
+// gives every lane of a wave something to do.
+int pick_vec(int dtype, int64_t D, int64_t ld0, int64_t ld1, const void* p0, const void* p1) {
+  const int size = dtype == GNET_F32 ? 4 : 2;
+  int v = 16 / size;
+  while (v > 1 && (D % v || ld0 % v || ld1 % v || ((uintptr_t)p0 | (uintptr_t)p1) % (v * size) || D < 64 * v)) v >>= 1;
+  return v;
+}
+template <template <int, int> class F, class A> void launch(int dtype, int vec, const A& a, unsigned grid, hipStream_t s) {
+#define GO(DT)                                                  \
+  switch (vec) {                                                \
+    case 1: F<DT, 1>::go(a, grid, s); break;                    \
+    case 2: F<DT, 2>::go(a, grid, s); break;                    \
+    case 4: F<DT, 4>::go(a, grid, s); break;                    \
+    default: F<DT, DT == GNET_F32 ? 4 : 8>::go(a, grid, s);     \
+  }
+  if (dtype == GNET_F32) { GO(GNET_F32) } else if (dtype == GNET_BF16) { GO(GNET_BF16) } else { GO(GNET_F16) }
+#undef GO
+}
+#define KERNEL_OF(name, kernel, args) \
+  template <int DT, int VEC> struct name { static void go(const args& a, unsigned grid, hipStream_t s) { kernel<DT, VEC><<<grid, 256, 0, s>>>(a); } }
+KERNEL_OF(GoForward, embed_rows_out, ForwardArgs);
+KERNEL_OF(GoRows, embed_rows, BackwardArgs);
+KERNEL_OF(GoHot, embed_hot, BackwardArgs);
+KERNEL_OF(GoHotRows, embed_hot_rows, BackwardArgs);
+KERNEL_OF(GoScale, embed_scale_grad, ScaleArgs);
+
+int check(int64_t M, int64_t V, int64_t D, int64_t ld, int dtype) {
+  if (dtype != GNET_F32 && dtype != GNET_BF16 && dtype != GNET_F16) return GNET_ERR_INVALID;
+  if (M < 0 || V < 1 || D < 1 || ld < D) return GNET_ERR_INVALID;
+  if (M > (1 << 24) || V > (1ll << 30) || D > (1 << 16)) return GNET_ERR_UNSUPPORTED;
+  return GNET_OK;
+}
+size_t keys_bytes(int64_t M) { return ((size_t)M * 8 + 255) & ~(size_t)255; }
+
+}  // namespace
+
+extern "C" int gnet_embed_forward(const void* ids, int32_t ids64, const void* table, int64_t ld_table, float scale, const float* token_scale,
+                                  int64_t M, int64_t V, int64_t D, int32_t dtype, void* y, gnet_stream_t stream) {
+  clear_hip_error();
+  if (const int e = check(M, V, D, ld_table, dtype)) return e;
+  if (M == 0) return GNET_OK;
+  if (!ids || !table || !y) return GNET_ERR_INVALID;
+  ForwardArgs a{ids, ids64, M, V, D, table, ld_table, scale, token_scale, y, 1};
+  const int vec = pick_vec(dtype, D, ld_table, D, table, y);
+  a.blocks = (int)((D + 64 * vec - 1) / (64 * vec));
+  launch<GoForward>(dtype, vec, a, (unsigned)((M * a.blocks + 3) / 4), (hipStream_t)stream);
+  return launch_status();
+}
+
+extern "C" size_t gnet_embed_workspace_bytes(int64_t M, int64_t D) {
+  if (M <= 0 || D <= 0 || M > (1 << 24) || D > (1 << 16)) return 0;
+  return 2 * keys_bytes(M) + (size_t)((M + HOT - 1) / HOT) * 2 * D * 4;
+}
+
+extern "C" int gnet_embed_backward(const void* ids, int32_t ids64, const void* dy, int64_t ld_dy, float scale, const float* token_scale,
+                                   int64_t M, int64_t V, int64_t D, int32_t dtype, void* dtable, int32_t accumulate, void* workspace,
+                                   size_t workspace_bytes, gnet_stream_t stream) {
+  clear_hip_error();
+  if (const int e = check(M, V, D, ld_dy, dtype)) return e;
+  if (!dtable || (M && (!ids || !dy))) return GNET_ERR_INVALID;
+  if (M == 0 && accumulate) return GNET_OK;
+  if (M && (!workspace || workspace_bytes < gnet_embed_workspace_bytes(M, D) || ((uintptr_t)workspace & 255))) return GNET_ERR_WORKSPACE;
+  hipStream_t s = (hipStream_t)stream;
+  u64* keys = (u64*)workspace;
+  u64* other = (u64*)((char*)workspace + keys_bytes(M));
+  float* part = (float*)((char*)workspace + 2 * keys_bytes(M));
+  if (M) {
+    int n = 64;
+    while (n < RUN && n < M) n <<= 1;
+    embed_sort<<<(unsigned)((M + RUN - 1) / RUN), 1024, 0, s>>>(ids, ids64, M, V, n, keys);
+    for (int64_t run = RUN; run < M; run *= WAY) {
+      embed_merge<<<(unsigned)((M + 255) / 256), 256, 0, s>>>(keys, other, M, run);
+      u64* t = keys; keys = other; other = t;
+    }
+  }
+  BackwardArgs a{keys, M, V, D, dy, ld_dy, scale, token_scale, dtable, D, accumulate, 4, part};
+  while (a.rows < MOST_ROWS && V / (2 * a.rows) >= 1024) a.rows *= 2;      // at least 1024 workgroups where the table allows it
+  const int vec = M ? pick_vec(dtype, D, ld_dy, D, dy, dtable) : pick_vec(dtype, D, D, D, dtable, dtable);
+  launch<GoRows>(dtype, vec, a, (unsigned)((V + a.rows - 1) / a.rows), s);
+  if (M > HOT) {
+    const unsigned segments = (unsigned)((M + HOT - 1) / HOT);
+    launch<GoHot>(dtype, vec, a, segments, s);
+    launch<GoHotRows>(dtype, vec, a, segments, s);
+  }
+  return launch_status();
+}
+
+extern "C" int gnet_embed_scale_backward(const void* ids, int32_t ids64, const void* table, int64_t ld_table, const void* dy, int64_t ld_dy,
+                                         float scale, int64_t M, int64_t V, int64_t D, int32_t dtype, float* dscale, gnet_stream_t stream) {
+  clear_hip_error();
+  if (const int e = check(M, V, D, ld_table < ld_dy ? ld_table : ld_dy, dtype)) return e;
+  if (M == 0) return GNET_OK;
+  if (!ids || !table || !dy || !dscale) return GNET_ERR_INVALID;
+  ScaleArgs a{ids, ids64, M, V, D, table, ld_table, dy, ld_dy, scale, dscale};
+  launch<GoScale>(dtype, pick_vec(dtype, D, ld_table, ld_dy, table, dy), a, (unsigned)((M + 3) / 4), (hipStream_t)stream);
+  return launch_status();
+}

@@ -1,0 +1,280 @@
+// The matrix products of the vocabulary losses (vocab.hip) on the 16-bit matrix pipe, fp32 accumulation:
+//   logits   z  = W . x^T      rows = vocabulary, columns = tokens, contraction over D      (both operands contraction-contiguous)
+//   d x^T       = W^T . dz^T   rows = features,   columns = tokens, contraction over V      (W contraction-strided)
+//   d W^T       = x^T . dz     rows = features,   columns = vocabulary, contraction over tokens  (both contraction-strided)
+// Rows sit in the accumulators' register direction (a lane of v_mfma_f32_16x16x32 holds four consecutive rows of one column),
+// so the softmax sums run inside a lane and every store is of consecutive elements of a row-major result.
+//
+// Operands of 32 bits are two fp16 planes, x s = hi + lo (s a power of two that puts the tensor's largest magnitude in
+// [2^13, 2^14)); a product is hi.hi + hi.lo + lo.hi, three passes ("segments") over the contraction into one accumulator.  What is
+// dropped or rounded is below 3 x 2^-24 of |a||b|, plus 2^-39 of the tensors' largest magnitudes where lo is subnormal.
+#pragma once
+#include "common.hpp"
+
+typedef unsigned short u16;
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+// ---- element types ----------------------------------------------------------------------------------------------
+struct Bf16T {
+  static __device__ __forceinline__ f32x4 mma(s16x8 a, s16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ u16 enc(float v) { return __builtin_bit_cast(u16, (__bf16)v); }
+  static __device__ __forceinline__ float dec(u16 v) { return __uint_as_float((unsigned)v << 16); }
+};
+struct F16T {
+  static __device__ __forceinline__ f32x4 mma(s16x8 a, s16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ u16 enc(float v) { return __builtin_bit_cast(u16, (_Float16)v); }
+  static __device__ __forceinline__ float dec(u16 v) { return (float)__builtin_bit_cast(_Float16, v); }
+};
+// a 32-bit value as the sum of two fp16
+__device__ __forceinline__ void split_f16(float v, u16& hi, u16& lo) {
+  hi = F16T::enc(v);
+  lo = F16T::enc(v - F16T::dec(hi));
+}
+
+// What the preparation kernels find out on the device.
+struct VocabMeta {
+  int rows;            // tokens that count (compacted)
+  float unscale_x;     // 1 / scale of the packed x (32-bit operands; else 1)
+  float unscale_w;
+  float unscale_g;     // one unit of the stored dz
+};
+
+constexpr int VG_BK = 64;      // contraction step
+
+struct VocabOperand {
+  const u16* p;        // first element (of plane 0)
+  int64_t ld;          // elements between rows as they lie in memory
+  int64_t plane;       // elements between the two planes of a 32-bit operand
+  int64_t rows;        // rows that may be read: a row index beyond is clamped to the last (its products are zero or not stored)
+  int cols;            // contraction-strided operands: elements of a row that may be read (a multiple of 8)
+};
+
+struct VocabGemm {
+  VocabOperand a, b;
+  int64_t k;                   // contraction length, a multiple of VG_BK (k_from_meta: meta->rows rounded up)
+  int k_from_meta;
+  int cols_from_meta;          // columns are tokens: column tiles behind meta->rows are left out
+  int segments;                // 1, or 3 with two planes
+  int row_tiles, col_tiles, splits;
+  const VocabMeta* meta;
+  // logits
+  float to_log2;               // log2(e) / temperature
+  int64_t valid_rows;          // vocabulary rows of this piece that exist
+  int first_row_tile, all_row_tiles;
+  float2* part;                // [column][all_row_tiles] running maximum and sum of a row tile
+  const float* lse2; const float* gscale;   // per column
+  u16* dz; int64_t ld_dz, plane_dz;
+  // products
+  float* slab; int64_t ld_slab, slab_stride; int accumulate;      // [split][column][ld_slab]
+  void* out; int64_t ld_out, out_rows, out_cols; int out_vec; int unscale_by_x;   // [column][row]; out_vec: four elements may be stored at once
+};
+
+enum { EPI_PART = 0, EPI_DZ = 1, EPI_SLAB = 2, EPI_OUT = 3 };
+
+// ---- staging of one operand tile, 16 bytes per lane straight into LDS ------------------------------------------------
+// Contraction-contiguous (STRIDED = false): LDS [T rows][64 k], 128 bytes a row; the 16-byte chunk c of row r lies at position
+// c ^ (r & 7), so that the 16 rows of a fragment read cover all banks.
+// Contraction-strided: LDS [64 k][T columns]; the 32-byte granule g of row k lies at g ^ h(k), so that the rows a transposing
+// read touches at once lie in different banks.
+template <int T> __device__ __forceinline__ int granule_swizzle(int k) {
+  return T >= 256 ? ((k & 3) | ((k >> 1) & 12)) : T >= 128 ? ((k & 3) | ((k >> 1) & 4)) : (k & (T / 16 - 1));
+}
+
+template <int T, bool STRIDED, int WAVES>
+__device__ __forceinline__ void stage_tile(char* lds, const VocabOperand& o, int64_t plane_off, int64_t t0, int64_t k0, int wave, int lane) {
+  constexpr int OPS = T * VG_BK * 2 / 1024;       // 1 KB per wave-wide load
+#pragma unroll
+  for (int op = wave; op < OPS; op += WAVES) {
+    const u16* src;
+    if (!STRIDED) {
+      const int r = op * 8 + (lane >> 3), c = (lane & 7) ^ (r & 7);
+      const int64_t row = min(t0 + r, o.rows - 1);
+      src = o.p + plane_off + row * o.ld + k0 + c * 8;
+    } else {
+      constexpr int CH = T / 8;                   // 16-byte chunks a row
+      const int idx = op * 64 + lane, r = idx / CH, p = idx % CH;
+      const int c = (((p >> 1) ^ granule_swizzle<T>(r)) << 1) | (p & 1);
+      const int64_t row = min(k0 + r, o.rows - 1);
+      const int64_t col = min(t0 + c * 8, (int64_t)o.cols - 8);
+      src = o.p + plane_off + row * o.ld + col;
+    }
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                     (__attribute__((address_space(3))) void*)(lds + op * 1024), 16, 0, 0);
+  }
+}
+
+// One 16 x 32 fragment: lane l gets row t + (l & 15), contraction elements 32 s + 8 (l >> 4) .. + 7.
+template <int T, bool STRIDED>
+__device__ __forceinline__ s16x8 read_frag(const char* lds, int t, int s, int lane) {
+  if (!STRIDED) {
+    const int r = t + (lane & 15), c = s * 4 + (lane >> 4);
+    return *reinterpret_cast<const s16x8*>(lds + r * 128 + ((c ^ (r & 7)) << 4));
+  } else {
+    const int i = lane & 15, k = s * 32 + (lane >> 4) * 8 + (i >> 2);
+    const int g = t >> 4;
+    const char* p0 = lds + k * (T * 2) + ((g ^ granule_swizzle<T>(k)) << 5) + (i & 3) * 8;
+    const char* p1 = lds + (k + 4) * (T * 2) + ((g ^ granule_swizzle<T>(k + 4)) << 5) + (i & 3) * 8;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p0);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p1);
+    return s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  }
+}
+
+template <class T, int BM, int BN, int WM, int WN, bool A_STRIDED, bool B_STRIDED, int EPI, int PLANES>
+__global__ void __launch_bounds__(64 * WM * WN) vocab_gemm(const VocabGemm g) {
+  constexpr int WAVES = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
+  __shared__ __attribute__((aligned(16))) char lds[(BM + BN) * VG_BK * 2];
+  char* const la = lds;
+  char* const lb = lds + BM * VG_BK * 2;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  const int id = blockIdx.x;
+  const int split = id % g.splits, tile = id / g.splits;
+  const int ct = tile % g.col_tiles, rt = tile / g.col_tiles;
+  const int64_t r0 = (int64_t)rt * BM, c0 = (int64_t)ct * BN;
+  const int rows = g.meta->rows;
+  // (the last step of a contraction over tokens reads dz up to the next multiple of its length)
+  if (g.cols_from_meta && c0 >= ((rows + VG_BK - 1) & ~(VG_BK - 1))) return;
+  const int64_t k_all = g.k_from_meta ? (int64_t)((rows + VG_BK - 1) / VG_BK) * VG_BK : g.k;
+  const int64_t steps = k_all / VG_BK, s0 = steps * split / g.splits, s1 = steps * (split + 1) / g.splits;
+
+  f32x4 acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  for (int seg = 0; seg < (PLANES == 1 ? 1 : 3); ++seg) {
+    const int64_t pa = PLANES == 1 || seg != 0 ? 0 : g.a.plane, pb = PLANES == 1 || seg != 1 ? 0 : g.b.plane;   // lo.hi, hi.lo, hi.hi
+    for (int64_t s = s0; s < s1; ++s) {
+      stage_tile<BM, A_STRIDED, WAVES>(la, g.a, pa, r0, s * VG_BK, wave, lane);
+      stage_tile<BN, B_STRIDED, WAVES>(lb, g.b, pb, c0, s * VG_BK, wave, lane);
+      __syncthreads();
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        s16x8 fa[FM], fb[FN];
+#pragma unroll
+        for (int i = 0; i < FM; ++i) fa[i] = read_frag<BM, A_STRIDED>(la, (wm * FM + i) * 16, ks, lane);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) fb[j] = read_frag<BN, B_STRIDED>(lb, (wn * FN + j) * 16, ks, lane);
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int j = 0; j < FN; ++j) acc[i][j] = T::mma(fa[i], fb[j], acc[i][j]);
+      }
+      __syncthreads();
+    }
+  }
+
+  const int col16 = lane & 15, quad = lane >> 4;
+  if constexpr (EPI == EPI_PART) {
+    // the tile's maximum and sum of 2^(z - max), z in units of log2, for each of its columns (tokens)
+    const float f = g.to_log2 * g.meta->unscale_x * g.meta->unscale_w;
+    float2* red = reinterpret_cast<float2*>(lds);        // [WM][BN]
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      float m = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int64_t row = r0 + (wm * FM + i) * 16 + quad * 4 + r;
+          const float z = row < g.valid_rows ? acc[i][j][r] * f : -INFINITY;
+          acc[i][j][r] = z;
+          m = fmaxf(m, z);
+        }
+      m = fmaxf(m, __shfl_xor(m, 16));
+      m = fmaxf(m, __shfl_xor(m, 32));
+      const float base = m == -INFINITY ? 0.f : m;       // nothing here yet: exp2(-inf - 0) = 0
+      float l = 0.f;
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) l += __builtin_amdgcn_exp2f(acc[i][j][r] - base);
+      l += __shfl_xor(l, 16);
+      l += __shfl_xor(l, 32);
+      if (quad == 0) red[wm * BN + (wn * FN + j) * 16 + col16] = make_float2(m, l);
+    }
+    __syncthreads();
+    for (int c = tid; c < BN; c += 64 * WAVES) {
+      if (c0 + c >= rows) continue;
+      float m = red[c].x;
+#pragma unroll
+      for (int w = 1; w < WM; ++w) m = fmaxf(m, red[w * BN + c].x);
+      const float base = m == -INFINITY ? 0.f : m;
+      float l = 0.f;
+#pragma unroll
+      for (int w = 0; w < WM; ++w) l += red[w * BN + c].y * __builtin_amdgcn_exp2f(red[w * BN + c].x - base);
+      g.part[(size_t)(c0 + c) * g.all_row_tiles + g.first_row_tile + rt] = make_float2(m, l);
+    }
+  } else if constexpr (EPI == EPI_DZ) {
+    const float f = g.to_log2 * g.meta->unscale_x * g.meta->unscale_w;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      const int64_t c = c0 + (wn * FN + j) * 16 + col16;
+      const bool some = c < rows;
+      const float lse = some ? g.lse2[c] : 0.f, gs = some ? g.gscale[c] : 0.f;
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        const int64_t row = r0 + (wm * FM + i) * 16 + quad * 4;
+        u16 v[4], lo[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          // padding (a token or a vocabulary row that does not exist) is zero: it takes part in the products
+          const float d = some && row + r < g.valid_rows ? __builtin_amdgcn_exp2f(acc[i][j][r] * f - lse) * gs : 0.f;
+          if (PLANES == 1) v[r] = T::enc(d); else split_f16(d, v[r], lo[r]);
+        }
+        *reinterpret_cast<s16x4*>(g.dz + c * g.ld_dz + row) = s16x4{(short)v[0], (short)v[1], (short)v[2], (short)v[3]};
+        if (PLANES == 2)
+          *reinterpret_cast<s16x4*>(g.dz + g.plane_dz + c * g.ld_dz + row) = s16x4{(short)lo[0], (short)lo[1], (short)lo[2], (short)lo[3]};
+      }
+    }
+  } else if constexpr (EPI == EPI_SLAB) {
+    float* slab = g.slab + split * g.slab_stride;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      const int64_t c = c0 + (wn * FN + j) * 16 + col16;
+      if (c >= g.out_cols) continue;
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        const int64_t row = r0 + (wm * FM + i) * 16 + quad * 4;
+        if (row >= g.ld_slab) continue;                  // ld_slab is a multiple of 64
+        f32x4* p = reinterpret_cast<f32x4*>(slab + c * g.ld_slab + row);
+        f32x4 v = acc[i][j];
+        if (g.accumulate) v += *p;
+        *p = v;
+      }
+    }
+  } else {
+    const float f = g.meta->unscale_g * (g.unscale_by_x ? g.meta->unscale_x : g.meta->unscale_w);
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      const int64_t c = c0 + (wn * FN + j) * 16 + col16;
+      if (c >= g.out_cols) continue;
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        const int64_t row = r0 + (wm * FM + i) * 16 + quad * 4;
+        if (PLANES == 2) {
+          float* p = (float*)g.out + c * g.ld_out + row;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) if (row + r < g.out_rows) p[r] = acc[i][j][r] * f;
+        } else {
+          u16* p = (u16*)g.out + c * g.ld_out + row;
+          if (g.out_vec && row + 3 < g.out_rows) {
+            *reinterpret_cast<s16x4*>(p) = s16x4{(short)T::enc(acc[i][j][0] * f), (short)T::enc(acc[i][j][1] * f),
+                                                 (short)T::enc(acc[i][j][2] * f), (short)T::enc(acc[i][j][3] * f)};
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) if (row + r < g.out_rows) p[r] = T::enc(acc[i][j][r] * f);
+          }
+        }
+      }
+    }
+  }
+}

@@ -1,0 +1,235 @@
+"""The two ends of a model over a large vocabulary on the HIP library (csrc/embed.hip, csrc/vocab.hip): rows of a [V, D] table by
+token id with the table's gradient, and softmax losses over the V rows of a [V, D] weight matrix with theirs.  Plain tensors in,
+plain tensors out, forward and backward as two calls (as in fc.py); PyTorch only owns the memory.
+
+    y = embed_forward(ids, table, scale)                          # features of the tokens
+    loss, lse, hit = xent_forward(x, w, labels)                   # one fp32 loss per token; sum or average as needed
+    dx, dw = xent_backward(x, w, labels, lse, hit, dloss)         # dloss: d(total) / d(loss), per token or one number
+    embed_backward(ids, dy, table, scale, out=dw)                 # a table that is also w: its second gradient is added
+
+Tokens may be laid out in any number of leading dimensions ([B, T] or flat); x, w, table, dy are float32, bfloat16 or float16,
+all of a call of one type; ids and labels int32 or int64.  An id or label outside [0, V) means "no token here" (padding): nothing
+is read or added for it.  Every result is reproducible bit for bit.  The calls run on the current stream of the tensors' device and
+may be captured into a graph; workspaces come from PyTorch's allocator for each call."""
+import ctypes as C
+
+import torch
+
+from . import _lib
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # GNET_F32, GNET_BF16, GNET_F16
+
+
+def _p(t):
+    return C.c_void_p(t.data_ptr()) if t is not None else C.c_void_p(0)
+
+
+def _stream(dev):
+    return C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _matrix(t, what, cols=None, dtype=None):
+    """A [..., D] tensor as rows of D consecutive elements (a view where its layout allows it)."""
+    if t.dim() < 1 or t.dtype not in _TYPES:
+        raise _lib.InvalidArgumentError("%s must be a float32, bfloat16 or float16 tensor with at least one dimension" % what)
+    if cols is not None and t.shape[-1] != cols:
+        raise _lib.InvalidArgumentError("%s must have %d columns, not %d" % (what, cols, t.shape[-1]))
+    if dtype is not None and t.dtype != dtype:
+        raise _lib.InvalidArgumentError("%s is %s where %s is expected" % (what, t.dtype, dtype))
+    if t.shape[-1] == 0:
+        raise _lib.InvalidArgumentError("%s has rows of no elements" % what)
+    t = t.detach()
+    t = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    return t
+
+
+def _ld(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _on_device(first, **others):
+    """The device of a call (after the checks of shapes and types)."""
+    if not first.is_cuda:
+        raise _lib.GnetError("the vocabulary operators have only device kernels: pass CUDA/HIP tensors")
+    for what, t in others.items():
+        if t is not None and t.device != first.device:
+            raise _lib.InvalidArgumentError("%s is on %s where %s is expected" % (what, t.device, first.device))
+    return first.device
+
+
+def _ids(t, what, shape=None):
+    if t.dtype not in (torch.int32, torch.int64):
+        raise _lib.InvalidArgumentError("%s must be int32 or int64, not %s" % (what, t.dtype))
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise _lib.InvalidArgumentError("%s has shape %s where %s is expected" % (what, tuple(t.shape), tuple(shape)))
+    return t.detach().contiguous()
+
+
+def _per_token(t, what, shape):
+    """fp32 values of the tokens' shape."""
+    if tuple(t.shape) != tuple(shape):
+        raise _lib.InvalidArgumentError("%s has shape %s where %s is expected" % (what, tuple(t.shape), tuple(shape)))
+    return t.detach().to(torch.float32).contiguous()
+
+
+def _workspace(nbytes, device):
+    """256-byte aligned scratch of this call.  From the caching allocator: ordered on the current stream, and part of the graph's own
+    memory while one is captured, so that no two calls in flight share it."""
+    buf = torch.empty(nbytes + 256, dtype=torch.uint8, device=device)
+    return buf, C.c_void_p((buf.data_ptr() + 255) // 256 * 256)
+
+
+# ---- token rows ----------------------------------------------------------------------------------------------------
+def embed_forward(ids, table, scale=1.0, token_scale=None):
+    """y [*ids.shape, D] = scale * token_scale * table[ids]; zero rows where an id is outside [0, V).
+    table [V, D]; token_scale: one factor per token, of ids' shape (a detection's score, for instance), or None."""
+    if table.dim() != 2 or table.shape[0] < 1:
+        raise _lib.InvalidArgumentError("table must be [V, D] with V >= 1")
+    t = _matrix(table, "table")
+    V, D = t.shape
+    i = _ids(ids, "ids")
+    s = _per_token(token_scale, "token_scale", ids.shape) if token_scale is not None else None
+    dev = _on_device(t, ids=i, token_scale=s)
+    y = torch.empty(tuple(ids.shape) + (D,), dtype=t.dtype, device=dev)
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        _lib.check(lib.gnet_embed_forward(_p(i), int(i.dtype == torch.int64), _p(t), _ld(t), float(scale), _p(s), i.numel(), V, D,
+                                          _TYPES[t.dtype], _p(y), _stream(dev)), "gnet_embed_forward")
+    return y
+
+
+def embed_backward(ids, dy, table, scale=1.0, token_scale=None, need_dscale=False, out=None):
+    """(dtable, dscale): gradients of embed_forward.  dtable [V, D] = scale * sum over the tokens of each id, in token order, of
+    token_scale * dy.  out: a contiguous [V, D] gradient of table's type that dtable is added to and that is returned (added in fp32,
+    rounded once; rows without a token keep their bits).  dscale (with need_dscale): fp32, of ids' shape, = scale * dy . table[ids]."""
+    if table.dim() != 2 or table.shape[0] < 1:
+        raise _lib.InvalidArgumentError("table must be [V, D] with V >= 1")
+    t = _matrix(table, "table")
+    V, D = t.shape
+    i = _ids(ids, "ids")
+    if tuple(dy.shape) != tuple(ids.shape) + (D,):
+        raise _lib.InvalidArgumentError("dy has shape %s where %s is expected" % (tuple(dy.shape), tuple(ids.shape) + (D,)))
+    g = _matrix(dy, "dy", D, t.dtype)
+    s = _per_token(token_scale, "token_scale", ids.shape) if token_scale is not None else None
+    if out is not None:
+        if tuple(out.shape) != (V, D) or out.dtype != t.dtype or not out.is_contiguous():
+            raise _lib.InvalidArgumentError("out must be a contiguous [%d, %d] tensor of type %s" % (V, D, t.dtype))
+    dev = _on_device(t, ids=i, dy=g, token_scale=s, out=out)
+    dtable = out.detach() if out is not None else torch.empty(V, D, dtype=t.dtype, device=dev)
+    M = i.numel()
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        nbytes = lib.gnet_embed_workspace_bytes(M, D)
+        buf, ws = _workspace(nbytes, dev)
+        _lib.check(lib.gnet_embed_backward(_p(i), int(i.dtype == torch.int64), _p(g), _ld(g), float(scale), _p(s), M, V, D, _TYPES[t.dtype],
+                                           _p(dtable), int(out is not None), ws, nbytes, _stream(dev)), "gnet_embed_backward")
+        dscale = None
+        if need_dscale:
+            dscale = torch.empty(tuple(ids.shape), dtype=torch.float32, device=dev)
+            _lib.check(lib.gnet_embed_scale_backward(_p(i), int(i.dtype == torch.int64), _p(t), _ld(t), _p(g), _ld(g), float(scale), M, V, D,
+                                                     _TYPES[t.dtype], _p(dscale), _stream(dev)), "gnet_embed_scale_backward")
+    return (out if out is not None else dtable), dscale
+
+
+# ---- softmax losses over the vocabulary ------------------------------------------------------------------------------
+def _features(x, w):
+    if w.dim() != 2 or w.shape[0] < 1:
+        raise _lib.InvalidArgumentError("w must be [V, D] with V >= 1")
+    wm = _matrix(w, "w")
+    return _matrix(x, "x", wm.shape[1], wm.dtype), wm
+
+
+def _teacher(top_ids, top_logits, x, temperature):
+    if not (temperature > 0 and temperature < float("inf")):
+        raise _lib.InvalidArgumentError("temperature must be positive and finite, not %s" % (temperature,))
+    lead = tuple(x.shape[:-1])
+    if top_ids.dim() != len(lead) + 1 or tuple(top_ids.shape[:-1]) != lead or top_ids.shape[-1] < 1:
+        raise _lib.InvalidArgumentError("top_ids must be [*tokens, K] with K >= 1, tokens %s" % (lead,))
+    return _ids(top_ids, "top_ids"), _per_token(top_logits, "top_logits", top_ids.shape)
+
+
+def _loss_gradient(dloss, lead):
+    """d(total) / d(loss) per token; one number (a tensor without dimensions) stands for all of them."""
+    if dloss.dim() == 0:
+        dloss = dloss.expand(lead)
+    return _per_token(dloss, "dloss", lead)
+
+
+def xent_forward(x, w, labels):
+    """(loss, lse, hit), fp32, of labels' shape: softmax cross entropy of the logits x . w^T (x [*tokens, D], w [V, D]) against
+    labels [*tokens], the logits' log-sum-exp and the label's logit.  All three are 0 where the label is outside [0, V)."""
+    xm, wm = _features(x, w)
+    lead = tuple(x.shape[:-1])
+    i = _ids(labels, "labels", lead)
+    dev = _on_device(wm, x=xm, labels=i)
+    (M, D), V = xm.shape, wm.shape[0]
+    loss, lse, hit = (torch.empty(lead, dtype=torch.float32, device=dev) for _ in range(3))
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        nbytes = lib.gnet_vocab_workspace_bytes(_p(wm), _ld(wm), M, V, D, 1, _TYPES[wm.dtype], 0)
+        buf, ws = _workspace(nbytes, dev)
+        _lib.check(lib.gnet_xent_forward(_p(xm), _ld(xm), _p(wm), _ld(wm), _p(i), int(i.dtype == torch.int64), M, V, D, _TYPES[wm.dtype],
+                                         _p(loss), _p(lse), _p(hit), ws, nbytes, _stream(dev)), "gnet_xent_forward")
+    return loss, lse, hit
+
+
+def xent_backward(x, w, labels, lse, hit, dloss, need_dx=True, need_dw=True):
+    """(dx, dw) of xent_forward, of x's and w's shapes and type, from its lse and hit and the losses' gradient dloss (labels' shape,
+    or a tensor without dimensions for all tokens).  None for what is not needed."""
+    xm, wm = _features(x, w)
+    lead = tuple(x.shape[:-1])
+    i = _ids(labels, "labels", lead)
+    return _backward(xm, wm, i, None, 1.0, _per_token(lse, "lse", lead), _per_token(hit, "hit", lead), _loss_gradient(dloss, lead), x.shape, 1, need_dx, need_dw)
+
+
+def distill_forward(x, w, top_ids, top_logits, temperature=1.0):
+    """(loss, lse, hit), fp32: divergence of the student's softmax(x . w^T / temperature) from the teacher's softmax over its K best
+    logits / temperature (top_ids, top_logits [*tokens, K]), the student's log-sum-exp [*tokens], and its logits / temperature at
+    top_ids [*tokens, K].  Slots with an id outside [0, V) or a logit of -inf are left out; a token without slots has loss 0."""
+    xm, wm = _features(x, w)
+    lead = tuple(x.shape[:-1])
+    i, t = _teacher(top_ids, top_logits, x, temperature)
+    dev = _on_device(wm, x=xm, top_ids=i, top_logits=t)
+    (M, D), V, K = xm.shape, wm.shape[0], i.shape[-1]
+    loss, lse = (torch.empty(lead, dtype=torch.float32, device=dev) for _ in range(2))
+    hit = torch.empty(lead + (K,), dtype=torch.float32, device=dev)
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        nbytes = lib.gnet_vocab_workspace_bytes(_p(wm), _ld(wm), M, V, D, K, _TYPES[wm.dtype], 0)
+        buf, ws = _workspace(nbytes, dev)
+        _lib.check(lib.gnet_distill_forward(_p(xm), _ld(xm), _p(wm), _ld(wm), _p(i), int(i.dtype == torch.int64), _p(t), float(temperature),
+                                            M, V, D, K, _TYPES[wm.dtype], _p(loss), _p(lse), _p(hit), ws, nbytes, _stream(dev)),
+                   "gnet_distill_forward")
+    return loss, lse, hit
+
+
+def distill_backward(x, w, top_ids, top_logits, lse, hit, dloss, temperature=1.0, need_dx=True, need_dw=True):
+    """(dx, dw) of distill_forward, of x's and w's shapes and type (the teacher's logits get no gradient)."""
+    xm, wm = _features(x, w)
+    lead = tuple(x.shape[:-1])
+    i, t = _teacher(top_ids, top_logits, x, temperature)
+    return _backward(xm, wm, i, t, temperature, _per_token(lse, "lse", lead), _per_token(hit, "hit", i.shape), _loss_gradient(dloss, lead), x.shape, i.shape[-1], need_dx, need_dw)
+
+
+def _backward(xm, wm, i, t, temperature, lse, hit, dloss, x_shape, K, need_dx, need_dw):
+    dev = _on_device(wm, x=xm, labels=i, top_logits=t, lse=lse, hit=hit, dloss=dloss)
+    (M, D), V, dt = xm.shape, wm.shape[0], _TYPES[wm.dtype]
+    dx = torch.empty(x_shape, dtype=xm.dtype, device=dev) if need_dx else None
+    dw = torch.empty(V, D, dtype=wm.dtype, device=dev) if need_dw else None
+    if not (need_dx or need_dw):
+        return dx, dw
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        nbytes = lib.gnet_vocab_workspace_bytes(_p(wm), _ld(wm), M, V, D, K, dt, 1)
+        buf, ws = _workspace(nbytes, dev)
+        ids64 = int(i.dtype == torch.int64)
+        if t is None:
+            _lib.check(lib.gnet_xent_backward(_p(xm), _ld(xm), _p(wm), _ld(wm), _p(i), ids64, _p(lse), _p(hit), _p(dloss), M, V, D, dt,
+                                              _p(dx), _p(dw), ws, nbytes, _stream(dev)), "gnet_xent_backward")
+        else:
+            _lib.check(lib.gnet_distill_backward(_p(xm), _ld(xm), _p(wm), _ld(wm), _p(i), ids64, _p(t), float(temperature), _p(lse), _p(hit),
+                                                 _p(dloss), M, V, D, K, dt, _p(dx), _p(dw), ws, nbytes, _stream(dev)),
+                       "gnet_distill_backward")
+    return dx, dw

@@ -297,6 +297,60 @@ int roi_pool_bwd_atomic_f32(const float* top_diff, const int32_t* argmax, const 
                             int32_t B, int32_t H, int32_t W, int32_t C, int32_t R, int32_t pooled_h,
                             int32_t pooled_w, float spatial_scale, float* bottom_diff, gnet_stream_t stream);
 
+/* ---- vocabulary operators: rows of a [V,D] table by token id, and softmax losses over the V rows of a [V,D] weight matrix (the
+ * two ends of a model over a large vocabulary; no reference counterpart).  Element types of x, w, table, dy and of the gradients of
+ * each: GNET_F32, GNET_BF16 or GNET_F16, one type a call.  Sums, softmax statistics, losses and per-token values are fp32.
+ * Ids are int32 or int64 (ids64 != 0) in device memory; an id outside [0, V) means "no token": it is never an error.
+ * Matrices are row-major with a row stride (ld, elements) where one is given, dense otherwise; workspaces 256-byte aligned.
+ * Two calls in flight at the same time must not share a workspace.
+ * Limits (GNET_ERR_UNSUPPORTED beyond): M <= 2^24 tokens, V <= 2^30, M V <= 2^44, D <= 2^16, K <= 1024. */
+#define GNET_F32 0
+#define GNET_BF16 1
+#define GNET_F16 2
+
+/* y[m] = scale * token_scale[m] * table[ids[m]]; zero where the id is outside [0, V).  token_scale: [M] or NULL (ones).  y [M,D]. */
+int gnet_embed_forward(const void* ids, int32_t ids64, const void* table, int64_t ld_table, float scale, const float* token_scale,
+                       int64_t M, int64_t V, int64_t D, int32_t dtype, void* y, gnet_stream_t stream);
+/* dtable [V,D] = scale * sum over the tokens with id v, in token order, of token_scale[m] * dy[m]: overwritten (rows without a token
+ * are zero), or, with accumulate != 0, added to (the sum is added in fp32 and rounded once; rows without a token are not touched).
+ * Reproducible: no atomics.  workspace: gnet_embed_workspace_bytes(M, D). */
+size_t gnet_embed_workspace_bytes(int64_t M, int64_t D);
+int gnet_embed_backward(const void* ids, int32_t ids64, const void* dy, int64_t ld_dy, float scale, const float* token_scale, int64_t M,
+                        int64_t V, int64_t D, int32_t dtype, void* dtable, int32_t accumulate, void* workspace,
+                        size_t workspace_bytes, gnet_stream_t stream);
+/* dscale[m] = scale * dy[m] . table[ids[m]] (the gradient of token_scale); zero where the id is outside [0, V). */
+int gnet_embed_scale_backward(const void* ids, int32_t ids64, const void* table, int64_t ld_table, const void* dy, int64_t ld_dy,
+                              float scale, int64_t M, int64_t V, int64_t D, int32_t dtype, float* dscale, gnet_stream_t stream);
+
+/* Softmax cross entropy of z = x . w^T (x [M,D], w [V,D]) against labels [M], without laying z out:
+ *   lse[m] = log sum_v exp z[m,v]     hit[m] = z[m,labels[m]]     loss[m] = lse[m] - hit[m] (never below 0)
+ * A token whose label is outside [0, V) is left out: loss, lse, hit and its row of dx are 0 and it adds nothing to dw, whatever its row
+ * of x holds.  Backward: from the forward pass's lse and hit and the losses' gradients dloss [M],
+ *   dz[m,v] = dloss[m] (exp(z[m,v] - lse[m]) - [v = labels[m]])     dx = dz . w     dw = dz^T . x
+ * dx [M,D] and dw [V,D] are overwritten; either may be NULL.  The logits are formed again, one piece of the vocabulary at a time;
+ * dz is kept in 16 bits (GNET_F32: two fp16 of together 22 bits) for the piece.  GNET_F32 operands must be finite.  Reproducible.
+ * workspace of all four calls: gnet_vocab_workspace_bytes(w, ldw, M, V, D, K, dtype, backward) (K = 1 for cross entropy). */
+size_t gnet_vocab_workspace_bytes(const void* w, int64_t ldw, int64_t M, int64_t V, int64_t D, int64_t K, int32_t dtype,
+                                  int32_t backward);
+int gnet_xent_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* labels, int32_t labels64, int64_t M,
+                      int64_t V, int64_t D, int32_t dtype, float* loss, float* lse, float* hit, void* workspace,
+                      size_t workspace_bytes, gnet_stream_t stream);
+int gnet_xent_backward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* labels, int32_t labels64,
+                       const float* lse, const float* hit, const float* dloss, int64_t M, int64_t V, int64_t D, int32_t dtype,
+                       void* dx, void* dw, void* workspace, size_t workspace_bytes, gnet_stream_t stream);
+/* Distillation from a teacher's K best logits per token (top_ids, top_logits [M,K]) at a temperature > 0: with
+ * z = x . w^T / temperature and q = softmax over the row's slots of top_logits / temperature,
+ *   loss[m] = sum_k q_k (log q_k - z[m,id_k] + lse[m])     lse[m] = log sum_v exp z[m,v]     hit[m,k] = z[m,id_k]
+ * (the divergence of the student from the teacher's renormalised head; no temperature^2 factor).  A slot whose id is outside [0, V) or
+ * whose logit is -inf is left out (hit 0), a token without any slot like a token without a label above.  An id may occur twice. */
+int gnet_distill_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* top_ids, int32_t ids64,
+                         const float* top_logits, float temperature, int64_t M, int64_t V, int64_t D, int64_t K, int32_t dtype,
+                         float* loss, float* lse, float* hit, void* workspace, size_t workspace_bytes, gnet_stream_t stream);
+int gnet_distill_backward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* top_ids, int32_t ids64,
+                          const float* top_logits, float temperature, const float* lse, const float* hit, const float* dloss,
+                          int64_t M, int64_t V, int64_t D, int64_t K, int32_t dtype, void* dx, void* dw, void* workspace,
+                          size_t workspace_bytes, gnet_stream_t stream);
+
 /* ---- optional per-kernel timing (measurement only; no reference counterpart) -------------
  * A caller-owned pool of HIP event pairs recorded on the launch stream around every kernel of the
  * selected classes.  gnet_profiler_read synchronises the recorded events, adds the elapsed
