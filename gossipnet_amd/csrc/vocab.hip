@@ -13,7 +13,7 @@
 
 namespace {
 
-constexpr int TILE = 128;
+constexpr int TILE = 256;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 __device__ __forceinline__ int64_t load_id(const void* p, int64_t i, int is64) {
@@ -383,7 +383,7 @@ Plan make_plan(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int pack_w
 }
 
 int needs_pack(const void* w, int64_t ldw, int64_t D, int dtype) {
-  return dtype == GNET_F32 || (D & 63) || (ldw & 7) || ((uintptr_t)w & 15);
+  return dtype == GNET_F32 || (D & 63) || (ldw & 7) || ldw > (1 << 22) || ((uintptr_t)w & 15);      // (2^22: 32-bit offsets in a tile)
 }
 
 struct Problem {
@@ -401,7 +401,7 @@ int check(const Problem& q) {
 
 template <int DT, class T, int PLANES> struct Run {
   template <bool AS, bool BS, int EPI> static void gemm(const VocabGemm& g, hipStream_t s) {
-    vocab_gemm<T, TILE, TILE, 2, 2, AS, BS, EPI, PLANES><<<(unsigned)((int64_t)g.row_tiles * g.col_tiles * g.splits), 256, 0, s>>>(g);
+    vocab_gemm<T, TILE, TILE, 2, 4, AS, BS, EPI, PLANES><<<(unsigned)((int64_t)g.row_tiles * g.col_tiles * g.splits), 512, 0, s>>>(g);
   }
 
   // targets, packing: everything in front of the first matrix product

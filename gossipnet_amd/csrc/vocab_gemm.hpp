@@ -86,28 +86,64 @@ template <int T> __device__ __forceinline__ int granule_swizzle(int k) {
   return T >= 256 ? ((k & 3) | ((k >> 1) & 12)) : T >= 128 ? ((k & 3) | ((k >> 1) & 4)) : (k & (T / 16 - 1));
 }
 
-template <int T, bool STRIDED, int WAVES>
-__device__ __forceinline__ void stage_tile(char* lds, const VocabOperand& o, int64_t plane_off, int64_t t0, int64_t k0, int wave, int lane) {
-  constexpr int OPS = T * VG_BK * 2 / 1024;       // 1 KB per wave-wide load
-#pragma unroll
-  for (int op = wave; op < OPS; op += WAVES) {
-    const u16* src;
-    if (!STRIDED) {
-      const int r = op * 8 + (lane >> 3), c = (lane & 7) ^ (r & 7);
-      const int64_t row = min(t0 + r, o.rows - 1);
-      src = o.p + plane_off + row * o.ld + k0 + c * 8;
-    } else {
-      constexpr int CH = T / 8;                   // 16-byte chunks a row
-      const int idx = op * 64 + lane, r = idx / CH, p = idx % CH;
-      const int c = (((p >> 1) ^ granule_swizzle<T>(r)) << 1) | (p & 1);
-      const int64_t row = min(k0 + r, o.rows - 1);
-      const int64_t col = min(t0 + c * 8, (int64_t)o.cols - 8);
-      src = o.p + plane_off + row * o.ld + col;
-    }
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                     (__attribute__((address_space(3))) void*)(lds + op * 1024), 16, 0, 0);
-  }
+// 64 lanes x 16 bytes from base + off (bytes, per lane) to 1 KB of LDS.  As a statement of its own: the compiler would order the builtin's
+// LDS write against every later LDS read with a wait for all loads, and with it end the overlap of one step's loads with the step
+// before.  It has no register result; the waits are in vocab_gemm's loop; nothing else in the kernel uses M0.
+__device__ __forceinline__ void load_to_lds(const char* base, unsigned off, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
 }
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+  return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
+}
+
+// A wave's share of one operand's tiles: OPS / WAVES loads of 1 KB a step, their lanes' byte offsets from the tile's first row (contraction-
+// contiguous) or the step's first row (contraction-strided) kept in registers.
+template <int T, bool STRIDED, int WAVES> struct Stager {
+  static constexpr int OPS = T * VG_BK * 2 / 1024, N = OPS / WAVES, CH = T / 8;      // CH: 16-byte chunks a strided row
+  static_assert(OPS % WAVES == 0, "a wave loads whole kilobytes");
+  const char* base;
+  unsigned off[N];
+  int64_t step_bytes, rows;
+  unsigned row_bytes;
+
+  __device__ __forceinline__ void init(const VocabOperand& o, int64_t t0, int64_t k0, int wave, int lane) {
+    row_bytes = (unsigned)(o.ld * 2);
+    rows = o.rows;
+    if (!STRIDED) {
+      base = (const char*)(o.p + t0 * o.ld + k0);
+      step_bytes = VG_BK * 2;
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+        const int r = (u * WAVES + wave) * 8 + (lane >> 3), c = (lane & 7) ^ (r & 7);
+        off[u] = (unsigned)min((int64_t)r, rows - 1 - t0) * row_bytes + c * 16;
+      }
+    } else {
+      base = (const char*)(o.p + k0 * o.ld);
+      step_bytes = VG_BK * o.ld * 2;
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+        const int idx = (u * WAVES + wave) * 64 + lane, r = idx / CH, p = idx % CH;
+        const int c = (((p >> 1) ^ granule_swizzle<T>(r)) << 1) | (p & 1);
+        off[u] = r * row_bytes + (unsigned)min(t0 + c * 8, (int64_t)o.cols - 8) * 2;
+      }
+    }
+  }
+  // step s counted from k0, at its byte offset `plane` further on
+  __device__ __forceinline__ void load(unsigned lds, int s, int64_t k, int64_t plane, int wave, int lane) const {
+    const char* from = base + s * step_bytes + plane;
+    if (STRIDED && k + VG_BK > rows) {                    // the last rows end inside this step
+      const unsigned last = (unsigned)(rows - 1 - k);
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+        const unsigned r = ((u * WAVES + wave) * 64 + lane) / CH;
+        load_to_lds(from, off[u] - (r > last ? r - last : 0) * row_bytes, lds + (u * WAVES + wave) * 1024);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < N; ++u) load_to_lds(from, off[u], lds + (u * WAVES + wave) * 1024);
+    }
+  }
+};
 
 // One 16 x 32 fragment: lane l gets row t + (l & 15), contraction elements 32 s + 8 (l >> 4) .. + 7.
 template <int T, bool STRIDED>
@@ -126,23 +162,32 @@ __device__ __forceinline__ s16x8 read_frag(const char* lds, int t, int s, int la
   }
 }
 
+// Workgroups are dealt to the eight XCDs in turn: give every XCD a contiguous share of the tiles, and within it run through four
+// row tiles at a time, so that the 32 workgroups that an XCD works on at once share four row panels and eight column panels in its L2.
+__device__ __forceinline__ void tile_of(int id, int row_tiles, int col_tiles, int splits, int& rt, int& ct, int& split) {
+  const int n = row_tiles * col_tiles * splits, x = id & 7, q = n >> 3, r = n & 7;
+  int t = x * q + min(x, r) + (id >> 3);
+  split = t / (row_tiles * col_tiles);
+  t -= split * row_tiles * col_tiles;
+  const int group = t / (4 * col_tiles), left = t - group * 4 * col_tiles, h = min(4, row_tiles - 4 * group);
+  ct = left / h;
+  rt = group * 4 + (left - ct * h);
+}
+
 template <class T, int BM, int BN, int WM, int WN, bool A_STRIDED, bool B_STRIDED, int EPI, int PLANES>
-__global__ void __launch_bounds__(64 * WM * WN) vocab_gemm(const VocabGemm g) {
-  constexpr int WAVES = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
-  __shared__ __attribute__((aligned(16))) char lds[(BM + BN) * VG_BK * 2];
-  char* const la = lds;
-  char* const lb = lds + BM * VG_BK * 2;
+__global__ void __launch_bounds__(64 * WM * WN, 2) vocab_gemm(const VocabGemm g) {
+  constexpr int WAVES = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16, STAGE = (BM + BN) * VG_BK * 2;
+  __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
-  const int id = blockIdx.x;
-  const int split = id % g.splits, tile = id / g.splits;
-  const int ct = tile % g.col_tiles, rt = tile / g.col_tiles;
+  int rt, ct, split;
+  tile_of(blockIdx.x, g.row_tiles, g.col_tiles, g.splits, rt, ct, split);
   const int64_t r0 = (int64_t)rt * BM, c0 = (int64_t)ct * BN;
   const int rows = g.meta->rows;
   // (the last step of a contraction over tokens reads dz up to the next multiple of its length)
   if (g.cols_from_meta && c0 >= ((rows + VG_BK - 1) & ~(VG_BK - 1))) return;
   const int64_t k_all = g.k_from_meta ? (int64_t)((rows + VG_BK - 1) / VG_BK) * VG_BK : g.k;
-  const int64_t steps = k_all / VG_BK, s0 = steps * split / g.splits, s1 = steps * (split + 1) / g.splits;
+  const int steps = (int)(k_all / VG_BK), s0 = (int)((int64_t)steps * split / g.splits), s1 = (int)((int64_t)steps * (split + 1) / g.splits);
 
   f32x4 acc[FM][FN];
 #pragma unroll
@@ -150,27 +195,43 @@ __global__ void __launch_bounds__(64 * WM * WN) vocab_gemm(const VocabGemm g) {
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  for (int seg = 0; seg < (PLANES == 1 ? 1 : 3); ++seg) {
-    const int64_t pa = PLANES == 1 || seg != 0 ? 0 : g.a.plane, pb = PLANES == 1 || seg != 1 ? 0 : g.b.plane;   // lo.hi, hi.lo, hi.hi
-    for (int64_t s = s0; s < s1; ++s) {
-      stage_tile<BM, A_STRIDED, WAVES>(la, g.a, pa, r0, s * VG_BK, wave, lane);
-      stage_tile<BN, B_STRIDED, WAVES>(lb, g.b, pb, c0, s * VG_BK, wave, lane);
-      __syncthreads();
+  // one step's loads are in flight while the step before is multiplied; one barrier a step: behind it the step's tiles are there and
+  // the other buffer is no longer read
+  const int n = (s1 - s0) * (PLANES == 1 ? 1 : 3);
+  Stager<BM, A_STRIDED, WAVES> sa;
+  Stager<BN, B_STRIDED, WAVES> sb;
+  sa.init(g.a, r0, (int64_t)s0 * VG_BK, wave, lane);
+  sb.init(g.b, c0, (int64_t)s0 * VG_BK, wave, lane);
+  const unsigned lds0 = lds_address(lds);
+  auto stage = [&](int it) {
+    const int seg = PLANES == 1 ? 0 : it / (s1 - s0), s = it - seg * (s1 - s0);
+    const unsigned to = lds0 + (it & 1) * STAGE;
+    const int64_t k = (int64_t)(s0 + s) * VG_BK;                                       // segments: lo.hi, hi.lo, hi.hi
+    sa.load(to, s, k, PLANES == 1 || seg != 0 ? 0 : g.a.plane * 2, wave, lane);
+    sb.load(to + BM * VG_BK * 2, s, k, PLANES == 1 || seg != 1 ? 0 : g.b.plane * 2, wave, lane);
+  };
+  if (n > 0) stage(0);
+  for (int it = 0; it < n; ++it) {
+    // (the reads of the step before have returned: their buffer is written next.  As one statement with a memory clobber, so that the
+    // compiler moves no LDS access across it; it keeps no loads in flight that this wait would not cover.)
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (it + 1 < n) stage(it + 1);
+    const char* const la = lds + (it & 1) * STAGE;
+    const char* const lb = la + BM * VG_BK * 2;
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        s16x8 fa[FM], fb[FN];
+    for (int ks = 0; ks < 2; ++ks) {
+      s16x8 fa[FM], fb[FN];
 #pragma unroll
-        for (int i = 0; i < FM; ++i) fa[i] = read_frag<BM, A_STRIDED>(la, (wm * FM + i) * 16, ks, lane);
+      for (int j = 0; j < FN; ++j) fb[j] = read_frag<BN, B_STRIDED>(lb, (wn * FN + j) * 16, ks, lane);
 #pragma unroll
-        for (int j = 0; j < FN; ++j) fb[j] = read_frag<BN, B_STRIDED>(lb, (wn * FN + j) * 16, ks, lane);
+      for (int i = 0; i < FM; ++i) fa[i] = read_frag<BM, A_STRIDED>(la, (wm * FM + i) * 16, ks, lane);
 #pragma unroll
-        for (int i = 0; i < FM; ++i)
+      for (int i = 0; i < FM; ++i)
 #pragma unroll
-          for (int j = 0; j < FN; ++j) acc[i][j] = T::mma(fa[i], fb[j], acc[i][j]);
-      }
-      __syncthreads();
+        for (int j = 0; j < FN; ++j) acc[i][j] = T::mma(fa[i], fb[j], acc[i][j]);
     }
   }
+  __syncthreads();                                 // the epilogue uses the LDS
 
   const int col16 = lane & 15, quad = lane >> 4;
   if constexpr (EPI == EPI_PART) {
