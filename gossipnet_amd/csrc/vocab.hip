@@ -2,10 +2,11 @@
 //   cross entropy   loss = lse(z) - z[label]                               (gnet_xent_*)
 //   distillation    loss = sum_k q_k (log q_k - z[id_k] + lse(z)),  q = softmax(teacher's logits / temperature)   (gnet_distill_*)
 // Cross entropy is distillation with one target of weight 1, so both run the same kernels:
-//   forward    vocab_targets  which tokens count, the targets' weights      vocab_pack   the tokens that count, moved together
-//              vocab_gemm<EPI_PART>  maximum and sum of 2^z per vocabulary tile         vocab_join   lse, the targets' logits, loss
+//   forward    vocab_targets  which tokens count, the teacher's weights      vocab_pack   the tokens that count, moved together
+//              vocab_gemm<EPI_PART>  maximum and sum of 2^z per vocabulary tile, the label's logit
+//              vocab_join, vocab_join_targets   lse, the teacher's ids' logits, loss
 //   backward   the first two, then for one piece of the vocabulary after the other
-//              vocab_gemm<EPI_DZ>  dz = g softmax(z) from recomputed logits       vocab_hits   dz at the targets, from fp32
+//              vocab_gemm<EPI_DZ>  dz = g (softmax(z) - label) from recomputed logits       vocab_hits   dz at the teacher's ids
 //              vocab_gemm<EPI_SLAB>  dx += dz . W (fp32)     vocab_gemm<EPI_OUT>  dW = dz^T . x     and at last vocab_finish  dx
 // A token whose targets are all outside [0, V) is left out of everything, whatever its row of x holds: it is not read again after
 // vocab_targets, its dx is zero.
@@ -13,16 +14,10 @@
 
 namespace {
 
-constexpr int TILE = 256;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 __device__ __forceinline__ int64_t load_id(const void* p, int64_t i, int is64) {
   return is64 ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
-}
-template <int DT> __device__ __forceinline__ float load_elem(const void* p, int64_t i) {
-  if (DT == GNET_F32) return ((const float*)p)[i];
-  if (DT == GNET_BF16) return Bf16T::dec(((const u16*)p)[i]);
-  return F16T::dec(((const u16*)p)[i]);
 }
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
@@ -34,100 +29,6 @@ __device__ __forceinline__ float wave_max(float v) {
   for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
   return v;
 }
-// the power of two that brings a magnitude into [2^top, 2^(top+1)); 1 for 0, infinities and NaN
-__device__ __forceinline__ int scale_exponent(float a, int top) {
-  if (!(a > 0.f) || !(a < INFINITY)) return 0;
-  return max(-126, min(126, top - ilogbf(a)));
-}
-
-struct Targets {
-  const void* ids; int ids64;          // [M,K]
-  const float* logits;                 // [M,K] teacher's logits, or NULL (one target of weight 1)
-  int64_t M; int K; int64_t V;
-  float to_log2;                       // log2(e) / temperature
-  float inv_temp;
-};
-__device__ __forceinline__ bool target_counts(const Targets& t, int64_t i, int64_t& id) {
-  id = load_id(t.ids, i, t.ids64);
-  return id >= 0 && id < t.V && !(t.logits && t.logits[i] == -INFINITY);
-}
-
-// One wave per token (and per padding byte of the flags): does it count; its targets' weights; in the backward pass weights of
-// equal ids added up in each of their slots.  Two passes over K logits, K <= 1024: latency.
-struct TargetsArgs {
-  Targets t;
-  int64_t flags_n;                     // M rounded up to 16
-  uint8_t* flag; float* q; float* q_sum; float* entropy;       // q_sum: backward pass; entropy: forward pass
-  const void* x; int64_t ldx, D; float* row_x;   // 32-bit x: the row's largest magnitude
-  const float* dloss; float* row_g;              // backward only
-};
-__global__ void __launch_bounds__(256) vocab_targets(const TargetsArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t m = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (m >= a.flags_n) return;
-  bool counts = false;
-  if (m < a.t.M) {
-    const int K = a.t.K;
-    float top = -INFINITY;
-    bool any = false;
-    for (int k = lane; k < K; k += 64) {
-      int64_t id;
-      if (target_counts(a.t, m * K + k, id)) { any = true; if (a.t.logits) top = fmaxf(top, a.t.logits[m * K + k]); }
-    }
-    counts = __any(any);
-    top = wave_max(top);
-    float sum = 0.f;
-    for (int k = lane; k < K; k += 64) {
-      int64_t id;
-      float e = 0.f;
-      if (target_counts(a.t, m * K + k, id)) e = a.t.logits ? exp2f((a.t.logits[m * K + k] - top) * a.t.to_log2) : 1.f;
-      a.q[m * K + k] = e;
-      sum += e;
-    }
-    sum = wave_sum(sum);
-    float ent = 0.f;
-    for (int k = lane; k < K; k += 64) {
-      const float e = a.q[m * K + k], q = counts ? e / sum : 0.f;
-      a.q[m * K + k] = q;
-      if (a.t.logits && q > 0.f) ent += q * ((a.t.logits[m * K + k] - top) * a.t.inv_temp - logf(sum));
-    }
-    if (a.entropy) { ent = wave_sum(ent); if (lane == 0) a.entropy[m] = ent; }
-    if (a.dloss && a.t.logits) {
-      // the same id twice in a row: each of its slots stands for the sum (read back what the wave itself wrote)
-      __threadfence_block();
-      for (int kb = 0; kb < K; kb += 64) {
-        const int k = kb + lane;
-        int64_t id = -1;
-        const bool c = k < K && target_counts(a.t, m * K + k, id);
-        float s = 0.f;
-        for (int j = 0; j < K; ++j)
-          if (c && load_id(a.t.ids, m * K + j, a.t.ids64) == id) s += a.q[m * K + j];
-        if (k < K) a.q_sum[m * K + k] = s;             // (an array of its own: later slots still read the single weights)
-      }
-    }
-    if (a.row_x) {
-      float mx = 0.f;
-      if (counts) for (int64_t d = lane; d < a.D; d += 64) mx = fmaxf(mx, fabsf(((const float*)a.x)[m * a.ldx + d]));
-      mx = wave_max(mx);
-      if (lane == 0) a.row_x[m] = mx;
-    }
-    if (a.row_g && lane == 0) a.row_g[m] = counts ? fabsf(a.dloss[m] * a.t.inv_temp) : 0.f;
-  }
-  if (lane == 0) a.flag[m] = counts;
-}
-
-// largest magnitude of a 32-bit matrix, one partial result per workgroup
-__global__ void __launch_bounds__(256) vocab_absmax(const float* __restrict__ w, int64_t ld, int64_t rows, int64_t D, float* __restrict__ part) {
-  __shared__ float red[4];
-  float mx = 0.f;
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x)
-    for (int64_t d = threadIdx.x; d < D; d += 256) mx = fmaxf(mx, fabsf(w[r * ld + d]));
-  mx = wave_max(mx);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = mx;
-  __syncthreads();
-  if (threadIdx.x == 0) part[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-}
-
 __device__ __forceinline__ int block_sum(int v, int* red) {
 #pragma unroll
   for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
@@ -143,98 +44,302 @@ __device__ __forceinline__ float block_max(float v, float* red) {
   __syncthreads();
   return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 }
+// the exponent of the power of two that brings a magnitude into [2^top, 2^(top+1)); 0 for 0, infinities and NaN
+__device__ __forceinline__ int scale_exponent(float a, int top) {
+  if (!(a > 0.f) || !(a < INFINITY)) return 0;
+  return max(-126, min(126, top - ilogbf(a)));
+}
 
-template <int DT> __device__ __forceinline__ void pack_row(const void* src, int64_t first, int64_t D, u16* dst, int64_t Dp, int64_t plane, float scale, int lane) {
-  for (int64_t d = lane; d < Dp; d += 64) {
-    if (DT == GNET_F32) {
-      u16 hi = 0, lo = 0;
-      if (d < D) split_f16(((const float*)src)[first + d] * scale, hi, lo);
-      dst[d] = hi; dst[plane + d] = lo;
+struct Targets {
+  const void* ids; int ids64;          // [M,K]
+  const float* logits;                 // [M,K] teacher's logits, or NULL (one target of weight 1: K = 1)
+  int64_t M; int K; int64_t V;
+  float to_log2;                       // log2(e) / temperature
+  float inv_temp;
+};
+__device__ __forceinline__ bool target_counts(const Targets& t, int64_t i, int64_t& id) {
+  id = load_id(t.ids, i, t.ids64);
+  return id >= 0 && id < t.V && !(t.logits && t.logits[i] == -INFINITY);
+}
+
+// ---- what is known before the first product ------------------------------------------------------------------------
+// Token workgroups, one wave per token (and per padding byte of the flags): does it count; its targets' weights; in the backward pass
+// the weights of equal ids added up in each of their slots.  Two passes over K <= 1024 logits: latency.
+// The remaining W_PARTS workgroups, 32-bit operands only: the largest magnitude of W, one partial result each.
+constexpr int W_PARTS = 1024;
+struct TargetsArgs {
+  Targets t;
+  int64_t flags_n;                     // M rounded up to 16
+  unsigned token_groups;
+  uint8_t* flag; float* q; float* q_sum; float* entropy;       // q, entropy: distillation; q_sum: its backward pass
+  const float* x; int64_t ldx, D; float* row_x;                // 32-bit x: the row's largest magnitude
+  const float* dloss; float* row_g;                            // backward only
+  const float* w; int64_t ldw; float* w_part; int w_vec;       // w_vec: rows of whole, aligned float4
+};
+__global__ void __launch_bounds__(256) vocab_targets(const TargetsArgs a) {
+  const int lane = threadIdx.x & 63;
+  if (blockIdx.x >= a.token_groups) {
+    __shared__ float red[4];
+    const unsigned part = blockIdx.x - a.token_groups;
+    float mx = 0.f;
+    if (a.w_vec) {
+      const int64_t per_row = a.D / 4, n = a.t.V * per_row;
+      const float4* w = (const float4*)a.w;
+      if (a.ldw == a.D) {
+        for (int64_t i = (int64_t)part * 256 + threadIdx.x; i < n; i += W_PARTS * 256ll) {
+          const float4 v = w[i];
+          mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+        }
+      } else {
+        for (int64_t r = part; r < a.t.V; r += W_PARTS)
+          for (int64_t d = threadIdx.x; d < per_row; d += 256) {
+            const float4 v = w[r * (a.ldw / 4) + d];
+            mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+          }
+      }
     } else {
-      dst[d] = d < D ? ((const u16*)src)[first + d] : (u16)0;
+      for (int64_t r = part; r < a.t.V; r += W_PARTS)
+        for (int64_t d = threadIdx.x; d < a.D; d += 256) mx = fmaxf(mx, fabsf(a.w[r * a.ldw + d]));
+    }
+    mx = block_max(mx, red);
+    if (threadIdx.x == 0) a.w_part[part] = mx;
+    return;
+  }
+  const int64_t m = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (m >= a.flags_n) return;
+  bool counts = false;
+  if (m < a.t.M) {
+    const int K = a.t.K;
+    if (!a.t.logits) {
+      int64_t id;
+      counts = target_counts(a.t, m, id);
+    } else {
+      float top = -INFINITY;
+      bool any = false;
+      for (int k = lane; k < K; k += 64) {
+        int64_t id;
+        if (target_counts(a.t, m * K + k, id)) { any = true; top = fmaxf(top, a.t.logits[m * K + k]); }
+      }
+      counts = __any(any);
+      top = wave_max(top);
+      float sum = 0.f;
+      for (int k = lane; k < K; k += 64) {
+        int64_t id;
+        const float e = target_counts(a.t, m * K + k, id) ? exp2f((a.t.logits[m * K + k] - top) * a.t.to_log2) : 0.f;
+        a.q[m * K + k] = e;
+        sum += e;
+      }
+      sum = wave_sum(sum);
+      float ent = 0.f;
+      for (int k = lane; k < K; k += 64) {
+        const float e = a.q[m * K + k], q = counts ? e / sum : 0.f;
+        a.q[m * K + k] = q;
+        if (q != 0.f) ent += q * ((a.t.logits[m * K + k] - top) * a.t.inv_temp - logf(sum));
+      }
+      if (a.entropy) { ent = wave_sum(ent); if (lane == 0) a.entropy[m] = ent; }
+      if (a.dloss) {
+        __threadfence_block();                             // the wave reads back what its other lanes wrote
+        for (int kb = 0; kb < K; kb += 64) {
+          const int k = kb + lane;
+          int64_t id = -1;
+          const bool c = k < K && target_counts(a.t, m * K + k, id);
+          float s = 0.f;
+          for (int j = 0; j < K; ++j)
+            if (c && load_id(a.t.ids, m * K + j, a.t.ids64) == id) s += a.q[m * K + j];
+          if (k < K) a.q_sum[m * K + k] = s;               // (an array of its own: later slots still read the single weights)
+        }
+      }
+    }
+    if (a.row_x) {
+      float mx = 0.f;
+      if (counts) for (int64_t d = lane; d < a.D; d += 64) mx = fmaxf(mx, fabsf(a.x[m * a.ldx + d]));
+      mx = wave_max(mx);
+      if (lane == 0) a.row_x[m] = mx;
+    }
+    if (a.row_g && lane == 0) a.row_g[m] = counts ? fabsf(a.dloss[m] * a.t.inv_temp) : 0.f;
+  }
+  if (lane == 0) a.flag[m] = counts;
+}
+
+// Rows copied to the matrix products' layout: Dp elements (a multiple of 64), zeros behind D; 32 bits as two fp16 planes.
+struct RowCopy { int64_t D, Dp, plane; float scale; int vec; };        // vec: 8 elements at a time (alignment and D allow it)
+template <int DT> __device__ __forceinline__ void copy_row(const void* src, int64_t first, bool zero, u16* dst, const RowCopy& c, int t, int threads) {
+  if (c.vec || zero) {
+    for (int64_t d = (int64_t)t * 8; d < c.Dp; d += (int64_t)threads * 8) {
+      s16x8 hi = {0, 0, 0, 0, 0, 0, 0, 0}, lo = hi;
+      if (!zero && d < c.D) {
+        if (DT == GNET_F32) {
+          const f32x4 v0 = *reinterpret_cast<const f32x4*>((const float*)src + first + d), v1 = *reinterpret_cast<const f32x4*>((const float*)src + first + d + 4);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            u16 h, l;
+            split_f16((i < 4 ? v0[i & 3] : v1[i & 3]) * c.scale, h, l);
+            hi[i] = (short)h; lo[i] = (short)l;
+          }
+        } else {
+          hi = *reinterpret_cast<const s16x8*>((const u16*)src + first + d);
+        }
+      }
+      *reinterpret_cast<s16x8*>(dst + d) = hi;
+      if (DT == GNET_F32) *reinterpret_cast<s16x8*>(dst + c.plane + d) = lo;
+    }
+  } else {
+    for (int64_t d = t; d < c.Dp; d += threads) {
+      u16 hi = 0, lo = 0;
+      if (d < c.D) {
+        if (DT == GNET_F32) split_f16(((const float*)src)[first + d] * c.scale, hi, lo);
+        else hi = ((const u16*)src)[first + d];
+      }
+      dst[d] = hi;
+      if (DT == GNET_F32) dst[c.plane + d] = lo;
     }
   }
 }
+// Rows of W that the matrix products cannot read where they lie (32 bits; widths that are no multiple of 64; alignment).
+struct PackW { const void* w; int64_t ldw, rows, rows_out; u16* dst; RowCopy c; };
+constexpr int PACK_W_ROWS = 16;
+template <int DT> __device__ __forceinline__ void pack_w_rows(const PackW& a, int64_t group, float scale) {
+  RowCopy c = a.c;
+  c.scale = scale;
+  for (int64_t r = group * PACK_W_ROWS + (threadIdx.x >> 6); r < min(a.rows_out, (group + 1) * PACK_W_ROWS); r += 4)
+    copy_row<DT>(a.w, r * a.ldw, r >= a.rows, a.dst + r * c.Dp, c, threadIdx.x & 63, 64);
+}
+template <int DT> __global__ void __launch_bounds__(256) vocab_pack_w(const PackW a, const VocabMeta* meta) {
+  pack_w_rows<DT>(a, blockIdx.x, DT == GNET_F32 ? 1.f / meta->unscale_w : 1.f);
+}
 
-// The tokens that count moved together, in order, rows padded to a multiple of 64 elements, zero rows behind them up to Mp.
-// Every workgroup counts the flags in front of its own rows: M bytes out of L2 instead of a scan in a launch of its own.
-constexpr int PACK_ROWS = 16;
+// Token workgroups: the tokens that count moved together, in order, zero rows behind them up to Mp.  Every workgroup counts the tokens
+// in front of its own rows: M bytes (or labels) out of L2 instead of a scan in a launch of its own.
+// The remaining workgroups pack the first piece of W.
 struct PackArgs {
-  const uint8_t* flag; int64_t flags_n, M, Mp;
-  const void* x; int64_t ldx, D, Dp; u16* xp; int64_t plane;
-  const float* row_x; const float* w_part; int w_parts;
-  const float* row_g; const float* dloss; const float* lse; float inv_temp; int top_g;
-  int32_t* pos; float* lse2; float* gscale;
+  Targets t;
+  const uint8_t* flag;                 // NULL: cross entropy's labels are looked at directly
+  int64_t flags_n, Mp; int rows;       // rows of a workgroup, a multiple of 4
+  unsigned token_groups;
+  const void* x; int64_t ldx; u16* xp; RowCopy c;
+  const float* row_x; const float* w_part;
+  const float* row_g; const float* dloss; const float* lse; int top_g;
+  int32_t* pos; int32_t* label; float* lse2; float* gscale;
   VocabMeta* meta;
+  PackW w;
 };
 template <int DT> __global__ void __launch_bounds__(256) vocab_pack(const PackArgs a) {
   __shared__ int ired[4];
   __shared__ float fred[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t r0 = (int64_t)blockIdx.x * PACK_ROWS;
+  int ew = 0;
+  if (DT == GNET_F32) {
+    float mw = 0.f;
+    for (int i = threadIdx.x; i < W_PARTS; i += 256) mw = fmaxf(mw, a.w_part[i]);
+    ew = scale_exponent(block_max(mw, fred), 13);
+  }
+  if (blockIdx.x >= a.token_groups) { pack_w_rows<DT>(a.w, blockIdx.x - a.token_groups, ldexpf(1.f, ew)); return; }
+  const int64_t r0 = (int64_t)blockIdx.x * a.rows, M = a.t.M;
+  auto counts = [&](int64_t i) { int64_t id; return a.flag ? a.flag[i] != 0 : target_counts(a.t, i, id); };
   int before = 0, all = 0;
-  for (int64_t i = (int64_t)threadIdx.x * 4; i < a.flags_n; i += 1024) {
-    const int n = __popc(*reinterpret_cast<const unsigned*>(a.flag + i));      // flags are 0 or 1
-    all += n;
-    if (i < r0) before += n;                                                   // r0 is a multiple of 16
+  float mg = 0.f, mx = 0.f;
+  if (a.flag) {
+    for (int64_t i = (int64_t)threadIdx.x * 4; i < a.flags_n; i += 1024) {
+      const int n = __popc(*reinterpret_cast<const unsigned*>(a.flag + i));      // flags are 0 or 1
+      all += n;
+      if (i < r0) before += n;                                                   // r0 is a multiple of 4
+    }
+    if (a.dloss) for (int64_t i = threadIdx.x; i < M; i += 256) mg = fmaxf(mg, a.row_g[i]);
+    if (DT == GNET_F32) for (int64_t i = threadIdx.x; i < M; i += 256) mx = fmaxf(mx, a.row_x[i]);
+  } else {
+    for (int64_t i = threadIdx.x; i < M; i += 256) {
+      const bool c = counts(i);
+      all += c;
+      if (i < r0) before += c;
+      if (a.dloss && c) mg = fmaxf(mg, fabsf(a.dloss[i] * a.t.inv_temp));
+    }
   }
   before = block_sum(before, ired);
   all = block_sum(all, ired);
-  float mx = 0.f, mw = 0.f, mg = 0.f;
-  if (DT == GNET_F32) {
-    for (int64_t i = threadIdx.x; i < a.M; i += 256) mx = fmaxf(mx, a.row_x[i]);
-    for (int i = threadIdx.x; i < a.w_parts; i += 256) mw = fmaxf(mw, a.w_part[i]);
-    mx = block_max(mx, fred);
-    mw = block_max(mw, fred);
-  }
-  if (a.row_g) {
-    for (int64_t i = threadIdx.x; i < a.M; i += 256) mg = fmaxf(mg, a.row_g[i]);
-    mg = block_max(mg, fred);
-  }
-  const int ex = DT == GNET_F32 ? scale_exponent(mx, 13) : 0, eg = a.row_g ? scale_exponent(mg, a.top_g) : 0;
+  if (a.dloss) mg = block_max(mg, fred);
+  if (DT == GNET_F32) mx = block_max(mx, fred);
+  const int ex = DT == GNET_F32 ? scale_exponent(mx, 13) : 0, eg = a.dloss ? scale_exponent(mg, a.top_g) : 0;
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     a.meta->rows = all;
     a.meta->unscale_x = ldexpf(1.f, -ex);
-    a.meta->unscale_w = DT == GNET_F32 ? ldexpf(1.f, -scale_exponent(mw, 13)) : 1.f;
+    a.meta->unscale_w = ldexpf(1.f, -ew);
     a.meta->unscale_g = ldexpf(1.f, -eg);
   }
-  const float sx = ldexpf(1.f, ex);
-  for (int j = wave; j < PACK_ROWS; j += 4) {
+  RowCopy c = a.c;
+  c.scale = ldexpf(1.f, ex);
+  const int wide = c.Dp >= 2048;                  // a whole workgroup a row, or a wave
+  const int t = wide ? threadIdx.x : threadIdx.x & 63;
+  for (int j = wide ? 0 : threadIdx.x >> 6; j < a.rows; j += wide ? 1 : 4) {
     const int64_t r = r0 + j;
-    if (r >= a.Mp) continue;
-    int f = 0;                                    // flags of this workgroup's rows in front of r; r's own
-    bool own = false;
-    for (int i = 0; i <= j; ++i) { const bool b = r0 + i < a.M && a.flag[r0 + i]; if (i < j) f += b; else own = b; }
-    const int64_t rank = before + f;              // tokens that count in front of r
-    if (r < a.M && lane == 0) a.pos[r] = own ? (int32_t)rank : -1;
+    if (r >= a.Mp) break;
+    int f = 0;                                    // tokens that count among this workgroup's in front of r
+    for (int i = 0; i < j; ++i) f += r0 + i < M && counts(r0 + i);
+    const bool own = r < M && counts(r);
+    const int64_t rank = before + f;
+    if (r < M && t == 0) a.pos[r] = own ? (int32_t)rank : -1;
     const int64_t to = own ? rank : all + (r - rank);        // the others' places behind them are zeroed
-    u16* dst = a.xp + to * a.Dp;
-    if (own) pack_row<DT>(a.x, r * a.ldx, a.D, dst, a.Dp, a.plane, sx, lane);
-    else pack_row<DT>(a.x, 0, 0, dst, a.Dp, a.plane, sx, lane);
-    if (own && a.row_g && lane == 0) {
-      a.lse2[to] = a.lse[r] * LOG2E;
-      a.gscale[to] = ldexpf(a.dloss[r] * a.inv_temp, eg);
+    copy_row<DT>(a.x, r * a.ldx, !own, a.xp + to * c.Dp, c, t, wide ? 256 : 64);
+    if (own && t == 0) {
+      if (a.label) a.label[to] = (int32_t)load_id(a.t.ids, r, a.t.ids64);
+      if (a.dloss) {
+        a.lse2[to] = a.lse[r] * LOG2E;
+        a.gscale[to] = ldexpf(a.dloss[r] * a.t.inv_temp, eg);
+      }
     }
   }
 }
 
-// Rows of W that the matrix products cannot read where they lie (32 bits; widths that are no multiple of 64; alignment).
-template <int DT> __global__ void __launch_bounds__(256) vocab_pack_w(const void* w, int64_t ldw, int64_t rows, int64_t D, u16* dst, int64_t Dp, int64_t plane, const VocabMeta* meta) {
-  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const float s = DT == GNET_F32 ? 1.f / meta->unscale_w : 1.f;
-  pack_row<DT>(w, r * ldw, r < rows ? D : 0, dst + r * Dp, Dp, plane, s, threadIdx.x & 63);
-}
-
-// One workgroup per token: lse from the vocabulary tiles' sums, the targets' logits as fp32 dot products, the loss.
+// ---- behind the products ---------------------------------------------------------------------------------------------
 struct JoinArgs {
   Targets t;
-  const int32_t* pos; const float2* part; int tiles;
-  const void* x; int64_t ldx; const void* w; int64_t ldw; int64_t D;
+  const int32_t* pos; const float2* part; int tiles; const float* hit2;      // hit2: cross entropy's label logits, compacted, log2 units
+  const void* x; int64_t ldx; const void* w; int64_t ldw; int64_t D; int vec;
   const float* q; const float* entropy;
   float* loss; float* lse; float* hit;
 };
-template <int DT> __global__ void __launch_bounds__(256) vocab_join(const JoinArgs a) {
-  __shared__ float red[4], red2[4];
+// log2 of a token's sum over the vocabulary from its tiles' maxima and sums, by one wave
+__device__ __forceinline__ float join_tiles(const float2* part, int tiles, int lane) {
+  float mx = -INFINITY, sum = 0.f;
+  for (int i = lane; i < tiles; i += 64) {
+    const float2 v = part[i];
+    const float n = fmaxf(mx, v.x), b = n == -INFINITY ? 0.f : n;
+    sum = sum * exp2f(mx - b) + v.y * exp2f(v.x - b);
+    mx = n;
+  }
+  const float all = wave_max(mx), base = all == -INFINITY ? 0.f : all;
+  return base + log2f(wave_sum(sum * exp2f(mx - base)));
+}
+// cross entropy: one wave per token
+__global__ void __launch_bounds__(256) vocab_join(const JoinArgs a) {
+  const int64_t m = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (m >= a.t.M) return;
+  const int p = a.pos[m], lane = threadIdx.x & 63;
+  float lse2 = 0.f, hit2 = 0.f;
+  if (p >= 0) { lse2 = join_tiles(a.part + (int64_t)p * a.tiles, a.tiles, lane); hit2 = a.hit2[p]; }
+  if (lane) return;
+  const float loss = (lse2 - hit2) * LN2;          // the same z in both: the rounding of z cancels where the label takes nearly everything
+  a.loss[m] = loss < 0.f ? 0.f : loss;             // (below 0 from rounding only; NaN stays)
+  a.lse[m] = lse2 * LN2;
+  a.hit[m] = hit2 * LN2;
+}
+template <int DT> __device__ __forceinline__ void dot8(const void* x, const void* w, float& s) {
+  if (DT == GNET_F32) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const f32x4 a = ((const f32x4*)x)[h], b = ((const f32x4*)w)[h];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s = fmaf(a[i], b[i], s);
+    }
+  } else {
+    const s16x8 a = *(const s16x8*)x, b = *(const s16x8*)w;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      s = DT == GNET_BF16 ? fmaf(Bf16T::dec((u16)a[i]), Bf16T::dec((u16)b[i]), s) : fmaf(F16T::dec((u16)a[i]), F16T::dec((u16)b[i]), s);
+  }
+}
+// distillation: one workgroup per token, a wave takes two of its targets at a time: their logits are fp32 dot products
+template <int DT> __global__ void __launch_bounds__(256) vocab_join_targets(const JoinArgs a) {
+  __shared__ float red[4];
+  constexpr int SIZE = DT == GNET_F32 ? 4 : 2;
   const int64_t m = blockIdx.x;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, K = a.t.K;
   const int p = a.pos[m];
@@ -243,48 +348,53 @@ template <int DT> __global__ void __launch_bounds__(256) vocab_join(const JoinAr
     if (threadIdx.x == 0) { a.loss[m] = 0.f; a.lse[m] = 0.f; }
     return;
   }
-  const float2* part = a.part + (int64_t)p * a.tiles;
-  float mx = -INFINITY, sum = 0.f;
-  for (int i = threadIdx.x; i < a.tiles; i += 256) {
-    const float2 v = part[i];
-    const float n = fmaxf(mx, v.x), b = n == -INFINITY ? 0.f : n;
-    sum = sum * exp2f(mx - b) + v.y * exp2f(v.x - b);
-    mx = n;
-  }
-  const float top = wave_max(mx);
-  if (lane == 0) red[wave] = top;
-  __syncthreads();
-  const float all = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), base = all == -INFINITY ? 0.f : all;
-  sum = wave_sum(sum * exp2f(mx - base));
-  if (lane == 0) red2[wave] = sum;
-  __syncthreads();
-  sum = (red2[0] + red2[1]) + (red2[2] + red2[3]);
-  const float lse = (base + log2f(sum)) * LN2;
+  const float lse = join_tiles(a.part + (int64_t)p * a.tiles, a.tiles, lane) * LN2;
   float loss = 0.f;
-  for (int k = wave; k < K; k += 4) {
-    int64_t id;
-    const bool c = target_counts(a.t, m * K + k, id);
-    float dot = 0.f;
-    if (c) {
-      for (int64_t d = lane; d < a.D; d += 64) dot = fmaf(load_elem<DT>(a.x, m * a.ldx + d), load_elem<DT>(a.w, id * a.ldw + d), dot);
-      dot = wave_sum(dot) * a.t.inv_temp;
-      const float q = a.q[m * K + k];
-      if (q != 0.f) loss += q * (lse - dot);       // (an infinite logit of a target without weight stays out)
+  const char* x = (const char*)a.x + m * a.ldx * SIZE;
+  for (int k = wave; k < K; k += 8) {
+    int64_t id[2];
+    bool c[2];
+    float dot[2] = {0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      c[u] = k + 4 * u < K && target_counts(a.t, m * K + k + 4 * u, id[u]);
+      if (!c[u]) id[u] = 0;
     }
-    if (lane == 0) a.hit[m * K + k] = dot;
+    const char* w0 = (const char*)a.w + id[0] * a.ldw * SIZE;
+    const char* w1 = (const char*)a.w + id[1] * a.ldw * SIZE;
+    if (a.vec) {
+      for (int64_t d = (int64_t)lane * 8; d < a.D; d += 512) {
+        dot8<DT>(x + d * SIZE, w0 + d * SIZE, dot[0]);
+        dot8<DT>(x + d * SIZE, w1 + d * SIZE, dot[1]);
+      }
+    } else {
+      for (int64_t d = lane; d < a.D; d += 64) {
+        const float v = DT == GNET_F32 ? ((const float*)x)[d] : DT == GNET_BF16 ? Bf16T::dec(((const u16*)x)[d]) : F16T::dec(((const u16*)x)[d]);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const char* w = u ? w1 : w0;
+          dot[u] = fmaf(v, DT == GNET_F32 ? ((const float*)w)[d] : DT == GNET_BF16 ? Bf16T::dec(((const u16*)w)[d]) : F16T::dec(((const u16*)w)[d]), dot[u]);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (k + 4 * u >= K) continue;
+      const int64_t i = m * K + k + 4 * u;
+      const float z = wave_sum(dot[u]) * a.t.inv_temp;
+      if (c[u]) { const float q = a.q[i]; if (q != 0.f) loss += q * (lse - z); }       // (an infinite logit of a target without weight stays out)
+      if (lane == 0) a.hit[i] = c[u] ? z : 0.f;
+    }
   }
-  __syncthreads();
   if (lane == 0) red[wave] = loss;
   __syncthreads();
   if (threadIdx.x == 0) {
-    loss = (red[0] + red[1]) + (red[2] + red[3]) + (a.t.logits ? a.entropy[m] : 0.f);
-    // cross entropy is >= 0: what is below comes from rounding (NaN stays).  Distillation with an id in two slots may be below 0.
-    a.loss[m] = !a.t.logits && loss < 0.f ? 0.f : loss;
+    a.loss[m] = (red[0] + red[1]) + (red[2] + red[3]) + a.entropy[m];
     a.lse[m] = lse;
   }
 }
 
-// dz at the targets of one piece of the vocabulary: (softmax - weight) g from the forward pass's fp32 logits, over what
+// dz at the teacher's ids of one piece of the vocabulary: (softmax - weight) g from the forward pass's fp32 logits, over what
 // vocab_gemm<EPI_DZ> stored there.  Slots with the same id store the same value.
 struct HitsArgs {
   Targets t;
@@ -304,79 +414,119 @@ template <class T, int PLANES> __global__ void __launch_bounds__(256) vocab_hits
   else { u16 hi, lo; split_f16(d, hi, lo); to[0] = hi; to[a.plane] = lo; }
 }
 
-// out[r][:] = unscale * sum over the splits' partial sums (ascending), zero for a row whose place is -1
+// out[r][:] = unscale * sum over the splits' partial sums (ascending), zero for a row whose place is -1; four elements a thread
 struct FinishArgs {
   const float* slab; int64_t ld, stride; int splits;
   const int32_t* pos;                                // NULL: row r of the slab
-  int64_t rows, D; void* out; int64_t ld_out;
+  int64_t rows, D; unsigned quads; void* out; int vec;        // quads: groups of four a row; vec: stored at once
   const VocabMeta* meta; int by_x;
 };
 template <int DT> __global__ void __launch_bounds__(256) vocab_finish(const FinishArgs a) {
   const float f = a.meta->unscale_g * (a.by_x ? a.meta->unscale_x : a.meta->unscale_w);
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t r = i / a.D, d = i % a.D;
+  const int64_t r = i / a.quads, d = (i - r * a.quads) * 4;
   if (r >= a.rows) return;
   const int64_t p = a.pos ? a.pos[r] : r;
-  float v = 0.f;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
   if (p >= 0) {
-    for (int s = 0; s < a.splits; ++s) v += a.slab[s * a.stride + p * a.ld + d];
+    for (int s = 0; s < a.splits; ++s) v += *reinterpret_cast<const f32x4*>(a.slab + s * a.stride + p * a.ld + d);
     v *= f;
   }
-  if (DT == GNET_F32) ((float*)a.out)[r * a.ld_out + d] = v;
-  else if (DT == GNET_BF16) ((u16*)a.out)[r * a.ld_out + d] = Bf16T::enc(v);
-  else ((u16*)a.out)[r * a.ld_out + d] = F16T::enc(v);
+  const int64_t at = r * a.D + d;
+  if (DT == GNET_F32) {
+    float* o = (float*)a.out + at;
+    if (a.vec) *reinterpret_cast<f32x4*>(o) = v;
+    else for (int k = 0; k < 4; ++k) if (d + k < a.D) o[k] = v[k];
+  } else {
+    u16* o = (u16*)a.out + at;
+    u16 e[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) e[k] = DT == GNET_BF16 ? Bf16T::enc(v[k]) : F16T::enc(v[k]);
+    if (a.vec) *reinterpret_cast<s16x4*>(o) = s16x4{(short)e[0], (short)e[1], (short)e[2], (short)e[3]};
+    else for (int k = 0; k < 4; ++k) if (d + k < a.D) o[k] = e[k];
+  }
 }
 
-// ---- the plan: sizes, pieces and where everything lies in the workspace ------------------------------------------------
+// ---- the plan: tiles, pieces and where everything lies in the workspace ------------------------------------------------
 inline int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
+inline int64_t tiles(int64_t v, int64_t a) { return (v + a - 1) / a; }
+
+// Tile shapes of the products.  256 x 256 runs a contraction step of 64 in SQUARE_US (one workgroup a CU), 128 x 128 in HALF_US (two a
+// CU) -- 1.29 against 1.0 PFLOP/s measured -- plus what a tile costs before and behind its steps.  128 x 64 and 128 x 32 are for
+// products with that few tokens, which wait for W: they only have to keep loads in flight.
+enum Shape { S256, S128, S64, S32 };
+struct ShapeInfo { int bm, bn; };
+constexpr ShapeInfo SHAPE[] = {{256, 256}, {128, 128}, {128, 64}, {128, 32}};
+struct Product { int shape, splits; };
+
+double product_us(int shape, int splits, int64_t rows, int64_t cols, int64_t steps) {
+  const int64_t n = tiles(rows, SHAPE[shape].bm) * tiles(cols, SHAPE[shape].bn) * splits;
+  const double round = shape == S256 ? tiles(steps, splits) * 1.67 + 8 : tiles(steps, splits) * 1.07 + 5;
+  const double joined = splits > 1 ? 5 + (double)rows * cols * 4 * (2 * splits) / 4e6 : 0;       // partial sums out and in at 4 TB/s
+  return tiles(n, shape == S256 ? 256 : 512) * round + joined;
+}
+// few_cols: the columns are tokens, for which the narrow shapes exist
+Product pick_product(int64_t rows, int64_t cols, int64_t steps, bool few_cols, bool may_split) {
+  Product best = {few_cols && cols <= 32 ? S32 : few_cols && cols <= 64 ? S64 : S256, 1};
+  if (best.shape == S256) {
+    double least = 1e30;
+    for (int shape = S256; shape <= S128; ++shape)
+      for (int splits = 1; splits <= (may_split ? 16 : 1) && (splits == 1 || steps / splits >= 4); ++splits) {
+        const double us = product_us(shape, splits, rows, cols, steps);
+        if (us < least) { least = us; best.shape = shape; best.splits = splits; }
+      }
+  } else if (may_split) {
+    const int64_t n = tiles(rows, SHAPE[best.shape].bm);
+    while (best.splits < 64 && n * best.splits < 768 && steps / (best.splits + 1) >= 8) ++best.splits;      // three workgroups a CU
+  }
+  return best;
+}
 
 struct Plan {
   int64_t Mp, Dp, flags_n, piece, pieces, w_tiles;
-  int planes, pack_w, dx_splits, dw_splits;
-  int64_t flag, q, entropy, row_x, row_g, w_part, meta, pos, lse2, gscale, xp, wp, part, dz, dx_slab, dw_slab, bytes;
+  int planes, pack_w, direct;
+  Product logits, dx, dw;
+  int64_t flag, q, entropy, row_x, row_g, w_part, meta, pos, label, hit2, lse2, gscale, xp, wp, part, dz, dx_slab, dw_slab, bytes;
 };
-constexpr int W_PARTS = 512;
 
-// One pass over the chip is 256 workgroups: a product with fewer tiles splits its contraction, down to eight steps a split.
-int pick_splits(int64_t tiles, int64_t steps) {
-  int s = 1;
-  while (tiles * s < 256 && steps / (2 * s) >= 8 && s < 64) s *= 2;
-  return s;
-}
-
-Plan make_plan(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int pack_w, int backward) {
+Plan make_plan(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int distill, int pack_w, int backward) {
   Plan p = {};
   p.planes = dtype == GNET_F32 ? 2 : 1;
+  const int segments = p.planes == 2 ? 3 : 1;
   p.pack_w = pack_w;
-  p.Mp = up(M, TILE); p.Dp = up(D, 64); p.flags_n = up(M, 16);
+  // cross entropy on 16 bits needs nothing of its tokens but the labels: up to 8192 of them the packing looks at them itself
+  p.direct = !distill && p.planes == 1 && M <= 8192;
+  p.Mp = up(M, VG_BK); p.Dp = up(D, 64); p.flags_n = up(M, 16);
   // A piece's dz and packed rows of W stay within the last-level cache (256 MB) for the products that read them again.
   const int64_t per_row = (int64_t)p.planes * 2 * ((backward ? p.Mp : 0) + (pack_w ? p.Dp : 0));
-  const int64_t Vp = up(V, TILE);
-  int64_t piece = per_row ? (128ll << 20) / per_row / TILE * TILE : Vp;
-  if (piece < 8 * TILE) piece = 8 * TILE;
-  p.pieces = (Vp + piece - 1) / piece;
-  p.piece = up((Vp + p.pieces - 1) / p.pieces, TILE);
-  p.pieces = (Vp + p.piece - 1) / p.piece;
-  p.w_tiles = Vp / TILE;
+  const int64_t Vp = up(V, 256);
+  int64_t piece = per_row ? (128ll << 20) / per_row / 256 * 256 : Vp;
+  if (piece < 2048) piece = 2048;
+  p.pieces = tiles(Vp, piece);
+  p.piece = up(tiles(Vp, p.pieces), 256);
+  p.pieces = tiles(Vp, p.piece);
+  p.logits = pick_product(p.piece, M, p.Dp / VG_BK * segments, true, false);
+  p.w_tiles = tiles(V, SHAPE[p.logits.shape].bm);
   int64_t o = 0;
   auto take = [&](int64_t bytes) { const int64_t at = o; o = up(o + bytes, 256); return at; };
-  p.flag = take(p.flags_n);
-  p.q = take(M * K * 4 * 2);
   p.meta = take(sizeof(VocabMeta));
   p.pos = take(M * 4);
   p.xp = take(p.planes * p.Mp * p.Dp * 2);
+  if (!p.direct) p.flag = take(p.flags_n);
+  if (distill) p.q = take(M * K * 4 * (backward ? 2 : 1)); else p.label = take(p.Mp * 4);
   if (p.planes == 2) { p.row_x = take(M * 4); p.w_part = take(W_PARTS * 4); }
   if (pack_w) p.wp = take(p.planes * p.piece * p.Dp * 2);
   if (!backward) {
     p.entropy = take(M * 4);
+    p.hit2 = take(p.Mp * 4);
     p.part = take(p.Mp * p.w_tiles * 8);
   } else {
     p.row_g = take(M * 4); p.lse2 = take(p.Mp * 4); p.gscale = take(p.Mp * 4);
     p.dz = take(p.planes * p.Mp * p.piece * 2);
-    p.dx_splits = pick_splits(up(p.Dp, TILE) / TILE * (p.Mp / TILE), p.piece / VG_BK);
-    p.dx_slab = take((int64_t)p.dx_splits * p.Mp * p.Dp * 4);
-    p.dw_splits = pick_splits(up(p.Dp, TILE) / TILE * (p.piece / TILE), p.Mp / VG_BK);
-    if (p.dw_splits > 1) p.dw_slab = take((int64_t)p.dw_splits * p.piece * p.Dp * 4);
+    p.dx = pick_product(p.Dp, M, p.piece / VG_BK * segments, true, true);
+    p.dx_slab = take((int64_t)p.dx.splits * p.Mp * p.Dp * 4);
+    p.dw = pick_product(p.Dp, p.piece, p.Mp / VG_BK * segments, false, true);
+    if (p.dw.splits > 1) p.dw_slab = take((int64_t)p.dw.splits * p.piece * p.Dp * 4);
   }
   p.bytes = o;
   return p;
@@ -384,6 +534,10 @@ Plan make_plan(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int pack_w
 
 int needs_pack(const void* w, int64_t ldw, int64_t D, int dtype) {
   return dtype == GNET_F32 || (D & 63) || (ldw & 7) || ldw > (1 << 22) || ((uintptr_t)w & 15);      // (2^22: 32-bit offsets in a tile)
+}
+// eight elements at a time
+int vec8(const void* p, int64_t ld, int64_t D, int dtype) {
+  return !(D & 7) && !((ld * (dtype == GNET_F32 ? 4 : 2)) & 15) && !((uintptr_t)p & 15);
 }
 
 struct Problem {
@@ -400,37 +554,65 @@ int check(const Problem& q) {
 }
 
 template <int DT, class T, int PLANES> struct Run {
-  template <bool AS, bool BS, int EPI> static void gemm(const VocabGemm& g, hipStream_t s) {
-    vocab_gemm<T, TILE, TILE, 2, 4, AS, BS, EPI, PLANES><<<(unsigned)((int64_t)g.row_tiles * g.col_tiles * g.splits), 512, 0, s>>>(g);
+  template <int BM, int BN, int WM, int WN, bool AS, bool BS, int EPI> static void launch(VocabGemm& g, int64_t rows, int64_t cols, int splits, hipStream_t s) {
+    g.row_tiles = (int)tiles(rows, BM); g.col_tiles = (int)tiles(cols, BN); g.splits = splits;
+    vocab_gemm<T, BM, BN, WM, WN, AS, BS, EPI, PLANES><<<(unsigned)((int64_t)g.row_tiles * g.col_tiles * splits), 64 * WM * WN, 0, s>>>(g);
+  }
+  // columns are tokens (all shapes) or vocabulary (the square ones)
+  template <bool AS, bool BS, int EPI> static void gemm(VocabGemm& g, const Product& p, int64_t rows, int64_t cols, hipStream_t s) {
+    if (p.shape == S256) return launch<256, 256, 2, 4, AS, BS, EPI>(g, rows, cols, p.splits, s);
+    if constexpr (!BS) {
+      if (p.shape == S64) return launch<128, 64, 4, 1, AS, BS, EPI>(g, rows, cols, p.splits, s);
+      if (p.shape == S32) return launch<128, 32, 4, 1, AS, BS, EPI>(g, rows, cols, p.splits, s);
+    }
+    launch<128, 128, 2, 2, AS, BS, EPI>(g, rows, cols, p.splits, s);
   }
 
-  // targets, packing: everything in front of the first matrix product
+  static PackW pack_of_w(const Problem& q, const Plan& p, char* ws, int64_t v0) {
+    PackW k = {};
+    k.w = (const char*)q.w + v0 * q.ldw * (DT == GNET_F32 ? 4 : 2);
+    k.ldw = q.ldw; k.rows = q.t.V - v0; k.rows_out = p.piece; k.dst = (u16*)(ws + p.wp);
+    k.c = RowCopy{q.D, p.Dp, p.piece * p.Dp, 1.f, vec8(q.w, q.ldw, q.D, DT)};
+    return k;
+  }
+  // everything in front of the first product, the first piece of W included
   static void prepare(const Problem& q, const Plan& p, char* ws, const float* dloss, const float* lse, hipStream_t s) {
     TargetsArgs a = {};
-    a.t = q.t; a.flags_n = p.flags_n;
-    a.flag = (uint8_t*)(ws + p.flag); a.q = (float*)(ws + p.q); a.q_sum = a.q + q.t.M * q.t.K; a.entropy = dloss ? nullptr : (float*)(ws + p.entropy);
-    a.x = q.x; a.ldx = q.ldx; a.D = q.D;
-    a.row_x = PLANES == 2 ? (float*)(ws + p.row_x) : nullptr;
-    a.dloss = dloss; a.row_g = dloss ? (float*)(ws + p.row_g) : nullptr;
-    vocab_targets<<<(unsigned)((p.flags_n + 3) / 4), 256, 0, s>>>(a);
-    if (PLANES == 2) vocab_absmax<<<W_PARTS, 256, 0, s>>>((const float*)q.w, q.ldw, q.t.V, q.D, (float*)(ws + p.w_part));
+    a.t = q.t; a.flags_n = p.flags_n; a.token_groups = (unsigned)tiles(p.flags_n, 4);
+    a.dloss = dloss;
+    if (!p.direct) {
+      a.flag = (uint8_t*)(ws + p.flag);
+      if (q.t.logits) { a.q = (float*)(ws + p.q); a.q_sum = a.q + q.t.M * q.t.K; if (!dloss) a.entropy = (float*)(ws + p.entropy); }
+      if (dloss) a.row_g = (float*)(ws + p.row_g);
+      a.ldx = q.ldx; a.D = q.D;
+      if (PLANES == 2) {
+        a.x = (const float*)q.x; a.row_x = (float*)(ws + p.row_x);
+        a.w = (const float*)q.w; a.ldw = q.ldw; a.w_part = (float*)(ws + p.w_part);
+        a.w_vec = !(q.D & 3) && !(q.ldw & 3) && !((uintptr_t)q.w & 15);
+      }
+      vocab_targets<<<a.token_groups + (PLANES == 2 ? W_PARTS : 0), 256, 0, s>>>(a);
+    }
     PackArgs k = {};
-    k.flag = a.flag; k.flags_n = p.flags_n; k.M = q.t.M; k.Mp = p.Mp;
-    k.x = q.x; k.ldx = q.ldx; k.D = q.D; k.Dp = p.Dp; k.xp = (u16*)(ws + p.xp); k.plane = p.Mp * p.Dp;
-    k.row_x = a.row_x; k.w_part = PLANES == 2 ? (float*)(ws + p.w_part) : nullptr; k.w_parts = W_PARTS;
-    k.row_g = a.row_g; k.dloss = dloss; k.lse = lse; k.inv_temp = q.t.inv_temp; k.top_g = DT == GNET_BF16 ? 0 : 14;
-    k.pos = (int32_t*)(ws + p.pos); k.lse2 = (float*)(ws + p.lse2); k.gscale = (float*)(ws + p.gscale);
+    k.t = q.t; k.flag = a.flag; k.flags_n = p.flags_n; k.Mp = p.Mp;
+    k.rows = 4;
+    while (tiles(p.Mp, k.rows) > 1024) k.rows *= 2;             // every workgroup looks at all M flags
+    k.token_groups = (unsigned)tiles(p.Mp, k.rows);
+    k.x = q.x; k.ldx = q.ldx; k.xp = (u16*)(ws + p.xp);
+    k.c = RowCopy{q.D, p.Dp, p.Mp * p.Dp, 1.f, vec8(q.x, q.ldx, q.D, DT)};
+    k.row_x = a.row_x; k.w_part = a.w_part;
+    k.row_g = a.row_g; k.dloss = dloss; k.lse = lse; k.top_g = DT == GNET_BF16 ? 0 : 14;
+    k.pos = (int32_t*)(ws + p.pos); k.label = q.t.logits ? nullptr : (int32_t*)(ws + p.label);
+    k.lse2 = (float*)(ws + p.lse2); k.gscale = (float*)(ws + p.gscale);
     k.meta = (VocabMeta*)(ws + p.meta);
-    vocab_pack<DT><<<(unsigned)((p.Mp + PACK_ROWS - 1) / PACK_ROWS), 256, 0, s>>>(k);
+    if (p.pack_w) k.w = pack_of_w(q, p, ws, 0);
+    vocab_pack<DT><<<k.token_groups + (p.pack_w ? (unsigned)tiles(p.piece, PACK_W_ROWS) : 0), 256, 0, s>>>(k);
   }
 
   // W rows v0 .. of one piece as an operand (packed first where needed)
   static VocabOperand piece_of_w(const Problem& q, const Plan& p, char* ws, int64_t v0, hipStream_t s) {
     VocabOperand o = {};
     if (p.pack_w) {
-      const int64_t rows = q.t.V - v0 < p.piece ? q.t.V - v0 : p.piece;
-      const char* from = (const char*)q.w + v0 * q.ldw * (DT == GNET_F32 ? 4 : 2);
-      vocab_pack_w<DT><<<(unsigned)(p.piece / 4), 256, 0, s>>>(from, q.ldw, rows, q.D, (u16*)(ws + p.wp), p.Dp, p.piece * p.Dp, (const VocabMeta*)(ws + p.meta));
+      if (v0) vocab_pack_w<DT><<<(unsigned)tiles(p.piece, PACK_W_ROWS), 256, 0, s>>>(pack_of_w(q, p, ws, v0), (const VocabMeta*)(ws + p.meta));
       o.p = (const u16*)(ws + p.wp); o.ld = p.Dp; o.plane = p.piece * p.Dp; o.rows = p.piece;
     } else {
       o.p = (const u16*)q.w + v0 * q.ldw; o.ld = q.ldw; o.plane = 0; o.rows = q.t.V - v0;
@@ -446,12 +628,10 @@ template <int DT, class T, int PLANES> struct Run {
   static VocabGemm logits(const Problem& q, const Plan& p, char* ws, const VocabOperand& w, int64_t v0) {
     VocabGemm g = {};
     g.a = w; g.b = packed_x(p, ws);
-    g.k = p.Dp; g.cols_from_meta = 1; g.segments = PLANES == 2 ? 3 : 1;
-    const int64_t rows = up(q.t.V - v0 < p.piece ? q.t.V - v0 : p.piece, TILE);
-    g.row_tiles = (int)(rows / TILE); g.col_tiles = (int)(p.Mp / TILE); g.splits = 1;
+    g.k = p.Dp; g.cols_from_meta = 1;
     g.meta = (const VocabMeta*)(ws + p.meta);
-    g.to_log2 = q.t.to_log2; g.valid_rows = q.t.V - v0;
-    g.first_row_tile = (int)(v0 / TILE); g.all_row_tiles = (int)p.w_tiles;
+    g.to_log2 = q.t.to_log2; g.valid_rows = q.t.V - v0; g.first_row = (int32_t)v0;
+    g.label = q.t.logits ? nullptr : (const int32_t*)(ws + p.label);
     return g;
   }
 
@@ -459,16 +639,24 @@ template <int DT, class T, int PLANES> struct Run {
     prepare(q, p, ws, nullptr, nullptr, s);
     for (int64_t v0 = 0; v0 < q.t.V; v0 += p.piece) {
       VocabGemm g = logits(q, p, ws, piece_of_w(q, p, ws, v0, s), v0);
-      g.part = (float2*)(ws + p.part);
-      gemm<false, false, EPI_PART>(g, s);
+      g.part = (float2*)(ws + p.part); g.hit = (float*)(ws + p.hit2);
+      g.first_row_tile = (int)(v0 / SHAPE[p.logits.shape].bm); g.all_row_tiles = (int)p.w_tiles;
+      gemm<false, false, EPI_PART>(g, p.logits, q.t.V - v0 < p.piece ? q.t.V - v0 : p.piece, q.t.M, s);
     }
     JoinArgs j = {};
-    j.t = q.t; j.pos = (const int32_t*)(ws + p.pos); j.part = (const float2*)(ws + p.part); j.tiles = (int)p.w_tiles;
-    j.x = q.x; j.ldx = q.ldx; j.w = q.w; j.ldw = q.ldw; j.D = q.D;
+    j.t = q.t; j.pos = (const int32_t*)(ws + p.pos); j.part = (const float2*)(ws + p.part); j.tiles = (int)p.w_tiles; j.hit2 = (const float*)(ws + p.hit2);
+    j.x = q.x; j.ldx = q.ldx; j.w = q.w; j.ldw = q.ldw; j.D = q.D; j.vec = vec8(q.x, q.ldx, q.D, DT) && vec8(q.w, q.ldw, q.D, DT);
     j.q = (const float*)(ws + p.q); j.entropy = (const float*)(ws + p.entropy);
     j.loss = loss; j.lse = lse; j.hit = hit;
-    vocab_join<DT><<<(unsigned)q.t.M, 256, 0, s>>>(j);
+    if (q.t.logits) vocab_join_targets<DT><<<(unsigned)q.t.M, 256, 0, s>>>(j);
+    else vocab_join<<<(unsigned)tiles(q.t.M, 4), 256, 0, s>>>(j);
     return launch_status();
+  }
+
+  static void finish(FinishArgs f, const Problem& q, hipStream_t s) {
+    f.D = q.D; f.quads = (unsigned)tiles(q.D, 4);
+    f.vec = !(q.D & 3) && !((uintptr_t)f.out & (DT == GNET_F32 ? 15 : 7));
+    vocab_finish<DT><<<(unsigned)tiles(f.rows * f.quads, 256), 256, 0, s>>>(f);
   }
 
   static int backward(const Problem& q, const Plan& p, char* ws, const float* lse, const float* hit, const float* dloss, void* dx, void* dw, hipStream_t s) {
@@ -480,47 +668,47 @@ template <int DT, class T, int PLANES> struct Run {
       const VocabOperand w = piece_of_w(q, p, ws, v0, s);
       VocabGemm g = logits(q, p, ws, w, v0);
       g.lse2 = (const float*)(ws + p.lse2); g.gscale = (const float*)(ws + p.gscale);
-      g.dz = (u16*)(ws + p.dz); g.ld_dz = p.piece; g.plane_dz = p.Mp * p.piece;
-      gemm<false, false, EPI_DZ>(g, s);
-      HitsArgs h = {};
-      h.t = q.t; h.pos = (const int32_t*)(ws + p.pos); h.lse = lse; h.hit = hit;
-      h.q = (const float*)(ws + p.q) + (q.t.logits ? q.t.M * q.t.K : 0);
-      h.gscale = g.gscale; h.dz = g.dz; h.ld_dz = g.ld_dz; h.plane = g.plane_dz; h.v0 = v0; h.v1 = v0 + rows;
-      vocab_hits<T, PLANES><<<(unsigned)((q.t.M * q.t.K + 255) / 256), 256, 0, s>>>(h);
+      g.dz = (u16*)(ws + p.dz); g.ld_dz = p.piece; g.plane_dz = p.Mp * p.piece; g.dz_cols = p.Mp;
+      gemm<false, false, EPI_DZ>(g, p.logits, rows, q.t.M, s);
+      if (q.t.logits) {
+        HitsArgs h = {};
+        h.t = q.t; h.pos = (const int32_t*)(ws + p.pos); h.lse = lse; h.hit = hit;
+        h.q = (const float*)(ws + p.q) + q.t.M * q.t.K;
+        h.gscale = g.gscale; h.dz = g.dz; h.ld_dz = g.ld_dz; h.plane = g.plane_dz; h.v0 = v0; h.v1 = v0 + rows;
+        vocab_hits<T, PLANES><<<(unsigned)tiles(q.t.M * q.t.K, 256), 256, 0, s>>>(h);
+      }
       VocabOperand dz = {};
       dz.p = g.dz; dz.ld = p.piece; dz.plane = g.plane_dz; dz.rows = p.Mp; dz.cols = (int)p.piece;
       if (dx) {
         VocabGemm d = {};
-        d.a = w; d.b = dz; d.k = rows64; d.cols_from_meta = 1; d.segments = g.segments;
-        d.row_tiles = (int)(up(p.Dp, TILE) / TILE); d.col_tiles = (int)(p.Mp / TILE); d.splits = p.dx_splits; d.meta = meta;
+        d.a = w; d.b = dz; d.k = rows64; d.cols_from_meta = 1; d.meta = meta;
         d.slab = (float*)(ws + p.dx_slab); d.ld_slab = p.Dp; d.slab_stride = p.Mp * p.Dp; d.accumulate = v0 > 0; d.out_cols = p.Mp;
-        gemm<true, false, EPI_SLAB>(d, s);
+        gemm<true, false, EPI_SLAB>(d, p.dx, p.Dp, q.t.M, s);
       }
       if (dw) {
         VocabGemm d = {};
-        d.a = packed_x(p, ws); d.b = dz; d.k_from_meta = 1; d.segments = g.segments;
-        d.row_tiles = (int)(up(p.Dp, TILE) / TILE); d.col_tiles = (int)(up(rows, TILE) / TILE); d.splits = p.dw_splits; d.meta = meta;
+        d.a = packed_x(p, ws); d.b = dz; d.k_from_meta = 1; d.meta = meta;
         d.out_cols = rows;
         void* out = (char*)dw + v0 * q.D * elem;
-        if (p.dw_splits == 1) {
+        if (p.dw.splits == 1) {
           d.out = out; d.ld_out = q.D; d.out_rows = q.D; d.unscale_by_x = 1;
           d.out_vec = (q.D & 3) == 0 && ((uintptr_t)dw & 7) == 0;
-          gemm<true, true, EPI_OUT>(d, s);
+          gemm<true, true, EPI_OUT>(d, p.dw, p.Dp, rows, s);
         } else {
           d.slab = (float*)(ws + p.dw_slab); d.ld_slab = p.Dp; d.slab_stride = p.piece * p.Dp;
-          gemm<true, true, EPI_SLAB>(d, s);
+          gemm<true, true, EPI_SLAB>(d, p.dw, p.Dp, rows, s);
           FinishArgs f = {};
-          f.slab = d.slab; f.ld = p.Dp; f.stride = d.slab_stride; f.splits = d.splits;
-          f.rows = rows; f.D = q.D; f.out = out; f.ld_out = q.D; f.meta = meta; f.by_x = 1;
-          vocab_finish<DT><<<(unsigned)((rows * q.D + 255) / 256), 256, 0, s>>>(f);
+          f.slab = d.slab; f.ld = p.Dp; f.stride = d.slab_stride; f.splits = p.dw.splits;
+          f.rows = rows; f.out = out; f.meta = meta; f.by_x = 1;
+          finish(f, q, s);
         }
       }
     }
     if (dx) {
       FinishArgs f = {};
-      f.slab = (const float*)(ws + p.dx_slab); f.ld = p.Dp; f.stride = p.Mp * p.Dp; f.splits = p.dx_splits;
-      f.pos = (const int32_t*)(ws + p.pos); f.rows = q.t.M; f.D = q.D; f.out = dx; f.ld_out = q.D; f.meta = meta;
-      vocab_finish<DT><<<(unsigned)((q.t.M * q.D + 255) / 256), 256, 0, s>>>(f);
+      f.slab = (const float*)(ws + p.dx_slab); f.ld = p.Dp; f.stride = p.Mp * p.Dp; f.splits = p.dx.splits;
+      f.pos = (const int32_t*)(ws + p.pos); f.rows = q.t.M; f.out = dx; f.meta = meta;
+      finish(f, q, s);
     }
     return launch_status();
   }
@@ -536,7 +724,7 @@ int run_forward(const Problem& q, float* loss, float* lse, float* hit, void* ws,
   if (const int e = check(q)) return e;
   if (q.t.M == 0) return GNET_OK;
   if (!loss || !lse || !hit) return GNET_ERR_INVALID;
-  const Plan p = make_plan(q.t.M, q.t.V, q.D, q.t.K, q.dtype, needs_pack(q.w, q.ldw, q.D, q.dtype), 0);
+  const Plan p = make_plan(q.t.M, q.t.V, q.D, q.t.K, q.dtype, q.t.logits != nullptr, needs_pack(q.w, q.ldw, q.D, q.dtype), 0);
   if (!ws || ws_bytes < (size_t)p.bytes || ((uintptr_t)ws & 255)) return GNET_ERR_WORKSPACE;
   switch (q.dtype) {
     case GNET_F32: return Run<GNET_F32, F16T, 2>::forward(q, p, (char*)ws, loss, lse, hit, s);
@@ -556,7 +744,7 @@ int run_backward(const Problem& q, const float* lse, const float* hit, const flo
     return launch_status();
   }
   if (!lse || !hit || !dloss) return GNET_ERR_INVALID;
-  const Plan p = make_plan(q.t.M, q.t.V, q.D, q.t.K, q.dtype, needs_pack(q.w, q.ldw, q.D, q.dtype), 1);
+  const Plan p = make_plan(q.t.M, q.t.V, q.D, q.t.K, q.dtype, q.t.logits != nullptr, needs_pack(q.w, q.ldw, q.D, q.dtype), 1);
   if (!ws || ws_bytes < (size_t)p.bytes || ((uintptr_t)ws & 255)) return GNET_ERR_WORKSPACE;
   switch (q.dtype) {
     case GNET_F32: return Run<GNET_F32, F16T, 2>::backward(q, p, (char*)ws, lse, hit, dloss, dx, dw, s);
@@ -578,8 +766,9 @@ Problem problem(const void* x, int64_t ldx, const void* w, int64_t ldw, const vo
 
 // ------------------------------------------------------------------------------------------
 extern "C" size_t gnet_vocab_workspace_bytes(const void* w, int64_t ldw, int64_t M, int64_t V, int64_t D, int64_t K, int32_t dtype, int32_t backward) {
-  if (M <= 0 || V < 1 || D < 1 || K < 1 || M > (1 << 24) || V > (1ll << 30) || D > (1 << 16) || K > 1024) return 0;
-  return (size_t)make_plan(M, V, D, K, dtype, needs_pack(w, ldw, D, dtype), backward).bytes;
+  if (M <= 0 || V < 1 || D < 1 || K < 0 || M > (1 << 24) || V > (1ll << 30) || D > (1 << 16) || K > 1024) return 0;
+  // K = 0: cross entropy
+  return (size_t)make_plan(M, V, D, K, dtype, K > 0, needs_pack(w, ldw, D, dtype), backward).bytes;
 }
 
 extern "C" int gnet_xent_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* labels, int32_t labels64, int64_t M,

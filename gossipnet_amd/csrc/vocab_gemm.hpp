@@ -60,16 +60,18 @@ struct VocabGemm {
   int64_t k;                   // contraction length, a multiple of VG_BK (k_from_meta: meta->rows rounded up)
   int k_from_meta;
   int cols_from_meta;          // columns are tokens: column tiles behind meta->rows are left out
-  int segments;                // 1, or 3 with two planes
   int row_tiles, col_tiles, splits;
   const VocabMeta* meta;
   // logits
   float to_log2;               // log2(e) / temperature
   int64_t valid_rows;          // vocabulary rows of this piece that exist
   int first_row_tile, all_row_tiles;
+  int32_t first_row;           // of the piece, in the vocabulary
+  const int32_t* label;        // per column: its one target, or NULL (several, see vocab_hits)
   float2* part;                // [column][all_row_tiles] running maximum and sum of a row tile
+  float* hit;                  // per column: the logit of its label, in units of log2
   const float* lse2; const float* gscale;   // per column
-  u16* dz; int64_t ld_dz, plane_dz;
+  u16* dz; int64_t ld_dz, plane_dz, dz_cols;
   // products
   float* slab; int64_t ld_slab, slab_stride; int accumulate;      // [split][column][ld_slab]
   void* out; int64_t ld_out, out_rows, out_cols; int out_vec; int unscale_by_x;   // [column][row]; out_vec: four elements may be stored at once
@@ -234,22 +236,33 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) vocab_gemm(const VocabGemm g)
   __syncthreads();                                 // the epilogue uses the LDS
 
   const int col16 = lane & 15, quad = lane >> 4;
+  // a column's label as a row of this wave's FM * 16 (outside: not here); a lane holds rows i * 16 + quad * 4 + r
+  auto label_row = [&](int64_t c) {
+    return g.label && c < rows ? (int64_t)g.label[c] - g.first_row - r0 - wm * FM * 16 - quad * 4 : (int64_t)-1;
+  };
   if constexpr (EPI == EPI_PART) {
     // the tile's maximum and sum of 2^(z - max), z in units of log2, for each of its columns (tokens)
     const float f = g.to_log2 * g.meta->unscale_x * g.meta->unscale_w;
+    const int64_t left = g.valid_rows - r0 - wm * FM * 16 - quad * 4;        // rows of the lane's that exist
     float2* red = reinterpret_cast<float2*>(lds);        // [WM][BN]
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
+      const int64_t c = c0 + (wn * FN + j) * 16 + col16;
+      const int64_t label = label_row(c);
       float m = -INFINITY;
 #pragma unroll
       for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int64_t row = r0 + (wm * FM + i) * 16 + quad * 4 + r;
-          const float z = row < g.valid_rows ? acc[i][j][r] * f : -INFINITY;
+          const float z = i * 16 + r < left ? acc[i][j][r] * f : -INFINITY;
           acc[i][j][r] = z;
           m = fmaxf(m, z);
         }
+      if (label >= 0 && label < FM * 16)
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) if (label == i * 16 + r) g.hit[c] = acc[i][j][r];
       m = fmaxf(m, __shfl_xor(m, 16));
       m = fmaxf(m, __shfl_xor(m, 32));
       const float base = m == -INFINITY ? 0.f : m;       // nothing here yet: exp2(-inf - 0) = 0
@@ -276,24 +289,33 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) vocab_gemm(const VocabGemm g)
     }
   } else if constexpr (EPI == EPI_DZ) {
     const float f = g.to_log2 * g.meta->unscale_x * g.meta->unscale_w;
+    const int64_t left = g.valid_rows - r0 - wm * FM * 16 - quad * 4;
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
       const int64_t c = c0 + (wn * FN + j) * 16 + col16;
+      if (c >= g.dz_cols) continue;
       const bool some = c < rows;
       const float lse = some ? g.lse2[c] : 0.f, gs = some ? g.gscale[c] : 0.f;
+      const int64_t label = label_row(c);
+      const bool here = label >= 0 && label < FM * 16;
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
-        const int64_t row = r0 + (wm * FM + i) * 16 + quad * 4;
         u16 v[4], lo[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           // padding (a token or a vocabulary row that does not exist) is zero: it takes part in the products
-          const float d = some && row + r < g.valid_rows ? __builtin_amdgcn_exp2f(acc[i][j][r] * f - lse) * gs : 0.f;
+          float p = __builtin_amdgcn_exp2f(acc[i][j][r] * f - lse);
+          if (here && label == i * 16 + r) p -= 1.f;
+          const float d = some && i * 16 + r < left ? p * gs : 0.f;
           if (PLANES == 1) v[r] = T::enc(d); else split_f16(d, v[r], lo[r]);
         }
-        *reinterpret_cast<s16x4*>(g.dz + c * g.ld_dz + row) = s16x4{(short)v[0], (short)v[1], (short)v[2], (short)v[3]};
-        if (PLANES == 2)
-          *reinterpret_cast<s16x4*>(g.dz + g.plane_dz + c * g.ld_dz + row) = s16x4{(short)lo[0], (short)lo[1], (short)lo[2], (short)lo[3]};
+        const int64_t at = c * g.ld_dz + r0 + (wm * FM + i) * 16 + quad * 4;
+        *reinterpret_cast<s16x4*>(g.dz + at) = s16x4{(short)v[0], (short)v[1], (short)v[2], (short)v[3]};
+        if (PLANES == 2) *reinterpret_cast<s16x4*>(g.dz + g.plane_dz + at) = s16x4{(short)lo[0], (short)lo[1], (short)lo[2], (short)lo[3]};
+        if (BN < VG_BK) {      // one column tile: the rest of the contraction's step over tokens
+          *reinterpret_cast<s16x4*>(g.dz + at + BN * g.ld_dz) = s16x4{0, 0, 0, 0};
+          if (PLANES == 2) *reinterpret_cast<s16x4*>(g.dz + g.plane_dz + at + BN * g.ld_dz) = s16x4{0, 0, 0, 0};
+        }
       }
     }
   } else if constexpr (EPI == EPI_SLAB) {

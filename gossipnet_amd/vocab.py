@@ -168,7 +168,7 @@ def xent_forward(x, w, labels):
     loss, lse, hit = (torch.empty(lead, dtype=torch.float32, device=dev) for _ in range(3))
     lib = _lib.load()
     with torch.cuda.device(dev):
-        nbytes = lib.gnet_vocab_workspace_bytes(_p(wm), _ld(wm), M, V, D, 1, _TYPES[wm.dtype], 0)
+        nbytes = lib.gnet_vocab_workspace_bytes(_p(wm), _ld(wm), M, V, D, 0, _TYPES[wm.dtype], 0)
         buf, ws = _workspace(nbytes, dev)
         _lib.check(lib.gnet_xent_forward(_p(xm), _ld(xm), _p(wm), _ld(wm), _p(i), int(i.dtype == torch.int64), M, V, D, _TYPES[wm.dtype],
                                          _p(loss), _p(lse), _p(hit), ws, nbytes, _stream(dev)), "gnet_xent_forward")
@@ -181,7 +181,7 @@ def xent_backward(x, w, labels, lse, hit, dloss, need_dx=True, need_dw=True):
     xm, wm = _features(x, w)
     lead = tuple(x.shape[:-1])
     i = _ids(labels, "labels", lead)
-    return _backward(xm, wm, i, None, 1.0, _per_token(lse, "lse", lead), _per_token(hit, "hit", lead), _loss_gradient(dloss, lead), x.shape, 1, need_dx, need_dw)
+    return _backward(xm, wm, i, None, 1.0, _per_token(lse, "lse", lead), _per_token(hit, "hit", lead), _loss_gradient(dloss, lead), x.shape, 0, need_dx, need_dw)
 
 
 def distill_forward(x, w, top_ids, top_logits, temperature=1.0):

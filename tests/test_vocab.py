@@ -91,7 +91,7 @@ def test_c_entries_refuse_before_they_launch():
         assert xent(**a) == _lib.ERR_INVALID, a
     for a in (dict(M=(1 << 24) + 1), dict(V=(1 << 30) + 1), dict(D=(1 << 16) + 1, ldx=1 << 17, ldw=1 << 17), dict(M=1 << 24, V=1 << 21)):
         assert xent(**a) == _lib.ERR_UNSUPPORTED, a
-    need = lib.gnet_vocab_workspace_bytes(p, 8, 4, 10, 8, 1, F32, 0)
+    need = lib.gnet_vocab_workspace_bytes(p, 8, 4, 10, 8, 0, F32, 0)
     assert need > 0
     for a in (dict(ws=None), dict(n=need - 1), dict(ws=odd)):
         assert xent(**a) == _lib.ERR_WORKSPACE, a
@@ -122,8 +122,8 @@ def test_workspaces_do_not_grow_with_the_logits():
     lib = _lib.load()
     p = C.c_void_p(1 << 20)
     M, V, D = 4096, 131072, 4096
-    assert lib.gnet_vocab_workspace_bytes(p, D, M, V, D, 1, BF16, 1) < M * V
-    assert lib.gnet_vocab_workspace_bytes(p, D, M, V, D, 1, BF16, 0) < M * V // 4
-    assert lib.gnet_vocab_workspace_bytes(p, D, 0, V, D, 1, BF16, 0) == 0
+    assert lib.gnet_vocab_workspace_bytes(p, D, M, V, D, 0, BF16, 1) < M * V
+    assert lib.gnet_vocab_workspace_bytes(p, D, M, V, D, 0, BF16, 0) < M * V // 4
+    assert lib.gnet_vocab_workspace_bytes(p, D, 0, V, D, 0, BF16, 0) == 0
     # a weight matrix that cannot be read where it lies is packed: only then is there room for it
-    assert lib.gnet_vocab_workspace_bytes(C.c_void_p((1 << 20) + 2), D, 64, V, D, 1, BF16, 0) > lib.gnet_vocab_workspace_bytes(p, D, 64, V, D, 1, BF16, 0)
+    assert lib.gnet_vocab_workspace_bytes(C.c_void_p((1 << 20) + 2), D, 64, V, D, 0, BF16, 0) > lib.gnet_vocab_workspace_bytes(p, D, 64, V, D, 0, BF16, 0)
