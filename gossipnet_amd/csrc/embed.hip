@@ -4,8 +4,8 @@
 //              d s[m] = scale * dy[m] . table[id[m]]
 // Every kernel here moves bytes: M rows in, M rows out; the backward pass reads M rows of dy and writes the V rows of the table's
 // gradient once, the rows without a token included.
-//   embed_sort    keys (id << 32 | token), distinct, sorted in LDS per 4096 tokens; embed_merge joins 16 sorted runs at a time by
-//                 binary searches in the others (no atomics: the order of every sum is fixed)
+//   embed_sort    keys (id << 32 | token), distinct, sorted per 4096 tokens; embed_merge joins 16 sorted runs at a time by binary
+//                 searches (no atomics: the order of every sum is fixed)
 //   embed_rows    a workgroup owns a range of the table's rows and finds their tokens by binary search; a row with more than HOT
 //                 tokens is left to
 //   embed_hot     one partial sum per HOT consecutive sorted tokens and run, and embed_hot_rows, which adds a run's partial sums
@@ -14,9 +14,11 @@
 namespace {
 
 typedef unsigned long long u64;
+constexpr unsigned NONE = 0xffffffffu;      // id of a token that is left out: sorted behind all others
 constexpr int RUN = 4096;          // tokens sorted by one workgroup: 32 KB of keys
 constexpr int WAY = 16;            // runs joined by one merge pass
-constexpr int HOT = 64;            // tokens a row's own wave adds up
+constexpr int HOT = 16;            // tokens a row's own wave adds up
+constexpr int BLOCKS = 4;          // column blocks of 64 * VEC elements a wave keeps sums of
 
 template <int DT> struct Elem { typedef u16 type; };
 template <> struct Elem<GNET_F32> { typedef float type; };
@@ -62,29 +64,78 @@ template <int DT, int VEC> __global__ void __launch_bounds__(256) embed_rows_out
 }
 
 // ---- the order of the tokens ------------------------------------------------------------------------------------------
-// Bitonic sort of one run in LDS; keys are distinct, so the result is the stable order.
-__global__ void __launch_bounds__(1024) embed_sort(const void* ids, int ids64, int64_t M, int64_t V, int n, u64* __restrict__ keys) {
-  __shared__ u64 s[RUN];
-  const int64_t base = (int64_t)blockIdx.x * RUN;
-  for (int i = threadIdx.x; i < n; i += 1024) {
-    u64 key = ~0ull;                                   // behind the last token
-    if (base + i < M) {
-      const int64_t id = load_id(ids, base + i, ids64);
-      key = ((id >= 0 && id < V ? (u64)id : 0xffffffffull) << 32) | (u64)(base + i);
-    }
-    s[i] = key;
+// Bitonic sort of one run, four consecutive keys a thread: partners up to 2 apart are the thread's own, up to 128 apart the wave's (lane
+// exchanges), the rest go through LDS -- 10 of the 78 steps.  KEY = 32 bits, id << 12 | place in the run, where ids fit into 20 bits,
+// else 64.  Keys are distinct, so the result is the stable order.
+template <int X> __device__ __forceinline__ unsigned lane_xor(unsigned v) {
+  if constexpr (X == 1) return __builtin_amdgcn_mov_dpp(v, 0xB1, 0xf, 0xf, true);
+  else if constexpr (X == 2) return __builtin_amdgcn_mov_dpp(v, 0x4E, 0xf, 0xf, true);
+  else if constexpr (X == 8) return __builtin_amdgcn_mov_dpp(v, 0x128, 0xf, 0xf, true);       // a rotation by 8 within 16
+  else if constexpr (X == 32) return __shfl_xor(v, 32);
+  else return __builtin_amdgcn_ds_swizzle(v, (X << 10) | 0x1f);
+}
+template <int X> __device__ __forceinline__ u64 lane_xor(u64 v) {
+  return (u64)lane_xor<X>((unsigned)(v >> 32)) << 32 | lane_xor<X>((unsigned)v);
+}
+template <class KEY> __device__ __forceinline__ void order(KEY& a, KEY& b, bool up) {
+  const KEY lo = a < b ? a : b, hi = a < b ? b : a;
+  a = up ? lo : hi;
+  b = up ? hi : lo;
+}
+template <class KEY, int X> __device__ __forceinline__ void lane_step(KEY (&v)[4], bool up) {
+  const bool low = !(threadIdx.x & X);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const KEY o = lane_xor<X>(v[i]);
+    v[i] = (v[i] < o) == (low == up) ? v[i] : o;
   }
-  for (int k = 2; k <= n; k <<= 1)
-    for (int j = k >> 1; j; j >>= 1) {
+}
+template <class KEY> __global__ void __launch_bounds__(RUN / 4) embed_sort(const void* ids, int ids64, int64_t M, int64_t V, int n, u64* __restrict__ keys) {
+  __shared__ __attribute__((aligned(16))) KEY s[RUN];
+  constexpr int PLACE = sizeof(KEY) == 4 ? 12 : 32;
+  constexpr KEY OUT = sizeof(KEY) == 4 ? (KEY)0xfffff : (KEY)NONE;            // behind every id: no token
+  const int64_t base = (int64_t)blockIdx.x * RUN;
+  const int t0 = threadIdx.x * 4;
+  KEY v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    KEY id = OUT;
+    if (base + t0 + i < M) {
+      const int64_t x = load_id(ids, base + t0 + i, ids64);
+      if (x >= 0 && x < V) id = (KEY)x;
+    }
+    v[i] = id << PLACE | (KEY)(t0 + i);
+  }
+  for (int k = 2; k <= n; k <<= 1) {
+    for (int j = k >> 1; j >= 256; j >>= 1) {
       __syncthreads();
-      for (int t = threadIdx.x; t < n / 2; t += 1024) {
-        const int i = ((t & ~(j - 1)) << 1) | (t & (j - 1));
-        const u64 x = s[i], y = s[i + j];
-        if ((x > y) == ((i & k) == 0)) { s[i] = y; s[i + j] = x; }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[t0 + i] = v[i];
+      __syncthreads();
+      const bool keep_low = !(t0 & j) == !(t0 & k);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const KEY o = s[(t0 ^ j) + i];
+        v[i] = (v[i] < o) == keep_low ? v[i] : o;
       }
     }
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += 1024) if (base + i < M) keys[base + i] = s[i];
+    const bool up = !(t0 & k);
+    if (k > 128) lane_step<KEY, 32>(v, up);
+    if (k > 64) lane_step<KEY, 16>(v, up);
+    if (k > 32) lane_step<KEY, 8>(v, up);
+    if (k > 16) lane_step<KEY, 4>(v, up);
+    if (k > 8) lane_step<KEY, 2>(v, up);
+    if (k > 4) lane_step<KEY, 1>(v, up);
+    if (k > 2) { order(v[0], v[2], up); order(v[1], v[3], up); order(v[0], v[1], up); order(v[2], v[3], up); }
+    else { order(v[0], v[1], true); order(v[2], v[3], false); }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const KEY id = v[i] >> PLACE;
+    const int64_t m = base + (int64_t)(v[i] & (((KEY)1 << PLACE) - 1));
+    // (places behind the last token of a short run sort behind the tokens that are left out: they came later)
+    if (base + t0 + i < M) keys[base + t0 + i] = (id == OUT ? (u64)NONE : (u64)id) << 32 | (u64)m;
+  }
 }
 
 // keys of [lo, hi) below `key`
@@ -95,15 +146,17 @@ __device__ __forceinline__ int64_t lower_bound(const u64* __restrict__ keys, int
   }
   return lo;
 }
+// WAY lanes a key: each counts the smaller keys of one run; their sum is the key's place
 __global__ void __launch_bounds__(256) embed_merge(const u64* __restrict__ in, u64* __restrict__ out, int64_t M, int64_t run) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= M) return;
-  const u64 key = in[i];
-  const int64_t own = i / run, first = own / WAY * WAY;
-  int64_t at = first * run + (i - own * run);
-  for (int64_t r = first; r < first + WAY && r * run < M; ++r)
-    if (r != own) at += lower_bound(in, r * run, min(M, (r + 1) * run), key) - r * run;
-  out[at] = key;
+  const int64_t i = (int64_t)blockIdx.x * (256 / WAY) + threadIdx.x / WAY;
+  const bool some = i < M;
+  const u64 key = some ? in[i] : 0;
+  const int64_t own = i / run, first = own / WAY * WAY, r = first + threadIdx.x % WAY;
+  int n = 0;
+  if (some && r * run < M) n = r == own ? (int)(i - own * run) : (int)(lower_bound(in, r * run, min(M, (r + 1) * run), key) - r * run);
+#pragma unroll
+  for (int o = WAY / 2; o; o >>= 1) n += __shfl_xor(n, o);
+  if (some && threadIdx.x % WAY == 0) out[first * run + n] = key;
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------------
@@ -115,12 +168,36 @@ struct BackwardArgs {
   float* part;                         // [segment][2][D]
 };
 
-template <int DT, int VEC> __device__ __forceinline__ void add_token(float (&sum)[VEC], const BackwardArgs& a, int64_t m, int64_t d) {
+// sums of the tokens [lo, hi) of the sorted order, in order, over `blocks` column blocks `step` elements apart from column d on; four
+// tokens' rows are on the way at a time
+template <int DT, int VEC> __device__ __forceinline__ void add_tokens(float (&sum)[BLOCKS][VEC], const BackwardArgs& a, int64_t lo, int64_t hi, int64_t d, int step, int blocks) {
   typedef typename Elem<DT>::type E;
-  const Pack<E, VEC> g = *reinterpret_cast<const Pack<E, VEC>*>((const E*)a.dy + m * a.ld + d);
-  const float s = a.token_scale ? a.token_scale[m] : 1.f;
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) sum[i] = fmaf(dec<DT>(g.v[i]), s, sum[i]);
+  for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) sum[b][i] = 0.f;
+  for (int64_t j = lo; j < hi; j += 4) {
+    Pack<E, VEC> g[4][BLOCKS];
+    float s[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (j + u >= hi) continue;
+      const int64_t m = (int64_t)(a.keys[j + u] & 0xffffffffull);
+      s[u] = a.token_scale ? a.token_scale[m] : 1.f;
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b)
+        if (b < blocks && d + b * step < a.D) g[u][b] = *reinterpret_cast<const Pack<E, VEC>*>((const E*)a.dy + m * a.ld + d + b * step);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (j + u >= hi) continue;
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b)
+        if (b < blocks && d + b * step < a.D)
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) sum[b][i] = fmaf(dec<DT>(g[u][b].v[i]), s[u], sum[b][i]);
+    }
+  }
 }
 template <int DT, int VEC> __device__ __forceinline__ void store_row(const float (&sum)[VEC], const BackwardArgs& a, int64_t v, int64_t d) {
   typedef typename Elem<DT>::type E;
@@ -142,62 +219,82 @@ template <int DT, int VEC> __global__ void __launch_bounds__(256) embed_rows(con
   for (int r = threadIdx.x >> 6; r < a.rows && v0 + r < a.V; r += 4) {
     const int64_t lo = start[r], hi = start[r + 1];
     if (hi - lo > HOT || (a.accumulate && lo == hi)) continue;
-    for (int64_t d = (int64_t)lane * VEC; d < a.D; d += 64 * VEC) {
-      float sum[VEC];
+    for (int64_t d = (int64_t)lane * VEC; d - lane * VEC < a.D; d += BLOCKS * 64 * VEC) {
+      const int blocks = (int)min((int64_t)BLOCKS, (a.D - (d - lane * VEC) + 64 * VEC - 1) / (64 * VEC));
+      float sum[BLOCKS][VEC];
+      add_tokens<DT, VEC>(sum, a, lo, hi, d, 64 * VEC, blocks);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) sum[i] = 0.f;
-      for (int64_t j = lo; j < hi; ++j) add_token<DT, VEC>(sum, a, (int64_t)(a.keys[j] & 0xffffffffull), d);
-      store_row<DT, VEC>(sum, a, v0 + r, d);
+      for (int b = 0; b < BLOCKS; ++b)
+        if (b < blocks && d + b * 64 * VEC < a.D) store_row<DT, VEC>(sum[b], a, v0 + r, d + b * 64 * VEC);
     }
   }
 }
 
 // The runs of more than HOT equal ids: a segment of HOT sorted tokens meets at most two, one that comes in over its first token
-// (slot 0: also a run that starts right there) and one that leaves over its last (slot 1).
-constexpr unsigned NONE = 0xffffffffu;      // id of a token that is left out: sorted behind all others
+// (slot 0: also a run that starts right there and leaves) and one that leaves over its last (slot 1).
 __device__ __forceinline__ unsigned id_at(const u64* keys, int64_t i) { return (unsigned)(keys[i] >> 32); }
+// does the run of `id` over place p have more than HOT tokens: are two of them HOT places apart, around p
+__device__ __forceinline__ bool hot_around(const u64* keys, int64_t M, int64_t p, unsigned id) {
+  const int64_t b = p - HOT + (threadIdx.x & 63), e = b + HOT;
+  return __any((threadIdx.x & 63) <= HOT && b >= 0 && e < M && id_at(keys, b) == id && id_at(keys, e) == id);
+}
 template <int DT, int VEC> __global__ void __launch_bounds__(256) embed_hot(const BackwardArgs a) {
   const int64_t seg = blockIdx.x, lo = seg * HOT, hi = min(a.M, lo + HOT);
   const unsigned first = id_at(a.keys, lo), last = id_at(a.keys, hi - 1);
-  const bool whole = first == last && hi < a.M && id_at(a.keys, hi) == first;
-  const bool in = first != NONE && (whole || (lo > 0 && id_at(a.keys, lo - 1) == first));
-  const bool out = first != last && last != NONE && hi < a.M && id_at(a.keys, hi) == last;
+  const bool leaves = last != NONE && hi < a.M && id_at(a.keys, hi) == last;
+  const bool in = first != NONE && lo > 0 && id_at(a.keys, lo - 1) == first;
   for (int slot = 0; slot < 2; ++slot) {
-    if (!(slot ? out : in)) continue;
-    const u64 id = slot ? last : first;
-    const int64_t run0 = lower_bound(a.keys, 0, hi, id << 32), run1 = lower_bound(a.keys, lo, a.M, (id + 1) << 32);
-    if (run1 - run0 <= HOT) continue;
-    const int64_t b = max(lo, run0), e = min(hi, run1);
+    // slot 0: comes in, or is the whole segment and leaves; slot 1: leaves and is not slot 0's
+    const unsigned id = slot ? last : first;
+    if (slot ? !(leaves && first != last) : !(in || (leaves && first == last))) continue;
+    if (!hot_around(a.keys, a.M, slot || !in ? hi : lo, id)) continue;
+    int64_t b = lo, e = hi;
+    if (slot) { while (id_at(a.keys, b) != id) ++b; } else { while (id_at(a.keys, e - 1) != id) --e; }
     for (int64_t d = (int64_t)threadIdx.x * VEC; d < a.D; d += 256 * VEC) {
-      float sum[VEC];
+      float sum[BLOCKS][VEC];
+      add_tokens<DT, VEC>(sum, a, b, e, d, 0, 1);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) sum[i] = 0.f;
-      for (int64_t j = b; j < e; ++j) add_token<DT, VEC>(sum, a, (int64_t)(a.keys[j] & 0xffffffffull), d);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) a.part[(seg * 2 + slot) * a.D + d + i] = sum[i];
+      for (int i = 0; i < VEC; ++i) a.part[(seg * 2 + slot) * a.D + d + i] = sum[0][i];
     }
   }
 }
+// The segment in which a hot run starts adds the run's partial sums: each wave a quarter of them in order, then the quarters in order.
 template <int DT, int VEC> __global__ void __launch_bounds__(256) embed_hot_rows(const BackwardArgs a) {
-  // the segment in which a run of more than HOT tokens starts adds its partial sums, in order
+  __shared__ float quarter[3][64 * VEC];
   const int64_t seg = blockIdx.x, lo = seg * HOT, hi = min(a.M, lo + HOT);
   if (hi >= a.M) return;
   const unsigned id = id_at(a.keys, hi - 1);
-  if (id == NONE || id_at(a.keys, hi) != id) return;              // no run leaves this segment
+  if (id == NONE || id_at(a.keys, hi) != id) return;                     // no run leaves this segment
   const bool whole = id_at(a.keys, lo) == id;
   if (whole && lo > 0 && id_at(a.keys, lo - 1) == id) return;            // it started earlier
-  const int64_t b = whole ? lo : lower_bound(a.keys, lo, hi, (u64)id << 32);
-  const int64_t e = lower_bound(a.keys, hi, a.M, ((u64)id + 1) << 32);
-  if (e - b <= HOT) return;                                              // embed_rows has it
-  const int64_t last = (e - 1) / HOT;
-  for (int64_t d = (int64_t)threadIdx.x * VEC; d < a.D; d += 256 * VEC) {
+  if (!hot_around(a.keys, a.M, hi, id)) return;                          // embed_rows has it
+  const int64_t n = (lower_bound(a.keys, hi, a.M, ((u64)id + 1) << 32) - 1) / HOT - seg;      // segments behind this one
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t s0 = seg + 1 + n * wave / 4, s1 = seg + 1 + n * (wave + 1) / 4;
+  for (int64_t d0 = 0; d0 < a.D; d0 += 64 * VEC) {
+    const int64_t d = d0 + lane * VEC;
     float sum[VEC];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) sum[i] = a.part[(seg * 2 + (whole ? 0 : 1)) * a.D + d + i];
-    for (int64_t s = seg + 1; s <= last; ++s)
+    for (int i = 0; i < VEC; ++i) sum[i] = 0.f;
+    if (d < a.D) {
+      if (wave == 0)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) sum[i] += a.part[s * 2 * a.D + d + i];
-    store_row<DT, VEC>(sum, a, id, d);
+        for (int i = 0; i < VEC; ++i) sum[i] = a.part[(seg * 2 + (whole ? 0 : 1)) * a.D + d + i];
+#pragma unroll 4
+      for (int64_t s = s0; s < s1; ++s)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) sum[i] += a.part[s * 2 * a.D + d + i];
+    }
+    __syncthreads();
+    if (wave)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) quarter[wave - 1][lane * VEC + i] = sum[i];
+    __syncthreads();
+    if (wave == 0 && d < a.D) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) sum[i] = ((sum[i] + quarter[0][lane * VEC + i]) + quarter[1][lane * VEC + i]) + quarter[2][lane * VEC + i];
+      store_row<DT, VEC>(sum, a, id, d);
+    }
   }
 }
 
@@ -292,11 +389,13 @@ extern "C" int gnet_embed_backward(const void* ids, int32_t ids64, const void* d
   u64* other = (u64*)((char*)workspace + keys_bytes(M));
   float* part = (float*)((char*)workspace + 2 * keys_bytes(M));
   if (M) {
-    int n = 64;
+    int n = 256;                                      // a whole wave
     while (n < RUN && n < M) n <<= 1;
-    embed_sort<<<(unsigned)((M + RUN - 1) / RUN), 1024, 0, s>>>(ids, ids64, M, V, n, keys);
+    const unsigned runs = (unsigned)((M + RUN - 1) / RUN);
+    if (V < (1 << 20) - 1) embed_sort<unsigned><<<runs, n / 4, 0, s>>>(ids, ids64, M, V, n, keys);
+    else embed_sort<u64><<<runs, n / 4, 0, s>>>(ids, ids64, M, V, n, keys);
     for (int64_t run = RUN; run < M; run *= WAY) {
-      embed_merge<<<(unsigned)((M + 255) / 256), 256, 0, s>>>(keys, other, M, run);
+      embed_merge<<<(unsigned)((M + 256 / WAY - 1) / (256 / WAY)), 256, 0, s>>>(keys, other, M, run);
       u64* t = keys; keys = other; other = t;
     }
   }

@@ -316,7 +316,7 @@ def test_gradient_against_differences():
 # ---- embedding rows -----------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("shape,V,D", [((1,), 1, 1), ((3, 5), 7, 3), ((1,), 100, 4096), ((130,), 50, 65), ((4097,), 81, 128), ((2, 700), 3000, 264), ((70000,), 33, 8),
-                                       ((9000,), 100000, 16)])
+                                       ((9000,), 100000, 16), ((5000,), 2 ** 20 - 2, 8), ((5000,), 2 ** 20 - 1, 8), ((300, 300), 2 ** 21, 2)])
 def test_embed(shape, V, D, dtype):
     from gossipnet_amd import vocab
     t = TYPES[dtype]
@@ -354,9 +354,9 @@ def test_embed(shape, V, D, dtype):
         near(ds, dot, mag * (D + 4) * U, "dscale")
 
 
-@pytest.mark.parametrize("M", [63, 64, 65, 128, 129, 4096, 4097, 65537])
+@pytest.mark.parametrize("M", [15, 16, 17, 32, 33, 64, 129, 4096, 4097, 65537, 70000])
 def test_embed_gradient_of_one_row_and_of_runs_around_the_hot_limit(M):
-    """All tokens the same id; and runs of 63, 64, 65 and more tokens at every place of the sorted order."""
+    """All tokens the same id; and runs of 15, 16, 17 and more tokens at every place of the sorted order."""
     from gossipnet_amd import vocab
     D = 24
     g = torch.Generator(device=DEV).manual_seed(M)
@@ -366,7 +366,7 @@ def test_embed_gradient_of_one_row_and_of_runs_around_the_hot_limit(M):
     for _ in range(2):
         want = torch.zeros(40, D, dtype=torch.float64, device=DEV).index_add_(0, ids, dy.double())
         assert torch.equal(vocab.embed_backward(ids, dy, table)[0].double(), want)
-        sizes = [63, 64, 65, 1, 127, 128, 129, 2, 64, 64, 200]
+        sizes = [15, 16, 17, 1, 31, 32, 33, 2, 16, 16, 48, 64, 200, 3, 17]
         ids = torch.repeat_interleave(torch.arange(len(sizes), device=DEV), torch.tensor(sizes, device=DEV))
         ids = ids.repeat(M // ids.numel() + 1)[:M][torch.randperm(M, device=DEV, generator=g)]
 
