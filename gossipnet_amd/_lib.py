@@ -61,7 +61,7 @@ EXPORTS = ["gnet_param_count", "gnet_graph_count", "gnet_graph_fill", "gnet_grap
            "roi_pool_fwd_f32", "roi_pool_bwd_f32", "roi_pool_bwd_atomic_f32", "gnet_version", "gnet_profiler_create", "gnet_profiler_read",
            "gnet_profiler_destroy", "gnet_profiler_set_stride", "gnet_profiler_begin", "gnet_profiler_end", "gnet_adam_step", "gnet_momentum_step", "gnet_clip_by_norm",
            "gnet_fc_workspace_bytes", "gnet_fc_forward", "gnet_fc_backward", "gnet_box_iou", "gnet_debug_gemm", "gnet_abi_version", "gnet_abi_sizes",
-           "gnet_embed_forward", "gnet_embed_workspace_bytes", "gnet_embed_backward", "gnet_embed_scale_backward", "gnet_vocab_workspace_bytes",
+           "gnet_embed_forward", "gnet_embed_workspace_bytes", "gnet_embed_backward", "gnet_vocab_workspace_bytes",
            "gnet_xent_forward", "gnet_xent_backward", "gnet_distill_forward", "gnet_distill_backward"]
 
 KCLASSES = ["graph", "pack", "pw_fwd", "node_fwd", "edge_fwd", "loss", "head_bwd", "winner_lists", "edge_bwd", "gather_winners",
@@ -209,9 +209,7 @@ def _bind(lib):
     lib.gnet_embed_workspace_bytes.restype = sz
     lib.gnet_embed_workspace_bytes.argtypes = [i64, i64]
     lib.gnet_embed_backward.restype = C.c_int
-    lib.gnet_embed_backward.argtypes = [vp, i32, vp, i64, f32, vp, i64, i64, i64, i32, vp, i32, vp, sz, vp]
-    lib.gnet_embed_scale_backward.restype = C.c_int
-    lib.gnet_embed_scale_backward.argtypes = [vp, i32, vp, i64, vp, i64, f32, i64, i64, i64, i32, vp, vp]
+    lib.gnet_embed_backward.argtypes = [vp, i32, vp, i64, f32, vp, i64, i64, i64, i32, vp, i32, vp, i64, vp, vp, sz, vp]
     lib.gnet_vocab_workspace_bytes.restype = sz
     lib.gnet_vocab_workspace_bytes.argtypes = [vp, i64, i64, i64, i64, i64, i32, i32]
     lib.gnet_xent_forward.restype = C.c_int

@@ -6,9 +6,9 @@
 // gradient once, the rows without a token included.
 //   embed_sort    keys (id << 32 | token), distinct, sorted per 4096 tokens; embed_merge joins 16 sorted runs at a time by binary
 //                 searches (no atomics: the order of every sum is fixed)
-//   embed_rows    a workgroup owns a range of the table's rows and finds their tokens by binary search; a row with more than HOT
-//                 tokens is left to
-//   embed_hot     one partial sum per HOT consecutive sorted tokens and run, and embed_hot_rows, which adds a run's partial sums
+//   embed_sums    four kinds of workgroups in one launch: sums of the runs of equal ids (a wave starts where a run starts), partial sums
+//                 of the runs of more than HOT tokens per HOT sorted tokens, zeros for the rows without a token, d s
+//   embed_hot_rows  adds a long run's partial sums
 #include "vocab_gemm.hpp"
 
 namespace {
@@ -19,6 +19,7 @@ constexpr int RUN = 4096;          // tokens sorted by one workgroup: 32 KB of k
 constexpr int WAY = 16;            // runs joined by one merge pass
 constexpr int HOT = 16;            // tokens a row's own wave adds up
 constexpr int BLOCKS = 4;          // column blocks of 64 * VEC elements a wave keeps sums of
+constexpr int FILL_ROWS = 64;      // table rows a workgroup looks for and fills with zeros
 
 template <int DT> struct Elem { typedef u16 type; };
 template <> struct Elem<GNET_F32> { typedef float type; };
@@ -164,35 +165,36 @@ struct BackwardArgs {
   const u64* keys; int64_t M, V, D;
   const void* dy; int64_t ld; float scale; const float* token_scale;
   void* out; int64_t ld_out; int accumulate;
-  int rows;                            // table rows of a workgroup
   float* part;                         // [segment][2][D]
+  unsigned run_groups, hot_groups, fill_groups;      // workgroups of each kind, in this order; d s gets the rest
+  const void* ids; int ids64; const void* table; int64_t ld_table; float* dscale;
 };
 
-// sums of the tokens [lo, hi) of the sorted order, in order, over `blocks` column blocks `step` elements apart from column d on; four
-// tokens' rows are on the way at a time
-template <int DT, int VEC> __device__ __forceinline__ void add_tokens(float (&sum)[BLOCKS][VEC], const BackwardArgs& a, int64_t lo, int64_t hi, int64_t d, int step, int blocks) {
+// sums of the tokens [lo, hi) of the sorted order, in order, over `blocks` <= NB column blocks `step` elements apart from column d on;
+// U tokens' rows are on the way at a time
+template <int DT, int VEC, int U, int NB> __device__ __forceinline__ void add_tokens(float (&sum)[NB][VEC], const BackwardArgs& a, int64_t lo, int64_t hi, int64_t d, int step, int blocks) {
   typedef typename Elem<DT>::type E;
 #pragma unroll
-  for (int b = 0; b < BLOCKS; ++b)
+  for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int i = 0; i < VEC; ++i) sum[b][i] = 0.f;
-  for (int64_t j = lo; j < hi; j += 4) {
-    Pack<E, VEC> g[4][BLOCKS];
-    float s[4];
+  for (int64_t j = lo; j < hi; j += U) {
+    Pack<E, VEC> g[U][NB];
+    float s[U];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < U; ++u) {
       if (j + u >= hi) continue;
       const int64_t m = (int64_t)(a.keys[j + u] & 0xffffffffull);
       s[u] = a.token_scale ? a.token_scale[m] : 1.f;
 #pragma unroll
-      for (int b = 0; b < BLOCKS; ++b)
+      for (int b = 0; b < NB; ++b)
         if (b < blocks && d + b * step < a.D) g[u][b] = *reinterpret_cast<const Pack<E, VEC>*>((const E*)a.dy + m * a.ld + d + b * step);
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < U; ++u) {
       if (j + u >= hi) continue;
 #pragma unroll
-      for (int b = 0; b < BLOCKS; ++b)
+      for (int b = 0; b < NB; ++b)
         if (b < blocks && d + b * step < a.D)
 #pragma unroll
           for (int i = 0; i < VEC; ++i) sum[b][i] = fmaf(dec<DT>(g[u][b].v[i]), s[u], sum[b][i]);
@@ -209,56 +211,102 @@ template <int DT, int VEC> __device__ __forceinline__ void store_row(const float
   *p = o;
 }
 
-constexpr int MOST_ROWS = 64;
-template <int DT, int VEC> __global__ void __launch_bounds__(256) embed_rows(const BackwardArgs a) {
-  __shared__ int64_t start[MOST_ROWS + 1];
-  const int64_t v0 = (int64_t)blockIdx.x * a.rows;
-  const int lane = threadIdx.x & 63;
-  if (threadIdx.x <= a.rows) start[threadIdx.x] = lower_bound(a.keys, 0, a.M, (u64)(v0 + threadIdx.x) << 32);
-  __syncthreads();
-  for (int r = threadIdx.x >> 6; r < a.rows && v0 + r < a.V; r += 4) {
-    const int64_t lo = start[r], hi = start[r + 1];
-    if (hi - lo > HOT || (a.accumulate && lo == hi)) continue;
-    for (int64_t d = (int64_t)lane * VEC; d - lane * VEC < a.D; d += BLOCKS * 64 * VEC) {
-      const int blocks = (int)min((int64_t)BLOCKS, (a.D - (d - lane * VEC) + 64 * VEC - 1) / (64 * VEC));
-      float sum[BLOCKS][VEC];
-      add_tokens<DT, VEC>(sum, a, lo, hi, d, 64 * VEC, blocks);
-#pragma unroll
-      for (int b = 0; b < BLOCKS; ++b)
-        if (b < blocks && d + b * 64 * VEC < a.D) store_row<DT, VEC>(sum[b], a, v0 + r, d + b * 64 * VEC);
-    }
-  }
-}
-
-// The runs of more than HOT equal ids: a segment of HOT sorted tokens meets at most two, one that comes in over its first token
-// (slot 0: also a run that starts right there and leaves) and one that leaves over its last (slot 1).
 __device__ __forceinline__ unsigned id_at(const u64* keys, int64_t i) { return (unsigned)(keys[i] >> 32); }
 // does the run of `id` over place p have more than HOT tokens: are two of them HOT places apart, around p
 __device__ __forceinline__ bool hot_around(const u64* keys, int64_t M, int64_t p, unsigned id) {
   const int64_t b = p - HOT + (threadIdx.x & 63), e = b + HOT;
   return __any((threadIdx.x & 63) <= HOT && b >= 0 && e < M && id_at(keys, b) == id && id_at(keys, e) == id);
 }
-template <int DT, int VEC> __global__ void __launch_bounds__(256) embed_hot(const BackwardArgs a) {
-  const int64_t seg = blockIdx.x, lo = seg * HOT, hi = min(a.M, lo + HOT);
+
+// A wave per place of the sorted order: where a run of at most HOT tokens starts, its sum.
+template <int DT, int VEC> __device__ __forceinline__ void run_sums(const BackwardArgs& a, int64_t i) {
+  if (i >= a.M) return;
+  const int lane = threadIdx.x & 63;
+  const unsigned id = id_at(a.keys, i);
+  if (id == NONE || (i > 0 && id_at(a.keys, i - 1) == id)) return;
+  const bool same = lane <= HOT && i + lane < a.M && id_at(a.keys, min(i + lane, a.M - 1)) == id;
+  const int n = __popcll(__ballot(same));                    // (equal ids are next to each other)
+  if (n > HOT) return;
+  for (int64_t d0 = 0; d0 < a.D; d0 += BLOCKS * 64 * VEC) {
+    const int blocks = (int)min((int64_t)BLOCKS, (a.D - d0 + 64 * VEC - 1) / (64 * VEC));
+    const int64_t d = d0 + lane * VEC;
+    float sum[BLOCKS][VEC];
+    add_tokens<DT, VEC, 4, BLOCKS>(sum, a, i, i + n, d, 64 * VEC, blocks);
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b)
+      if (b < blocks && d + b * 64 * VEC < a.D) store_row<DT, VEC>(sum[b], a, id, d + b * 64 * VEC);
+  }
+}
+
+// The runs of more than HOT equal ids: a segment of HOT sorted tokens meets at most two, one that comes in over its first token
+// (slot 0: also a run that starts right there and leaves) and one that leaves over its last (slot 1).
+template <int DT, int VEC> __device__ __forceinline__ void hot_sums(const BackwardArgs& a, int64_t seg) {
+  const int64_t lo = seg * HOT, hi = min(a.M, lo + HOT);
   const unsigned first = id_at(a.keys, lo), last = id_at(a.keys, hi - 1);
   const bool leaves = last != NONE && hi < a.M && id_at(a.keys, hi) == last;
   const bool in = first != NONE && lo > 0 && id_at(a.keys, lo - 1) == first;
   for (int slot = 0; slot < 2; ++slot) {
-    // slot 0: comes in, or is the whole segment and leaves; slot 1: leaves and is not slot 0's
     const unsigned id = slot ? last : first;
     if (slot ? !(leaves && first != last) : !(in || (leaves && first == last))) continue;
     if (!hot_around(a.keys, a.M, slot || !in ? hi : lo, id)) continue;
     int64_t b = lo, e = hi;
     if (slot) { while (id_at(a.keys, b) != id) ++b; } else { while (id_at(a.keys, e - 1) != id) --e; }
     for (int64_t d = (int64_t)threadIdx.x * VEC; d < a.D; d += 256 * VEC) {
-      float sum[BLOCKS][VEC];
-      add_tokens<DT, VEC>(sum, a, b, e, d, 0, 1);
+      float sum[1][VEC];
+      add_tokens<DT, VEC, HOT, 1>(sum, a, b, e, d, 0, 1);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) a.part[(seg * 2 + slot) * a.D + d + i] = sum[0][i];
     }
   }
 }
-// The segment in which a hot run starts adds the run's partial sums: each wave a quarter of them in order, then the quarters in order.
+
+// Zeros for those of FILL_ROWS rows that no token has (each row's tokens by binary search).
+template <int DT, int VEC> __device__ __forceinline__ void fill_rows(const BackwardArgs& a, int64_t group, int64_t* start) {
+  typedef typename Elem<DT>::type E;
+  const int64_t v0 = group * FILL_ROWS;
+  if (threadIdx.x <= FILL_ROWS) start[threadIdx.x] = lower_bound(a.keys, 0, a.M, (u64)(v0 + threadIdx.x) << 32);
+  __syncthreads();
+  Pack<E, VEC> zero;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) zero.v[i] = enc<DT>(0.f);
+  for (int r = threadIdx.x >> 6; r < FILL_ROWS && v0 + r < a.V; r += 4)
+    if (start[r] == start[r + 1])
+      for (int64_t d = (int64_t)(threadIdx.x & 63) * VEC; d < a.D; d += 64 * VEC) *reinterpret_cast<Pack<E, VEC>*>((E*)a.out + (v0 + r) * a.ld_out + d) = zero;
+}
+
+template <int DT, int VEC> __device__ __forceinline__ void scale_gradient(const BackwardArgs& a, int64_t m) {
+  typedef typename Elem<DT>::type E;
+  if (m >= a.M) return;
+  const int64_t id = load_id(a.ids, m, a.ids64);
+  float dot = 0.f;
+  if (id >= 0 && id < a.V) {
+#pragma unroll 4
+    for (int64_t d = (int64_t)(threadIdx.x & 63) * VEC; d < a.D; d += 64 * VEC) {
+      const Pack<E, VEC> t = *reinterpret_cast<const Pack<E, VEC>*>((const E*)a.table + id * a.ld_table + d);
+      const Pack<E, VEC> g = *reinterpret_cast<const Pack<E, VEC>*>((const E*)a.dy + m * a.ld + d);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) dot = fmaf(dec<DT>(t.v[i]), dec<DT>(g.v[i]), dot);
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) dot += __shfl_xor(dot, o);
+  }
+  if ((threadIdx.x & 63) == 0) a.dscale[m] = dot * a.scale;
+}
+
+template <int DT, int VEC> __global__ void __launch_bounds__(256) embed_sums(const BackwardArgs a) {
+  __shared__ int64_t start[FILL_ROWS + 1];
+  unsigned g = blockIdx.x;
+  const int wave = threadIdx.x >> 6;
+  if (g < a.run_groups) return run_sums<DT, VEC>(a, (int64_t)g * 4 + wave);
+  g -= a.run_groups;
+  if (g < a.hot_groups) return hot_sums<DT, VEC>(a, g);
+  g -= a.hot_groups;
+  if (g < a.fill_groups) return fill_rows<DT, VEC>(a, g, start);
+  scale_gradient<DT, VEC>(a, (int64_t)(g - a.fill_groups) * 4 + wave);
+}
+
+// The segment in which a hot run starts adds the run's partial sums, a workgroup per column block: each wave a quarter of them in order,
+// then the quarters in order.
 template <int DT, int VEC> __global__ void __launch_bounds__(256) embed_hot_rows(const BackwardArgs a) {
   __shared__ float quarter[3][64 * VEC];
   const int64_t seg = blockIdx.x, lo = seg * HOT, hi = min(a.M, lo + HOT);
@@ -267,58 +315,32 @@ template <int DT, int VEC> __global__ void __launch_bounds__(256) embed_hot_rows
   if (id == NONE || id_at(a.keys, hi) != id) return;                     // no run leaves this segment
   const bool whole = id_at(a.keys, lo) == id;
   if (whole && lo > 0 && id_at(a.keys, lo - 1) == id) return;            // it started earlier
-  if (!hot_around(a.keys, a.M, hi, id)) return;                          // embed_rows has it
+  if (!hot_around(a.keys, a.M, hi, id)) return;                          // run_sums has it
   const int64_t n = (lower_bound(a.keys, hi, a.M, ((u64)id + 1) << 32) - 1) / HOT - seg;      // segments behind this one
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t s0 = seg + 1 + n * wave / 4, s1 = seg + 1 + n * (wave + 1) / 4;
-  for (int64_t d0 = 0; d0 < a.D; d0 += 64 * VEC) {
-    const int64_t d = d0 + lane * VEC;
-    float sum[VEC];
+  const int64_t d = ((int64_t)blockIdx.y * 64 + lane) * VEC;
+  float sum[VEC];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) sum[i] = 0.f;
-    if (d < a.D) {
-      if (wave == 0)
+  for (int i = 0; i < VEC; ++i) sum[i] = 0.f;
+  if (d < a.D) {
+    if (wave == 0)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) sum[i] = a.part[(seg * 2 + (whole ? 0 : 1)) * a.D + d + i];
+      for (int i = 0; i < VEC; ++i) sum[i] = a.part[(seg * 2 + (whole ? 0 : 1)) * a.D + d + i];
 #pragma unroll 4
-      for (int64_t s = s0; s < s1; ++s)
+    for (int64_t s = s0; s < s1; ++s)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) sum[i] += a.part[s * 2 * a.D + d + i];
-    }
-    __syncthreads();
-    if (wave)
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) quarter[wave - 1][lane * VEC + i] = sum[i];
-    __syncthreads();
-    if (wave == 0 && d < a.D) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) sum[i] = ((sum[i] + quarter[0][lane * VEC + i]) + quarter[1][lane * VEC + i]) + quarter[2][lane * VEC + i];
-      store_row<DT, VEC>(sum, a, id, d);
-    }
+      for (int i = 0; i < VEC; ++i) sum[i] += a.part[s * 2 * a.D + d + i];
   }
-}
-
-struct ScaleArgs {
-  const void* ids; int ids64; int64_t M, V, D;
-  const void* table; int64_t ld; const void* dy; int64_t ld_dy; float scale; float* dscale;
-};
-template <int DT, int VEC> __global__ void __launch_bounds__(256) embed_scale_grad(const ScaleArgs a) {
-  typedef typename Elem<DT>::type E;
-  const int64_t m = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (m >= a.M) return;
-  const int64_t id = load_id(a.ids, m, a.ids64);
-  float dot = 0.f;
-  if (id >= 0 && id < a.V) {
-    for (int64_t d = (int64_t)(threadIdx.x & 63) * VEC; d < a.D; d += 64 * VEC) {
-      const Pack<E, VEC> t = *reinterpret_cast<const Pack<E, VEC>*>((const E*)a.table + id * a.ld + d);
-      const Pack<E, VEC> g = *reinterpret_cast<const Pack<E, VEC>*>((const E*)a.dy + m * a.ld_dy + d);
+  if (wave)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) dot = fmaf(dec<DT>(t.v[i]), dec<DT>(g.v[i]), dot);
-    }
+    for (int i = 0; i < VEC; ++i) quarter[wave - 1][lane * VEC + i] = sum[i];
+  __syncthreads();
+  if (wave == 0 && d < a.D) {
 #pragma unroll
-    for (int o = 32; o; o >>= 1) dot += __shfl_xor(dot, o);
+    for (int i = 0; i < VEC; ++i) sum[i] = ((sum[i] + quarter[0][lane * VEC + i]) + quarter[1][lane * VEC + i]) + quarter[2][lane * VEC + i];
+    store_row<DT, VEC>(sum, a, id, d);
   }
-  if ((threadIdx.x & 63) == 0) a.dscale[m] = dot * a.scale;
 }
 
 // Elements a lane takes at once: the widest access that width, row strides and addresses allow (16 bytes at most) and that still
@@ -329,7 +351,7 @@ int pick_vec(int dtype, int64_t D, int64_t ld0, int64_t ld1, const void* p0, con
   while (v > 1 && (D % v || ld0 % v || ld1 % v || ((uintptr_t)p0 | (uintptr_t)p1) % (v * size) || D < 64 * v)) v >>= 1;
   return v;
 }
-template <template <int, int> class F, class A> void launch(int dtype, int vec, const A& a, unsigned grid, hipStream_t s) {
+template <template <int, int> class F, class A> void launch(int dtype, int vec, const A& a, dim3 grid, hipStream_t s) {
 #define GO(DT)                                                  \
   switch (vec) {                                                \
     case 1: F<DT, 1>::go(a, grid, s); break;                    \
@@ -341,12 +363,10 @@ template <template <int, int> class F, class A> void launch(int dtype, int vec, 
 #undef GO
 }
 #define KERNEL_OF(name, kernel, args) \
-  template <int DT, int VEC> struct name { static void go(const args& a, unsigned grid, hipStream_t s) { kernel<DT, VEC><<<grid, 256, 0, s>>>(a); } }
+  template <int DT, int VEC> struct name { static void go(const args& a, dim3 grid, hipStream_t s) { kernel<DT, VEC><<<grid, 256, 0, s>>>(a); } }
 KERNEL_OF(GoForward, embed_rows_out, ForwardArgs);
-KERNEL_OF(GoRows, embed_rows, BackwardArgs);
-KERNEL_OF(GoHot, embed_hot, BackwardArgs);
+KERNEL_OF(GoSums, embed_sums, BackwardArgs);
 KERNEL_OF(GoHotRows, embed_hot_rows, BackwardArgs);
-KERNEL_OF(GoScale, embed_scale_grad, ScaleArgs);
 
 int check(int64_t M, int64_t V, int64_t D, int64_t ld, int dtype) {
   if (dtype != GNET_F32 && dtype != GNET_BF16 && dtype != GNET_F16) return GNET_ERR_INVALID;
@@ -377,12 +397,11 @@ extern "C" size_t gnet_embed_workspace_bytes(int64_t M, int64_t D) {
 }
 
 extern "C" int gnet_embed_backward(const void* ids, int32_t ids64, const void* dy, int64_t ld_dy, float scale, const float* token_scale,
-                                   int64_t M, int64_t V, int64_t D, int32_t dtype, void* dtable, int32_t accumulate, void* workspace,
-                                   size_t workspace_bytes, gnet_stream_t stream) {
+                                   int64_t M, int64_t V, int64_t D, int32_t dtype, void* dtable, int32_t accumulate, const void* table,
+                                   int64_t ld_table, float* dscale, void* workspace, size_t workspace_bytes, gnet_stream_t stream) {
   clear_hip_error();
   if (const int e = check(M, V, D, ld_dy, dtype)) return e;
-  if (!dtable || (M && (!ids || !dy))) return GNET_ERR_INVALID;
-  if (M == 0 && accumulate) return GNET_OK;
+  if (!dtable || (M && (!ids || !dy)) || (dscale && M && (!table || ld_table < D))) return GNET_ERR_INVALID;
   if (M && (!workspace || workspace_bytes < gnet_embed_workspace_bytes(M, D) || ((uintptr_t)workspace & 255))) return GNET_ERR_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
   u64* keys = (u64*)workspace;
@@ -399,25 +418,18 @@ extern "C" int gnet_embed_backward(const void* ids, int32_t ids64, const void* d
       u64* t = keys; keys = other; other = t;
     }
   }
-  BackwardArgs a{keys, M, V, D, dy, ld_dy, scale, token_scale, dtable, D, accumulate, 4, part};
-  while (a.rows < MOST_ROWS && V / (2 * a.rows) >= 1024) a.rows *= 2;      // at least 1024 workgroups where the table allows it
-  const int vec = M ? pick_vec(dtype, D, ld_dy, D, dy, dtable) : pick_vec(dtype, D, D, D, dtable, dtable);
-  launch<GoRows>(dtype, vec, a, (unsigned)((V + a.rows - 1) / a.rows), s);
-  if (M > HOT) {
-    const unsigned segments = (unsigned)((M + HOT - 1) / HOT);
-    launch<GoHot>(dtype, vec, a, segments, s);
-    launch<GoHotRows>(dtype, vec, a, segments, s);
+  BackwardArgs a{keys, M, V, D, dy, ld_dy, scale, token_scale, dtable, D, accumulate, part, 0, 0, 0, ids, ids64, table, ld_table, dscale};
+  int vec = M ? pick_vec(dtype, D, ld_dy, D, dy, dtable) : pick_vec(dtype, D, D, D, dtable, dtable);
+  if (dscale && M) {
+    const int of_table = pick_vec(dtype, D, ld_table, D, table, dtable);
+    vec = of_table < vec ? of_table : vec;
   }
-  return launch_status();
-}
-
-extern "C" int gnet_embed_scale_backward(const void* ids, int32_t ids64, const void* table, int64_t ld_table, const void* dy, int64_t ld_dy,
-                                         float scale, int64_t M, int64_t V, int64_t D, int32_t dtype, float* dscale, gnet_stream_t stream) {
-  clear_hip_error();
-  if (const int e = check(M, V, D, ld_table < ld_dy ? ld_table : ld_dy, dtype)) return e;
-  if (M == 0) return GNET_OK;
-  if (!ids || !table || !dy || !dscale) return GNET_ERR_INVALID;
-  ScaleArgs a{ids, ids64, M, V, D, table, ld_table, dy, ld_dy, scale, dscale};
-  launch<GoScale>(dtype, pick_vec(dtype, D, ld_table, ld_dy, table, dy), a, (unsigned)((M + 3) / 4), (hipStream_t)stream);
+  const unsigned segments = (unsigned)((M + HOT - 1) / HOT);
+  a.run_groups = (unsigned)((M + 3) / 4);
+  a.hot_groups = M > HOT ? segments : 0;
+  a.fill_groups = accumulate ? 0 : (unsigned)((V + FILL_ROWS - 1) / FILL_ROWS);
+  const unsigned groups = a.run_groups + a.hot_groups + a.fill_groups + (dscale ? a.run_groups : 0);
+  if (groups) launch<GoSums>(dtype, vec, a, groups, s);
+  if (M > HOT) launch<GoHotRows>(dtype, vec, a, dim3(segments, (unsigned)((D + 64 * vec - 1) / (64 * vec))), s);
   return launch_status();
 }

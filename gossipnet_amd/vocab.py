@@ -120,16 +120,12 @@ def embed_backward(ids, dy, table, scale=1.0, token_scale=None, need_dscale=Fals
     dtable = out.detach() if out is not None else torch.empty(V, D, dtype=t.dtype, device=dev)
     M = i.numel()
     lib = _lib.load()
+    dscale = torch.empty(tuple(ids.shape), dtype=torch.float32, device=dev) if need_dscale else None
     with torch.cuda.device(dev):
         nbytes = lib.gnet_embed_workspace_bytes(M, D)
         buf, ws = _workspace(nbytes, dev)
         _lib.check(lib.gnet_embed_backward(_p(i), int(i.dtype == torch.int64), _p(g), _ld(g), float(scale), _p(s), M, V, D, _TYPES[t.dtype],
-                                           _p(dtable), int(out is not None), ws, nbytes, _stream(dev)), "gnet_embed_backward")
-        dscale = None
-        if need_dscale:
-            dscale = torch.empty(tuple(ids.shape), dtype=torch.float32, device=dev)
-            _lib.check(lib.gnet_embed_scale_backward(_p(i), int(i.dtype == torch.int64), _p(t), _ld(t), _p(g), _ld(g), float(scale), M, V, D,
-                                                     _TYPES[t.dtype], _p(dscale), _stream(dev)), "gnet_embed_scale_backward")
+                                           _p(dtable), int(out is not None), _p(t), _ld(t), _p(dscale), ws, nbytes, _stream(dev)), "gnet_embed_backward")
     return (out if out is not None else dtable), dscale
 
 

@@ -313,14 +313,12 @@ int gnet_embed_forward(const void* ids, int32_t ids64, const void* table, int64_
                        int64_t M, int64_t V, int64_t D, int32_t dtype, void* y, gnet_stream_t stream);
 /* dtable [V,D] = scale * sum over the tokens with id v, in token order, of token_scale[m] * dy[m]: overwritten (rows without a token
  * are zero), or, with accumulate != 0, added to (the sum is added in fp32 and rounded once; rows without a token are not touched).
- * Reproducible: no atomics.  workspace: gnet_embed_workspace_bytes(M, D). */
+ * dscale (NULL: not needed): [M] = scale * dy[m] . table[ids[m]], the gradient of token_scale; zero where the id is outside [0, V); it
+ * alone reads table.  Reproducible: no atomics.  workspace: gnet_embed_workspace_bytes(M, D). */
 size_t gnet_embed_workspace_bytes(int64_t M, int64_t D);
 int gnet_embed_backward(const void* ids, int32_t ids64, const void* dy, int64_t ld_dy, float scale, const float* token_scale, int64_t M,
-                        int64_t V, int64_t D, int32_t dtype, void* dtable, int32_t accumulate, void* workspace,
-                        size_t workspace_bytes, gnet_stream_t stream);
-/* dscale[m] = scale * dy[m] . table[ids[m]] (the gradient of token_scale); zero where the id is outside [0, V). */
-int gnet_embed_scale_backward(const void* ids, int32_t ids64, const void* table, int64_t ld_table, const void* dy, int64_t ld_dy,
-                              float scale, int64_t M, int64_t V, int64_t D, int32_t dtype, float* dscale, gnet_stream_t stream);
+                        int64_t V, int64_t D, int32_t dtype, void* dtable, int32_t accumulate, const void* table, int64_t ld_table,
+                        float* dscale, void* workspace, size_t workspace_bytes, gnet_stream_t stream);
 
 /* Softmax cross entropy of z = x . w^T (x [M,D], w [V,D]) against labels [M], without laying z out:
  *   lse[m] = log sum_v exp z[m,v]     hit[m] = z[m,labels[m]]     loss[m] = lse[m] - hit[m] (never below 0)

@@ -105,16 +105,15 @@ def test_c_entries_refuse_before_they_launch():
         assert distill(**a) == _lib.ERR_INVALID, a
     assert distill(K=1025) == _lib.ERR_UNSUPPORTED
 
-    def embed(ids=p, ld=8, M=4, V=10, D=8, dtype=BF16, out=p, ws=p, n=1 << 30):
-        return lib.gnet_embed_backward(ids, 0, p, ld, 1.0, None, M, V, D, dtype, out, 0, ws, n, None)
-    for a in (dict(M=-1), dict(V=0), dict(D=0), dict(ld=7), dict(dtype=-1), dict(ids=None), dict(out=None)):
+    def embed(ids=p, ld=8, M=4, V=10, D=8, dtype=BF16, out=p, table=p, ld_table=8, dscale=p, ws=p, n=1 << 30):
+        return lib.gnet_embed_backward(ids, 0, p, ld, 1.0, None, M, V, D, dtype, out, 0, table, ld_table, dscale, ws, n, None)
+    for a in (dict(M=-1), dict(V=0), dict(D=0), dict(ld=7), dict(dtype=-1), dict(ids=None), dict(out=None), dict(table=None), dict(ld_table=7)):
         assert embed(**a) == _lib.ERR_INVALID, a
     for a in (dict(ws=None), dict(n=8), dict(ws=odd)):
         assert embed(**a) == _lib.ERR_WORKSPACE, a
     assert lib.gnet_embed_forward(p, 0, p, 7, 1.0, None, 4, 10, 8, BF16, p, None) == _lib.ERR_INVALID
     assert lib.gnet_embed_forward(None, 0, p, 8, 1.0, None, 4, 10, 8, BF16, p, None) == _lib.ERR_INVALID
     assert lib.gnet_embed_forward(None, 0, None, 8, 1.0, None, 0, 10, 8, BF16, None, None) == _lib.OK
-    assert lib.gnet_embed_scale_backward(p, 0, p, 8, p, 7, 1.0, 4, 10, 8, BF16, p, None) == _lib.ERR_INVALID
 
 
 def test_workspaces_do_not_grow_with_the_logits():
