@@ -18,7 +18,7 @@ constexpr unsigned NONE = 0xffffffffu;      // id of a token that is left out: s
 constexpr int RUN = 4096;          // tokens sorted by one workgroup: 32 KB of keys
 constexpr int WAY = 16;            // runs joined by one merge pass
 constexpr int HOT = 16;            // tokens a row's own wave adds up
-constexpr int BLOCKS = 4;          // column blocks of 64 * VEC elements a wave keeps sums of
+constexpr int BLOCKS = 2;          // column blocks of 64 * VEC elements a wave keeps sums of
 constexpr int FILL_ROWS = 64;      // table rows a workgroup looks for and fills with zeros
 
 template <int DT> struct Elem { typedef u16 type; };
@@ -166,25 +166,25 @@ struct BackwardArgs {
   const void* dy; int64_t ld; float scale; const float* token_scale;
   void* out; int64_t ld_out; int accumulate;
   float* part;                         // [segment][2][D]
-  unsigned run_groups, hot_groups, fill_groups;      // workgroups of each kind, in this order; d s gets the rest
+  unsigned hot_groups, run_groups, scale_groups;     // workgroups of each kind, in this order; the zero rows get the rest
   const void* ids; int ids64; const void* table; int64_t ld_table; float* dscale;
 };
 
-// sums of the tokens [lo, hi) of the sorted order, in order, over `blocks` <= NB column blocks `step` elements apart from column d on;
-// U tokens' rows are on the way at a time
-template <int DT, int VEC, int U, int NB> __device__ __forceinline__ void add_tokens(float (&sum)[NB][VEC], const BackwardArgs& a, int64_t lo, int64_t hi, int64_t d, int step, int blocks) {
+// Sums over tokens held by the wave's lanes [lo, hi), in order, for `blocks` <= NB column blocks `step` elements apart from column d on;
+// U tokens' rows are on the way at a time.
+template <int DT, int VEC, int U, int NB> __device__ __forceinline__ void add_tokens(float (&sum)[NB][VEC], const BackwardArgs& a, int token, int lo, int hi, int64_t d, int step, int blocks) {
   typedef typename Elem<DT>::type E;
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int i = 0; i < VEC; ++i) sum[b][i] = 0.f;
-  for (int64_t j = lo; j < hi; j += U) {
+  for (int j = lo; j < hi; j += U) {
     Pack<E, VEC> g[U][NB];
     float s[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (j + u >= hi) continue;
-      const int64_t m = (int64_t)(a.keys[j + u] & 0xffffffffull);
+      const int64_t m = __builtin_amdgcn_readlane(token, j + u);
       s[u] = a.token_scale ? a.token_scale[m] : 1.f;
 #pragma unroll
       for (int b = 0; b < NB; ++b)
@@ -211,27 +211,30 @@ template <int DT, int VEC> __device__ __forceinline__ void store_row(const float
   *p = o;
 }
 
-__device__ __forceinline__ unsigned id_at(const u64* keys, int64_t i) { return (unsigned)(keys[i] >> 32); }
-// does the run of `id` over place p have more than HOT tokens: are two of them HOT places apart, around p
-__device__ __forceinline__ bool hot_around(const u64* keys, int64_t M, int64_t p, unsigned id) {
-  const int64_t b = p - HOT + (threadIdx.x & 63), e = b + HOT;
-  return __any((threadIdx.x & 63) <= HOT && b >= 0 && e < M && id_at(keys, b) == id && id_at(keys, e) == id);
+// 64 consecutive keys from place p on, one a lane: id (NONE outside the order) and token
+__device__ __forceinline__ void load_keys(const BackwardArgs& a, int64_t p, unsigned& id, int& token) {
+  const int64_t i = p + (threadIdx.x & 63);
+  const u64 key = i >= 0 && i < a.M ? a.keys[i] : ~0ull;
+  id = (unsigned)(key >> 32);
+  token = (int)(unsigned)key;
 }
 
 // A wave per place of the sorted order: where a run of at most HOT tokens starts, its sum.
-template <int DT, int VEC> __device__ __forceinline__ void run_sums(const BackwardArgs& a, int64_t i) {
-  if (i >= a.M) return;
-  const int lane = threadIdx.x & 63;
-  const unsigned id = id_at(a.keys, i);
-  if (id == NONE || (i > 0 && id_at(a.keys, i - 1) == id)) return;
-  const bool same = lane <= HOT && i + lane < a.M && id_at(a.keys, min(i + lane, a.M - 1)) == id;
-  const int n = __popcll(__ballot(same));                    // (equal ids are next to each other)
+template <int DT, int VEC> __device__ __forceinline__ void run_sums(const BackwardArgs& a, int64_t p) {
+  if (p >= a.M) return;
+  unsigned ids;
+  int token;
+  load_keys(a, p - 1, ids, token);                           // lane 0: the place in front
+  const unsigned id = __builtin_amdgcn_readlane(ids, 1);
+  if (id == NONE || (p > 0 && (unsigned)__builtin_amdgcn_readlane(ids, 0) == id)) return;
+  const int n = __popcll(__ballot(ids == id));               // (equal ids are next to each other)
   if (n > HOT) return;
+  const int lane = threadIdx.x & 63;
   for (int64_t d0 = 0; d0 < a.D; d0 += BLOCKS * 64 * VEC) {
     const int blocks = (int)min((int64_t)BLOCKS, (a.D - d0 + 64 * VEC - 1) / (64 * VEC));
     const int64_t d = d0 + lane * VEC;
     float sum[BLOCKS][VEC];
-    add_tokens<DT, VEC, 4, BLOCKS>(sum, a, i, i + n, d, 64 * VEC, blocks);
+    add_tokens<DT, VEC, 4, BLOCKS>(sum, a, token, 1, 1 + n, d, 64 * VEC, blocks);
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b)
       if (b < blocks && d + b * 64 * VEC < a.D) store_row<DT, VEC>(sum[b], a, id, d + b * 64 * VEC);
@@ -239,21 +242,27 @@ template <int DT, int VEC> __device__ __forceinline__ void run_sums(const Backwa
 }
 
 // The runs of more than HOT equal ids: a segment of HOT sorted tokens meets at most two, one that comes in over its first token
-// (slot 0: also a run that starts right there and leaves) and one that leaves over its last (slot 1).
+// (slot 0: also a run that starts right there and leaves) and one that leaves over its last (slot 1).  A run that crosses a border of
+// the segment has more than HOT tokens if the HOT places on either side of it hold that many.
+static_assert(3 * HOT <= 64, "a segment and its neighbours are a wave's keys");
 template <int DT, int VEC> __device__ __forceinline__ void hot_sums(const BackwardArgs& a, int64_t seg) {
-  const int64_t lo = seg * HOT, hi = min(a.M, lo + HOT);
-  const unsigned first = id_at(a.keys, lo), last = id_at(a.keys, hi - 1);
-  const bool leaves = last != NONE && hi < a.M && id_at(a.keys, hi) == last;
-  const bool in = first != NONE && lo > 0 && id_at(a.keys, lo - 1) == first;
+  const int64_t lo = seg * HOT;
+  unsigned ids;
+  int token;
+  load_keys(a, lo - HOT, ids, token);                        // lanes HOT .. 2 HOT - 1: the segment
+  const int end = (int)min((int64_t)HOT, a.M - lo) + HOT;
+  const unsigned first = __builtin_amdgcn_readlane(ids, HOT), last = __builtin_amdgcn_readlane(ids, end - 1);
+  const bool in = first != NONE && (unsigned)__builtin_amdgcn_readlane(ids, HOT - 1) == first;
+  const bool leaves = last != NONE && (unsigned)__builtin_amdgcn_readlane(ids, end) == last;
   for (int slot = 0; slot < 2; ++slot) {
     const unsigned id = slot ? last : first;
     if (slot ? !(leaves && first != last) : !(in || (leaves && first == last))) continue;
-    if (!hot_around(a.keys, a.M, slot || !in ? hi : lo, id)) continue;
-    int64_t b = lo, e = hi;
-    if (slot) { while (id_at(a.keys, b) != id) ++b; } else { while (id_at(a.keys, e - 1) != id) --e; }
+    const u64 run = __ballot(ids == id);                     // the run as far as these keys show it
+    if (__popcll(run) <= HOT) continue;
+    const int b = max(HOT, (int)__builtin_ctzll(run)), e = min(end, 64 - (int)__builtin_clzll(run));
     for (int64_t d = (int64_t)threadIdx.x * VEC; d < a.D; d += 256 * VEC) {
       float sum[1][VEC];
-      add_tokens<DT, VEC, HOT, 1>(sum, a, b, e, d, 0, 1);
+      add_tokens<DT, VEC, 8, 1>(sum, a, token, b, e, d, 0, 1);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) a.part[(seg * 2 + slot) * a.D + d + i] = sum[0][i];
     }
@@ -297,25 +306,28 @@ template <int DT, int VEC> __global__ void __launch_bounds__(256) embed_sums(con
   __shared__ int64_t start[FILL_ROWS + 1];
   unsigned g = blockIdx.x;
   const int wave = threadIdx.x >> 6;
-  if (g < a.run_groups) return run_sums<DT, VEC>(a, (int64_t)g * 4 + wave);
-  g -= a.run_groups;
   if (g < a.hot_groups) return hot_sums<DT, VEC>(a, g);
   g -= a.hot_groups;
-  if (g < a.fill_groups) return fill_rows<DT, VEC>(a, g, start);
-  scale_gradient<DT, VEC>(a, (int64_t)(g - a.fill_groups) * 4 + wave);
+  if (g < a.run_groups) return run_sums<DT, VEC>(a, (int64_t)g * 4 + wave);
+  g -= a.run_groups;
+  if (g < a.scale_groups) return scale_gradient<DT, VEC>(a, (int64_t)g * 4 + wave);
+  fill_rows<DT, VEC>(a, g - a.scale_groups, start);
 }
 
 // The segment in which a hot run starts adds the run's partial sums, a workgroup per column block: each wave a quarter of them in order,
 // then the quarters in order.
 template <int DT, int VEC> __global__ void __launch_bounds__(256) embed_hot_rows(const BackwardArgs a) {
   __shared__ float quarter[3][64 * VEC];
-  const int64_t seg = blockIdx.x, lo = seg * HOT, hi = min(a.M, lo + HOT);
+  const int64_t seg = blockIdx.x, lo = seg * HOT, hi = lo + HOT;
   if (hi >= a.M) return;
-  const unsigned id = id_at(a.keys, hi - 1);
-  if (id == NONE || id_at(a.keys, hi) != id) return;                     // no run leaves this segment
-  const bool whole = id_at(a.keys, lo) == id;
-  if (whole && lo > 0 && id_at(a.keys, lo - 1) == id) return;            // it started earlier
-  if (!hot_around(a.keys, a.M, hi, id)) return;                          // run_sums has it
+  unsigned ids;
+  int token;
+  load_keys(a, lo - HOT, ids, token);
+  const unsigned id = __builtin_amdgcn_readlane(ids, 2 * HOT - 1);
+  if (id == NONE || (unsigned)__builtin_amdgcn_readlane(ids, 2 * HOT) != id) return;         // no run leaves this segment
+  const bool whole = (unsigned)__builtin_amdgcn_readlane(ids, HOT) == id;
+  if (whole && (unsigned)__builtin_amdgcn_readlane(ids, HOT - 1) == id) return;              // it started earlier
+  if (__popcll(__ballot(ids == id)) <= HOT) return;                                          // run_sums has it
   const int64_t n = (lower_bound(a.keys, hi, a.M, ((u64)id + 1) << 32) - 1) / HOT - seg;      // segments behind this one
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t s0 = seg + 1 + n * wave / 4, s1 = seg + 1 + n * (wave + 1) / 4;
@@ -425,10 +437,10 @@ extern "C" int gnet_embed_backward(const void* ids, int32_t ids64, const void* d
     vec = of_table < vec ? of_table : vec;
   }
   const unsigned segments = (unsigned)((M + HOT - 1) / HOT);
-  a.run_groups = (unsigned)((M + 3) / 4);
   a.hot_groups = M > HOT ? segments : 0;
-  a.fill_groups = accumulate ? 0 : (unsigned)((V + FILL_ROWS - 1) / FILL_ROWS);
-  const unsigned groups = a.run_groups + a.hot_groups + a.fill_groups + (dscale ? a.run_groups : 0);
+  a.run_groups = (unsigned)((M + 3) / 4);
+  a.scale_groups = dscale ? a.run_groups : 0;
+  const unsigned groups = a.hot_groups + a.run_groups + a.scale_groups + (accumulate ? 0 : (unsigned)((V + FILL_ROWS - 1) / FILL_ROWS));
   if (groups) launch<GoSums>(dtype, vec, a, groups, s);
   if (M > HOT) launch<GoHotRows>(dtype, vec, a, dim3(segments, (unsigned)((D + 64 * vec - 1) / (64 * vec))), s);
   return launch_status();
