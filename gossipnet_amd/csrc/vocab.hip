@@ -554,18 +554,18 @@ int check(const Problem& q) {
 }
 
 template <int DT, class T, int PLANES> struct Run {
-  template <int BM, int BN, int WM, int WN, bool AS, bool BS, int EPI> static void launch(VocabGemm& g, int64_t rows, int64_t cols, int splits, hipStream_t s) {
+  template <int BM, int BN, int WM, int WN, int STAGES, bool AS, bool BS, int EPI> static void launch(VocabGemm& g, int64_t rows, int64_t cols, int splits, hipStream_t s) {
     g.row_tiles = (int)tiles(rows, BM); g.col_tiles = (int)tiles(cols, BN); g.splits = splits;
-    vocab_gemm<T, BM, BN, WM, WN, AS, BS, EPI, PLANES><<<(unsigned)((int64_t)g.row_tiles * g.col_tiles * splits), 64 * WM * WN, 0, s>>>(g);
+    vocab_gemm<T, BM, BN, WM, WN, STAGES, AS, BS, EPI, PLANES><<<(unsigned)((int64_t)g.row_tiles * g.col_tiles * splits), 64 * WM * WN, 0, s>>>(g);
   }
   // columns are tokens (all shapes) or vocabulary (the square ones)
   template <bool AS, bool BS, int EPI> static void gemm(VocabGemm& g, const Product& p, int64_t rows, int64_t cols, hipStream_t s) {
-    if (p.shape == S256) return launch<256, 256, 2, 4, AS, BS, EPI>(g, rows, cols, p.splits, s);
+    if (p.shape == S256) return launch<256, 256, 2, 4, 2, AS, BS, EPI>(g, rows, cols, p.splits, s);
     if constexpr (!BS) {
-      if (p.shape == S64) return launch<128, 64, 4, 1, AS, BS, EPI>(g, rows, cols, p.splits, s);
-      if (p.shape == S32) return launch<128, 32, 4, 1, AS, BS, EPI>(g, rows, cols, p.splits, s);
+      if (p.shape == S64) return launch<128, 64, 4, 1, 2, AS, BS, EPI>(g, rows, cols, p.splits, s);
+      if (p.shape == S32) return launch<128, 32, 4, 1, 2, AS, BS, EPI>(g, rows, cols, p.splits, s);
     }
-    launch<128, 128, 2, 2, AS, BS, EPI>(g, rows, cols, p.splits, s);
+    launch<128, 128, 2, 2, 2, AS, BS, EPI>(g, rows, cols, p.splits, s);
   }
 
   static PackW pack_of_w(const Problem& q, const Plan& p, char* ws, int64_t v0) {

@@ -10,6 +10,7 @@
 // dropped or rounded is below 3 x 2^-24 of |a||b|, plus 2^-39 of the tensors' largest magnitudes where lo is subnormal.
 #pragma once
 #include "common.hpp"
+#include <type_traits>
 
 typedef unsigned short u16;
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -45,7 +46,7 @@ struct VocabMeta {
   float unscale_g;     // one unit of the stored dz
 };
 
-constexpr int VG_BK = 64;      // contraction step
+constexpr int VG_BK = 64;      // contraction elements of a stage; contractions are a multiple of it
 
 struct VocabOperand {
   const u16* p;        // first element (of plane 0)
@@ -81,11 +82,11 @@ enum { EPI_PART = 0, EPI_DZ = 1, EPI_SLAB = 2, EPI_OUT = 3 };
 
 // ---- staging of one operand tile, 16 bytes per lane straight into LDS ------------------------------------------------
 // Contraction-contiguous (STRIDED = false): LDS [T rows][64 k], 128 bytes a row; the 16-byte chunk c of row r lies at position
-// c ^ (r & 7), so that the 16 rows of a fragment read cover all banks.
+// c ^ (r & 7), so that the rows a fragment read touches at once cover all banks.  (Rows of 32 k, loaded 64 bytes at a time, cost 5 %.)
 // Contraction-strided: LDS [64 k][T columns]; the 32-byte granule g of row k lies at g ^ h(k), so that the rows a transposing
-// read touches at once lie in different banks.
+// read touches at once lie in different banks.  (h(k + 4) = h(k) for k < 4 modulo 8, h(k + 32) = h(k).)
 template <int T> __device__ __forceinline__ int granule_swizzle(int k) {
-  return T >= 256 ? ((k & 3) | ((k >> 1) & 12)) : T >= 128 ? ((k & 3) | ((k >> 1) & 4)) : (k & (T / 16 - 1));
+  return T >= 256 ? ((k & 3) | ((k >> 1) & 12)) : ((k & 3) | ((k >> 1) & 4));
 }
 
 // 64 lanes x 16 bytes from base + off (bytes, per lane) to 1 KB of LDS.  As a statement of its own: the compiler would order the builtin's
@@ -94,20 +95,25 @@ template <int T> __device__ __forceinline__ int granule_swizzle(int k) {
 __device__ __forceinline__ void load_to_lds(const char* base, unsigned off, unsigned lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
 }
+__device__ __forceinline__ void load_to_lds(const char* from, unsigned lds) {      // every lane's own address
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory");
+}
 __device__ __forceinline__ unsigned lds_address(const void* p) {
   return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
 
-// A wave's share of one operand's tiles: OPS / WAVES loads of 1 KB a step, their lanes' byte offsets from the tile's first row (contraction-
-// contiguous) or the step's first row (contraction-strided) kept in registers.
+// A wave's share of one operand's stages: N loads of 1 KB, their lanes' byte offsets from the tile's first row (contraction-contiguous)
+// or the stage's first row (contraction-strided) kept in registers.  (Fewer kilobytes than waves: some are loaded twice, so that
+// every wave has the same number of loads on the way.)
 template <int T, bool STRIDED, int WAVES> struct Stager {
-  static constexpr int OPS = T * VG_BK * 2 / 1024, N = OPS / WAVES, CH = T / 8;      // CH: 16-byte chunks a strided row
-  static_assert(OPS % WAVES == 0, "a wave loads whole kilobytes");
+  static constexpr int OPS = T * VG_BK * 2 / 1024, N = OPS < WAVES ? 1 : OPS / WAVES, CH = T / 8;      // CH: 16-byte chunks a strided row
+  static_assert(OPS % WAVES == 0 || WAVES % OPS == 0, "whole kilobytes");
   const char* base;
   unsigned off[N];
   int64_t step_bytes, rows;
   unsigned row_bytes;
 
+  static __device__ __forceinline__ int op(int u, int wave) { return (u * WAVES + wave) % OPS; }
   __device__ __forceinline__ void init(const VocabOperand& o, int64_t t0, int64_t k0, int wave, int lane) {
     row_bytes = (unsigned)(o.ld * 2);
     rows = o.rows;
@@ -116,7 +122,7 @@ template <int T, bool STRIDED, int WAVES> struct Stager {
       step_bytes = VG_BK * 2;
 #pragma unroll
       for (int u = 0; u < N; ++u) {
-        const int r = (u * WAVES + wave) * 8 + (lane >> 3), c = (lane & 7) ^ (r & 7);
+        const int r = op(u, wave) * 8 + (lane >> 3), c = (lane & 7) ^ (r & 7);
         off[u] = (unsigned)min((int64_t)r, rows - 1 - t0) * row_bytes + c * 16;
       }
     } else {
@@ -124,45 +130,47 @@ template <int T, bool STRIDED, int WAVES> struct Stager {
       step_bytes = VG_BK * o.ld * 2;
 #pragma unroll
       for (int u = 0; u < N; ++u) {
-        const int idx = (u * WAVES + wave) * 64 + lane, r = idx / CH, p = idx % CH;
+        const int idx = op(u, wave) * 64 + lane, r = idx / CH, p = idx % CH;
         const int c = (((p >> 1) ^ granule_swizzle<T>(r)) << 1) | (p & 1);
         off[u] = r * row_bytes + (unsigned)min(t0 + c * 8, (int64_t)o.cols - 8) * 2;
       }
     }
   }
-  // step s counted from k0, at its byte offset `plane` further on
-  __device__ __forceinline__ void load(unsigned lds, int s, int64_t k, int64_t plane, int wave, int lane) const {
+  // stage s counted from k0, whose contraction index is k, `plane` bytes further on; CLAMP: the rows may end inside or in front of it
+  template <bool CLAMP> __device__ __forceinline__ void load(unsigned lds, int s, int64_t k, int64_t plane, int wave, int lane) const {
     const char* from = base + s * step_bytes + plane;
-    if (STRIDED && k + VG_BK > rows) {                    // the last rows end inside this step
-      const unsigned last = (unsigned)(rows - 1 - k);
 #pragma unroll
-      for (int u = 0; u < N; ++u) {
-        const unsigned r = ((u * WAVES + wave) * 64 + lane) / CH;
-        load_to_lds(from, off[u] - (r > last ? r - last : 0) * row_bytes, lds + (u * WAVES + wave) * 1024);
-      }
-    } else {
-#pragma unroll
-      for (int u = 0; u < N; ++u) load_to_lds(from, off[u], lds + (u * WAVES + wave) * 1024);
+    for (int u = 0; u < N; ++u) {
+      const unsigned to = lds + op(u, wave) * 1024;
+      if (!CLAMP) { load_to_lds(from, off[u], to); continue; }
+      const int64_t beyond = STRIDED ? max(k + (op(u, wave) * 64 + lane) / CH - (rows - 1), (int64_t)0) : 0;
+      load_to_lds(from + off[u] - beyond * row_bytes, to);
     }
   }
 };
 
-// One 16 x 32 fragment: lane l gets row t + (l & 15), contraction elements 32 s + 8 (l >> 4) .. + 7.
-template <int T, bool STRIDED>
-__device__ __forceinline__ s16x8 read_frag(const char* lds, int t, int s, int lane) {
-  if (!STRIDED) {
-    const int r = t + (lane & 15), c = s * 4 + (lane >> 4);
-    return *reinterpret_cast<const s16x8*>(lds + r * 128 + ((c ^ (r & 7)) << 4));
-  } else {
-    const int i = lane & 15, k = s * 32 + (lane >> 4) * 8 + (i >> 2);
-    const int g = t >> 4;
-    const char* p0 = lds + k * (T * 2) + ((g ^ granule_swizzle<T>(k)) << 5) + (i & 3) * 8;
-    const char* p1 = lds + (k + 4) * (T * 2) + ((g ^ granule_swizzle<T>(k + 4)) << 5) + (i & 3) * 8;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p0);
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p1);
+// 16 x 32 fragments: lane l gets row t + (l & 15), contraction elements 32 half + 8 (l >> 4) .. + 7 of the stage, t = 16 (first + i).
+template <int T, bool STRIDED, int F> struct Fragments {
+  int at[STRIDED ? F : 2];
+  __device__ __forceinline__ void init(int first, int lane) {
+    const int i = lane & 15, quad = lane >> 4;
+    if (!STRIDED) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) at[half] = (first * 16 + i) * (VG_BK * 2) + (((half * 4 + quad) ^ (i & 7)) << 4);
+    } else {
+      const int k = quad * 8 + (i >> 2);
+#pragma unroll
+      for (int f = 0; f < F; ++f) at[f] = k * (T * 2) + (((first + f) ^ granule_swizzle<T>(k)) << 5) + (i & 3) * 8;
+    }
+  }
+  __device__ __forceinline__ s16x8 read(const char* lds, int f, int half) const {
+    if (!STRIDED) return *reinterpret_cast<const s16x8*>(lds + at[half] + f * 16 * VG_BK * 2);
+    typedef __attribute__((address_space(3))) s16x4* Lds;
+    const char* p = lds + at[f] + half * 32 * T * 2;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)p), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(p + 4 * T * 2));
     return s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   }
-}
+};
 
 // Workgroups are dealt to the eight XCDs in turn: give every XCD a contiguous share of the tiles, and within it run through four
 // row tiles at a time, so that the 32 workgroups that an XCD works on at once share four row panels and eight column panels in its L2.
@@ -176,10 +184,13 @@ __device__ __forceinline__ void tile_of(int id, int row_tiles, int col_tiles, in
   rt = group * 4 + (left - ct * h);
 }
 
-template <class T, int BM, int BN, int WM, int WN, bool A_STRIDED, bool B_STRIDED, int EPI, int PLANES>
+// The pipeline, per stage of 64 contraction elements in two halves: the products of a half run from registers while the next half is
+// read from LDS into the other set of registers, and while the following stages are on their way from memory.  One barrier a stage, in its
+// middle: behind it the next stage is there for every wave, and nobody reads this stage any more, whose place is loaded next.
+template <class T, int BM, int BN, int WM, int WN, int STAGES, bool A_STRIDED, bool B_STRIDED, int EPI, int PLANES>
 __global__ void __launch_bounds__(64 * WM * WN, 2) vocab_gemm(const VocabGemm g) {
   constexpr int WAVES = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16, STAGE = (BM + BN) * VG_BK * 2;
-  __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
+  __shared__ __attribute__((aligned(16))) char lds[STAGES * STAGE];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
   int rt, ct, split;
@@ -189,7 +200,8 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) vocab_gemm(const VocabGemm g)
   // (the last step of a contraction over tokens reads dz up to the next multiple of its length)
   if (g.cols_from_meta && c0 >= ((rows + VG_BK - 1) & ~(VG_BK - 1))) return;
   const int64_t k_all = g.k_from_meta ? (int64_t)((rows + VG_BK - 1) / VG_BK) * VG_BK : g.k;
-  const int steps = (int)(k_all / VG_BK), s0 = (int)((int64_t)steps * split / g.splits), s1 = (int)((int64_t)steps * (split + 1) / g.splits);
+  const int64_t steps = k_all / VG_BK, k0 = steps * split / g.splits * VG_BK, k1 = steps * (split + 1) / g.splits * VG_BK;
+  const int per_segment = (int)((k1 - k0) / VG_BK), n = per_segment * (PLANES == 1 ? 1 : 3);
 
   f32x4 acc[FM][FN];
 #pragma unroll
@@ -197,40 +209,83 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) vocab_gemm(const VocabGemm g)
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  // one step's loads are in flight while the step before is multiplied; one barrier a step: behind it the step's tiles are there and
-  // the other buffer is no longer read
-  const int n = (s1 - s0) * (PLANES == 1 ? 1 : 3);
   Stager<BM, A_STRIDED, WAVES> sa;
   Stager<BN, B_STRIDED, WAVES> sb;
-  sa.init(g.a, r0, (int64_t)s0 * VG_BK, wave, lane);
-  sb.init(g.b, c0, (int64_t)s0 * VG_BK, wave, lane);
+  sa.init(g.a, r0, k0, wave, lane);
+  sb.init(g.b, c0, k0, wave, lane);
+  Fragments<BM, A_STRIDED, FM> ra;
+  Fragments<BN, B_STRIDED, FN> rb;
+  ra.init(wm * FM, lane);
+  rb.init(wn * FN, lane);
   const unsigned lds0 = lds_address(lds);
-  auto stage = [&](int it) {
-    const int seg = PLANES == 1 ? 0 : it / (s1 - s0), s = it - seg * (s1 - s0);
-    const unsigned to = lds0 + (it & 1) * STAGE;
-    const int64_t k = (int64_t)(s0 + s) * VG_BK;                                       // segments: lo.hi, hi.lo, hi.hi
-    sa.load(to, s, k, PLANES == 1 || seg != 0 ? 0 : g.a.plane * 2, wave, lane);
-    sb.load(to + BM * VG_BK * 2, s, k, PLANES == 1 || seg != 1 ? 0 : g.b.plane * 2, wave, lane);
+  constexpr int LOADS = Stager<BM, A_STRIDED, WAVES>::N + Stager<BN, B_STRIDED, WAVES>::N;        // a wave's, per stage
+  int place = 0, loaded = 0;                           // where the next stage goes, and which one it is
+  auto load = [&](auto clamp) {
+    const unsigned to = lds0 + place * STAGE;
+    // segments: lo.hi, hi.lo, hi.hi (in integers: selects by a condition end up in vector registers)
+    const int first = PLANES == 1 ? -1 : (loaded - per_segment) >> 31, second = PLANES == 1 ? -1 : (loaded - 2 * per_segment) >> 31;
+    const int s = PLANES == 1 ? loaded : loaded - (per_segment & ~first) - (per_segment & ~second);
+    const int64_t k = k0 + (int64_t)s * VG_BK;
+    sa.template load<decltype(clamp)::value>(to, s, k, PLANES == 1 ? 0 : g.a.plane * 2 & (int64_t)first, wave, lane);
+    sb.template load<decltype(clamp)::value>(to + BM * VG_BK * 2, s, k, PLANES == 1 ? 0 : g.b.plane * 2 & (int64_t)(second & ~first), wave, lane);
+    place = place + 1 == STAGES ? 0 : place + 1;
+    ++loaded;
   };
-  if (n > 0) stage(0);
-  for (int it = 0; it < n; ++it) {
-    // (the reads of the step before have returned: their buffer is written next.  As one statement with a memory clobber, so that the
-    // compiler moves no LDS access across it; it keeps no loads in flight that this wait would not cover.)
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (it + 1 < n) stage(it + 1);
-    const char* const la = lds + (it & 1) * STAGE;
-    const char* const lb = la + BM * VG_BK * 2;
+  // The wave's LDS reads have returned (as a builtin, which the compiler counts); at most `stages` stages' loads are still on their way;
+  // everybody is here.  With a memory clobber, so that the compiler moves no LDS access across it; it keeps no loads of its own in
+  // flight here.
+  auto sync = [&](auto stages) {
+    __builtin_amdgcn_s_waitcnt(0xC07F);                // lgkmcnt(0)
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(LOADS * decltype(stages)::value) : "memory");
+  };
+  typedef std::integral_constant<int, STAGES - 1> Others;
+  typedef std::integral_constant<int, STAGES - 2> Later;
+  typedef std::integral_constant<int, 0> None;
+  s16x8 fa[2][FM], fb[2][FN];
+  int from = 0;
+  auto read = [&](int half) {
+    const char* const la = lds + from * STAGE;
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      s16x8 fa[FM], fb[FN];
+    for (int j = 0; j < FN; ++j) fb[half][j] = rb.read(la + BM * VG_BK * 2, j, half);
 #pragma unroll
-      for (int j = 0; j < FN; ++j) fb[j] = read_frag<BN, B_STRIDED>(lb, (wn * FN + j) * 16, ks, lane);
+    for (int i = 0; i < FM; ++i) fa[half][i] = ra.read(la, i, half);
+  };
+  auto multiply = [&](int h) {
 #pragma unroll
-      for (int i = 0; i < FM; ++i) fa[i] = read_frag<BM, A_STRIDED>(la, (wm * FM + i) * 16, ks, lane);
+    for (int i = 0; i < FM; ++i)
 #pragma unroll
-      for (int i = 0; i < FM; ++i)
+      for (int j = 0; j < FN; ++j) acc[i][j] = T::mma(fa[h][i], fb[h][j], acc[i][j]);
+    // the next half's LDS reads go between the first products, one by one
+    constexpr int READS = FM * (A_STRIDED ? 2 : 1) + FN * (B_STRIDED ? 2 : 1), EACH = (READS + FM * FN - 1) / (FM * FN), GROUPS = (READS + EACH - 1) / EACH;
 #pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = T::mma(fa[i], fb[j], acc[i][j]);
+    for (int i = 0; i < GROUPS; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, EACH, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, FM * FN - GROUPS, 0);
+  };
+  auto next = [&] { from = from + 1 == STAGES ? 0 : from + 1; };
+  if (n > 0) {
+    for (int i = 0; i < STAGES && i < n; ++i) load(std::true_type());
+    if (n < STAGES) sync(None()); else sync(Others());       // stage 0 is there
+    read(0);
+    int it = 0;
+    for (; it + STAGES + 1 < n; ++it) {                      // (the last stage of the contraction may end early: not loaded here)
+      read(1);
+      multiply(0);
+      sync(Later());
+      load(std::false_type());
+      next();
+      read(0);
+      multiply(1);
+    }
+    for (; it < n; ++it) {
+      read(1);
+      multiply(0);
+      if (it + STAGES < n) { sync(Later()); load(std::true_type()); } else sync(None());
+      next();
+      read(0);                                               // (behind the last stage: of no use, and of no harm)
+      multiply(1);
     }
   }
   __syncthreads();                                 // the epilogue uses the LDS
@@ -258,11 +313,15 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) vocab_gemm(const VocabGemm g)
           acc[i][j][r] = z;
           m = fmaxf(m, z);
         }
-      if (label >= 0 && label < FM * 16)
+      if (__any(label >= 0 && label < FM * 16)) {
+        float z = 0.f;
+        bool mine = false;
 #pragma unroll
         for (int i = 0; i < FM; ++i)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) if (label == i * 16 + r) g.hit[c] = acc[i][j][r];
+          for (int r = 0; r < 4; ++r) { const bool is = label == i * 16 + r; z = is ? acc[i][j][r] : z; mine |= is; }
+        if (mine) g.hit[c] = z;
+      }
       m = fmaxf(m, __shfl_xor(m, 16));
       m = fmaxf(m, __shfl_xor(m, 32));
       const float base = m == -INFINITY ? 0.f : m;       // nothing here yet: exp2(-inf - 0) = 0
