@@ -421,14 +421,15 @@ struct FinishArgs {
   int64_t rows, D; unsigned quads; void* out; int vec;        // quads: groups of four a row; vec: stored at once
   const VocabMeta* meta; int by_x;
 };
-template <int DT> __global__ void __launch_bounds__(256) vocab_finish(const FinishArgs a) {
+template <int DT> __global__ void __launch_bounds__(64) vocab_finish(const FinishArgs a) {
   const float f = a.meta->unscale_g * (a.by_x ? a.meta->unscale_x : a.meta->unscale_w);
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t i = (int64_t)blockIdx.x * 64 + threadIdx.x;
   const int64_t r = i / a.quads, d = (i - r * a.quads) * 4;
   if (r >= a.rows) return;
   const int64_t p = a.pos ? a.pos[r] : r;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
   if (p >= 0) {
+#pragma unroll 8
     for (int s = 0; s < a.splits; ++s) v += *reinterpret_cast<const f32x4*>(a.slab + s * a.stride + p * a.ld + d);
     v *= f;
   }
@@ -656,7 +657,7 @@ template <int DT, class T, int PLANES> struct Run {
   static void finish(FinishArgs f, const Problem& q, hipStream_t s) {
     f.D = q.D; f.quads = (unsigned)tiles(q.D, 4);
     f.vec = !(q.D & 3) && !((uintptr_t)f.out & (DT == GNET_F32 ? 15 : 7));
-    vocab_finish<DT><<<(unsigned)tiles(f.rows * f.quads, 256), 256, 0, s>>>(f);
+    vocab_finish<DT><<<(unsigned)tiles(f.rows * f.quads, 64), 64, 0, s>>>(f);
   }
 
   static int backward(const Problem& q, const Plan& p, char* ws, const float* lse, const float* hit, const float* dloss, void* dx, void* dw, hipStream_t s) {
@@ -692,7 +693,7 @@ template <int DT, class T, int PLANES> struct Run {
         void* out = (char*)dw + v0 * q.D * elem;
         if (p.dw.splits == 1) {
           d.out = out; d.ld_out = q.D; d.out_rows = q.D; d.unscale_by_x = 1;
-          d.out_vec = (q.D & 3) == 0 && ((uintptr_t)dw & 7) == 0;
+          d.out_vec = vec8(dw, q.D, q.D, DT);
           gemm<true, true, EPI_OUT>(d, p.dw, p.Dp, rows, s);
         } else {
           d.slab = (float*)(ws + p.dw_slab); d.ld_slab = p.Dp; d.slab_stride = p.piece * p.Dp;
