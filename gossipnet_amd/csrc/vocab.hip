@@ -195,6 +195,12 @@ template <int DT> __device__ __forceinline__ void copy_row(const void* src, int6
     }
   }
 }
+template <int DT> __device__ __forceinline__ void zero_row(void* out, int64_t first, int64_t D, int t, int threads) {
+  for (int64_t d = t; d < D; d += threads) {
+    if (DT == GNET_F32) ((float*)out)[first + d] = 0.f;
+    else ((u16*)out)[first + d] = 0;
+  }
+}
 // Rows of W that the matrix products cannot read where they lie (32 bits; widths that are no multiple of 64; alignment).
 struct PackW { const void* w; int64_t ldw, rows, rows_out; u16* dst; RowCopy c; };
 constexpr int PACK_W_ROWS = 16;
@@ -219,7 +225,8 @@ struct PackArgs {
   const void* x; int64_t ldx; u16* xp; RowCopy c;
   const float* row_x; const float* w_part;
   const float* row_g; const float* dloss; const float* lse; int top_g;
-  int32_t* pos; int32_t* label; float* lse2; float* gscale;
+  int32_t* pos; int32_t* label; int32_t* row_of; float* lse2; float* gscale;
+  void* dx;                            // its rows of tokens that do not count are zeroed here; NULL: later
   VocabMeta* meta;
   PackW w;
 };
@@ -266,23 +273,37 @@ template <int DT> __global__ void __launch_bounds__(256) vocab_pack(const PackAr
   }
   RowCopy c = a.c;
   c.scale = ldexpf(1.f, ex);
+  __shared__ int place[256];                      // of 256 rows of the group: how many that count in front, ~ of it for one that does not
   const int wide = c.Dp >= 2048;                  // a whole workgroup a row, or a wave
-  const int t = wide ? threadIdx.x : threadIdx.x & 63;
-  for (int j = wide ? 0 : threadIdx.x >> 6; j < a.rows; j += wide ? 1 : 4) {
-    const int64_t r = r0 + j;
-    if (r >= a.Mp) break;
-    int f = 0;                                    // tokens that count among this workgroup's in front of r
-    for (int i = 0; i < j; ++i) f += r0 + i < M && counts(r0 + i);
-    const bool own = r < M && counts(r);
-    const int64_t rank = before + f;
-    if (r < M && t == 0) a.pos[r] = own ? (int32_t)rank : -1;
-    const int64_t to = own ? rank : all + (r - rank);        // the others' places behind them are zeroed
-    copy_row<DT>(a.x, r * a.ldx, !own, a.xp + to * c.Dp, c, t, wide ? 256 : 64);
-    if (own && t == 0) {
-      if (a.label) a.label[to] = (int32_t)load_id(a.t.ids, r, a.t.ids64);
-      if (a.dloss) {
-        a.lse2[to] = a.lse[r] * LOG2E;
-        a.gscale[to] = ldexpf(a.dloss[r] * a.t.inv_temp, eg);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = wide ? threadIdx.x : lane;
+  for (int j0 = 0; j0 < a.rows; j0 += 256) {
+    const int64_t base = r0 + j0, mine = base + threadIdx.x;
+    const bool c256 = threadIdx.x < a.rows - j0 && mine < M && counts(mine);
+    const unsigned long long mask = __ballot(c256);
+    __syncthreads();
+    if (lane == 0) ired[wave] = __popcll(mask);
+    __syncthreads();
+    int rank = before + __popcll(mask & ((1ull << lane) - 1));
+    for (int w = 0; w < wave; ++w) rank += ired[w];
+    place[threadIdx.x] = c256 ? rank : ~rank;
+    if (mine < M && threadIdx.x < a.rows - j0) a.pos[mine] = c256 ? rank : -1;
+    before += ired[0] + ired[1] + ired[2] + ired[3];
+    __syncthreads();
+    const int n = (int)min((int64_t)min(256, a.rows - j0), a.Mp - base);
+    for (int j = wide ? 0 : wave; j < n; j += wide ? 1 : 4) {
+      const int64_t r = base + j;
+      const int at = place[j];
+      const bool own = at >= 0;
+      const int64_t to = own ? at : all + (r - ~at);           // the others' places behind them are zeroed
+      copy_row<DT>(a.x, r * a.ldx, !own, a.xp + to * c.Dp, c, t, wide ? 256 : 64);
+      if (a.dx && !own && r < M) zero_row<DT>(a.dx, r * c.D, c.D, t, wide ? 256 : 64);
+      if (own && t == 0) {
+        if (a.label) a.label[to] = (int32_t)load_id(a.t.ids, r, a.t.ids64);
+        if (a.row_of) a.row_of[to] = (int32_t)r;
+        if (a.dloss) {
+          a.lse2[to] = a.lse[r] * LOG2E;
+          a.gscale[to] = ldexpf(a.dloss[r] * a.t.inv_temp, eg);
+        }
       }
     }
   }
@@ -452,9 +473,10 @@ template <int DT> __global__ void __launch_bounds__(64) vocab_finish(const Finis
 inline int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 inline int64_t tiles(int64_t v, int64_t a) { return (v + a - 1) / a; }
 
-// Tile shapes of the products.  256 x 256 runs a contraction step of 64 in SQUARE_US (one workgroup a CU), 128 x 128 in HALF_US (two a
-// CU) -- 1.29 against 1.0 PFLOP/s measured -- plus what a tile costs before and behind its steps.  128 x 64 and 128 x 32 are for
-// products with that few tokens, which wait for W: they only have to keep loads in flight.
+// Tile shapes of the products.  A contraction step of 64 takes 256 x 256 tiles 1.5 us (one workgroup a CU: 1.4 PFLOP/s) and 128 x 128
+// tiles 0.9 us (two a CU: 1.2), and every tile 6 or 3.5 us before and behind its steps (fitted to 4096 x 131072 x 4096, 833 x 50257 x 1024 and
+// 464 x 65537 x 1536).  128 x 64 and 128 x 32 are for products with that few tokens, which wait for W: they only have to keep
+// loads in flight.
 enum Shape { S256, S128, S64, S32 };
 struct ShapeInfo { int bm, bn; };
 constexpr ShapeInfo SHAPE[] = {{256, 256}, {128, 128}, {128, 64}, {128, 32}};
@@ -462,7 +484,7 @@ struct Product { int shape, splits; };
 
 double product_us(int shape, int splits, int64_t rows, int64_t cols, int64_t steps) {
   const int64_t n = tiles(rows, SHAPE[shape].bm) * tiles(cols, SHAPE[shape].bn) * splits;
-  const double round = shape == S256 ? tiles(steps, splits) * 1.67 + 8 : tiles(steps, splits) * 1.07 + 5;
+  const double round = shape == S256 ? tiles(steps, splits) * 1.5 + 6 : tiles(steps, splits) * 0.9 + 3.5;
   const double joined = splits > 1 ? 5 + (double)rows * cols * 4 * (2 * splits) / 4e6 : 0;       // partial sums out and in at 4 TB/s
   return tiles(n, shape == S256 ? 256 : 512) * round + joined;
 }
@@ -485,9 +507,9 @@ Product pick_product(int64_t rows, int64_t cols, int64_t steps, bool few_cols, b
 
 struct Plan {
   int64_t Mp, Dp, flags_n, piece, pieces, w_tiles;
-  int planes, pack_w, direct;
+  int planes, pack_w, direct, dx_direct;
   Product logits, dx, dw;
-  int64_t flag, q, entropy, row_x, row_g, w_part, meta, pos, label, hit2, lse2, gscale, xp, wp, part, dz, dx_slab, dw_slab, bytes;
+  int64_t flag, q, entropy, row_x, row_g, w_part, meta, pos, label, row_of, hit2, lse2, gscale, xp, wp, part, dz, dx_slab, dw_slab, bytes;
 };
 
 Plan make_plan(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int distill, int pack_w, int backward) {
@@ -498,10 +520,11 @@ Plan make_plan(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int distil
   // cross entropy on 16 bits needs nothing of its tokens but the labels: up to 8192 of them the packing looks at them itself
   p.direct = !distill && p.planes == 1 && M <= 8192;
   p.Mp = up(M, VG_BK); p.Dp = up(D, 64); p.flags_n = up(M, 16);
-  // A piece's dz and packed rows of W stay within the last-level cache (256 MB) for the products that read them again.
+  // A piece's dz and packed rows of W take 256 MB at most: that is what the last-level cache holds for the products that read them
+  // again, though larger pieces measured the same (2048 x 100352 x 2048: 2.25 ms; 64 MB 2.22, 512 MB 2.17; 4096 x 131072 x 4096: 9.85, 9.77, 9.79).
   const int64_t per_row = (int64_t)p.planes * 2 * ((backward ? p.Mp : 0) + (pack_w ? p.Dp : 0));
   const int64_t Vp = up(V, 256);
-  int64_t piece = per_row ? (128ll << 20) / per_row / 256 * 256 : Vp;
+  int64_t piece = per_row ? (256ll << 20) / per_row / 256 * 256 : Vp;
   if (piece < 2048) piece = 2048;
   p.pieces = tiles(Vp, piece);
   p.piece = up(tiles(Vp, p.pieces), 256);
@@ -525,7 +548,9 @@ Plan make_plan(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int distil
     p.row_g = take(M * 4); p.lse2 = take(p.Mp * 4); p.gscale = take(p.Mp * 4);
     p.dz = take(p.planes * p.Mp * p.piece * 2);
     p.dx = pick_product(p.Dp, M, p.piece / VG_BK * segments, true, true);
-    p.dx_slab = take((int64_t)p.dx.splits * p.Mp * p.Dp * 4);
+    p.dx_direct = p.pieces == 1 && p.dx.splits == 1;          // one sum: straight to its rows
+    p.row_of = take(p.Mp * 4);
+    if (!p.dx_direct) p.dx_slab = take((int64_t)p.dx.splits * p.Mp * p.Dp * 4);
     p.dw = pick_product(p.Dp, p.piece, p.Mp / VG_BK * segments, false, true);
     if (p.dw.splits > 1) p.dw_slab = take((int64_t)p.dw.splits * p.piece * p.Dp * 4);
   }
@@ -577,7 +602,7 @@ template <int DT, class T, int PLANES> struct Run {
     return k;
   }
   // everything in front of the first product, the first piece of W included
-  static void prepare(const Problem& q, const Plan& p, char* ws, const float* dloss, const float* lse, hipStream_t s) {
+  static void prepare(const Problem& q, const Plan& p, char* ws, const float* dloss, const float* lse, void* dx, hipStream_t s) {
     TargetsArgs a = {};
     a.t = q.t; a.flags_n = p.flags_n; a.token_groups = (unsigned)tiles(p.flags_n, 4);
     a.dloss = dloss;
@@ -605,6 +630,7 @@ template <int DT, class T, int PLANES> struct Run {
     k.pos = (int32_t*)(ws + p.pos); k.label = q.t.logits ? nullptr : (int32_t*)(ws + p.label);
     k.lse2 = (float*)(ws + p.lse2); k.gscale = (float*)(ws + p.gscale);
     k.meta = (VocabMeta*)(ws + p.meta);
+    if (dx && p.dx_direct) { k.dx = dx; k.row_of = (int32_t*)(ws + p.row_of); }
     if (p.pack_w) k.w = pack_of_w(q, p, ws, 0);
     vocab_pack<DT><<<k.token_groups + (p.pack_w ? (unsigned)tiles(p.piece, PACK_W_ROWS) : 0), 256, 0, s>>>(k);
   }
@@ -637,7 +663,7 @@ template <int DT, class T, int PLANES> struct Run {
   }
 
   static int forward(const Problem& q, const Plan& p, char* ws, float* loss, float* lse, float* hit, hipStream_t s) {
-    prepare(q, p, ws, nullptr, nullptr, s);
+    prepare(q, p, ws, nullptr, nullptr, nullptr, s);
     for (int64_t v0 = 0; v0 < q.t.V; v0 += p.piece) {
       VocabGemm g = logits(q, p, ws, piece_of_w(q, p, ws, v0, s), v0);
       g.part = (float2*)(ws + p.part); g.hit = (float*)(ws + p.hit2);
@@ -661,7 +687,7 @@ template <int DT, class T, int PLANES> struct Run {
   }
 
   static int backward(const Problem& q, const Plan& p, char* ws, const float* lse, const float* hit, const float* dloss, void* dx, void* dw, hipStream_t s) {
-    prepare(q, p, ws, dloss, lse, s);
+    prepare(q, p, ws, dloss, lse, dx, s);
     const VocabMeta* meta = (const VocabMeta*)(ws + p.meta);
     const int elem = DT == GNET_F32 ? 4 : 2;
     for (int64_t v0 = 0; v0 < q.t.V; v0 += p.piece) {
@@ -682,9 +708,15 @@ template <int DT, class T, int PLANES> struct Run {
       dz.p = g.dz; dz.ld = p.piece; dz.plane = g.plane_dz; dz.rows = p.Mp; dz.cols = (int)p.piece;
       if (dx) {
         VocabGemm d = {};
-        d.a = w; d.b = dz; d.k = rows64; d.cols_from_meta = 1; d.meta = meta;
-        d.slab = (float*)(ws + p.dx_slab); d.ld_slab = p.Dp; d.slab_stride = p.Mp * p.Dp; d.accumulate = v0 > 0; d.out_cols = p.Mp;
-        gemm<true, false, EPI_SLAB>(d, p.dx, p.Dp, q.t.M, s);
+        d.a = w; d.b = dz; d.k = rows64; d.cols_from_meta = 1; d.meta = meta; d.out_cols = p.Mp;
+        if (p.dx_direct) {
+          d.out = dx; d.ld_out = q.D; d.out_rows = q.D; d.out_vec = vec8(dx, q.D, q.D, DT);
+          d.row_of = (const int32_t*)(ws + p.row_of);
+          gemm<true, false, EPI_OUT>(d, p.dx, p.Dp, q.t.M, s);
+        } else {
+          d.slab = (float*)(ws + p.dx_slab); d.ld_slab = p.Dp; d.slab_stride = p.Mp * p.Dp; d.accumulate = v0 > 0;
+          gemm<true, false, EPI_SLAB>(d, p.dx, p.Dp, q.t.M, s);
+        }
       }
       if (dw) {
         VocabGemm d = {};
@@ -705,7 +737,7 @@ template <int DT, class T, int PLANES> struct Run {
         }
       }
     }
-    if (dx) {
+    if (dx && !p.dx_direct) {
       FinishArgs f = {};
       f.slab = (const float*)(ws + p.dx_slab); f.ld = p.Dp; f.stride = p.Mp * p.Dp; f.splits = p.dx.splits;
       f.pos = (const int32_t*)(ws + p.pos); f.rows = q.t.M; f.out = dx; f.meta = meta;

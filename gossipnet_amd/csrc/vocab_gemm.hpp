@@ -75,6 +75,7 @@ struct VocabGemm {
   u16* dz; int64_t ld_dz, plane_dz, dz_cols;
   // products
   float* slab; int64_t ld_slab, slab_stride; int accumulate;      // [split][column][ld_slab]
+  const int32_t* row_of;       // the output row of a column (tokens that count), or NULL
   void* out; int64_t ld_out, out_rows, out_cols; int out_vec; int unscale_by_x;   // [column][row]; out_vec: 16 bytes may be stored at once
 };
 
@@ -434,28 +435,29 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) vocab_gemm(const VocabGemm g)
     }
   } else {
     const float f = g.meta->unscale_g * (g.unscale_by_x ? g.meta->unscale_x : g.meta->unscale_w);
+    const int64_t cols = g.row_of ? (int64_t)rows : g.out_cols;
     if constexpr (PLANES == 2) {
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
         const int64_t c = c0 + (wn * FN + j) * 16 + col16;
-        if (c >= g.out_cols) continue;
+        if (c >= cols) continue;
+        float* out = (float*)g.out + (g.row_of ? g.row_of[c] : c) * g.ld_out;
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
           const int64_t row = r0 + (wm * FM + i) * 16 + quad * 4;
-          float* p = (float*)g.out + c * g.ld_out + row;
           if (g.out_vec) {
-            if (row < g.out_rows) *reinterpret_cast<f32x4*>(p) = acc[i][j] * f;
+            if (row < g.out_rows) *reinterpret_cast<f32x4*>(out + row) = acc[i][j] * f;
           } else {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) if (row + r < g.out_rows) p[r] = acc[i][j][r] * f;
+            for (int r = 0; r < 4; ++r) if (row + r < g.out_rows) out[row + r] = acc[i][j][r] * f;
           }
         }
       }
     } else {
       store_tile<BM, BN, WM, WN>(lds, tid, [&](int i, int j, int r) { return T::enc(acc[i][j][r] * f); }, [&](int v, int d, s16x8 x) {
         const int64_t c = c0 + v, row = r0 + d;
-        if (c >= g.out_cols) return;
-        u16* p = (u16*)g.out + c * g.ld_out + row;
+        if (c >= cols) return;
+        u16* p = (u16*)g.out + (g.row_of ? g.row_of[c] : c) * g.ld_out + row;
         if (g.out_vec) {
           if (row < g.out_rows) *reinterpret_cast<s16x8*>(p) = x;
         } else {

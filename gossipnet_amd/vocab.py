@@ -11,8 +11,6 @@ Tokens may be laid out in any number of leading dimensions ([B, T] or flat); x, 
 all of a call of one type; ids and labels int32 or int64.  An id or label outside [0, V) means "no token here" (padding): nothing
 is read or added for it.  Every result is reproducible bit for bit.  The calls run on the current stream of the tensors' device and
 may be captured into a graph; workspaces come from PyTorch's allocator for each call."""
-import ctypes as C
-
 import torch
 
 from . import _lib
@@ -21,11 +19,27 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # GNET_F32,
 
 
 def _p(t):
-    return C.c_void_p(t.data_ptr()) if t is not None else C.c_void_p(0)
+    return t.data_ptr() if t is not None else None
 
 
 def _stream(dev):
-    return C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+class _Here(object):
+    """Nothing to switch: the call's device is the current one (torch.cuda.device costs microseconds that a small call feels)."""
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *_):
+        pass
+
+
+_HERE = _Here()
+
+
+def _device(dev):
+    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
 def _matrix(t, what, cols=None, dtype=None):
@@ -78,7 +92,7 @@ def _workspace(nbytes, device):
     """256-byte aligned scratch of this call.  From the caching allocator: ordered on the current stream, and part of the graph's own
     memory while one is captured, so that no two calls in flight share it."""
     buf = torch.empty(nbytes + 256, dtype=torch.uint8, device=device)
-    return buf, C.c_void_p((buf.data_ptr() + 255) // 256 * 256)
+    return buf, (buf.data_ptr() + 255) // 256 * 256
 
 
 # ---- token rows ----------------------------------------------------------------------------------------------------
@@ -94,7 +108,7 @@ def embed_forward(ids, table, scale=1.0, token_scale=None):
     dev = _on_device(t, ids=i, token_scale=s)
     y = torch.empty(tuple(ids.shape) + (D,), dtype=t.dtype, device=dev)
     lib = _lib.load()
-    with torch.cuda.device(dev):
+    with _device(dev):
         _lib.check(lib.gnet_embed_forward(_p(i), int(i.dtype == torch.int64), _p(t), _ld(t), float(scale), _p(s), i.numel(), V, D,
                                           _TYPES[t.dtype], _p(y), _stream(dev)), "gnet_embed_forward")
     return y
@@ -121,7 +135,7 @@ def embed_backward(ids, dy, table, scale=1.0, token_scale=None, need_dscale=Fals
     M = i.numel()
     lib = _lib.load()
     dscale = torch.empty(tuple(ids.shape), dtype=torch.float32, device=dev) if need_dscale else None
-    with torch.cuda.device(dev):
+    with _device(dev):
         nbytes = lib.gnet_embed_workspace_bytes(M, D)
         buf, ws = _workspace(nbytes, dev)
         _lib.check(lib.gnet_embed_backward(_p(i), int(i.dtype == torch.int64), _p(g), _ld(g), float(scale), _p(s), M, V, D, _TYPES[t.dtype],
@@ -163,7 +177,7 @@ def xent_forward(x, w, labels):
     (M, D), V = xm.shape, wm.shape[0]
     loss, lse, hit = (torch.empty(lead, dtype=torch.float32, device=dev) for _ in range(3))
     lib = _lib.load()
-    with torch.cuda.device(dev):
+    with _device(dev):
         nbytes = lib.gnet_vocab_workspace_bytes(_p(wm), _ld(wm), M, V, D, 0, _TYPES[wm.dtype], 0)
         buf, ws = _workspace(nbytes, dev)
         _lib.check(lib.gnet_xent_forward(_p(xm), _ld(xm), _p(wm), _ld(wm), _p(i), int(i.dtype == torch.int64), M, V, D, _TYPES[wm.dtype],
@@ -192,7 +206,7 @@ def distill_forward(x, w, top_ids, top_logits, temperature=1.0):
     loss, lse = (torch.empty(lead, dtype=torch.float32, device=dev) for _ in range(2))
     hit = torch.empty(lead + (K,), dtype=torch.float32, device=dev)
     lib = _lib.load()
-    with torch.cuda.device(dev):
+    with _device(dev):
         nbytes = lib.gnet_vocab_workspace_bytes(_p(wm), _ld(wm), M, V, D, K, _TYPES[wm.dtype], 0)
         buf, ws = _workspace(nbytes, dev)
         _lib.check(lib.gnet_distill_forward(_p(xm), _ld(xm), _p(wm), _ld(wm), _p(i), int(i.dtype == torch.int64), _p(t), float(temperature),
@@ -217,7 +231,7 @@ def _backward(xm, wm, i, t, temperature, lse, hit, dloss, x_shape, K, need_dx, n
     if not (need_dx or need_dw):
         return dx, dw
     lib = _lib.load()
-    with torch.cuda.device(dev):
+    with _device(dev):
         nbytes = lib.gnet_vocab_workspace_bytes(_p(wm), _ld(wm), M, V, D, K, dt, 1)
         buf, ws = _workspace(nbytes, dev)
         ids64 = int(i.dtype == torch.int64)
