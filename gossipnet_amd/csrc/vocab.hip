@@ -14,8 +14,6 @@
 
 namespace {
 
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-
 __device__ __forceinline__ int64_t load_id(const void* p, int64_t i, int is64) {
   return is64 ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
 }
@@ -225,7 +223,7 @@ struct PackArgs {
   const void* x; int64_t ldx; u16* xp; RowCopy c;
   const float* row_x; const float* w_part;
   const float* row_g; const float* dloss; const float* lse; int top_g;
-  int32_t* pos; int32_t* label; int32_t* row_of; float* lse2; float* gscale;
+  int32_t* pos; int32_t* label; int32_t* row_of; float* lse_c; float* gscale;
   void* dx;                            // its rows of tokens that do not count are zeroed here; NULL: later
   VocabMeta* meta;
   PackW w;
@@ -301,7 +299,7 @@ template <int DT> __global__ void __launch_bounds__(256) vocab_pack(const PackAr
         if (a.label) a.label[to] = (int32_t)load_id(a.t.ids, r, a.t.ids64);
         if (a.row_of) a.row_of[to] = (int32_t)r;
         if (a.dloss) {
-          a.lse2[to] = a.lse[r] * LOG2E;
+          a.lse_c[to] = a.lse[r];
           a.gscale[to] = ldexpf(a.dloss[r] * a.t.inv_temp, eg);
         }
       }
@@ -312,35 +310,36 @@ template <int DT> __global__ void __launch_bounds__(256) vocab_pack(const PackAr
 // ---- behind the products ---------------------------------------------------------------------------------------------
 struct JoinArgs {
   Targets t;
-  const int32_t* pos; const float2* part; int tiles; const float* hit2;      // hit2: cross entropy's label logits, compacted, log2 units
+  const int32_t* pos; const float2* part; int tiles; const float* hit_c;     // hit_c: cross entropy's label logits, compacted
   const void* x; int64_t ldx; const void* w; int64_t ldw; int64_t D; int vec;
   const float* q; const float* entropy;
   float* loss; float* lse; float* hit;
 };
-// log2 of a token's sum over the vocabulary from its tiles' maxima and sums, by one wave
-__device__ __forceinline__ float join_tiles(const float2* part, int tiles, int lane) {
+// a token's largest logit and the log of the sum over the vocabulary of exp(z - largest), from its tiles', by one wave
+__device__ __forceinline__ void join_tiles(const float2* part, int tiles, int lane, float& top, float& log_sum) {
   float mx = -INFINITY, sum = 0.f;
   for (int i = lane; i < tiles; i += 64) {
     const float2 v = part[i];
     const float n = fmaxf(mx, v.x), b = n == -INFINITY ? 0.f : n;
-    sum = sum * exp2f(mx - b) + v.y * exp2f(v.x - b);
+    sum = sum * exp2f((mx - b) * LOG2E) + v.y * exp2f((v.x - b) * LOG2E);
     mx = n;
   }
-  const float all = wave_max(mx), base = all == -INFINITY ? 0.f : all;
-  return base + log2f(wave_sum(sum * exp2f(mx - base)));
+  const float all = wave_max(mx);
+  top = all == -INFINITY ? 0.f : all;
+  log_sum = logf(wave_sum(sum * exp2f((mx - top) * LOG2E)));
 }
 // cross entropy: one wave per token
 __global__ void __launch_bounds__(256) vocab_join(const JoinArgs a) {
   const int64_t m = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (m >= a.t.M) return;
   const int p = a.pos[m], lane = threadIdx.x & 63;
-  float lse2 = 0.f, hit2 = 0.f;
-  if (p >= 0) { lse2 = join_tiles(a.part + (int64_t)p * a.tiles, a.tiles, lane); hit2 = a.hit2[p]; }
+  float top = 0.f, log_sum = 0.f, hit = 0.f;
+  if (p >= 0) { join_tiles(a.part + (int64_t)p * a.tiles, a.tiles, lane, top, log_sum); hit = a.hit_c[p]; }
   if (lane) return;
-  const float loss = (lse2 - hit2) * LN2;          // the same z in both: the rounding of z cancels where the label takes nearly everything
+  const float loss = (top - hit) + log_sum;        // both from the same products: where the label takes nearly everything nothing cancels
   a.loss[m] = loss < 0.f ? 0.f : loss;             // (below 0 from rounding only; NaN stays)
-  a.lse[m] = lse2 * LN2;
-  a.hit[m] = hit2 * LN2;
+  a.lse[m] = top + log_sum;
+  a.hit[m] = hit;
 }
 template <int DT> __device__ __forceinline__ void dot8(const void* x, const void* w, float& s) {
   if (DT == GNET_F32) {
@@ -369,7 +368,9 @@ template <int DT> __global__ void __launch_bounds__(256) vocab_join_targets(cons
     if (threadIdx.x == 0) { a.loss[m] = 0.f; a.lse[m] = 0.f; }
     return;
   }
-  const float lse = join_tiles(a.part + (int64_t)p * a.tiles, a.tiles, lane) * LN2;
+  float top, log_sum;
+  join_tiles(a.part + (int64_t)p * a.tiles, a.tiles, lane, top, log_sum);
+  const float lse = top + log_sum;
   float loss = 0.f;
   const char* x = (const char*)a.x + m * a.ldx * SIZE;
   for (int k = wave; k < K; k += 8) {
@@ -509,7 +510,7 @@ struct Plan {
   int64_t Mp, Dp, flags_n, piece, pieces, w_tiles;
   int planes, pack_w, direct, dx_direct;
   Product logits, dx, dw;
-  int64_t flag, q, entropy, row_x, row_g, w_part, meta, pos, label, row_of, hit2, lse2, gscale, xp, wp, part, dz, dx_slab, dw_slab, bytes;
+  int64_t flag, q, entropy, row_x, row_g, w_part, meta, pos, label, row_of, hit_c, lse_c, gscale, xp, wp, part, dz, dx_slab, dw_slab, bytes;
 };
 
 Plan make_plan(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int distill, int pack_w, int backward) {
@@ -530,6 +531,7 @@ Plan make_plan(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int distil
   p.piece = up(tiles(Vp, p.pieces), 256);
   p.pieces = tiles(Vp, p.piece);
   p.logits = pick_product(p.piece, M, p.Dp / VG_BK * segments, true, false);
+  if (V <= SHAPE[S128].bm && p.logits.shape == S256) p.logits.shape = S128;          // (a vocabulary of one tile: EPI_DZ_ONE)
   p.w_tiles = tiles(V, SHAPE[p.logits.shape].bm);
   int64_t o = 0;
   auto take = [&](int64_t bytes) { const int64_t at = o; o = up(o + bytes, 256); return at; };
@@ -542,10 +544,10 @@ Plan make_plan(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int distil
   if (pack_w) p.wp = take(p.planes * p.piece * p.Dp * 2);
   if (!backward) {
     p.entropy = take(M * 4);
-    p.hit2 = take(p.Mp * 4);
+    p.hit_c = take(p.Mp * 4);
     p.part = take(p.Mp * p.w_tiles * 8);
   } else {
-    p.row_g = take(M * 4); p.lse2 = take(p.Mp * 4); p.gscale = take(p.Mp * 4);
+    p.row_g = take(M * 4); p.lse_c = take(p.Mp * 4); p.gscale = take(p.Mp * 4);
     p.dz = take(p.planes * p.Mp * p.piece * 2);
     p.dx = pick_product(p.Dp, M, p.piece / VG_BK * segments, true, true);
     p.dx_direct = p.pieces == 1 && p.dx.splits == 1;          // one sum: straight to its rows
@@ -586,7 +588,7 @@ template <int DT, class T, int PLANES> struct Run {
   }
   // columns are tokens (all shapes) or vocabulary (the square ones)
   template <bool AS, bool BS, int EPI> static void gemm(VocabGemm& g, const Product& p, int64_t rows, int64_t cols, hipStream_t s) {
-    if (p.shape == S256) return launch<256, 256, 2, 4, 2, AS, BS, EPI>(g, rows, cols, p.splits, s);
+    if constexpr (EPI != EPI_DZ_ONE) { if (p.shape == S256) return launch<256, 256, 2, 4, 2, AS, BS, EPI>(g, rows, cols, p.splits, s); }
     if constexpr (!BS) {
       if (p.shape == S64) return launch<128, 64, 4, 1, 2, AS, BS, EPI>(g, rows, cols, p.splits, s);
       if (p.shape == S32) return launch<128, 32, 4, 1, 2, AS, BS, EPI>(g, rows, cols, p.splits, s);
@@ -628,7 +630,7 @@ template <int DT, class T, int PLANES> struct Run {
     k.row_x = a.row_x; k.w_part = a.w_part;
     k.row_g = a.row_g; k.dloss = dloss; k.lse = lse; k.top_g = DT == GNET_BF16 ? 0 : 14;
     k.pos = (int32_t*)(ws + p.pos); k.label = q.t.logits ? nullptr : (int32_t*)(ws + p.label);
-    k.lse2 = (float*)(ws + p.lse2); k.gscale = (float*)(ws + p.gscale);
+    k.lse_c = (float*)(ws + p.lse_c); k.gscale = (float*)(ws + p.gscale);
     k.meta = (VocabMeta*)(ws + p.meta);
     if (dx && p.dx_direct) { k.dx = dx; k.row_of = (int32_t*)(ws + p.row_of); }
     if (p.pack_w) k.w = pack_of_w(q, p, ws, 0);
@@ -657,7 +659,7 @@ template <int DT, class T, int PLANES> struct Run {
     g.a = w; g.b = packed_x(p, ws);
     g.k = p.Dp; g.cols_from_meta = 1;
     g.meta = (const VocabMeta*)(ws + p.meta);
-    g.to_log2 = q.t.to_log2; g.valid_rows = q.t.V - v0; g.first_row = (int32_t)v0;
+    g.inv_temp = q.t.inv_temp; g.valid_rows = q.t.V - v0; g.first_row = (int32_t)v0;
     g.label = q.t.logits ? nullptr : (const int32_t*)(ws + p.label);
     return g;
   }
@@ -666,12 +668,12 @@ template <int DT, class T, int PLANES> struct Run {
     prepare(q, p, ws, nullptr, nullptr, nullptr, s);
     for (int64_t v0 = 0; v0 < q.t.V; v0 += p.piece) {
       VocabGemm g = logits(q, p, ws, piece_of_w(q, p, ws, v0, s), v0);
-      g.part = (float2*)(ws + p.part); g.hit = (float*)(ws + p.hit2);
+      g.part = (float2*)(ws + p.part); g.hit = (float*)(ws + p.hit_c);
       g.first_row_tile = (int)(v0 / SHAPE[p.logits.shape].bm); g.all_row_tiles = (int)p.w_tiles;
       gemm<false, false, EPI_PART>(g, p.logits, q.t.V - v0 < p.piece ? q.t.V - v0 : p.piece, q.t.M, s);
     }
     JoinArgs j = {};
-    j.t = q.t; j.pos = (const int32_t*)(ws + p.pos); j.part = (const float2*)(ws + p.part); j.tiles = (int)p.w_tiles; j.hit2 = (const float*)(ws + p.hit2);
+    j.t = q.t; j.pos = (const int32_t*)(ws + p.pos); j.part = (const float2*)(ws + p.part); j.tiles = (int)p.w_tiles; j.hit_c = (const float*)(ws + p.hit_c);
     j.x = q.x; j.ldx = q.ldx; j.w = q.w; j.ldw = q.ldw; j.D = q.D; j.vec = vec8(q.x, q.ldx, q.D, DT) && vec8(q.w, q.ldw, q.D, DT);
     j.q = (const float*)(ws + p.q); j.entropy = (const float*)(ws + p.entropy);
     j.loss = loss; j.lse = lse; j.hit = hit;
@@ -694,9 +696,10 @@ template <int DT, class T, int PLANES> struct Run {
       const int64_t rows = q.t.V - v0 < p.piece ? q.t.V - v0 : p.piece, rows64 = up(rows, VG_BK);
       const VocabOperand w = piece_of_w(q, p, ws, v0, s);
       VocabGemm g = logits(q, p, ws, w, v0);
-      g.lse2 = (const float*)(ws + p.lse2); g.gscale = (const float*)(ws + p.gscale);
+      g.lse = (const float*)(ws + p.lse_c); g.gscale = (const float*)(ws + p.gscale);
       g.dz = (u16*)(ws + p.dz); g.ld_dz = p.piece; g.plane_dz = p.Mp * p.piece; g.dz_cols = p.Mp;
-      gemm<false, false, EPI_DZ>(g, p.logits, rows, q.t.M, s);
+      if (p.logits.shape != S256 && q.t.V <= SHAPE[p.logits.shape].bm) gemm<false, false, EPI_DZ_ONE>(g, p.logits, rows, q.t.M, s);
+      else gemm<false, false, EPI_DZ>(g, p.logits, rows, q.t.M, s);
       if (q.t.logits) {
         HitsArgs h = {};
         h.t = q.t; h.pos = (const int32_t*)(ws + p.pos); h.lse = lse; h.hit = hit;

@@ -38,6 +38,8 @@ __device__ __forceinline__ void split_f16(float v, u16& hi, u16& lo) {
   lo = F16T::enc(v - F16T::dec(hi));
 }
 
+constexpr float LOG2E = 1.4426950408889634f;
+
 // What the preparation kernels find out on the device.
 struct VocabMeta {
   int rows;            // tokens that count (compacted)
@@ -64,14 +66,14 @@ struct VocabGemm {
   int row_tiles, col_tiles, splits;
   const VocabMeta* meta;
   // logits
-  float to_log2;               // log2(e) / temperature
+  float inv_temp;
   int64_t valid_rows;          // vocabulary rows of this piece that exist
   int first_row_tile, all_row_tiles;
   int32_t first_row;           // of the piece, in the vocabulary
   const int32_t* label;        // per column: its one target, or NULL (several, see vocab_hits)
-  float2* part;                // [column][all_row_tiles] running maximum and sum of a row tile
-  float* hit;                  // per column: the logit of its label, in units of log2
-  const float* lse2; const float* gscale;   // per column
+  float2* part;                // [column][all_row_tiles] maximum z and sum of exp(z - maximum) of a row tile
+  float* hit;                  // per column: the logit of its label
+  const float* lse; const float* gscale;   // per column
   u16* dz; int64_t ld_dz, plane_dz, dz_cols;
   // products
   float* slab; int64_t ld_slab, slab_stride; int accumulate;      // [split][column][ld_slab]
@@ -79,7 +81,7 @@ struct VocabGemm {
   void* out; int64_t ld_out, out_rows, out_cols; int out_vec; int unscale_by_x;   // [column][row]; out_vec: 16 bytes may be stored at once
 };
 
-enum { EPI_PART = 0, EPI_DZ = 1, EPI_SLAB = 2, EPI_OUT = 3 };
+enum { EPI_PART = 0, EPI_DZ = 1, EPI_SLAB = 2, EPI_OUT = 3, EPI_DZ_ONE = 4 };      // EPI_DZ_ONE: the vocabulary is one row tile
 
 // ---- staging of one operand tile, 16 bytes per lane straight into LDS ------------------------------------------------
 // Contraction-contiguous (STRIDED = false): LDS [T rows][64 k], 128 bytes a row; the 16-byte chunk c of row r lies at position
@@ -321,24 +323,53 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) vocab_gemm(const VocabGemm g)
   auto label_row = [&](int64_t c) {
     return g.label && c < rows ? (int64_t)g.label[c] - g.first_row - r0 - wm * FM * 16 - quad * 4 : (int64_t)-1;
   };
+  const int64_t left = g.valid_rows - r0 - wm * FM * 16 - quad * 4;          // rows of the lane's that exist
+  auto scale = [&](float f) {
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[i][j][r] = i * 16 + r < left ? acc[i][j][r] * f : -INFINITY;
+  };
+  // The tile's maximum and sum of exp(z - maximum) of each column (token): every wave's share into `red`, then put together by column.
+  // The difference is taken before the change to base 2: z itself (exact at temperature 1) stays what the backward pass forms again, and
+  // no rounding is relative to a large z.
+  float2* const red = reinterpret_cast<float2*>(lds);        // [WM][BN]
+  auto wave_stats = [&](int j) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) m = fmaxf(m, acc[i][j][r]);
+    m = fmaxf(m, __shfl_xor(m, 16));
+    m = fmaxf(m, __shfl_xor(m, 32));
+    const float base = m == -INFINITY ? 0.f : m;             // nothing here: exp(-inf - 0) = 0
+    float l = 0.f;
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) l += __builtin_amdgcn_exp2f((acc[i][j][r] - base) * LOG2E);
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (quad == 0) red[wm * BN + (wn * FN + j) * 16 + col16] = make_float2(m, l);
+  };
+  auto tile_stats = [&](int c) {
+    float m = red[c].x;
+#pragma unroll
+    for (int w = 1; w < WM; ++w) m = fmaxf(m, red[w * BN + c].x);
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+#pragma unroll
+    for (int w = 0; w < WM; ++w) l += red[w * BN + c].y * __builtin_amdgcn_exp2f((red[w * BN + c].x - base) * LOG2E);
+    return make_float2(m, l);
+  };
   if constexpr (EPI == EPI_PART) {
-    // the tile's maximum and sum of 2^(z - max), z in units of log2, for each of its columns (tokens)
-    const float f = g.to_log2 * g.meta->unscale_x * g.meta->unscale_w;
-    const int64_t left = g.valid_rows - r0 - wm * FM * 16 - quad * 4;        // rows of the lane's that exist
-    float2* red = reinterpret_cast<float2*>(lds);        // [WM][BN]
+    scale(g.inv_temp * (g.meta->unscale_x * g.meta->unscale_w));
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
       const int64_t c = c0 + (wn * FN + j) * 16 + col16;
       const int64_t label = label_row(c);
-      float m = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float z = i * 16 + r < left ? acc[i][j][r] * f : -INFINITY;
-          acc[i][j][r] = z;
-          m = fmaxf(m, z);
-        }
       if (__any(label >= 0 && label < FM * 16)) {
         float z = 0.f;
         bool mine = false;
@@ -348,38 +379,29 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) vocab_gemm(const VocabGemm g)
           for (int r = 0; r < 4; ++r) { const bool is = label == i * 16 + r; z = is ? acc[i][j][r] : z; mine |= is; }
         if (mine) g.hit[c] = z;
       }
-      m = fmaxf(m, __shfl_xor(m, 16));
-      m = fmaxf(m, __shfl_xor(m, 32));
-      const float base = m == -INFINITY ? 0.f : m;       // nothing here yet: exp2(-inf - 0) = 0
-      float l = 0.f;
-#pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) l += __builtin_amdgcn_exp2f(acc[i][j][r] - base);
-      l += __shfl_xor(l, 16);
-      l += __shfl_xor(l, 32);
-      if (quad == 0) red[wm * BN + (wn * FN + j) * 16 + col16] = make_float2(m, l);
+      wave_stats(j);
     }
     __syncthreads();
-    for (int c = tid; c < BN; c += 64 * WAVES) {
-      if (c0 + c >= rows) continue;
-      float m = red[c].x;
+    for (int c = tid; c < BN; c += 64 * WAVES)
+      if (c0 + c < rows) g.part[(size_t)(c0 + c) * g.all_row_tiles + g.first_row_tile + rt] = tile_stats(c);
+  } else if constexpr (EPI == EPI_DZ || EPI == EPI_DZ_ONE) {
+    // A vocabulary of one tile: the sum is formed here again instead of from lse, whose 32 bits are half a step of its own magnitude off --
+    // more than what is left of 1 - p in a confident row.
+    float f = g.inv_temp * (g.meta->unscale_x * g.meta->unscale_w);
+    if constexpr (EPI == EPI_DZ_ONE) {
+      scale(f);
+      f = 1.f;
 #pragma unroll
-      for (int w = 1; w < WM; ++w) m = fmaxf(m, red[w * BN + c].x);
-      const float base = m == -INFINITY ? 0.f : m;
-      float l = 0.f;
-#pragma unroll
-      for (int w = 0; w < WM; ++w) l += red[w * BN + c].y * __builtin_amdgcn_exp2f(red[w * BN + c].x - base);
-      g.part[(size_t)(c0 + c) * g.all_row_tiles + g.first_row_tile + rt] = make_float2(m, l);
+      for (int j = 0; j < FN; ++j) wave_stats(j);
+      __syncthreads();
     }
-  } else if constexpr (EPI == EPI_DZ) {
-    const float f = g.to_log2 * g.meta->unscale_x * g.meta->unscale_w;
-    const int64_t left = g.valid_rows - r0 - wm * FM * 16 - quad * 4;
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
       const int64_t c = c0 + (wn * FN + j) * 16 + col16;
       const bool some = c < rows;
-      const float lse = some ? g.lse2[c] : 0.f, gs = some ? g.gscale[c] : 0.f;
+      float lse = some ? g.lse[c] : 0.f, over = 1.f;
+      if constexpr (EPI == EPI_DZ_ONE) { const float2 s = tile_stats((wn * FN + j) * 16 + col16); lse = s.x; over = 1.f / s.y; }
+      const float gs = some ? g.gscale[c] : 0.f;
       const int64_t label = label_row(c);
       const bool here = __any(label >= 0 && label < FM * 16);
 #pragma unroll
@@ -387,11 +409,12 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) vocab_gemm(const VocabGemm g)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           // padding (a token or a vocabulary row that does not exist) is zero: it takes part in the products
-          float p = __builtin_amdgcn_exp2f(acc[i][j][r] * f - lse);
+          float p = __builtin_amdgcn_exp2f((acc[i][j][r] * f - lse) * LOG2E) * over;
           if (here && label == i * 16 + r) p -= 1.f;
           acc[i][j][r] = some && i * 16 + r < left ? p * gs : 0.f;
         }
     }
+    if (EPI == EPI_DZ_ONE) __syncthreads();
     if constexpr (PLANES == 1) {
       store_tile<BM, BN, WM, WN>(lds, tid, [&](int i, int j, int r) { return T::enc(acc[i][j][r]); },
                                  [&](int v, int d, s16x8 x) { if (c0 + v < g.dz_cols) *reinterpret_cast<s16x8*>(g.dz + (c0 + v) * g.ld_dz + r0 + d) = x; });
