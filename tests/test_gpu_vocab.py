@@ -133,7 +133,7 @@ def check_distill(x, w, ids, logits, tau, dloss):
 
 
 SIZES = [(1, 1, 1), (1, 2, 3), (3, 5, 7), (2, 300, 64), (17, 130, 65), (64, 127, 64), (128, 128, 128), (129, 257, 192), (65, 1000, 100),
-         (300, 513, 256), (5, 8191, 72), (31, 4099, 320), (513, 81, 128), (1100, 1030, 136)]
+         (300, 513, 256), (5, 8191, 72), (31, 4099, 320), (513, 81, 128), (1100, 1030, 136), (3, 200, 8200), (9001, 130, 64), (270000, 40, 8)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
@@ -148,7 +148,7 @@ def test_xent(M, V, D, dtype):
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("M,V,D,K,tau", [(1, 1, 1, 1, 1.0), (1, 70, 64, 70, 2.0), (3, 5, 7, 2, 0.5), (17, 130, 65, 3, 4.0), (64, 500, 128, 64, 1.5), (200, 1111, 72, 65, 1.0),
-                                         (130, 300, 256, 8, 2.0), (5, 5000, 96, 200, 3.0)])
+                                         (130, 300, 256, 8, 2.0), (5, 5000, 96, 200, 3.0), (3, 3000, 64, 1024, 2.0), (9001, 100, 64, 3, 1.0)])
 def test_distill(M, V, D, K, tau, dtype):
     x, w, ids, dloss, logits = make(M, V, D, dtype, M + V + K, K)
     check_distill(x, w, ids, logits, tau, dloss)                       # random ids: some occur twice in a row
@@ -272,6 +272,29 @@ def test_several_pieces_of_the_vocabulary(dtype, M, V, D):
     x, w, labels, dloss = make(M, V, D, dtype, 12)
     labels[::7] = -1
     check_xent(x, w, labels, dloss)
+
+
+def test_two_calls_at_once():
+    """Two streams with calls of different shapes in flight: each gives what it gives alone."""
+    from gossipnet_amd import vocab
+    a, b = make(900, 20000, 512, "bf16", 30), make(300, 6000, 256, "f32", 31)
+
+    def run(x, w, labels, dloss):
+        loss, lse, hit = vocab.xent_forward(x, w, labels)
+        return (loss, lse, hit) + vocab.xent_backward(x, w, labels, lse, hit, dloss) + (vocab.embed_backward(labels, x, w)[0],)
+    want = [run(*a), run(*b)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(6):
+        for k, (s, args) in enumerate(zip(streams, (a, b))):
+            with torch.cuda.stream(s):
+                got[k].append(run(*args))
+    torch.cuda.synchronize()
+    for k in (0, 1):
+        for out in got[k]:
+            for p, q in zip(out, want[k]):
+                assert torch.equal(p, q)
 
 
 def test_repeats_are_bitwise_equal():
