@@ -27,13 +27,10 @@ __device__ __forceinline__ float wave_max(float v) {
   for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
   return v;
 }
-__device__ __forceinline__ int block_sum(int v, int* red) {
+__device__ __forceinline__ int wave_isum(int v) {
 #pragma unroll
   for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return red[0] + red[1] + red[2] + red[3];
+  return v;
 }
 __device__ __forceinline__ float block_max(float v, float* red) {
   v = wave_max(v);
@@ -229,39 +226,52 @@ struct PackArgs {
   PackW w;
 };
 template <int DT> __global__ void __launch_bounds__(256) vocab_pack(const PackArgs a) {
-  __shared__ int ired[4];
-  __shared__ float fred[4];
-  int ew = 0;
-  if (DT == GNET_F32) {
-    float mw = 0.f;
-    for (int i = threadIdx.x; i < W_PARTS; i += 256) mw = fmaxf(mw, a.w_part[i]);
-    ew = scale_exponent(block_max(mw, fred), 13);
-  }
-  if (blockIdx.x >= a.token_groups) { pack_w_rows<DT>(a.w, blockIdx.x - a.token_groups, ldexpf(1.f, ew)); return; }
+  __shared__ int ired[2][4];
+  __shared__ float fred[3][4];
+  __shared__ int place[256];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const bool packs_w = blockIdx.x >= a.token_groups;
   const int64_t r0 = (int64_t)blockIdx.x * a.rows, M = a.t.M;
   auto counts = [&](int64_t i) { int64_t id; return a.flag ? a.flag[i] != 0 : target_counts(a.t, i, id); };
+  // all that is looked through first, then one exchange between the waves
   int before = 0, all = 0;
-  float mg = 0.f, mx = 0.f;
-  if (a.flag) {
-    for (int64_t i = (int64_t)threadIdx.x * 4; i < a.flags_n; i += 1024) {
-      const int n = __popc(*reinterpret_cast<const unsigned*>(a.flag + i));      // flags are 0 or 1
-      all += n;
-      if (i < r0) before += n;                                                   // r0 is a multiple of 4
-    }
-    if (a.dloss) for (int64_t i = threadIdx.x; i < M; i += 256) mg = fmaxf(mg, a.row_g[i]);
-    if (DT == GNET_F32) for (int64_t i = threadIdx.x; i < M; i += 256) mx = fmaxf(mx, a.row_x[i]);
-  } else {
-    for (int64_t i = threadIdx.x; i < M; i += 256) {
-      const bool c = counts(i);
-      all += c;
-      if (i < r0) before += c;
-      if (a.dloss && c) mg = fmaxf(mg, fabsf(a.dloss[i] * a.t.inv_temp));
+  float mw = 0.f, mg = 0.f, mx = 0.f;
+  if (DT == GNET_F32)
+    for (int i = threadIdx.x; i < W_PARTS; i += 256) mw = fmaxf(mw, a.w_part[i]);
+  if (!packs_w) {
+    if (a.flag) {
+#pragma unroll 4
+      for (int64_t i = (int64_t)threadIdx.x * 4; i < a.flags_n; i += 1024) {
+        const int n = __popc(*reinterpret_cast<const unsigned*>(a.flag + i));      // flags are 0 or 1
+        all += n;
+        if (i < r0) before += n;                                                   // r0 is a multiple of 4
+      }
+      if (a.dloss)
+#pragma unroll 4
+        for (int64_t i = threadIdx.x; i < M; i += 256) mg = fmaxf(mg, a.row_g[i]);
+      if (DT == GNET_F32)
+#pragma unroll 4
+        for (int64_t i = threadIdx.x; i < M; i += 256) mx = fmaxf(mx, a.row_x[i]);
+    } else {
+#pragma unroll 4
+      for (int64_t i = threadIdx.x; i < M; i += 256) {
+        const bool c = counts(i);
+        all += c;
+        if (i < r0) before += c;
+        if (a.dloss && c) mg = fmaxf(mg, fabsf(a.dloss[i] * a.t.inv_temp));
+      }
     }
   }
-  before = block_sum(before, ired);
-  all = block_sum(all, ired);
-  if (a.dloss) mg = block_max(mg, fred);
-  if (DT == GNET_F32) mx = block_max(mx, fred);
+  before = wave_isum(before);
+  all = wave_isum(all);
+  if (DT == GNET_F32) { mw = wave_max(mw); mx = wave_max(mx); }
+  if (a.dloss) mg = wave_max(mg);
+  if (lane == 0) { ired[0][wave] = before; ired[1][wave] = all; fred[0][wave] = mw; fred[1][wave] = mx; fred[2][wave] = mg; }
+  __syncthreads();
+  before = all = 0;
+  for (int w = 0; w < 4; ++w) { before += ired[0][w]; all += ired[1][w]; mw = fmaxf(mw, fred[0][w]); mx = fmaxf(mx, fred[1][w]); mg = fmaxf(mg, fred[2][w]); }
+  const int ew = DT == GNET_F32 ? scale_exponent(mw, 13) : 0;
+  if (packs_w) { pack_w_rows<DT>(a.w, blockIdx.x - a.token_groups, ldexpf(1.f, ew)); return; }
   const int ex = DT == GNET_F32 ? scale_exponent(mx, 13) : 0, eg = a.dloss ? scale_exponent(mg, a.top_g) : 0;
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     a.meta->rows = all;
@@ -271,21 +281,21 @@ template <int DT> __global__ void __launch_bounds__(256) vocab_pack(const PackAr
   }
   RowCopy c = a.c;
   c.scale = ldexpf(1.f, ex);
-  __shared__ int place[256];                      // of 256 rows of the group: how many that count in front, ~ of it for one that does not
   const int wide = c.Dp >= 2048;                  // a whole workgroup a row, or a wave
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = wide ? threadIdx.x : lane;
+  const int t = wide ? threadIdx.x : lane;
+  // 256 rows of the group at a time: place[] = how many that count are in front of a row, or ~ of it for a row that does not
   for (int j0 = 0; j0 < a.rows; j0 += 256) {
     const int64_t base = r0 + j0, mine = base + threadIdx.x;
     const bool c256 = threadIdx.x < a.rows - j0 && mine < M && counts(mine);
     const unsigned long long mask = __ballot(c256);
     __syncthreads();
-    if (lane == 0) ired[wave] = __popcll(mask);
+    if (lane == 0) ired[0][wave] = __popcll(mask);
     __syncthreads();
     int rank = before + __popcll(mask & ((1ull << lane) - 1));
-    for (int w = 0; w < wave; ++w) rank += ired[w];
+    for (int w = 0; w < wave; ++w) rank += ired[0][w];
     place[threadIdx.x] = c256 ? rank : ~rank;
     if (mine < M && threadIdx.x < a.rows - j0) a.pos[mine] = c256 ? rank : -1;
-    before += ired[0] + ired[1] + ired[2] + ired[3];
+    before += ired[0][0] + ired[0][1] + ired[0][2] + ired[0][3];
     __syncthreads();
     const int n = (int)min((int64_t)min(256, a.rows - j0), a.Mp - base);
     for (int j = wide ? 0 : wave; j < n; j += wide ? 1 : 4) {
@@ -318,15 +328,13 @@ struct JoinArgs {
 // a token's largest logit and the log of the sum over the vocabulary of exp(z - largest), from its tiles', by one wave
 __device__ __forceinline__ void join_tiles(const float2* part, int tiles, int lane, float& top, float& log_sum) {
   float mx = -INFINITY, sum = 0.f;
-  for (int i = lane; i < tiles; i += 64) {
-    const float2 v = part[i];
-    const float n = fmaxf(mx, v.x), b = n == -INFINITY ? 0.f : n;
-    sum = sum * exp2f((mx - b) * LOG2E) + v.y * exp2f((v.x - b) * LOG2E);
-    mx = n;
-  }
-  const float all = wave_max(mx);
-  top = all == -INFINITY ? 0.f : all;
-  log_sum = logf(wave_sum(sum * exp2f((mx - top) * LOG2E)));
+#pragma unroll 8
+  for (int i = lane; i < tiles; i += 64) mx = fmaxf(mx, part[i].x);
+  mx = wave_max(mx);
+  top = mx == -INFINITY ? 0.f : mx;
+#pragma unroll 8
+  for (int i = lane; i < tiles; i += 64) sum += part[i].y * exp2f((part[i].x - top) * LOG2E);
+  log_sum = logf(wave_sum(sum));
 }
 // cross entropy: one wave per token
 __global__ void __launch_bounds__(256) vocab_join(const JoinArgs a) {
