@@ -219,7 +219,7 @@ struct PackArgs {
   unsigned token_groups;
   const void* x; int64_t ldx; u16* xp; RowCopy c;
   const float* row_x; const float* w_part;
-  const float* row_g; const float* dloss; const float* lse; int top_g;
+  const float* row_g; const float* dloss; const float* lse; float top_g;
   int32_t* pos; int32_t* label; int32_t* row_of; float* lse_c; float* gscale;
   void* dx;                            // its rows of tokens that do not count are zeroed here; NULL: later
   VocabMeta* meta;
@@ -272,12 +272,15 @@ template <int DT> __global__ void __launch_bounds__(256) vocab_pack(const PackAr
   for (int w = 0; w < 4; ++w) { before += ired[0][w]; all += ired[1][w]; mw = fmaxf(mw, fred[0][w]); mx = fmaxf(mx, fred[1][w]); mg = fmaxf(mg, fred[2][w]); }
   const int ew = DT == GNET_F32 ? scale_exponent(mw, 13) : 0;
   if (packs_w) { pack_w_rows<DT>(a.w, blockIdx.x - a.token_groups, ldexpf(1.f, ew)); return; }
-  const int ex = DT == GNET_F32 ? scale_exponent(mx, 13) : 0, eg = a.dloss ? scale_exponent(mg, a.top_g) : 0;
+  const int ex = DT == GNET_F32 ? scale_exponent(mx, 13) : 0;
+  // dz is stored in units of the largest |dloss|, not of a power of two: with one dloss for all tokens what is rounded to 16 bits is
+  // softmax - target itself, and the -1 of a label and the rest of its row are not off by different shares (top_g: 2^15 for fp16)
+  const float unit_g = mg >= 1.17549435e-38f && mg < INFINITY ? mg : 1.f;
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     a.meta->rows = all;
     a.meta->unscale_x = ldexpf(1.f, -ex);
     a.meta->unscale_w = ldexpf(1.f, -ew);
-    a.meta->unscale_g = ldexpf(1.f, -eg);
+    a.meta->unscale_g = unit_g / a.top_g;
   }
   RowCopy c = a.c;
   c.scale = ldexpf(1.f, ex);
@@ -310,7 +313,7 @@ template <int DT> __global__ void __launch_bounds__(256) vocab_pack(const PackAr
         if (a.row_of) a.row_of[to] = (int32_t)r;
         if (a.dloss) {
           a.lse_c[to] = a.lse[r];
-          a.gscale[to] = ldexpf(a.dloss[r] * a.t.inv_temp, eg);
+          a.gscale[to] = a.dloss[r] * a.t.inv_temp / unit_g * a.top_g;
         }
       }
     }
@@ -636,7 +639,7 @@ template <int DT, class T, int PLANES> struct Run {
     k.x = q.x; k.ldx = q.ldx; k.xp = (u16*)(ws + p.xp);
     k.c = RowCopy{q.D, p.Dp, p.Mp * p.Dp, 1.f, vec8(q.x, q.ldx, q.D, DT)};
     k.row_x = a.row_x; k.w_part = a.w_part;
-    k.row_g = a.row_g; k.dloss = dloss; k.lse = lse; k.top_g = DT == GNET_BF16 ? 0 : 14;
+    k.row_g = a.row_g; k.dloss = dloss; k.lse = lse; k.top_g = DT == GNET_BF16 ? 1.f : 32768.f;
     k.pos = (int32_t*)(ws + p.pos); k.label = q.t.logits ? nullptr : (int32_t*)(ws + p.label);
     k.lse_c = (float*)(ws + p.lse_c); k.gscale = (float*)(ws + p.gscale);
     k.meta = (VocabMeta*)(ws + p.meta);
