@@ -204,6 +204,16 @@ def test_large_logits_and_confident_rows(dtype):
     check_xent(x * 0, w, labels, dloss)                                # uniform
 
 
+def test_outliers_in_fp32():
+    """One power of two scales a whole tensor: rows and single values far above and far below the rest."""
+    x, w, labels, dloss = make(90, 400, 128, "f32", 16)
+    x[5, 3], x[6] = 3e4, x[6] * 1e-6
+    w[7], w[8], w[9, 1] = w[7] * 1e-8, w[8] * 50, 2000.0
+    check_xent(x, w, labels, dloss)
+    check_xent(x * 1e-20, w * 1e-15, labels, dloss)
+    check_xent(x * 1e12, w * 1e-12, labels, dloss * 1e9)
+
+
 def test_loss_gradients_of_all_sizes():
     x, w, labels, dloss = make(64, 300, 128, "f16", 10)
     for scale in (1e-30, 1e-3, 1e4, 0.0):
@@ -250,6 +260,22 @@ def test_strides_and_alignment(dtype):
     loss, lse, hit = vocab.xent_forward(x.reshape(7, 10, D), w, y)
     dx, dw = vocab.xent_backward(x.reshape(7, 10, D), w, y, lse, hit, dloss.reshape(7, 10))
     assert torch.equal(loss.flatten(), want[0]) and torch.equal(dx.reshape(M, D), want[3]) and torch.equal(dw, want[4])
+
+
+def test_one_token_without_dimensions():
+    from gossipnet_amd import vocab
+    x, w, labels, _ = make(1, 90, 64, "bf16", 15)
+    one = torch.tensor(1.0, device=DEV)
+    loss, lse, hit = vocab.xent_forward(x[0], w, labels[0])
+    dx, dw = vocab.xent_backward(x[0], w, labels[0], lse, hit, one)
+    a = vocab.xent_forward(x, w, labels)
+    b = vocab.xent_backward(x, w, labels, a[1], a[2], one)
+    assert loss.shape == lse.shape == hit.shape == () and float(loss) == float(a[0]) and dx.shape == (64,)
+    assert torch.equal(dx, b[0][0]) and torch.equal(dw, b[1])
+    y = vocab.embed_forward(labels[0], w)
+    assert y.shape == (64,) and torch.equal(y, w[labels[0]])
+    dt, ds = vocab.embed_backward(labels[0], y, w, need_dscale=True)
+    assert ds.shape == () and torch.equal(dt[labels[0]], y)
 
 
 def test_no_tokens():
