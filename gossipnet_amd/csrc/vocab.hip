@@ -2,9 +2,10 @@
 //   cross entropy   loss = lse(z) - z[label]                               (gnet_xent_*)
 //   distillation    loss = sum_k q_k (log q_k - z[id_k] + lse(z)),  q = softmax(teacher's logits / temperature)   (gnet_distill_*)
 // Cross entropy is distillation with one target of weight 1, so both run the same kernels:
-//   forward    vocab_targets  which tokens count, the teacher's weights      vocab_pack   the tokens that count, moved together
+//   forward    vocab_targets  which tokens count, the teacher's weights      vocab_pack   the tokens that count, moved together;
+//              the logits at the teacher's ids
 //              vocab_gemm<EPI_PART>  maximum and sum of 2^z per vocabulary tile, the label's logit
-//              vocab_join, vocab_join_targets   lse, the teacher's ids' logits, loss
+//              vocab_join   lse, loss
 //   backward   the first two, then for one piece of the vocabulary after the other
 //              vocab_gemm<EPI_DZ>  dz = g (softmax(z) - label) from recomputed logits       vocab_hits   dz at the teacher's ids
 //              vocab_gemm<EPI_SLAB>  dx += dz . W (fp32)     vocab_gemm<EPI_OUT>  dW = dz^T . x     and at last vocab_finish  dx
@@ -134,14 +135,22 @@ __global__ void __launch_bounds__(256) vocab_targets(const TargetsArgs a) {
       if (a.entropy) { ent = wave_sum(ent); if (lane == 0) a.entropy[m] = ent; }
       if (a.dloss) {
         __threadfence_block();                             // the wave reads back what its other lanes wrote
-        for (int kb = 0; kb < K; kb += 64) {
-          const int k = kb + lane;
+        auto slot = [&](int k, int& id32, float& q) {      // (an id that counts is below 2^30)
           int64_t id = -1;
           const bool c = k < K && target_counts(a.t, m * K + k, id);
-          float s = 0.f;
-          for (int j = 0; j < K; ++j)
-            if (c && load_id(a.t.ids, m * K + j, a.t.ids64) == id) s += a.q[m * K + j];
-          if (k < K) a.q_sum[m * K + k] = s;               // (an array of its own: later slots still read the single weights)
+          id32 = c ? (int)id : -1;
+          q = c ? a.q[m * K + k] : 0.f;
+        };
+        for (int kb = 0; kb < K; kb += 64) {
+          int id, other;
+          float q, s = 0.f;
+          slot(kb + lane, id, q);
+          for (int jb = 0; jb < K; jb += 64) {
+            slot(jb + lane, other, q);
+            for (int l = 0; l < min(64, K - jb); ++l)
+              if (__builtin_amdgcn_readlane(other, l) == id) s += __int_as_float(__builtin_amdgcn_readlane(__float_as_int(q), l));
+          }
+          if (kb + lane < K) a.q_sum[m * K + kb + lane] = s;       // (an array of its own: later slots still read the single weights)
         }
       }
     }
@@ -209,9 +218,75 @@ template <int DT> __global__ void __launch_bounds__(256) vocab_pack_w(const Pack
   pack_w_rows<DT>(a, blockIdx.x, DT == GNET_F32 ? 1.f / meta->unscale_w : 1.f);
 }
 
+// The student's logits at the teacher's ids, distillation's forward pass: fp32 dot products, four slots of a token a wave.
+template <int DT> __device__ __forceinline__ void dot8(const s16x8 (&x)[DT == GNET_F32 ? 2 : 1], const void* w, float& s) {
+  if constexpr (DT == GNET_F32) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const f32x4 a = __builtin_bit_cast(f32x4, x[h]), b = ((const f32x4*)w)[h];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s = fmaf(a[i], b[i], s);
+    }
+  } else {
+    const s16x8 b = *(const s16x8*)w;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      s = DT == GNET_BF16 ? fmaf(Bf16T::dec((u16)x[0][i]), Bf16T::dec((u16)b[i]), s) : fmaf(F16T::dec((u16)x[0][i]), F16T::dec((u16)b[i]), s);
+  }
+}
+template <int DT> __device__ __forceinline__ float load_elem(const void* p, int64_t i) {
+  if (DT == GNET_F32) return ((const float*)p)[i];
+  if (DT == GNET_BF16) return Bf16T::dec(((const u16*)p)[i]);
+  return F16T::dec(((const u16*)p)[i]);
+}
+struct DotArgs { const void* x; int64_t ldx; const void* w; int64_t ldw, D; int vec; float* hit; int per_token; };      // per_token: waves
+template <int DT> __device__ __forceinline__ void target_dots(const Targets& t, const DotArgs& a, int64_t unit) {
+  constexpr int SIZE = DT == GNET_F32 ? 4 : 2, U = 4;
+  const int64_t m = unit / a.per_token;
+  if (m >= t.M) return;
+  const int lane = threadIdx.x & 63, k0 = (int)(unit - m * a.per_token) * U;
+  const char* x = (const char*)a.x + m * a.ldx * SIZE;
+  const char* w[U];
+  bool c[U];
+  float dot[U];
+  bool some = false;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    int64_t id = 0;
+    c[u] = k0 + u < t.K && target_counts(t, m * t.K + k0 + u, id);
+    w[u] = (const char*)a.w + (c[u] ? id : 0) * a.ldw * SIZE;
+    dot[u] = 0.f;
+    some |= c[u];
+  }
+  if (some) {                                        // (a token that does not count: its x is not read)
+    if (a.vec) {
+#pragma unroll 2
+      for (int64_t d = (int64_t)lane * 8; d < a.D; d += 512) {
+        s16x8 xv[DT == GNET_F32 ? 2 : 1];
+#pragma unroll
+        for (int h = 0; h < (DT == GNET_F32 ? 2 : 1); ++h) xv[h] = ((const s16x8*)(x + d * SIZE))[h];
+#pragma unroll
+        for (int u = 0; u < U; ++u) dot8<DT>(xv, w[u] + d * SIZE, dot[u]);
+      }
+    } else {
+#pragma unroll 4
+      for (int64_t d = lane; d < a.D; d += 64) {
+        const float v = load_elem<DT>(x, d);
+#pragma unroll
+        for (int u = 0; u < U; ++u) dot[u] = fmaf(v, load_elem<DT>(w[u], d), dot[u]);
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const float z = wave_sum(dot[u]) * t.inv_temp;
+    if (lane == 0 && k0 + u < t.K) a.hit[m * t.K + k0 + u] = c[u] ? z : 0.f;
+  }
+}
+
 // Token workgroups: the tokens that count moved together, in order, zero rows behind them up to Mp.  Every workgroup counts the tokens
 // in front of its own rows: M bytes (or labels) out of L2 instead of a scan in a launch of its own.
-// The remaining workgroups pack the first piece of W.
+// Then workgroups that pack the first piece of W, and those of the targets' logits.
 struct PackArgs {
   Targets t;
   const uint8_t* flag;                 // NULL: cross entropy's labels are looked at directly
@@ -223,13 +298,15 @@ struct PackArgs {
   int32_t* pos; int32_t* label; int32_t* row_of; float* lse_c; float* gscale;
   void* dx;                            // its rows of tokens that do not count are zeroed here; NULL: later
   VocabMeta* meta;
-  PackW w;
+  PackW w; unsigned w_groups;
+  DotArgs dots;
 };
 template <int DT> __global__ void __launch_bounds__(256) vocab_pack(const PackArgs a) {
   __shared__ int ired[2][4];
   __shared__ float fred[3][4];
   __shared__ int place[256];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (blockIdx.x >= a.token_groups + a.w_groups) return target_dots<DT>(a.t, a.dots, (int64_t)(blockIdx.x - a.token_groups - a.w_groups) * 4 + (threadIdx.x >> 6));
   const bool packs_w = blockIdx.x >= a.token_groups;
   const int64_t r0 = (int64_t)blockIdx.x * a.rows, M = a.t.M;
   auto counts = [&](int64_t i) { int64_t id; return a.flag ? a.flag[i] != 0 : target_counts(a.t, i, id); };
@@ -324,9 +401,8 @@ template <int DT> __global__ void __launch_bounds__(256) vocab_pack(const PackAr
 struct JoinArgs {
   Targets t;
   const int32_t* pos; const float2* part; int tiles; const float* hit_c;     // hit_c: cross entropy's label logits, compacted
-  const void* x; int64_t ldx; const void* w; int64_t ldw; int64_t D; int vec;
   const float* q; const float* entropy;
-  float* loss; float* lse; float* hit;
+  float* loss; float* lse; float* hit;                                       // hit: distillation's comes from vocab_pack
 };
 // a token's largest logit and the log of the sum over the vocabulary of exp(z - largest), from its tiles', by one wave
 __device__ __forceinline__ void join_tiles(const float2* part, int tiles, int lane, float& top, float& log_sum) {
@@ -339,92 +415,27 @@ __device__ __forceinline__ void join_tiles(const float2* part, int tiles, int la
   for (int i = lane; i < tiles; i += 64) sum += part[i].y * exp2f((part[i].x - top) * LOG2E);
   log_sum = logf(wave_sum(sum));
 }
-// cross entropy: one wave per token
+// one wave per token
 __global__ void __launch_bounds__(256) vocab_join(const JoinArgs a) {
   const int64_t m = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (m >= a.t.M) return;
-  const int p = a.pos[m], lane = threadIdx.x & 63;
-  float top = 0.f, log_sum = 0.f, hit = 0.f;
-  if (p >= 0) { join_tiles(a.part + (int64_t)p * a.tiles, a.tiles, lane, top, log_sum); hit = a.hit_c[p]; }
-  if (lane) return;
-  const float loss = (top - hit) + log_sum;        // both from the same products: where the label takes nearly everything nothing cancels
-  a.loss[m] = loss < 0.f ? 0.f : loss;             // (below 0 from rounding only; NaN stays)
-  a.lse[m] = top + log_sum;
-  a.hit[m] = hit;
-}
-template <int DT> __device__ __forceinline__ void dot8(const void* x, const void* w, float& s) {
-  if (DT == GNET_F32) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const f32x4 a = ((const f32x4*)x)[h], b = ((const f32x4*)w)[h];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s = fmaf(a[i], b[i], s);
-    }
-  } else {
-    const s16x8 a = *(const s16x8*)x, b = *(const s16x8*)w;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      s = DT == GNET_BF16 ? fmaf(Bf16T::dec((u16)a[i]), Bf16T::dec((u16)b[i]), s) : fmaf(F16T::dec((u16)a[i]), F16T::dec((u16)b[i]), s);
-  }
-}
-// distillation: one workgroup per token, a wave takes two of its targets at a time: their logits are fp32 dot products
-template <int DT> __global__ void __launch_bounds__(256) vocab_join_targets(const JoinArgs a) {
-  __shared__ float red[4];
-  constexpr int SIZE = DT == GNET_F32 ? 4 : 2;
-  const int64_t m = blockIdx.x;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, K = a.t.K;
-  const int p = a.pos[m];
-  if (p < 0) {
-    for (int k = threadIdx.x; k < K; k += 256) a.hit[m * K + k] = 0.f;
-    if (threadIdx.x == 0) { a.loss[m] = 0.f; a.lse[m] = 0.f; }
-    return;
-  }
-  float top, log_sum;
-  join_tiles(a.part + (int64_t)p * a.tiles, a.tiles, lane, top, log_sum);
+  const int p = a.pos[m], lane = threadIdx.x & 63, K = a.t.K;
+  float top = 0.f, log_sum = 0.f, loss = 0.f;
+  if (p >= 0) join_tiles(a.part + (int64_t)p * a.tiles, a.tiles, lane, top, log_sum);
   const float lse = top + log_sum;
-  float loss = 0.f;
-  const char* x = (const char*)a.x + m * a.ldx * SIZE;
-  for (int k = wave; k < K; k += 8) {
-    int64_t id[2];
-    bool c[2];
-    float dot[2] = {0.f, 0.f};
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      c[u] = k + 4 * u < K && target_counts(a.t, m * K + k + 4 * u, id[u]);
-      if (!c[u]) id[u] = 0;
+  if (!a.t.logits) {
+    const float hit = p >= 0 ? a.hit_c[p] : 0.f;
+    loss = (top - hit) + log_sum;                  // both from the same products: where the label takes nearly everything nothing cancels
+    if (loss < 0.f) loss = 0.f;                    // (below 0 from rounding only; NaN stays)
+    if (lane == 0) a.hit[m] = hit;
+  } else if (p >= 0) {
+    for (int k = lane; k < K; k += 64) {
+      const float q = a.q[m * K + k];
+      if (q != 0.f) loss += q * (lse - a.hit[m * K + k]);      // (an infinite logit of a target without weight stays out)
     }
-    const char* w0 = (const char*)a.w + id[0] * a.ldw * SIZE;
-    const char* w1 = (const char*)a.w + id[1] * a.ldw * SIZE;
-    if (a.vec) {
-      for (int64_t d = (int64_t)lane * 8; d < a.D; d += 512) {
-        dot8<DT>(x + d * SIZE, w0 + d * SIZE, dot[0]);
-        dot8<DT>(x + d * SIZE, w1 + d * SIZE, dot[1]);
-      }
-    } else {
-      for (int64_t d = lane; d < a.D; d += 64) {
-        const float v = DT == GNET_F32 ? ((const float*)x)[d] : DT == GNET_BF16 ? Bf16T::dec(((const u16*)x)[d]) : F16T::dec(((const u16*)x)[d]);
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const char* w = u ? w1 : w0;
-          dot[u] = fmaf(v, DT == GNET_F32 ? ((const float*)w)[d] : DT == GNET_BF16 ? Bf16T::dec(((const u16*)w)[d]) : F16T::dec(((const u16*)w)[d]), dot[u]);
-        }
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      if (k + 4 * u >= K) continue;
-      const int64_t i = m * K + k + 4 * u;
-      const float z = wave_sum(dot[u]) * a.t.inv_temp;
-      if (c[u]) { const float q = a.q[i]; if (q != 0.f) loss += q * (lse - z); }       // (an infinite logit of a target without weight stays out)
-      if (lane == 0) a.hit[i] = c[u] ? z : 0.f;
-    }
+    loss = wave_sum(loss) + a.entropy[m];
   }
-  if (lane == 0) red[wave] = loss;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    a.loss[m] = (red[0] + red[1]) + (red[2] + red[3]) + a.entropy[m];
-    a.lse[m] = lse;
-  }
+  if (lane == 0) { a.loss[m] = loss; a.lse[m] = lse; }
 }
 
 // dz at the teacher's ids of one piece of the vocabulary: (softmax - weight) g from the forward pass's fp32 logits, over what
@@ -615,7 +626,7 @@ template <int DT, class T, int PLANES> struct Run {
     return k;
   }
   // everything in front of the first product, the first piece of W included
-  static void prepare(const Problem& q, const Plan& p, char* ws, const float* dloss, const float* lse, void* dx, hipStream_t s) {
+  static void prepare(const Problem& q, const Plan& p, char* ws, const float* dloss, const float* lse, void* dx, float* hit, hipStream_t s) {
     TargetsArgs a = {};
     a.t = q.t; a.flags_n = p.flags_n; a.token_groups = (unsigned)tiles(p.flags_n, 4);
     a.dloss = dloss;
@@ -644,8 +655,13 @@ template <int DT, class T, int PLANES> struct Run {
     k.lse_c = (float*)(ws + p.lse_c); k.gscale = (float*)(ws + p.gscale);
     k.meta = (VocabMeta*)(ws + p.meta);
     if (dx && p.dx_direct) { k.dx = dx; k.row_of = (int32_t*)(ws + p.row_of); }
-    if (p.pack_w) k.w = pack_of_w(q, p, ws, 0);
-    vocab_pack<DT><<<k.token_groups + (p.pack_w ? (unsigned)tiles(p.piece, PACK_W_ROWS) : 0), 256, 0, s>>>(k);
+    if (p.pack_w) { k.w = pack_of_w(q, p, ws, 0); k.w_groups = (unsigned)tiles(p.piece, PACK_W_ROWS); }
+    unsigned groups = k.token_groups + k.w_groups;
+    if (hit && q.t.logits) {
+      k.dots = DotArgs{q.x, q.ldx, q.w, q.ldw, q.D, vec8(q.x, q.ldx, q.D, DT) && vec8(q.w, q.ldw, q.D, DT), hit, (q.t.K + 3) / 4};
+      groups += (unsigned)tiles(q.t.M * k.dots.per_token, 4);
+    }
+    vocab_pack<DT><<<groups, 256, 0, s>>>(k);
   }
 
   // W rows v0 .. of one piece as an operand (packed first where needed)
@@ -676,7 +692,7 @@ template <int DT, class T, int PLANES> struct Run {
   }
 
   static int forward(const Problem& q, const Plan& p, char* ws, float* loss, float* lse, float* hit, hipStream_t s) {
-    prepare(q, p, ws, nullptr, nullptr, nullptr, s);
+    prepare(q, p, ws, nullptr, nullptr, nullptr, hit, s);
     for (int64_t v0 = 0; v0 < q.t.V; v0 += p.piece) {
       VocabGemm g = logits(q, p, ws, piece_of_w(q, p, ws, v0, s), v0);
       g.part = (float2*)(ws + p.part); g.hit = (float*)(ws + p.hit_c);
@@ -685,11 +701,9 @@ template <int DT, class T, int PLANES> struct Run {
     }
     JoinArgs j = {};
     j.t = q.t; j.pos = (const int32_t*)(ws + p.pos); j.part = (const float2*)(ws + p.part); j.tiles = (int)p.w_tiles; j.hit_c = (const float*)(ws + p.hit_c);
-    j.x = q.x; j.ldx = q.ldx; j.w = q.w; j.ldw = q.ldw; j.D = q.D; j.vec = vec8(q.x, q.ldx, q.D, DT) && vec8(q.w, q.ldw, q.D, DT);
     j.q = (const float*)(ws + p.q); j.entropy = (const float*)(ws + p.entropy);
     j.loss = loss; j.lse = lse; j.hit = hit;
-    if (q.t.logits) vocab_join_targets<DT><<<(unsigned)q.t.M, 256, 0, s>>>(j);
-    else vocab_join<<<(unsigned)tiles(q.t.M, 4), 256, 0, s>>>(j);
+    vocab_join<<<(unsigned)tiles(q.t.M, 4), 256, 0, s>>>(j);
     return launch_status();
   }
 
@@ -700,7 +714,7 @@ template <int DT, class T, int PLANES> struct Run {
   }
 
   static int backward(const Problem& q, const Plan& p, char* ws, const float* lse, const float* hit, const float* dloss, void* dx, void* dw, hipStream_t s) {
-    prepare(q, p, ws, dloss, lse, dx, s);
+    prepare(q, p, ws, dloss, lse, dx, nullptr, s);
     const VocabMeta* meta = (const VocabMeta*)(ws + p.meta);
     const int elem = DT == GNET_F32 ? 4 : 2;
     for (int64_t v0 = 0; v0 < q.t.V; v0 += p.piece) {
