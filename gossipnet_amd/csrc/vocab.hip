@@ -205,7 +205,7 @@ template <int DT> __device__ __forceinline__ void zero_row(void* out, int64_t fi
     else ((u16*)out)[first + d] = 0;
   }
 }
-// Rows of W that the matrix products cannot read where they lie (32 bits; widths that are no multiple of 64; alignment).
+// Rows of W that the matrix products cannot read where they lie (32 bits; widths that are no multiple of 8; alignment).
 struct PackW { const void* w; int64_t ldw, rows, rows_out; u16* dst; RowCopy c; };
 constexpr int PACK_W_ROWS = 16;
 template <int DT> __device__ __forceinline__ void pack_w_rows(const PackW& a, int64_t group, float scale) {
@@ -583,7 +583,7 @@ Plan make_plan(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int distil
 }
 
 int needs_pack(const void* w, int64_t ldw, int64_t D, int dtype) {
-  return dtype == GNET_F32 || (D & 63) || (ldw & 7) || ldw > (1 << 22) || ((uintptr_t)w & 15);      // (2^22: 32-bit offsets in a tile)
+  return dtype == GNET_F32 || (D & 7) || (ldw & 7) || ldw > (1 << 22) || ((uintptr_t)w & 15);      // (2^22: 32-bit offsets in a tile)
 }
 // eight elements at a time
 int vec8(const void* p, int64_t ld, int64_t D, int dtype) {
@@ -673,7 +673,7 @@ template <int DT, class T, int PLANES> struct Run {
     } else {
       o.p = (const u16*)q.w + v0 * q.ldw; o.ld = q.ldw; o.plane = 0; o.rows = q.t.V - v0;
     }
-    o.cols = (int)p.Dp;
+    o.cols = (int)(p.pack_w ? p.Dp : q.D);
     return o;
   }
   static VocabOperand packed_x(const Plan& p, char* ws) {

@@ -55,7 +55,7 @@ struct VocabOperand {
   int64_t ld;          // elements between rows as they lie in memory
   int64_t plane;       // elements between the two planes of a 32-bit operand
   int64_t rows;        // rows that may be read: a row index beyond is clamped to the last (its products are zero or not stored)
-  int cols;            // contraction-strided operands: elements of a row that may be read (a multiple of 8)
+  int cols;            // elements of a row that may be read (a multiple of 8): a chunk beyond is replaced by the last (zeros of the other operand)
 };
 
 struct VocabGemm {
@@ -115,11 +115,13 @@ template <int T, bool STRIDED, int WAVES> struct Stager {
   unsigned off[N];
   int64_t step_bytes, rows;
   unsigned row_bytes;
+  int cols;
 
   static __device__ __forceinline__ int op(int u, int wave) { return (u * WAVES + wave) % OPS; }
   __device__ __forceinline__ void init(const VocabOperand& o, int64_t t0, int64_t k0, int wave, int lane) {
     row_bytes = (unsigned)(o.ld * 2);
     rows = o.rows;
+    cols = o.cols;
     if (!STRIDED) {
       base = (const char*)(o.p + t0 * o.ld + k0);
       step_bytes = VG_BK * 2;
@@ -139,15 +141,16 @@ template <int T, bool STRIDED, int WAVES> struct Stager {
       }
     }
   }
-  // stage s counted from k0, whose contraction index is k, `plane` bytes further on; CLAMP: the rows may end inside or in front of it
+  // stage s counted from k0, whose contraction index is k, `plane` bytes further on; CLAMP: the contraction may end inside or in front of it
   template <bool CLAMP> __device__ __forceinline__ void load(unsigned lds, int s, int64_t k, int64_t plane, int wave, int lane) const {
     const char* from = base + s * step_bytes + plane;
 #pragma unroll
     for (int u = 0; u < N; ++u) {
       const unsigned to = lds + op(u, wave) * 1024;
       if (!CLAMP) { load_to_lds(from, off[u], to); continue; }
-      const int64_t beyond = STRIDED ? max(k + (op(u, wave) * 64 + lane) / CH - (rows - 1), (int64_t)0) : 0;
-      load_to_lds(from + off[u] - beyond * row_bytes, to);
+      // (contraction-strided: rows beyond the last; contraction-contiguous: elements beyond a row's)
+      const int64_t beyond = STRIDED ? (k + (op(u, wave) * 64 + lane) / CH - (rows - 1)) * row_bytes : (k + ((lane & 7) ^ (lane >> 3)) * 8 - (cols - 8)) * 2;
+      load_to_lds(from + off[u] - max(beyond, (int64_t)0), to);
     }
   }
 };
