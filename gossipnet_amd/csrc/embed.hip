@@ -33,7 +33,26 @@ template <int DT> __device__ __forceinline__ typename Elem<DT>::type enc(float v
   else if constexpr (DT == GNET_BF16) return Bf16T::enc(v);
   else return F16T::enc(v);
 }
-template <class E, int VEC> struct alignas(sizeof(E) * VEC) Pack { E v[VEC]; };
+// VEC elements of a row at once, at the alignment of an element; what is left behind the last whole VEC one by one
+template <class E, int VEC> struct Pack {
+  typedef E V __attribute__((ext_vector_type(VEC)));
+  typedef E U __attribute__((ext_vector_type(VEC), aligned(sizeof(E))));
+  V v;
+};
+template <class E, int VEC> __device__ __forceinline__ Pack<E, VEC> load_pack(const E* p, int64_t left) {
+  Pack<E, VEC> o;
+  if (left >= VEC) o.v = *reinterpret_cast<const typename Pack<E, VEC>::U*>(p);
+  else
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) o.v[i] = i < left ? p[i] : (E)0;
+  return o;
+}
+template <class E, int VEC> __device__ __forceinline__ void store_pack(E* p, const Pack<E, VEC>& o, int64_t left) {
+  if (left >= VEC) *reinterpret_cast<typename Pack<E, VEC>::U*>(p) = o.v;
+  else
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) if (i < left) p[i] = o.v[i];
+}
 
 __device__ __forceinline__ int64_t load_id(const void* p, int64_t i, int is64) {
   return is64 ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
@@ -53,7 +72,7 @@ template <int DT, int VEC> __global__ void __launch_bounds__(256) embed_rows_out
   const int64_t id = load_id(a.ids, m, a.ids64);
   Pack<E, VEC> o;
   if (id >= 0 && id < a.V) {
-    const Pack<E, VEC> t = *reinterpret_cast<const Pack<E, VEC>*>((const E*)a.table + id * a.ld + d);
+    const Pack<E, VEC> t = load_pack<E, VEC>((const E*)a.table + id * a.ld + d, a.D - d);
     const float s = a.token_scale ? a.scale * a.token_scale[m] : a.scale;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) o.v[i] = enc<DT>(dec<DT>(t.v[i]) * s);
@@ -61,7 +80,7 @@ template <int DT, int VEC> __global__ void __launch_bounds__(256) embed_rows_out
 #pragma unroll
     for (int i = 0; i < VEC; ++i) o.v[i] = enc<DT>(0.f);
   }
-  *reinterpret_cast<Pack<E, VEC>*>((E*)a.y + m * a.D + d) = o;
+  store_pack<E, VEC>((E*)a.y + m * a.D + d, o, a.D - d);
 }
 
 // ---- the order of the tokens ------------------------------------------------------------------------------------------
@@ -165,7 +184,7 @@ struct BackwardArgs {
   const u64* keys; int64_t M, V, D;
   const void* dy; int64_t ld; float scale; const float* token_scale;
   void* out; int64_t ld_out; int accumulate;
-  float* part;                         // [segment][2][D]
+  float* part; int64_t ld_part;        // [segment][2][D rounded up to 8]
   unsigned hot_groups, run_groups, scale_groups;     // workgroups of each kind, in this order; the zero rows get the rest
   const void* ids; int ids64; const void* table; int64_t ld_table; float* dscale;
 };
@@ -188,7 +207,7 @@ template <int DT, int VEC, int U, int NB> __device__ __forceinline__ void add_to
       s[u] = a.token_scale ? a.token_scale[m] : 1.f;
 #pragma unroll
       for (int b = 0; b < NB; ++b)
-        if (b < blocks && d + b * step < a.D) g[u][b] = *reinterpret_cast<const Pack<E, VEC>*>((const E*)a.dy + m * a.ld + d + b * step);
+        if (b < blocks && d + b * step < a.D) g[u][b] = load_pack<E, VEC>((const E*)a.dy + m * a.ld + d + b * step, a.D - d - b * step);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -203,12 +222,12 @@ template <int DT, int VEC, int U, int NB> __device__ __forceinline__ void add_to
 }
 template <int DT, int VEC> __device__ __forceinline__ void store_row(const float (&sum)[VEC], const BackwardArgs& a, int64_t v, int64_t d) {
   typedef typename Elem<DT>::type E;
-  Pack<E, VEC>* p = reinterpret_cast<Pack<E, VEC>*>((E*)a.out + v * a.ld_out + d);
+  E* p = (E*)a.out + v * a.ld_out + d;
   Pack<E, VEC> o;
-  if (a.accumulate) o = *p;
+  if (a.accumulate) o = load_pack<E, VEC>(p, a.D - d);
 #pragma unroll
   for (int i = 0; i < VEC; ++i) o.v[i] = enc<DT>(a.accumulate ? dec<DT>(o.v[i]) + sum[i] * a.scale : sum[i] * a.scale);
-  *p = o;
+  store_pack<E, VEC>(p, o, a.D - d);
 }
 
 // 64 consecutive keys from place p on, one a lane: id (NONE outside the order) and token
@@ -264,7 +283,7 @@ template <int DT, int VEC> __device__ __forceinline__ void hot_sums(const Backwa
       float sum[1][VEC];
       add_tokens<DT, VEC, 8, 1>(sum, a, token, b, e, d, 0, 1);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) a.part[(seg * 2 + slot) * a.D + d + i] = sum[0][i];
+      for (int i = 0; i < VEC; ++i) a.part[(seg * 2 + slot) * a.ld_part + d + i] = sum[0][i];
     }
   }
 }
@@ -280,7 +299,7 @@ template <int DT, int VEC> __device__ __forceinline__ void fill_rows(const Backw
   for (int i = 0; i < VEC; ++i) zero.v[i] = enc<DT>(0.f);
   for (int r = threadIdx.x >> 6; r < FILL_ROWS && v0 + r < a.V; r += 4)
     if (start[r] == start[r + 1])
-      for (int64_t d = (int64_t)(threadIdx.x & 63) * VEC; d < a.D; d += 64 * VEC) *reinterpret_cast<Pack<E, VEC>*>((E*)a.out + (v0 + r) * a.ld_out + d) = zero;
+      for (int64_t d = (int64_t)(threadIdx.x & 63) * VEC; d < a.D; d += 64 * VEC) store_pack<E, VEC>((E*)a.out + (v0 + r) * a.ld_out + d, zero, a.D - d);
 }
 
 template <int DT, int VEC> __device__ __forceinline__ void scale_gradient(const BackwardArgs& a, int64_t m) {
@@ -291,8 +310,8 @@ template <int DT, int VEC> __device__ __forceinline__ void scale_gradient(const 
   if (id >= 0 && id < a.V) {
 #pragma unroll 4
     for (int64_t d = (int64_t)(threadIdx.x & 63) * VEC; d < a.D; d += 64 * VEC) {
-      const Pack<E, VEC> t = *reinterpret_cast<const Pack<E, VEC>*>((const E*)a.table + id * a.ld_table + d);
-      const Pack<E, VEC> g = *reinterpret_cast<const Pack<E, VEC>*>((const E*)a.dy + m * a.ld + d);
+      const Pack<E, VEC> t = load_pack<E, VEC>((const E*)a.table + id * a.ld_table + d, a.D - d);
+      const Pack<E, VEC> g = load_pack<E, VEC>((const E*)a.dy + m * a.ld + d, a.D - d);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) dot = fmaf(dec<DT>(t.v[i]), dec<DT>(g.v[i]), dot);
     }
@@ -338,11 +357,11 @@ template <int DT, int VEC> __global__ void __launch_bounds__(256) embed_hot_rows
   if (d < a.D) {
     if (wave == 0)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) sum[i] = a.part[(seg * 2 + (whole ? 0 : 1)) * a.D + d + i];
+      for (int i = 0; i < VEC; ++i) sum[i] = a.part[(seg * 2 + (whole ? 0 : 1)) * a.ld_part + d + i];
 #pragma unroll 4
     for (int64_t s = s0; s < s1; ++s)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) sum[i] += a.part[s * 2 * a.D + d + i];
+      for (int i = 0; i < VEC; ++i) sum[i] += a.part[s * 2 * a.ld_part + d + i];
   }
   if (wave)
 #pragma unroll
@@ -355,12 +374,10 @@ template <int DT, int VEC> __global__ void __launch_bounds__(256) embed_hot_rows
   }
 }
 
-// Elements a lane takes at once: the widest access that width, row strides and addresses allow (16 bytes at most) and that still
-// gives every lane of a wave something to do.
-int pick_vec(int dtype, int64_t D, int64_t ld0, int64_t ld1, const void* p0, const void* p1) {
-  const int size = dtype == GNET_F32 ? 4 : 2;
-  int v = 16 / size;
-  while (v > 1 && (D % v || ld0 % v || ld1 % v || ((uintptr_t)p0 | (uintptr_t)p1) % (v * size) || D < 64 * v)) v >>= 1;
+// Elements a lane takes at once: 16 bytes, or as many as still give every lane of a wave something to do.
+int pick_vec(int dtype, int64_t D) {
+  int v = dtype == GNET_F32 ? 4 : 8;
+  while (v > 1 && D < 64 * v) v >>= 1;
   return v;
 }
 template <template <int, int> class F, class A> void launch(int dtype, int vec, const A& a, dim3 grid, hipStream_t s) {
@@ -397,7 +414,7 @@ extern "C" int gnet_embed_forward(const void* ids, int32_t ids64, const void* ta
   if (M == 0) return GNET_OK;
   if (!ids || !table || !y) return GNET_ERR_INVALID;
   ForwardArgs a{ids, ids64, M, V, D, table, ld_table, scale, token_scale, y, 1};
-  const int vec = pick_vec(dtype, D, ld_table, D, table, y);
+  const int vec = pick_vec(dtype, D);
   a.blocks = (int)((D + 64 * vec - 1) / (64 * vec));
   launch<GoForward>(dtype, vec, a, (unsigned)((M * a.blocks + 3) / 4), (hipStream_t)stream);
   return launch_status();
@@ -405,7 +422,7 @@ extern "C" int gnet_embed_forward(const void* ids, int32_t ids64, const void* ta
 
 extern "C" size_t gnet_embed_workspace_bytes(int64_t M, int64_t D) {
   if (M <= 0 || D <= 0 || M > (1 << 24) || D > (1 << 16)) return 0;
-  return 2 * keys_bytes(M) + (size_t)((M + HOT - 1) / HOT) * 2 * D * 4;
+  return 2 * keys_bytes(M) + (size_t)((M + HOT - 1) / HOT) * 2 * ((D + 7) & ~7ll) * 4;
 }
 
 extern "C" int gnet_embed_backward(const void* ids, int32_t ids64, const void* dy, int64_t ld_dy, float scale, const float* token_scale,
@@ -430,12 +447,8 @@ extern "C" int gnet_embed_backward(const void* ids, int32_t ids64, const void* d
       u64* t = keys; keys = other; other = t;
     }
   }
-  BackwardArgs a{keys, M, V, D, dy, ld_dy, scale, token_scale, dtable, D, accumulate, part, 0, 0, 0, ids, ids64, table, ld_table, dscale};
-  int vec = M ? pick_vec(dtype, D, ld_dy, D, dy, dtable) : pick_vec(dtype, D, D, D, dtable, dtable);
-  if (dscale && M) {
-    const int of_table = pick_vec(dtype, D, ld_table, D, table, dtable);
-    vec = of_table < vec ? of_table : vec;
-  }
+  BackwardArgs a{keys, M, V, D, dy, ld_dy, scale, token_scale, dtable, D, accumulate, part, (D + 7) & ~7ll, 0, 0, 0, ids, ids64, table, ld_table, dscale};
+  const int vec = pick_vec(dtype, D);
   const unsigned segments = (unsigned)((M + HOT - 1) / HOT);
   a.hot_groups = M > HOT ? segments : 0;
   a.run_groups = (unsigned)((M + 3) / 4);

@@ -40,6 +40,13 @@ __device__ __forceinline__ float block_max(float v, float* red) {
   __syncthreads();
   return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 }
+__device__ __forceinline__ float block_sum(float v, float* red) {
+  v = wave_sum(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return (red[0] + red[1]) + (red[2] + red[3]);
+}
 // the exponent of the power of two that brings a magnitude into [2^top, 2^(top+1)); 0 for 0, infinities and NaN
 __device__ __forceinline__ int scale_exponent(float a, int top) {
   if (!(a > 0.f) || !(a < INFINITY)) return 0;
@@ -70,33 +77,27 @@ struct TargetsArgs {
   uint8_t* flag; float* q; float* q_sum; float* entropy;       // q, entropy: distillation; q_sum: its backward pass
   const float* x; int64_t ldx, D; float* row_x;                // 32-bit x: the row's largest magnitude
   const float* dloss; float* row_g;                            // backward only
-  const float* w; int64_t ldw; float* w_part; int w_vec;       // w_vec: rows of whole, aligned float4
+  const float* w; int64_t ldw; float* w_part;
 };
+// the largest magnitude of a thread's share of n consecutive values
+__device__ __forceinline__ float magnitude(const float* p, int64_t n, int64_t t, int64_t threads) {
+  float mx = 0.f;
+#pragma unroll 4
+  for (int64_t i = t; i < n / 4; i += threads) {
+    const f32x4 v = *reinterpret_cast<const f32x4u*>(p + i * 4);
+    mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))));
+  }
+  for (int64_t i = n / 4 * 4 + t; i < n; i += threads) mx = fmaxf(mx, fabsf(p[i]));
+  return mx;
+}
 __global__ void __launch_bounds__(256) vocab_targets(const TargetsArgs a) {
   const int lane = threadIdx.x & 63;
   if (blockIdx.x >= a.token_groups) {
     __shared__ float red[4];
     const unsigned part = blockIdx.x - a.token_groups;
     float mx = 0.f;
-    if (a.w_vec) {
-      const int64_t per_row = a.D / 4, n = a.t.V * per_row;
-      const float4* w = (const float4*)a.w;
-      if (a.ldw == a.D) {
-        for (int64_t i = (int64_t)part * 256 + threadIdx.x; i < n; i += W_PARTS * 256ll) {
-          const float4 v = w[i];
-          mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
-        }
-      } else {
-        for (int64_t r = part; r < a.t.V; r += W_PARTS)
-          for (int64_t d = threadIdx.x; d < per_row; d += 256) {
-            const float4 v = w[r * (a.ldw / 4) + d];
-            mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
-          }
-      }
-    } else {
-      for (int64_t r = part; r < a.t.V; r += W_PARTS)
-        for (int64_t d = threadIdx.x; d < a.D; d += 256) mx = fmaxf(mx, fabsf(a.w[r * a.ldw + d]));
-    }
+    if (a.ldw == a.D) mx = magnitude(a.w, a.t.V * a.D, (int64_t)part * 256 + threadIdx.x, W_PARTS * 256ll);
+    else for (int64_t r = part; r < a.t.V; r += W_PARTS) mx = fmaxf(mx, magnitude(a.w + r * a.ldw, a.D, threadIdx.x, 256));
     mx = block_max(mx, red);
     if (threadIdx.x == 0) a.w_part[part] = mx;
     return;
@@ -156,7 +157,7 @@ __global__ void __launch_bounds__(256) vocab_targets(const TargetsArgs a) {
     }
     if (a.row_x) {
       float mx = 0.f;
-      if (counts) for (int64_t d = lane; d < a.D; d += 64) mx = fmaxf(mx, fabsf(a.x[m * a.ldx + d]));
+      if (counts) mx = magnitude(a.x + m * a.ldx, a.D, lane, 64);
       mx = wave_max(mx);
       if (lane == 0) a.row_x[m] = mx;
     }
@@ -166,37 +167,38 @@ __global__ void __launch_bounds__(256) vocab_targets(const TargetsArgs a) {
 }
 
 // Rows copied to the matrix products' layout: Dp elements (a multiple of 64), zeros behind D; 32 bits as two fp16 planes.
-struct RowCopy { int64_t D, Dp, plane; float scale; int vec; };        // vec: 8 elements at a time (alignment and D allow it)
+struct RowCopy { int64_t D, Dp, plane; float scale; };
 template <int DT> __device__ __forceinline__ void copy_row(const void* src, int64_t first, bool zero, u16* dst, const RowCopy& c, int t, int threads) {
-  if (c.vec || zero) {
-    for (int64_t d = (int64_t)t * 8; d < c.Dp; d += (int64_t)threads * 8) {
-      s16x8 hi = {0, 0, 0, 0, 0, 0, 0, 0}, lo = hi;
-      if (!zero && d < c.D) {
-        if (DT == GNET_F32) {
-          const f32x4 v0 = *reinterpret_cast<const f32x4*>((const float*)src + first + d), v1 = *reinterpret_cast<const f32x4*>((const float*)src + first + d + 4);
+  for (int64_t d = (int64_t)t * 8; d < c.Dp; d += (int64_t)threads * 8) {
+    s16x8 hi = {0, 0, 0, 0, 0, 0, 0, 0}, lo = hi;
+    if (!zero) {
+      if (DT == GNET_F32) {
+        const float* p = (const float*)src + first + d;
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (d + 8 <= c.D) {
+          const f32x4 v0 = *reinterpret_cast<const f32x4u*>(p), v1 = *reinterpret_cast<const f32x4u*>(p + 4);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            u16 h, l;
-            split_f16((i < 4 ? v0[i & 3] : v1[i & 3]) * c.scale, h, l);
-            hi[i] = (short)h; lo[i] = (short)l;
-          }
+          for (int i = 0; i < 8; ++i) v[i] = i < 4 ? v0[i & 3] : v1[i & 3];
         } else {
-          hi = *reinterpret_cast<const s16x8*>((const u16*)src + first + d);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) if (d + i < c.D) v[i] = p[i];
         }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          u16 h, l;
+          split_f16(v[i] * c.scale, h, l);
+          hi[i] = (short)h; lo[i] = (short)l;
+        }
+      } else {
+        const u16* p = (const u16*)src + first + d;
+        if (d + 8 <= c.D) hi = *reinterpret_cast<const s16x8u*>(p);
+        else
+#pragma unroll
+          for (int i = 0; i < 8; ++i) if (d + i < c.D) hi[i] = (short)p[i];
       }
-      *reinterpret_cast<s16x8*>(dst + d) = hi;
-      if (DT == GNET_F32) *reinterpret_cast<s16x8*>(dst + c.plane + d) = lo;
     }
-  } else {
-    for (int64_t d = t; d < c.Dp; d += threads) {
-      u16 hi = 0, lo = 0;
-      if (d < c.D) {
-        if (DT == GNET_F32) split_f16(((const float*)src)[first + d] * c.scale, hi, lo);
-        else hi = ((const u16*)src)[first + d];
-      }
-      dst[d] = hi;
-      if (DT == GNET_F32) dst[c.plane + d] = lo;
-    }
+    *reinterpret_cast<s16x8*>(dst + d) = hi;
+    if (DT == GNET_F32) *reinterpret_cast<s16x8*>(dst + c.plane + d) = lo;
   }
 }
 template <int DT> __device__ __forceinline__ void zero_row(void* out, int64_t first, int64_t D, int t, int threads) {
@@ -223,12 +225,12 @@ template <int DT> __device__ __forceinline__ void dot8(const s16x8 (&x)[DT == GN
   if constexpr (DT == GNET_F32) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const f32x4 a = __builtin_bit_cast(f32x4, x[h]), b = ((const f32x4*)w)[h];
+      const f32x4 a = __builtin_bit_cast(f32x4, x[h]), b = ((const f32x4u*)w)[h];
 #pragma unroll
       for (int i = 0; i < 4; ++i) s = fmaf(a[i], b[i], s);
     }
   } else {
-    const s16x8 b = *(const s16x8*)w;
+    const s16x8 b = *(const s16x8u*)w;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       s = DT == GNET_BF16 ? fmaf(Bf16T::dec((u16)x[0][i]), Bf16T::dec((u16)b[i]), s) : fmaf(F16T::dec((u16)x[0][i]), F16T::dec((u16)b[i]), s);
@@ -239,7 +241,7 @@ template <int DT> __device__ __forceinline__ float load_elem(const void* p, int6
   if (DT == GNET_BF16) return Bf16T::dec(((const u16*)p)[i]);
   return F16T::dec(((const u16*)p)[i]);
 }
-struct DotArgs { const void* x; int64_t ldx; const void* w; int64_t ldw, D; int vec; float* hit; int per_token; };      // per_token: waves
+struct DotArgs { const void* x; int64_t ldx; const void* w; int64_t ldw, D; float* hit; int per_token; };      // per_token: waves
 template <int DT> __device__ __forceinline__ void target_dots(const Targets& t, const DotArgs& a, int64_t unit) {
   constexpr int SIZE = DT == GNET_F32 ? 4 : 2, U = 4;
   const int64_t m = unit / a.per_token;
@@ -259,22 +261,19 @@ template <int DT> __device__ __forceinline__ void target_dots(const Targets& t, 
     some |= c[u];
   }
   if (some) {                                        // (a token that does not count: its x is not read)
-    if (a.vec) {
 #pragma unroll 2
-      for (int64_t d = (int64_t)lane * 8; d < a.D; d += 512) {
-        s16x8 xv[DT == GNET_F32 ? 2 : 1];
+    for (int64_t d = (int64_t)lane * 8; d + 8 <= a.D; d += 512) {
+      s16x8 xv[DT == GNET_F32 ? 2 : 1];
 #pragma unroll
-        for (int h = 0; h < (DT == GNET_F32 ? 2 : 1); ++h) xv[h] = ((const s16x8*)(x + d * SIZE))[h];
+      for (int h = 0; h < (DT == GNET_F32 ? 2 : 1); ++h) xv[h] = ((const s16x8u*)(x + d * SIZE))[h];
 #pragma unroll
-        for (int u = 0; u < U; ++u) dot8<DT>(xv, w[u] + d * SIZE, dot[u]);
-      }
-    } else {
-#pragma unroll 4
-      for (int64_t d = lane; d < a.D; d += 64) {
-        const float v = load_elem<DT>(x, d);
+      for (int u = 0; u < U; ++u) dot8<DT>(xv, w[u] + d * SIZE, dot[u]);
+    }
+    const int64_t d = (a.D & ~7ll) + lane;           // what is left of eight
+    if (d < a.D) {
+      const float v = load_elem<DT>(x, d);
 #pragma unroll
-        for (int u = 0; u < U; ++u) dot[u] = fmaf(v, load_elem<DT>(w[u], d), dot[u]);
-      }
+      for (int u = 0; u < U; ++u) dot[u] = fmaf(v, load_elem<DT>(w[u], d), dot[u]);
     }
   }
 #pragma unroll
@@ -438,6 +437,89 @@ __global__ void __launch_bounds__(256) vocab_join(const JoinArgs a) {
   if (lane == 0) { a.loss[m] = loss; a.lse[m] = lse; }
 }
 
+// Few tiles and a long contraction: the logits' product is split along its contraction, and what fits into 64 MB of partial sums goes
+// on by rows, a workgroup a token: its logits are the splits' sums, and the whole row's maximum and sum are at hand in both directions.
+// forward: loss, lse, hit in place of the tiles' sums and vocab_join;  backward: dz, normalised by the row itself.
+struct RowsArgs {
+  Targets t;
+  const float* slab; int64_t ld, stride; int splits;
+  const VocabMeta* meta;
+  const int32_t* pos; const float* q; const float* entropy; float* loss; float* lse; float* hit;       // forward
+  const int32_t* label; const float* gscale; u16* dz; int64_t ld_dz, plane;                            // backward
+};
+template <class T, int PLANES, bool BACKWARD> __global__ void __launch_bounds__(256) vocab_rows(const RowsArgs a) {
+  __shared__ float red[4];
+  const int64_t m = blockIdx.x;                        // forward: token; backward: place
+  const int rows = a.meta->rows, K = a.t.K;
+  const int p = BACKWARD ? (m < rows ? (int)m : -1) : a.pos[m];
+  if (p < 0) {
+    if (BACKWARD) {
+      for (int64_t v = threadIdx.x * 4; v < a.ld; v += 1024)
+#pragma unroll
+        for (int i = 0; i < PLANES; ++i) *reinterpret_cast<s16x4*>(a.dz + i * a.plane + m * a.ld_dz + v) = s16x4{0, 0, 0, 0};
+    } else {
+      if (!a.t.logits && threadIdx.x == 0) a.hit[m] = 0.f;
+      if (threadIdx.x == 0) { a.loss[m] = 0.f; a.lse[m] = 0.f; }
+    }
+    return;
+  }
+  const float f = a.t.inv_temp * (a.meta->unscale_x * a.meta->unscale_w);
+  auto logit = [&](int64_t v) {                        // of rows v .. v + 3
+    f32x4 z = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.splits; ++s) z += *reinterpret_cast<const f32x4*>(a.slab + s * a.stride + p * a.ld + v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) z[i] = v + i < a.t.V ? z[i] * f : -INFINITY;
+    return z;
+  };
+  float top = -INFINITY, sum = 0.f;
+  for (int64_t v = threadIdx.x * 4; v < a.t.V; v += 1024) {
+    const f32x4 z = logit(v);
+    top = fmaxf(top, fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])));
+  }
+  top = block_max(top, red);
+  if (top == -INFINITY) top = 0.f;
+  for (int64_t v = threadIdx.x * 4; v < a.t.V; v += 1024) {
+    const f32x4 z = logit(v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum += exp2f((z[i] - top) * LOG2E);
+  }
+  sum = block_sum(sum, red);
+  if constexpr (BACKWARD) {
+    const float over = 1.f / sum, gs = a.gscale[p];
+    const int64_t label = a.label ? a.label[p] : -1;
+    for (int64_t v = threadIdx.x * 4; v < a.ld; v += 1024) {
+      u16 hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
+      if (v < a.t.V) {
+        const f32x4 z = logit(v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float d = (exp2f((z[i] - top) * LOG2E) * over - (v + i == label ? 1.f : 0.f)) * gs;      // (behind V: exp(-inf) = 0)
+          if (PLANES == 1) hi[i] = T::enc(v + i < a.t.V ? d : 0.f); else split_f16(v + i < a.t.V ? d : 0.f, hi[i], lo[i]);
+        }
+      }
+      *reinterpret_cast<s16x4*>(a.dz + m * a.ld_dz + v) = s16x4{(short)hi[0], (short)hi[1], (short)hi[2], (short)hi[3]};
+      if (PLANES == 2) *reinterpret_cast<s16x4*>(a.dz + a.plane + m * a.ld_dz + v) = s16x4{(short)lo[0], (short)lo[1], (short)lo[2], (short)lo[3]};
+    }
+  } else {
+    const float log_sum = logf(sum), lse = top + log_sum;
+    float loss = 0.f;
+    if (!a.t.logits) {
+      const int64_t label = load_id(a.t.ids, m, a.t.ids64);
+      const float hit = logit(label & ~3ll)[label & 3];
+      loss = (top - hit) + log_sum;
+      if (loss < 0.f) loss = 0.f;
+      if (threadIdx.x == 0) a.hit[m] = hit;
+    } else {
+      for (int k = threadIdx.x; k < K; k += 256) {
+        const float q = a.q[m * K + k];
+        if (q != 0.f) loss += q * (lse - a.hit[m * K + k]);
+      }
+      loss = block_sum(loss, red) + a.entropy[m];
+    }
+    if (threadIdx.x == 0) { a.loss[m] = loss; a.lse[m] = lse; }
+  }
+}
+
 // dz at the teacher's ids of one piece of the vocabulary: (softmax - weight) g from the forward pass's fp32 logits, over what
 // vocab_gemm<EPI_DZ> stored there.  Slots with the same id store the same value.
 struct HitsArgs {
@@ -462,7 +544,7 @@ template <class T, int PLANES> __global__ void __launch_bounds__(256) vocab_hits
 struct FinishArgs {
   const float* slab; int64_t ld, stride; int splits;
   const int32_t* pos;                                // NULL: row r of the slab
-  int64_t rows, D; unsigned quads; void* out; int vec;        // quads: groups of four a row; vec: stored at once
+  int64_t rows, D; unsigned quads; void* out;                 // quads: groups of four a row
   const VocabMeta* meta; int by_x;
 };
 template <int DT> __global__ void __launch_bounds__(64) vocab_finish(const FinishArgs a) {
@@ -480,15 +562,15 @@ template <int DT> __global__ void __launch_bounds__(64) vocab_finish(const Finis
   const int64_t at = r * a.D + d;
   if (DT == GNET_F32) {
     float* o = (float*)a.out + at;
-    if (a.vec) *reinterpret_cast<f32x4*>(o) = v;
+    if (d + 4 <= a.D) *reinterpret_cast<f32x4u*>(o) = v;
     else for (int k = 0; k < 4; ++k) if (d + k < a.D) o[k] = v[k];
   } else {
     u16* o = (u16*)a.out + at;
-    u16 e[4];
+    s16x4 e;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) e[k] = DT == GNET_BF16 ? Bf16T::enc(v[k]) : F16T::enc(v[k]);
-    if (a.vec) *reinterpret_cast<s16x4*>(o) = s16x4{(short)e[0], (short)e[1], (short)e[2], (short)e[3]};
-    else for (int k = 0; k < 4; ++k) if (d + k < a.D) o[k] = e[k];
+    for (int k = 0; k < 4; ++k) e[k] = (short)(DT == GNET_BF16 ? Bf16T::enc(v[k]) : F16T::enc(v[k]));
+    if (d + 4 <= a.D) *reinterpret_cast<s16x4u*>(o) = e;
+    else for (int k = 0; k < 4; ++k) if (d + k < a.D) o[k] = (u16)e[k];
   }
 }
 
@@ -528,11 +610,26 @@ Product pick_product(int64_t rows, int64_t cols, int64_t steps, bool few_cols, b
   return best;
 }
 
+// Splits of the logits' contraction where the tiles leave more than half of the chip idle.  A tile alone on its CU takes 0.6 us a step of
+// 64; the partial sums are then read twice by one workgroup a token, about 20 bytes a nanosecond.  The forward
+// product and the kernel behind it, in one and split: 165 x 2283 x 2240 fp32 67 and 29 us, 40 x 1000 x 4096 fp16 39 and 15 us, 5 x 154 x 3088 bf16
+// 30 and 14 us, 700 x 512 x 1024 bf16 19 and 15 us; 31 x 16278 x 1183 fp16 17 us in one, where the second kernel alone took 20 us.
+int logits_splits(int shape, int64_t V, int64_t M, int64_t steps, int64_t slab_bytes) {
+  const int64_t n = tiles(V, SHAPE[shape].bm) * tiles(M, SHAPE[shape].bn);
+  int best = 1;
+  double least = steps * 0.6;
+  for (int s = 2; n * s <= 256 && steps / s >= 8 && slab_bytes * s <= 64ll << 20; ++s) {
+    const double us = tiles(steps, s) * 0.6 + 4 + (double)V * s * 8 / 20e3 * (M > 1024 ? M / 1024. : 1.);
+    if (us < least) { least = us; best = s; }
+  }
+  return best;
+}
+
 struct Plan {
   int64_t Mp, Dp, flags_n, piece, pieces, w_tiles;
   int planes, pack_w, direct, dx_direct;
   Product logits, dx, dw;
-  int64_t flag, q, entropy, row_x, row_g, w_part, meta, pos, label, row_of, hit_c, lse_c, gscale, xp, wp, part, dz, dx_slab, dw_slab, bytes;
+  int64_t flag, q, entropy, row_x, row_g, w_part, meta, pos, label, row_of, hit_c, lse_c, gscale, xp, wp, part, z_slab, dz, dx_slab, dw_slab, bytes;
 };
 
 Plan make_plan(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int distill, int pack_w, int backward) {
@@ -552,8 +649,9 @@ Plan make_plan(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int distil
   p.pieces = tiles(Vp, piece);
   p.piece = up(tiles(Vp, p.pieces), 256);
   p.pieces = tiles(Vp, p.piece);
-  p.logits = pick_product(p.piece, M, p.Dp / VG_BK * segments, true, false);
+  p.logits = pick_product(V < p.piece ? V : p.piece, M, p.Dp / VG_BK * segments, true, false);
   if (V <= SHAPE[S128].bm && p.logits.shape == S256) p.logits.shape = S128;          // (a vocabulary of one tile: EPI_DZ_ONE)
+  if (p.pieces == 1) p.logits.splits = logits_splits(p.logits.shape, V, M, p.Dp / VG_BK * segments, (int64_t)p.Mp * p.piece * 4);
   p.w_tiles = tiles(V, SHAPE[p.logits.shape].bm);
   int64_t o = 0;
   auto take = [&](int64_t bytes) { const int64_t at = o; o = up(o + bytes, 256); return at; };
@@ -564,10 +662,11 @@ Plan make_plan(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int distil
   if (distill) p.q = take(M * K * 4 * (backward ? 2 : 1)); else p.label = take(p.Mp * 4);
   if (p.planes == 2) { p.row_x = take(M * 4); p.w_part = take(W_PARTS * 4); }
   if (pack_w) p.wp = take(p.planes * p.piece * p.Dp * 2);
+  if (p.logits.splits > 1) p.z_slab = take((int64_t)p.logits.splits * p.Mp * p.piece * 4);
   if (!backward) {
     p.entropy = take(M * 4);
     p.hit_c = take(p.Mp * 4);
-    p.part = take(p.Mp * p.w_tiles * 8);
+    if (p.logits.splits == 1) p.part = take(p.Mp * p.w_tiles * 8);
   } else {
     p.row_g = take(M * 4); p.lse_c = take(p.Mp * 4); p.gscale = take(p.Mp * 4);
     p.dz = take(p.planes * p.Mp * p.piece * 2);
@@ -585,11 +684,6 @@ Plan make_plan(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int distil
 int needs_pack(const void* w, int64_t ldw, int64_t D, int dtype) {
   return dtype == GNET_F32 || (D & 7) || (ldw & 7) || ldw > (1 << 22) || ((uintptr_t)w & 15);      // (2^22: 32-bit offsets in a tile)
 }
-// eight elements at a time
-int vec8(const void* p, int64_t ld, int64_t D, int dtype) {
-  return !(D & 7) && !((ld * (dtype == GNET_F32 ? 4 : 2)) & 15) && !((uintptr_t)p & 15);
-}
-
 struct Problem {
   const void* x; int64_t ldx; const void* w; int64_t ldw; Targets t; int64_t D; int dtype;
 };
@@ -622,7 +716,7 @@ template <int DT, class T, int PLANES> struct Run {
     PackW k = {};
     k.w = (const char*)q.w + v0 * q.ldw * (DT == GNET_F32 ? 4 : 2);
     k.ldw = q.ldw; k.rows = q.t.V - v0; k.rows_out = p.piece; k.dst = (u16*)(ws + p.wp);
-    k.c = RowCopy{q.D, p.Dp, p.piece * p.Dp, 1.f, vec8(q.w, q.ldw, q.D, DT)};
+    k.c = RowCopy{q.D, p.Dp, p.piece * p.Dp, 1.f};
     return k;
   }
   // everything in front of the first product, the first piece of W included
@@ -638,7 +732,6 @@ template <int DT, class T, int PLANES> struct Run {
       if (PLANES == 2) {
         a.x = (const float*)q.x; a.row_x = (float*)(ws + p.row_x);
         a.w = (const float*)q.w; a.ldw = q.ldw; a.w_part = (float*)(ws + p.w_part);
-        a.w_vec = !(q.D & 3) && !(q.ldw & 3) && !((uintptr_t)q.w & 15);
       }
       vocab_targets<<<a.token_groups + (PLANES == 2 ? W_PARTS : 0), 256, 0, s>>>(a);
     }
@@ -648,7 +741,7 @@ template <int DT, class T, int PLANES> struct Run {
     while (tiles(p.Mp, k.rows) > 1024) k.rows *= 2;             // every workgroup looks at all M flags
     k.token_groups = (unsigned)tiles(p.Mp, k.rows);
     k.x = q.x; k.ldx = q.ldx; k.xp = (u16*)(ws + p.xp);
-    k.c = RowCopy{q.D, p.Dp, p.Mp * p.Dp, 1.f, vec8(q.x, q.ldx, q.D, DT)};
+    k.c = RowCopy{q.D, p.Dp, p.Mp * p.Dp, 1.f};
     k.row_x = a.row_x; k.w_part = a.w_part;
     k.row_g = a.row_g; k.dloss = dloss; k.lse = lse; k.top_g = DT == GNET_BF16 ? 1.f : 32768.f;
     k.pos = (int32_t*)(ws + p.pos); k.label = q.t.logits ? nullptr : (int32_t*)(ws + p.label);
@@ -658,7 +751,7 @@ template <int DT, class T, int PLANES> struct Run {
     if (p.pack_w) { k.w = pack_of_w(q, p, ws, 0); k.w_groups = (unsigned)tiles(p.piece, PACK_W_ROWS); }
     unsigned groups = k.token_groups + k.w_groups;
     if (hit && q.t.logits) {
-      k.dots = DotArgs{q.x, q.ldx, q.w, q.ldw, q.D, vec8(q.x, q.ldx, q.D, DT) && vec8(q.w, q.ldw, q.D, DT), hit, (q.t.K + 3) / 4};
+      k.dots = DotArgs{q.x, q.ldx, q.w, q.ldw, q.D, hit, (q.t.K + 3) / 4};
       groups += (unsigned)tiles(q.t.M * k.dots.per_token, 4);
     }
     vocab_pack<DT><<<groups, 256, 0, s>>>(k);
@@ -691,8 +784,26 @@ template <int DT, class T, int PLANES> struct Run {
     return g;
   }
 
+  // the logits' partial sums, all of them
+  static RowsArgs split_logits(VocabGemm g, const Problem& q, const Plan& p, char* ws, hipStream_t s) {
+    g.slab = (float*)(ws + p.z_slab); g.ld_slab = p.piece; g.slab_stride = p.Mp * p.piece; g.out_cols = p.Mp;
+    gemm<false, false, EPI_SLAB>(g, p.logits, q.t.V, q.t.M, s);
+    RowsArgs r = {};
+    r.t = q.t; r.slab = g.slab; r.ld = p.piece; r.stride = g.slab_stride; r.splits = p.logits.splits; r.meta = g.meta;
+    return r;
+  }
+
   static int forward(const Problem& q, const Plan& p, char* ws, float* loss, float* lse, float* hit, hipStream_t s) {
     prepare(q, p, ws, nullptr, nullptr, nullptr, hit, s);
+    const int32_t* pos = (const int32_t*)(ws + p.pos);
+    const float* weights = (const float*)(ws + p.q);
+    const float* entropy = (const float*)(ws + p.entropy);
+    if (p.logits.splits > 1) {
+      RowsArgs r = split_logits(logits(q, p, ws, piece_of_w(q, p, ws, 0, s), 0), q, p, ws, s);
+      r.pos = pos; r.q = weights; r.entropy = entropy; r.loss = loss; r.lse = lse; r.hit = hit;
+      vocab_rows<T, PLANES, false><<<(unsigned)q.t.M, 256, 0, s>>>(r);
+      return launch_status();
+    }
     for (int64_t v0 = 0; v0 < q.t.V; v0 += p.piece) {
       VocabGemm g = logits(q, p, ws, piece_of_w(q, p, ws, v0, s), v0);
       g.part = (float2*)(ws + p.part); g.hit = (float*)(ws + p.hit_c);
@@ -700,8 +811,8 @@ template <int DT, class T, int PLANES> struct Run {
       gemm<false, false, EPI_PART>(g, p.logits, q.t.V - v0 < p.piece ? q.t.V - v0 : p.piece, q.t.M, s);
     }
     JoinArgs j = {};
-    j.t = q.t; j.pos = (const int32_t*)(ws + p.pos); j.part = (const float2*)(ws + p.part); j.tiles = (int)p.w_tiles; j.hit_c = (const float*)(ws + p.hit_c);
-    j.q = (const float*)(ws + p.q); j.entropy = (const float*)(ws + p.entropy);
+    j.t = q.t; j.pos = pos; j.part = (const float2*)(ws + p.part); j.tiles = (int)p.w_tiles; j.hit_c = (const float*)(ws + p.hit_c);
+    j.q = weights; j.entropy = entropy;
     j.loss = loss; j.lse = lse; j.hit = hit;
     vocab_join<<<(unsigned)tiles(q.t.M, 4), 256, 0, s>>>(j);
     return launch_status();
@@ -709,7 +820,6 @@ template <int DT, class T, int PLANES> struct Run {
 
   static void finish(FinishArgs f, const Problem& q, hipStream_t s) {
     f.D = q.D; f.quads = (unsigned)tiles(q.D, 4);
-    f.vec = !(q.D & 3) && !((uintptr_t)f.out & (DT == GNET_F32 ? 15 : 7));
     vocab_finish<DT><<<(unsigned)tiles(f.rows * f.quads, 64), 64, 0, s>>>(f);
   }
 
@@ -723,7 +833,11 @@ template <int DT, class T, int PLANES> struct Run {
       VocabGemm g = logits(q, p, ws, w, v0);
       g.lse = (const float*)(ws + p.lse_c); g.gscale = (const float*)(ws + p.gscale);
       g.dz = (u16*)(ws + p.dz); g.ld_dz = p.piece; g.plane_dz = p.Mp * p.piece; g.dz_cols = p.Mp;
-      if (p.logits.shape != S256 && q.t.V <= SHAPE[p.logits.shape].bm) gemm<false, false, EPI_DZ_ONE>(g, p.logits, rows, q.t.M, s);
+      if (p.logits.splits > 1) {
+        RowsArgs r = split_logits(g, q, p, ws, s);
+        r.label = g.label; r.gscale = g.gscale; r.dz = g.dz; r.ld_dz = g.ld_dz; r.plane = g.plane_dz;
+        vocab_rows<T, PLANES, true><<<(unsigned)p.Mp, 256, 0, s>>>(r);
+      } else if (p.logits.shape != S256 && q.t.V <= SHAPE[p.logits.shape].bm) gemm<false, false, EPI_DZ_ONE>(g, p.logits, rows, q.t.M, s);
       else gemm<false, false, EPI_DZ>(g, p.logits, rows, q.t.M, s);
       if (q.t.logits) {
         HitsArgs h = {};
@@ -738,7 +852,7 @@ template <int DT, class T, int PLANES> struct Run {
         VocabGemm d = {};
         d.a = w; d.b = dz; d.k = rows64; d.cols_from_meta = 1; d.meta = meta; d.out_cols = p.Mp;
         if (p.dx_direct) {
-          d.out = dx; d.ld_out = q.D; d.out_rows = q.D; d.out_vec = vec8(dx, q.D, q.D, DT);
+          d.out = dx; d.ld_out = q.D; d.out_rows = q.D;
           d.row_of = (const int32_t*)(ws + p.row_of);
           gemm<true, false, EPI_OUT>(d, p.dx, p.Dp, q.t.M, s);
         } else {
@@ -753,7 +867,6 @@ template <int DT, class T, int PLANES> struct Run {
         void* out = (char*)dw + v0 * q.D * elem;
         if (p.dw.splits == 1) {
           d.out = out; d.ld_out = q.D; d.out_rows = q.D; d.unscale_by_x = 1;
-          d.out_vec = vec8(dw, q.D, q.D, DT);
           gemm<true, true, EPI_OUT>(d, p.dw, p.Dp, rows, s);
         } else {
           d.slab = (float*)(ws + p.dw_slab); d.ld_slab = p.Dp; d.slab_stride = p.piece * p.Dp;

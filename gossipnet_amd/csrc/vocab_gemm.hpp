@@ -17,6 +17,11 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 
+// vectors at the alignment of their elements (the hardware's global accesses of 16 bytes need no more)
+typedef short s16x8u __attribute__((ext_vector_type(8), aligned(2)));
+typedef short s16x4u __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+
 // ---- element types ----------------------------------------------------------------------------------------------
 struct Bf16T {
   static __device__ __forceinline__ f32x4 mma(s16x8 a, s16x8 b, f32x4 c) {
@@ -78,7 +83,7 @@ struct VocabGemm {
   // products
   float* slab; int64_t ld_slab, slab_stride; int accumulate;      // [split][column][ld_slab]
   const int32_t* row_of;       // the output row of a column (tokens that count), or NULL
-  void* out; int64_t ld_out, out_rows, out_cols; int out_vec; int unscale_by_x;   // [column][row]; out_vec: 16 bytes may be stored at once
+  void* out; int64_t ld_out, out_rows, out_cols; int unscale_by_x;   // [column][row]
 };
 
 enum { EPI_PART = 0, EPI_DZ = 1, EPI_SLAB = 2, EPI_OUT = 3, EPI_DZ_ONE = 4 };      // EPI_DZ_ONE: the vocabulary is one row tile
@@ -471,12 +476,11 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) vocab_gemm(const VocabGemm g)
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
           const int64_t row = r0 + (wm * FM + i) * 16 + quad * 4;
-          if (g.out_vec) {
-            if (row < g.out_rows) *reinterpret_cast<f32x4*>(out + row) = acc[i][j] * f;
-          } else {
+          const f32x4 v = acc[i][j] * f;
+          if (row + 4 <= g.out_rows) *reinterpret_cast<f32x4u*>(out + row) = v;
+          else
 #pragma unroll
-            for (int r = 0; r < 4; ++r) if (row + r < g.out_rows) out[row + r] = acc[i][j][r] * f;
-          }
+            for (int r = 0; r < 4; ++r) if (row + r < g.out_rows) out[row + r] = v[r];
         }
       }
     } else {
@@ -484,12 +488,10 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) vocab_gemm(const VocabGemm g)
         const int64_t c = c0 + v, row = r0 + d;
         if (c >= cols) return;
         u16* p = (u16*)g.out + (g.row_of ? g.row_of[c] : c) * g.ld_out + row;
-        if (g.out_vec) {
-          if (row < g.out_rows) *reinterpret_cast<s16x8*>(p) = x;
-        } else {
+        if (row + 8 <= g.out_rows) *reinterpret_cast<s16x8u*>(p) = x;
+        else
 #pragma unroll
           for (int r = 0; r < 8; ++r) if (row + r < g.out_rows) p[r] = (u16)x[r];
-        }
       });
     }
   }
