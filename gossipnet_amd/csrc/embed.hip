@@ -9,6 +9,7 @@
 //   embed_sums    four kinds of workgroups in one launch: sums of the runs of equal ids (a wave starts where a run starts), partial sums
 //                 of the runs of more than HOT tokens per HOT sorted tokens, zeros for the rows without a token, d s
 //   embed_hot_rows  adds a long run's partial sums
+// or, for few tokens and a small table, embed_few alone.
 #include "vocab_gemm.hpp"
 
 namespace {
@@ -374,6 +375,62 @@ template <int DT, int VEC> __global__ void __launch_bounds__(256) embed_hot_rows
   }
 }
 
+// A small table and few tokens: no order is needed.  A workgroup per row of the table and column block looks through all ids, its 16 waves
+// a share of the tokens each, and adds up those of its row; more workgroups for d s.  One launch for three.
+constexpr int FEW = 2048, FEW_WAVES = 16;          // tokens at most
+template <int DT, int VEC> __global__ void __launch_bounds__(64 * FEW_WAVES) embed_few(const BackwardArgs a) {
+  __shared__ int list[FEW_WAVES][FEW / FEW_WAVES];
+  __shared__ float sums[FEW_WAVES][64 * VEC];
+  __shared__ int found[FEW_WAVES];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (blockIdx.x < a.scale_groups) {
+    if (blockIdx.y == 0) scale_gradient<DT, VEC>(a, (int64_t)blockIdx.x * FEW_WAVES + wave);
+    return;
+  }
+  const int64_t v = blockIdx.x - a.scale_groups, d0 = (int64_t)blockIdx.y * 64 * VEC, d = d0 + lane * VEC;
+  const int share = (int)((a.M + 64 * FEW_WAVES - 1) / (64 * FEW_WAVES)) * 64, first = wave * share;
+  bool mine[FEW / FEW_WAVES / 64];
+#pragma unroll
+  for (int i = 0; i < FEW / FEW_WAVES / 64; ++i) {
+    const int m = first + i * 64 + lane;
+    mine[i] = i * 64 < share && m < a.M && load_id(a.ids, m, a.ids64) == v;
+  }
+  int n = 0;
+#pragma unroll
+  for (int i = 0; i < FEW / FEW_WAVES / 64; ++i) {
+    const u64 all = __ballot(mine[i]);
+    if (mine[i]) list[wave][n + __popcll(all & ((1ull << lane) - 1))] = first + i * 64 + lane;
+    n += __popcll(all);
+  }
+  if (lane == 0) found[wave] = n;
+  float sum[1][VEC], more[1][VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) sum[0][i] = 0.f;
+  for (int j = 0; j < n; j += 64) {                  // (a wave reads what it wrote itself)
+    const int token = j + lane < n ? list[wave][j + lane] : 0;
+    add_tokens<DT, VEC, 8, 1>(more, a, token, 0, min(64, n - j), d, 0, 1);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) sum[0][i] += more[0][i];
+  }
+  if (n)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) sums[wave][lane * VEC + i] = sum[0][i];
+  __syncthreads();
+  int total = 0;
+#pragma unroll
+  for (int w = 0; w < FEW_WAVES; ++w) total += found[w];
+  const int c = threadIdx.x;
+  if (c >= 64 * VEC || d0 + c >= a.D || (a.accumulate && !total)) return;
+  float all[1] = {0.f};
+#pragma unroll
+  for (int w = 0; w < FEW_WAVES; ++w)
+    if (found[w]) all[0] += sums[w][c];
+  store_row<DT, 1>(all, a, v, d0 + c);
+}
+// Measured against the sorted order: 2000 tokens, a table of 81 x 128 8 and 18 us, of 2048 x 64 10 and 18; 16 tokens, 4096 x 64 (not taken)
+// 12 and 9.  The worst case, all tokens of one row, is bound by what one CU can fetch: 2000 tokens 28 and 21 us, 4096 (not taken) 53 and 28.
+bool few(int64_t M, int64_t V, int64_t column_blocks) { return M <= FEW && V * column_blocks <= 2048; }
+
 // Elements a lane takes at once: 16 bytes, or as many as still give every lane of a wave something to do.
 int pick_vec(int dtype, int64_t D) {
   int v = dtype == GNET_F32 ? 4 : 8;
@@ -391,11 +448,12 @@ template <template <int, int> class F, class A> void launch(int dtype, int vec, 
   if (dtype == GNET_F32) { GO(GNET_F32) } else if (dtype == GNET_BF16) { GO(GNET_BF16) } else { GO(GNET_F16) }
 #undef GO
 }
-#define KERNEL_OF(name, kernel, args) \
-  template <int DT, int VEC> struct name { static void go(const args& a, dim3 grid, hipStream_t s) { kernel<DT, VEC><<<grid, 256, 0, s>>>(a); } }
-KERNEL_OF(GoForward, embed_rows_out, ForwardArgs);
-KERNEL_OF(GoSums, embed_sums, BackwardArgs);
-KERNEL_OF(GoHotRows, embed_hot_rows, BackwardArgs);
+#define KERNEL_OF(name, kernel, args, threads) \
+  template <int DT, int VEC> struct name { static void go(const args& a, dim3 grid, hipStream_t s) { kernel<DT, VEC><<<grid, threads, 0, s>>>(a); } }
+KERNEL_OF(GoForward, embed_rows_out, ForwardArgs, 256);
+KERNEL_OF(GoSums, embed_sums, BackwardArgs, 256);
+KERNEL_OF(GoHotRows, embed_hot_rows, BackwardArgs, 256);
+KERNEL_OF(GoFew, embed_few, BackwardArgs, 64 * FEW_WAVES);
 
 int check(int64_t M, int64_t V, int64_t D, int64_t ld, int dtype) {
   if (dtype != GNET_F32 && dtype != GNET_BF16 && dtype != GNET_F16) return GNET_ERR_INVALID;
@@ -436,6 +494,14 @@ extern "C" int gnet_embed_backward(const void* ids, int32_t ids64, const void* d
   u64* keys = (u64*)workspace;
   u64* other = (u64*)((char*)workspace + keys_bytes(M));
   float* part = (float*)((char*)workspace + 2 * keys_bytes(M));
+  BackwardArgs a{keys, M, V, D, dy, ld_dy, scale, token_scale, dtable, D, accumulate, part, (D + 7) & ~7ll, 0, 0, 0, ids, ids64, table, ld_table, dscale};
+  const int vec = pick_vec(dtype, D);
+  const unsigned column_blocks = (unsigned)((D + 64 * vec - 1) / (64 * vec));
+  if (M && few(M, V, column_blocks)) {
+    a.scale_groups = dscale ? (unsigned)((M + FEW_WAVES - 1) / FEW_WAVES) : 0;
+    launch<GoFew>(dtype, vec, a, dim3(a.scale_groups + (unsigned)V, column_blocks), s);
+    return launch_status();
+  }
   if (M) {
     int n = 256;                                      // a whole wave
     while (n < RUN && n < M) n <<= 1;
@@ -447,14 +513,13 @@ extern "C" int gnet_embed_backward(const void* ids, int32_t ids64, const void* d
       u64* t = keys; keys = other; other = t;
     }
   }
-  BackwardArgs a{keys, M, V, D, dy, ld_dy, scale, token_scale, dtable, D, accumulate, part, (D + 7) & ~7ll, 0, 0, 0, ids, ids64, table, ld_table, dscale};
-  const int vec = pick_vec(dtype, D);
+  a.keys = keys;
   const unsigned segments = (unsigned)((M + HOT - 1) / HOT);
   a.hot_groups = M > HOT ? segments : 0;
   a.run_groups = (unsigned)((M + 3) / 4);
   a.scale_groups = dscale ? a.run_groups : 0;
   const unsigned groups = a.hot_groups + a.run_groups + a.scale_groups + (accumulate ? 0 : (unsigned)((V + FILL_ROWS - 1) / FILL_ROWS));
   if (groups) launch<GoSums>(dtype, vec, a, groups, s);
-  if (M > HOT) launch<GoHotRows>(dtype, vec, a, dim3(segments, (unsigned)((D + 64 * vec - 1) / (64 * vec))), s);
+  if (M > HOT) launch<GoHotRows>(dtype, vec, a, dim3(segments, column_blocks), s);
   return launch_status();
 }

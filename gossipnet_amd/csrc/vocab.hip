@@ -11,6 +11,7 @@
 //              vocab_gemm<EPI_SLAB>  dx += dz . W (fp32)     vocab_gemm<EPI_OUT>  dW = dz^T . x     and at last vocab_finish  dx
 // A token whose targets are all outside [0, V) is left out of everything, whatever its row of x holds: it is not read again after
 // vocab_targets, its dx is zero.
+// A small vocabulary takes other kernels (vocab_small.hpp), few tiles of logits others for the softmax (logits_splits).
 #include "vocab_gemm.hpp"
 
 namespace {
@@ -64,6 +65,8 @@ __device__ __forceinline__ bool target_counts(const Targets& t, int64_t i, int64
   id = load_id(t.ids, i, t.ids64);
   return id >= 0 && id < t.V && !(t.logits && t.logits[i] == -INFINITY);
 }
+
+#include "vocab_small.hpp"
 
 // ---- what is known before the first product ------------------------------------------------------------------------
 // Token workgroups, one wave per token (and per padding byte of the flags): does it count; its targets' weights; in the backward pass
@@ -625,6 +628,17 @@ int logits_splits(int shape, int64_t V, int64_t M, int64_t steps, int64_t slab_b
   return best;
 }
 
+// Where the small vocabulary's kernels run (vocab_small.hpp).  A workgroup reads all of W and computes its tokens' logits on the fp32
+// matrix pipe, which is 1/16 of what 16 bits and a third of what two fp16 planes get: past some V D and M V D the general path is faster.
+// Forward and backward together, here and there: fp32 2000 x 81 x 128 26 and 68 us, 4096 x 256 x 256 69 and 88, 2000 x 256 x 512 (not
+// taken) 105 and 84; bf16 2000 x 81 x 128 28 and 48, 4096 x 128 x 256 47 and 58, 2000 x 256 x 256 (not taken) 60 and 51; distillation with
+// K = 32, 2000 x 81 x 128: fp32 30 and 85, bf16 32 and 67.
+bool small(int64_t M, int64_t V, int64_t D, int64_t K, int dtype) {
+  const int64_t most = dtype == GNET_F32 ? 1 << 16 : 1 << 15;
+  return V <= 256 && K <= SMALL_K && M <= 8192 && V * D <= most && M * V * D <= 4096 * most;
+}
+size_t small_bytes(int64_t M, int64_t V) { return (size_t)up(M, 16) * (up(V, 16) + 1) * 4; }
+
 struct Plan {
   int64_t Mp, Dp, flags_n, piece, pieces, w_tiles;
   int planes, pack_w, direct, dx_direct;
@@ -678,6 +692,7 @@ Plan make_plan(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int distil
     if (p.dw.splits > 1) p.dw_slab = take((int64_t)p.dw.splits * p.piece * p.Dp * 4);
   }
   p.bytes = o;
+  if (backward && small(M, V, D, K, dtype) && (size_t)p.bytes < small_bytes(M, V)) p.bytes = (int64_t)small_bytes(M, V);
   return p;
 }
 
@@ -696,6 +711,33 @@ int check(const Problem& q) {
   if (!q.w || (q.t.M && (!q.x || !q.t.ids))) return GNET_ERR_INVALID;
   return GNET_OK;
 }
+
+// ---- a small vocabulary ------------------------------------------------------------------------------------------------
+template <int DT> struct Small {
+  static SmallArgs args(const Problem& q) {
+    SmallArgs a = {};
+    a.t = q.t; a.x = q.x; a.ldx = q.ldx; a.w = q.w; a.ldw = q.ldw; a.D = q.D;
+    a.ld_z = (int)up(q.t.V, 64) + 4;
+    return a;
+  }
+  static int forward(const Problem& q, float* loss, float* lse, float* hit, hipStream_t s) {
+    SmallArgs a = args(q);
+    a.loss = loss; a.lse = lse; a.hit = hit;
+    vocab_small<DT, false><<<(unsigned)tiles(q.t.M, SMALL_TOKENS), 64 * SMALL_WAVES, SMALL_TOKENS * a.ld_z * 4, s>>>(a);
+    return launch_status();
+  }
+  static int backward(const Problem& q, char* ws, const float* dloss, void* dx, void* dw, hipStream_t s) {
+    SmallArgs a = args(q);
+    a.dloss = dloss; a.dx = dx;
+    a.dz = (float*)ws; a.ld_dz = up(q.t.V, 16); a.alive = (int*)(a.dz + up(q.t.M, 16) * a.ld_dz);
+    vocab_small<DT, true><<<(unsigned)tiles(q.t.M, SMALL_TOKENS), 64 * SMALL_WAVES, SMALL_TOKENS * a.ld_z * 4, s>>>(a);
+    if (dw) {
+      const SmallDwArgs d{q.x, q.ldx, q.t.M, q.t.V, q.D, a.dz, a.ld_dz, a.alive, dw};
+      vocab_small_dw<DT><<<dim3((unsigned)tiles(q.t.V, 16), (unsigned)tiles(q.D, 16)), 64 * SMALL_DW_WAVES, 0, s>>>(d);
+    }
+    return launch_status();
+  }
+};
 
 template <int DT, class T, int PLANES> struct Run {
   template <int BM, int BN, int WM, int WN, int STAGES, bool AS, bool BS, int EPI> static void launch(VocabGemm& g, int64_t rows, int64_t cols, int splits, hipStream_t s) {
@@ -900,6 +942,11 @@ int run_forward(const Problem& q, float* loss, float* lse, float* hit, void* ws,
   if (!loss || !lse || !hit) return GNET_ERR_INVALID;
   const Plan p = make_plan(q.t.M, q.t.V, q.D, q.t.K, q.dtype, q.t.logits != nullptr, needs_pack(q.w, q.ldw, q.D, q.dtype), 0);
   if (!ws || ws_bytes < (size_t)p.bytes || ((uintptr_t)ws & 255)) return GNET_ERR_WORKSPACE;
+  if (small(q.t.M, q.t.V, q.D, q.t.K, q.dtype)) switch (q.dtype) {
+    case GNET_F32: return Small<GNET_F32>::forward(q, loss, lse, hit, s);
+    case GNET_BF16: return Small<GNET_BF16>::forward(q, loss, lse, hit, s);
+    default: return Small<GNET_F16>::forward(q, loss, lse, hit, s);
+  }
   switch (q.dtype) {
     case GNET_F32: return Run<GNET_F32, F16T, 2>::forward(q, p, (char*)ws, loss, lse, hit, s);
     case GNET_BF16: return Run<GNET_BF16, Bf16T, 1>::forward(q, p, (char*)ws, loss, lse, hit, s);
@@ -920,6 +967,11 @@ int run_backward(const Problem& q, const float* lse, const float* hit, const flo
   if (!lse || !hit || !dloss) return GNET_ERR_INVALID;
   const Plan p = make_plan(q.t.M, q.t.V, q.D, q.t.K, q.dtype, q.t.logits != nullptr, needs_pack(q.w, q.ldw, q.D, q.dtype), 1);
   if (!ws || ws_bytes < (size_t)p.bytes || ((uintptr_t)ws & 255)) return GNET_ERR_WORKSPACE;
+  if (small(q.t.M, q.t.V, q.D, q.t.K, q.dtype)) switch (q.dtype) {
+    case GNET_F32: return Small<GNET_F32>::backward(q, (char*)ws, dloss, dx, dw, s);
+    case GNET_BF16: return Small<GNET_BF16>::backward(q, (char*)ws, dloss, dx, dw, s);
+    default: return Small<GNET_F16>::backward(q, (char*)ws, dloss, dx, dw, s);
+  }
   switch (q.dtype) {
     case GNET_F32: return Run<GNET_F32, F16T, 2>::backward(q, p, (char*)ws, lse, hit, dloss, dx, dw, s);
     case GNET_BF16: return Run<GNET_BF16, Bf16T, 1>::backward(q, p, (char*)ws, lse, hit, dloss, dx, dw, s);

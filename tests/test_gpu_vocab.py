@@ -134,7 +134,8 @@ def check_distill(x, w, ids, logits, tau, dloss):
 
 SIZES = [(1, 1, 1), (1, 2, 3), (3, 5, 7), (2, 300, 64), (17, 130, 65), (64, 127, 64), (128, 128, 128), (129, 257, 192), (65, 1000, 100),
          (300, 513, 256), (5, 8191, 72), (31, 4099, 320), (513, 81, 128), (1100, 1030, 136), (3, 200, 8200), (9001, 130, 64), (270000, 40, 8),
-         (165, 2283, 2240), (5, 154, 2050), (300, 129, 1100)]
+         (165, 2283, 2240), (5, 154, 2050), (300, 129, 1100),
+         (20, 120, 600), (50, 100, 700), (9000, 81, 128), (33, 256, 128), (17, 255, 129), (2000, 81, 128), (8192, 9, 30)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
@@ -149,7 +150,8 @@ def test_xent(M, V, D, dtype):
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("M,V,D,K,tau", [(1, 1, 1, 1, 1.0), (1, 70, 64, 70, 2.0), (3, 5, 7, 2, 0.5), (17, 130, 65, 3, 4.0), (64, 500, 128, 64, 1.5), (200, 1111, 72, 65, 1.0),
-                                         (40, 1000, 4100, 13, 2.5), (130, 300, 256, 8, 2.0), (5, 5000, 96, 200, 3.0), (3, 3000, 64, 1024, 2.0), (9001, 100, 64, 3, 1.0)])
+                                         (40, 1000, 4100, 13, 2.5), (130, 300, 256, 8, 2.0), (5, 5000, 96, 200, 3.0), (3, 3000, 64, 1024, 2.0), (9001, 100, 64, 3, 1.0),
+                                         (30, 200, 64, 64, 1.5), (517, 81, 100, 33, 2.0)])
 def test_distill(M, V, D, K, tau, dtype):
     x, w, ids, dloss, logits = make(M, V, D, dtype, M + V + K, K)
     check_distill(x, w, ids, logits, tau, dloss)                       # random ids: some occur twice in a row
@@ -160,8 +162,9 @@ def test_distill(M, V, D, K, tau, dtype):
     check_distill(x, w, ids, logits, tau, dloss)
 
 
-def test_same_id_in_every_slot_and_lowest_logits():
-    x, w, ids, dloss, logits = make(40, 200, 64, "bf16", 5, 6)
+@pytest.mark.parametrize("V", [200, 700])
+def test_same_id_in_every_slot_and_lowest_logits(V):
+    x, w, ids, dloss, logits = make(40, V, 64, "bf16", 5, 6)
     ids[:] = ids[:, :1]
     check_distill(x, w, ids, logits, 2.0, dloss)
     ids = torch.arange(6, device=DEV).repeat(40, 1) * 30
@@ -174,9 +177,10 @@ def test_same_id_in_every_slot_and_lowest_logits():
     assert not bool(e.some.any())
 
 
-def test_labels_outside_the_vocabulary():
+@pytest.mark.parametrize("D", [64, 1000])
+def test_labels_outside_the_vocabulary(D):
     from gossipnet_amd import vocab
-    x, w, labels, dloss = make(9, 50, 64, "bf16", 3)
+    x, w, labels, dloss = make(9, 50, D, "bf16", 3)
     labels[:] = torch.tensor([-1, 50, -100, 2 ** 32 + 1, -2 ** 40, 51, 2 ** 31, 7, 2 ** 62], device=DEV)
     e = check_xent(x, w, labels, dloss)
     assert e.some.tolist() == [False] * 7 + [True, False]
@@ -187,9 +191,10 @@ def test_labels_outside_the_vocabulary():
         assert not bool(t.any())
 
 
+@pytest.mark.parametrize("V", [120, 333])
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-def test_infinities_and_nan_in_rows_that_are_left_out(dtype):
-    x, w, labels, dloss = make(150, 333, 128, dtype, 8)
+def test_infinities_and_nan_in_rows_that_are_left_out(dtype, V):
+    x, w, labels, dloss = make(150, V, 128, dtype, 8)
     x[3], x[77], x[149] = math.nan, math.inf, -math.inf
     labels[3] = labels[77] = labels[149] = -1
     dloss[3], dloss[77] = math.nan, math.inf
@@ -197,17 +202,19 @@ def test_infinities_and_nan_in_rows_that_are_left_out(dtype):
     check_xent(x, w, labels, dloss)
 
 
+@pytest.mark.parametrize("V", [90, 700])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-def test_large_logits_and_confident_rows(dtype):
-    x, w, labels, dloss = make(100, 700, 192, dtype, 9)
+def test_large_logits_and_confident_rows(dtype, V):
+    x, w, labels, dloss = make(100, V, 192, dtype, 9)
     check_xent(x * 300, w, labels, dloss)                              # far beyond exp's range
     check_xent(w[labels] * 40, w, labels, dloss)                       # the label takes nearly everything
     check_xent(x * 0, w, labels, dloss)                                # uniform
 
 
-def test_outliers_in_fp32():
+@pytest.mark.parametrize("V", [200, 600])
+def test_outliers_in_fp32(V):
     """One power of two scales a whole tensor: rows and single values far above and far below the rest."""
-    x, w, labels, dloss = make(90, 400, 128, "f32", 16)
+    x, w, labels, dloss = make(90, V, 128, "f32", 16)
     x[5, 3], x[6] = 3e4, x[6] * 1e-6
     w[7], w[8], w[9, 1] = w[7] * 1e-8, w[8] * 50, 2000.0
     check_xent(x, w, labels, dloss)
@@ -215,8 +222,9 @@ def test_outliers_in_fp32():
     check_xent(x * 1e12, w * 1e-12, labels, dloss * 1e9)
 
 
-def test_loss_gradients_of_all_sizes():
-    x, w, labels, dloss = make(64, 300, 128, "f16", 10)
+@pytest.mark.parametrize("V", [100, 300])
+def test_loss_gradients_of_all_sizes(V):
+    x, w, labels, dloss = make(64, V, 128, "f16", 10)
     for scale in (1e-30, 1e-3, 1e4, 0.0):
         from gossipnet_amd import vocab
         e = Exact(x, w, labels)
@@ -235,11 +243,12 @@ def test_loss_gradients_of_all_sizes():
     assert dw is None and torch.equal(dx, a[0])
 
 
+@pytest.mark.parametrize("V", [100, 260, 700])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-def test_strides_and_alignment(dtype):
+def test_strides_and_alignment(dtype, V):
     """Rows inside wider ones, addresses that are no multiple of 16, transposed and expanded tensors: the dense call's results."""
     from gossipnet_amd import vocab
-    M, V, D = 70, 260, 128
+    M, D = 70, 128
     x, w, labels, dloss = make(M, V, D, dtype, 11)
 
     def run(x, w):
@@ -404,29 +413,31 @@ def test_embed(shape, V, D, dtype):
         near(ds, dot, mag * (D + 4) * U, "dscale")
 
 
-@pytest.mark.parametrize("M", [15, 16, 17, 32, 33, 64, 129, 4096, 4097, 65537, 70000])
-def test_embed_gradient_of_one_row_and_of_runs_around_the_hot_limit(M):
+@pytest.mark.parametrize("V", [40, 4000])
+@pytest.mark.parametrize("M", [15, 16, 17, 32, 33, 64, 129, 2048, 2049, 4096, 4097, 65537, 70000])
+def test_embed_gradient_of_one_row_and_of_runs_around_the_hot_limit(M, V):
     """All tokens the same id; and runs of 15, 16, 17 and more tokens at every place of the sorted order."""
     from gossipnet_amd import vocab
     D = 24
     g = torch.Generator(device=DEV).manual_seed(M)
     dy = torch.randint(-8, 9, (M, D), device=DEV, generator=g).float()       # sums of small whole numbers: exact
-    table = torch.zeros(40, D, device=DEV)
+    table = torch.zeros(V, D, device=DEV)
     ids = torch.full((M,), 17, device=DEV)
     for _ in range(2):
-        want = torch.zeros(40, D, dtype=torch.float64, device=DEV).index_add_(0, ids, dy.double())
+        want = torch.zeros(V, D, dtype=torch.float64, device=DEV).index_add_(0, ids, dy.double())
         assert torch.equal(vocab.embed_backward(ids, dy, table)[0].double(), want)
         sizes = [15, 16, 17, 1, 31, 32, 33, 2, 16, 16, 48, 64, 200, 3, 17]
         ids = torch.repeat_interleave(torch.arange(len(sizes), device=DEV), torch.tensor(sizes, device=DEV))
         ids = ids.repeat(M // ids.numel() + 1)[:M][torch.randperm(M, device=DEV, generator=g)]
 
 
-def test_embed_strides():
+@pytest.mark.parametrize("V", [50, 3000])
+def test_embed_strides(V):
     from gossipnet_amd import vocab
-    table = torch.randn(50, 64, device=DEV, dtype=torch.bfloat16)
-    ids = torch.randint(0, 50, (200,), device=DEV)
+    table = torch.randn(V, 64, device=DEV, dtype=torch.bfloat16)
+    ids = torch.randint(0, V, (200,), device=DEV)
     dy = torch.randn(200, 64, device=DEV, dtype=torch.bfloat16)
-    wide, dwide = torch.zeros(50, 77, device=DEV, dtype=torch.bfloat16), torch.zeros(200, 99, device=DEV, dtype=torch.bfloat16)
+    wide, dwide = torch.zeros(V, 77, device=DEV, dtype=torch.bfloat16), torch.zeros(200, 99, device=DEV, dtype=torch.bfloat16)
     wide[:, 5:69], dwide[:, 1:65] = table, dy
     assert torch.equal(vocab.embed_forward(ids, wide[:, 5:69], 2.0), vocab.embed_forward(ids, table, 2.0))
     assert torch.equal(vocab.embed_forward(ids, table.t().contiguous().t(), 2.0), vocab.embed_forward(ids, table, 2.0))
@@ -516,10 +527,11 @@ def test_tied_training_step_against_autograd():
     assert float((total.double().cpu() - W.grad).abs().max()) <= 64 * V * U * scale
 
 
-def test_other_streams_and_captured_graphs():
+@pytest.mark.parametrize("sizes", [[(40, 600, 128), (300, 2000, 64)], [(40, 100, 64), (300, 81, 128)], [(20, 300, 2048), (2100, 81, 64)]])
+def test_other_streams_and_captured_graphs(sizes):
     """Eager calls on a side stream, and a captured step replayed with new inputs, two graphs in turn, eager work between them."""
     steps = []
-    for seed, (M, V, D) in enumerate([(40, 600, 128), (300, 2000, 64)]):
+    for seed, (M, V, D) in enumerate(sizes):
         x, w, ids, _, logits = make(M, V, D, "bf16", seed, 4)
         steps.append([x, w, ids[:, 0].contiguous(), ids, logits, w])
     eager = [_step(*s) for s in steps]
