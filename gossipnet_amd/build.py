@@ -67,7 +67,8 @@ def build(force=False, verbose=False):
 
 def _build_locked(force, verbose, objdir):
     srcs = [os.path.join(CSRC, s) for s in SOURCES if os.path.exists(os.path.join(CSRC, s))]
-    deps = srcs + [os.path.join(CSRC, "common.hpp"), os.path.join(CSRC, "backward_edge.hpp"), os.path.join(CSRC, "vocab_gemm.hpp"), os.path.join(CSRC, "vocab_small.hpp"),
+    deps = srcs + [os.path.join(CSRC, "common.hpp"), os.path.join(CSRC, "backward_edge.hpp"), os.path.join(CSRC, "vocab_gemm.hpp"),
+                   os.path.join(CSRC, "vocab_small.hpp"), os.path.join(CSRC, "vocab_few.hpp"),
                    os.path.join(HERE, "..", "include", "gossipnet_hip.h")]
     hdr_mtime = max(os.path.getmtime(d) for d in deps[len(srcs):])
     objs, procs = [], []

@@ -11,7 +11,8 @@
 //              vocab_gemm<EPI_SLAB>  dx += dz . W (fp32)     vocab_gemm<EPI_OUT>  dW = dz^T . x     and at last vocab_finish  dx
 // A token whose targets are all outside [0, V) is left out of everything, whatever its row of x holds: it is not read again after
 // vocab_targets, its dx is zero.
-// A small vocabulary takes other kernels (vocab_small.hpp), few tiles of logits others for the softmax (logits_splits).
+// A small vocabulary takes other kernels (vocab_small.hpp), and so do few tokens on a W that would have to be laid out (vocab_few.hpp); few
+// tiles of logits take another softmax (logits_splits).
 #include "vocab_gemm.hpp"
 
 namespace {
@@ -67,6 +68,7 @@ __device__ __forceinline__ bool target_counts(const Targets& t, int64_t i, int64
 }
 
 #include "vocab_small.hpp"
+#include "vocab_few.hpp"
 
 // ---- what is known before the first product ------------------------------------------------------------------------
 // Token workgroups, one wave per token (and per padding byte of the flags): does it count; its targets' weights; in the backward pass
@@ -629,7 +631,7 @@ int logits_splits(int shape, int64_t V, int64_t M, int64_t steps, int64_t slab_b
 }
 
 // Where the small vocabulary's kernels run (vocab_small.hpp).  A workgroup reads all of W and computes its tokens' logits on the fp32
-// matrix pipe, which is 1/16 of what 16 bits and a third of what two fp16 planes get: past some V D and M V D the general path is faster.
+// matrix pipe, at a sixteenth of the 16-bit rate and a fifth of two fp16 planes': past some V D and M V D the general path is faster.
 // Forward and backward together, here and there: fp32 2000 x 81 x 128 26 and 68 us, 4096 x 256 x 256 69 and 88, 2000 x 256 x 512 (not
 // taken) 105 and 84; bf16 2000 x 81 x 128 28 and 48, 4096 x 128 x 256 47 and 58, 2000 x 256 x 256 (not taken) 60 and 51; distillation with
 // K = 32, 2000 x 81 x 128: fp32 30 and 85, bf16 32 and 67.
@@ -696,6 +698,29 @@ Plan make_plan(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int distil
   return p;
 }
 
+// Few tokens and a W that would have to be laid out (vocab_few.hpp).
+// (The vocabulary has to be larger than one tile: in a small one the sums are formed again in the backward pass, where 1 - p needs them.)
+struct FewPlan { int tokens; int64_t ld_z, dx_rows, splits, ld_slab, z, part, flag, q, entropy, slab, bytes; };
+bool few_tokens(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int pack_w) {
+  return pack_w && M <= FEW_TOKENS && V > SHAPE[S128].bm && up(M, 16) * up(V, 64) * 4 <= FEW_LOGITS && !small(M, V, D, K, dtype);
+}
+FewPlan few_plan(int64_t M, int64_t V, int64_t D, int64_t K, bool distill, int backward) {
+  FewPlan p = {};
+  p.tokens = M <= 16 ? 16 : 32;
+  p.ld_z = up(V, 64); p.ld_slab = up(D, 64);
+  const int64_t blocks = p.ld_slab / 64;
+  // workgroups for the whole chip, four a CU; their partial sums stay below 16 MB
+  p.dx_rows = up(tiles(V, blocks < 1024 ? 1024 / blocks : 1), 64); p.splits = tiles(V, p.dx_rows);
+  int64_t o = 0;
+  auto take = [&](int64_t bytes) { const int64_t at = o; o = up(o + bytes, 256); return at; };
+  p.z = take(p.tokens * p.ld_z * 4);
+  if (distill) { p.flag = take(up(M, 16)); p.q = take(M * K * 4 * (backward ? 2 : 1)); }
+  if (backward) p.slab = take(p.splits * p.tokens * p.ld_slab * 4);
+  else { p.part = take(M * (p.ld_z / FEW_ROWS) * 8); p.entropy = take(M * 4); }
+  p.bytes = o;
+  return p;
+}
+
 int needs_pack(const void* w, int64_t ldw, int64_t D, int dtype) {
   return dtype == GNET_F32 || (D & 7) || (ldw & 7) || ldw > (1 << 22) || ((uintptr_t)w & 15);      // (2^22: 32-bit offsets in a tile)
 }
@@ -736,6 +761,61 @@ template <int DT> struct Small {
       vocab_small_dw<DT><<<dim3((unsigned)tiles(q.t.V, 16), (unsigned)tiles(q.D, 16)), 64 * SMALL_DW_WAVES, 0, s>>>(d);
     }
     return launch_status();
+  }
+};
+
+// ---- few tokens ------------------------------------------------------------------------------------------------------
+template <int DT> struct Few {
+  static void targets(const Problem& q, const FewPlan& p, char* ws, const float* dloss, hipStream_t s) {
+    TargetsArgs a = {};
+    a.t = q.t; a.flags_n = up(q.t.M, 16); a.token_groups = (unsigned)tiles(a.flags_n, 4);
+    a.dloss = dloss; a.flag = (uint8_t*)(ws + p.flag); a.q = (float*)(ws + p.q); a.q_sum = a.q + q.t.M * q.t.K;
+    if (!dloss) a.entropy = (float*)(ws + p.entropy);
+    vocab_targets<<<a.token_groups, 256, 0, s>>>(a);
+  }
+  static FewArgs args(const Problem& q, const FewPlan& p, char* ws) {
+    FewArgs a = {};
+    a.t = q.t; a.flag = q.t.logits ? (const uint8_t*)(ws + p.flag) : nullptr;
+    a.x = q.x; a.ldx = q.ldx; a.w = q.w; a.ldw = q.ldw; a.D = q.D;
+    a.z = (float*)(ws + p.z); a.ld_z = p.ld_z;
+    return a;
+  }
+  template <int NT> static int forward(const Problem& q, const FewPlan& p, char* ws, float* loss, float* lse, float* hit, hipStream_t s) {
+    if (q.t.logits) targets(q, p, ws, nullptr, s);
+    FewArgs a = args(q, p, ws);
+    a.part = (float2*)(ws + p.part);
+    vocab_few_logits<DT, NT, false><<<(unsigned)(p.ld_z / FEW_ROWS), 256, 0, s>>>(a);
+    vocab_few_join<<<(unsigned)q.t.M, 256, 0, s>>>(FewJoinArgs{q.t, a.flag, a.z, p.ld_z, a.part, (const float*)(ws + p.q), (const float*)(ws + p.entropy), loss, lse, hit});
+    return launch_status();
+  }
+  template <int NT> static int backward(const Problem& q, const FewPlan& p, char* ws, const float* lse, const float* hit, const float* dloss, void* dx, void* dw, hipStream_t s) {
+    if (q.t.logits) targets(q, p, ws, dloss, s);
+    FewArgs a = args(q, p, ws);
+    a.lse = lse; a.dloss = dloss;
+    vocab_few_logits<DT, NT, true><<<(unsigned)(p.ld_z / FEW_ROWS), 256, 0, s>>>(a);
+    if (q.t.logits)
+      vocab_few_hits<<<(unsigned)tiles(q.t.M * q.t.K, 256), 256, 0, s>>>(q.t, lse, hit, (const float*)(ws + p.q) + q.t.M * q.t.K, dloss, a.z, p.ld_z);
+    if (dx) {
+      float* slab = (float*)(ws + p.slab);
+      vocab_few_dx<DT, NT><<<(unsigned)(p.ld_slab / 64 * up(p.splits, 8)), 256, 0, s>>>(FewDxArgs{q.w, q.ldw, q.t.V, q.D, a.z, p.ld_z, p.dx_rows, p.splits, slab, p.ld_slab});
+      vocab_few_finish<DT><<<dim3((unsigned)tiles(q.D, 256), (unsigned)q.t.M), 256, 0, s>>>(q.t, a.flag, slab, p.ld_slab, p.tokens * p.ld_slab, (int)p.splits, q.D, dx);
+    }
+    if (dw) {
+      const int64_t rows = p.ld_z / FEW_ROWS, most = tiles(q.D, 256), parts = most * rows < 1024 ? most : tiles(1024, rows);
+      const int64_t features = up(tiles(q.D, parts), 256);
+      vocab_few_dw<DT, NT><<<dim3((unsigned)rows, (unsigned)tiles(q.D, features)), 256, 0, s>>>(FewDwArgs{q.t, a.flag, q.x, q.ldx, q.D, a.z, p.ld_z, features, dw});
+    }
+    return launch_status();
+  }
+  static int forward(const Problem& q, void* ws, size_t ws_bytes, float* loss, float* lse, float* hit, hipStream_t s) {
+    const FewPlan p = few_plan(q.t.M, q.t.V, q.D, q.t.K, q.t.logits != nullptr, 0);
+    if (!ws || ws_bytes < (size_t)p.bytes || ((uintptr_t)ws & 255)) return GNET_ERR_WORKSPACE;
+    return p.tokens == 16 ? forward<1>(q, p, (char*)ws, loss, lse, hit, s) : forward<2>(q, p, (char*)ws, loss, lse, hit, s);
+  }
+  static int backward(const Problem& q, void* ws, size_t ws_bytes, const float* lse, const float* hit, const float* dloss, void* dx, void* dw, hipStream_t s) {
+    const FewPlan p = few_plan(q.t.M, q.t.V, q.D, q.t.K, q.t.logits != nullptr, 1);
+    if (!ws || ws_bytes < (size_t)p.bytes || ((uintptr_t)ws & 255)) return GNET_ERR_WORKSPACE;
+    return p.tokens == 16 ? backward<1>(q, p, (char*)ws, lse, hit, dloss, dx, dw, s) : backward<2>(q, p, (char*)ws, lse, hit, dloss, dx, dw, s);
   }
 };
 
@@ -940,7 +1020,13 @@ int run_forward(const Problem& q, float* loss, float* lse, float* hit, void* ws,
   if (const int e = check(q)) return e;
   if (q.t.M == 0) return GNET_OK;
   if (!loss || !lse || !hit) return GNET_ERR_INVALID;
-  const Plan p = make_plan(q.t.M, q.t.V, q.D, q.t.K, q.dtype, q.t.logits != nullptr, needs_pack(q.w, q.ldw, q.D, q.dtype), 0);
+  const int pack_w = needs_pack(q.w, q.ldw, q.D, q.dtype);
+  if (few_tokens(q.t.M, q.t.V, q.D, q.t.K, q.dtype, pack_w)) switch (q.dtype) {
+    case GNET_F32: return Few<GNET_F32>::forward(q, ws, ws_bytes, loss, lse, hit, s);
+    case GNET_BF16: return Few<GNET_BF16>::forward(q, ws, ws_bytes, loss, lse, hit, s);
+    default: return Few<GNET_F16>::forward(q, ws, ws_bytes, loss, lse, hit, s);
+  }
+  const Plan p = make_plan(q.t.M, q.t.V, q.D, q.t.K, q.dtype, q.t.logits != nullptr, pack_w, 0);
   if (!ws || ws_bytes < (size_t)p.bytes || ((uintptr_t)ws & 255)) return GNET_ERR_WORKSPACE;
   if (small(q.t.M, q.t.V, q.D, q.t.K, q.dtype)) switch (q.dtype) {
     case GNET_F32: return Small<GNET_F32>::forward(q, loss, lse, hit, s);
@@ -965,7 +1051,13 @@ int run_backward(const Problem& q, const float* lse, const float* hit, const flo
     return launch_status();
   }
   if (!lse || !hit || !dloss) return GNET_ERR_INVALID;
-  const Plan p = make_plan(q.t.M, q.t.V, q.D, q.t.K, q.dtype, q.t.logits != nullptr, needs_pack(q.w, q.ldw, q.D, q.dtype), 1);
+  const int pack_w = needs_pack(q.w, q.ldw, q.D, q.dtype);
+  if (few_tokens(q.t.M, q.t.V, q.D, q.t.K, q.dtype, pack_w)) switch (q.dtype) {
+    case GNET_F32: return Few<GNET_F32>::backward(q, ws, ws_bytes, lse, hit, dloss, dx, dw, s);
+    case GNET_BF16: return Few<GNET_BF16>::backward(q, ws, ws_bytes, lse, hit, dloss, dx, dw, s);
+    default: return Few<GNET_F16>::backward(q, ws, ws_bytes, lse, hit, dloss, dx, dw, s);
+  }
+  const Plan p = make_plan(q.t.M, q.t.V, q.D, q.t.K, q.dtype, q.t.logits != nullptr, pack_w, 1);
   if (!ws || ws_bytes < (size_t)p.bytes || ((uintptr_t)ws & 255)) return GNET_ERR_WORKSPACE;
   if (small(q.t.M, q.t.V, q.D, q.t.K, q.dtype)) switch (q.dtype) {
     case GNET_F32: return Small<GNET_F32>::backward(q, (char*)ws, dloss, dx, dw, s);
@@ -993,8 +1085,10 @@ Problem problem(const void* x, int64_t ldx, const void* w, int64_t ldw, const vo
 // ------------------------------------------------------------------------------------------
 extern "C" size_t gnet_vocab_workspace_bytes(const void* w, int64_t ldw, int64_t M, int64_t V, int64_t D, int64_t K, int32_t dtype, int32_t backward) {
   if (M <= 0 || V < 1 || D < 1 || K < 0 || M > (1 << 24) || V > (1ll << 30) || D > (1 << 16) || K > 1024) return 0;
+  const int pack_w = needs_pack(w, ldw, D, dtype);
   // K = 0: cross entropy
-  return (size_t)make_plan(M, V, D, K, dtype, K > 0, needs_pack(w, ldw, D, dtype), backward).bytes;
+  if (few_tokens(M, V, D, K, dtype, pack_w)) return (size_t)few_plan(M, V, D, K, K > 0, backward).bytes;
+  return (size_t)make_plan(M, V, D, K, dtype, K > 0, pack_w, backward).bytes;
 }
 
 extern "C" int gnet_xent_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* labels, int32_t labels64, int64_t M,

@@ -11,21 +11,47 @@
 // Bound by latency: 2000 x 81 x 128 fp32 takes 7 us forward, 11 and 9 us backward, of which an empty launch is 2 to 3.
 #pragma once
 
-
 // N consecutive elements as they lie in memory, at an element's alignment
 template <int DT, int N> struct SmallRaw {
   typedef std::conditional_t<DT == GNET_F32, float, short> E;
   typedef E V __attribute__((ext_vector_type(N)));
   typedef E U __attribute__((ext_vector_type(N), aligned(sizeof(E))));
   V v;
-  __device__ __forceinline__ void load(const void* p, int64_t i) { v = *reinterpret_cast<const U*>((const E*)p + i); }
-  __device__ __forceinline__ void load(const void* p, int64_t i, int64_t left) {       // `left` of them exist
+  // (16 bits at an odd address: the dwords that hold them, shifted.  A vector load that starts inside a dword takes 190 cycles a wave, one
+  // at a dword's start 16; what the first and last dword hold besides is not used.)
+  __device__ __forceinline__ void load(const void* p, int64_t i) {
+    if constexpr (DT == GNET_F32 || N < 4) v = *reinterpret_cast<const U*>((const E*)p + i);
+    else {
+      typedef unsigned W __attribute__((ext_vector_type(N / 2)));
+      typedef unsigned WU __attribute__((ext_vector_type(N / 2), aligned(4)));
+      const uintptr_t at = (uintptr_t)((const E*)p + i);
+      const W lo = *reinterpret_cast<const WU*>(at & ~(uintptr_t)3);
+      const unsigned hi = *reinterpret_cast<const unsigned*>((at + 2 * N - 2) & ~(uintptr_t)3), shift = (unsigned)(at & 2) * 8;
+      W o;
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = j < left ? ((const E*)p)[i + j] : (E)0;
+      for (int k = 0; k < N / 2; ++k) o[k] = __builtin_amdgcn_alignbit(k + 1 < N / 2 ? lo[k + 1 < N / 2 ? k + 1 : k] : hi, lo[k], shift);
+      v = __builtin_bit_cast(V, o);
+    }
+  }
+  // `left` of them exist, maybe none, but the row has at least one: the last one in place of the others
+  __device__ __forceinline__ void load(const void* p, int64_t i, int64_t left) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = ((const E*)p)[i + min((int64_t)j, left - 1)];
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = j < left ? v[j] : (E)0;
   }
   __device__ __forceinline__ float get(int j) const {
     if constexpr (DT == GNET_F32) return v[j];
     else return DT == GNET_BF16 ? Bf16T::dec((u16)v[j]) : F16T::dec((u16)v[j]);
+  }
+  __device__ __forceinline__ void set(int j, float f) {
+    if constexpr (DT == GNET_F32) v[j] = f;
+    else v[j] = (short)(DT == GNET_BF16 ? Bf16T::enc(f) : F16T::enc(f));
+  }
+  __device__ __forceinline__ void store(void* p, int64_t i, int64_t left) const {
+    if (left >= N) { *reinterpret_cast<U*>((E*)p + i) = v; return; }
+#pragma unroll
+    for (int j = 0; j < N; ++j) if (j < left) ((E*)p)[i + j] = v[j];
   }
 };
 template <int DT> __device__ __forceinline__ void small_store(void* p, int64_t i, float v) {
