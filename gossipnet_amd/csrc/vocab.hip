@@ -11,7 +11,7 @@
 //              vocab_gemm<EPI_SLAB>  dx += dz . W (fp32)     vocab_gemm<EPI_OUT>  dW = dz^T . x     and at last vocab_finish  dx
 // A token whose targets are all outside [0, V) is left out of everything, whatever its row of x holds: it is not read again after
 // vocab_targets, its dx is zero.
-// A small vocabulary takes other kernels (vocab_small.hpp), and so do few tokens on a W that would have to be laid out (vocab_few.hpp); few
+// A small vocabulary takes other kernels (vocab_small.hpp), and so do few tokens on a W that would have to be laid out (vocab_few.hpp) or on little of it; few
 // tiles of logits take another softmax (logits_splits).
 #include "vocab_gemm.hpp"
 
@@ -698,11 +698,14 @@ Plan make_plan(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int distil
   return p;
 }
 
-// Few tokens and a W that would have to be laid out (vocab_few.hpp).
+// Few tokens and a W that would have to be laid out, or so little work that the general path is its launches (vocab_few.hpp).  bf16 weights
+// that need no layout, both directions, here and there: 16 x 1000 x 128 22 and 33 us, 16 x 16000 x 128 34 and 37, 16 x 4000 x 512 34 and 38;
+// 32 x 4000 x 512 (not taken) 43 and 39, 16 x 1000 x 4096 (not taken) 93 and 54.
 // (The vocabulary has to be larger than one tile: in a small one the sums are formed again in the backward pass, where 1 - p needs them.)
 struct FewPlan { int tokens; int64_t ld_z, dx_rows, splits, ld_slab, z, part, flag, q, entropy, slab, bytes; };
 bool few_tokens(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int pack_w) {
-  return pack_w && M <= FEW_TOKENS && V > SHAPE[S128].bm && up(M, 16) * up(V, 64) * 4 <= FEW_LOGITS && !small(M, V, D, K, dtype);
+  const bool little = D <= 1024 && up(M, 16) * V * D <= 1 << 25;
+  return (pack_w || little) && M <= FEW_TOKENS && V > SHAPE[S128].bm && up(M, 16) * up(V, 64) * 4 <= FEW_LOGITS && !small(M, V, D, K, dtype);
 }
 FewPlan few_plan(int64_t M, int64_t V, int64_t D, int64_t K, bool distill, int backward) {
   FewPlan p = {};

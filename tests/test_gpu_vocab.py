@@ -136,7 +136,7 @@ SIZES = [(1, 1, 1), (1, 2, 3), (3, 5, 7), (2, 300, 64), (17, 130, 65), (64, 127,
          (300, 513, 256), (5, 8191, 72), (31, 4099, 320), (513, 81, 128), (1100, 1030, 136), (3, 200, 8200), (9001, 130, 64), (270000, 40, 8),
          (165, 2283, 2240), (5, 154, 2050), (300, 129, 1100),
          (20, 120, 600), (50, 100, 700), (9000, 81, 128), (33, 256, 128), (17, 255, 129), (2000, 81, 128), (8192, 9, 30),
-         (5, 3001, 129), (16, 1000, 592), (17, 700, 301), (32, 5000, 75), (32, 2049, 515), (33, 2049, 515), (20, 129, 1000)]
+         (5, 3001, 129), (16, 1000, 592), (17, 700, 301), (32, 5000, 75), (32, 2049, 515), (33, 2049, 515), (20, 129, 1000), (16, 2048, 1024), (17, 2048, 1024), (2, 5000, 1032)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
