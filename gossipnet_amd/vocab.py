@@ -22,8 +22,12 @@ def _p(t):
     return t.data_ptr() if t is not None else None
 
 
+# (torch.cuda.current_stream makes an object first: 2 us of a call that takes 8)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(dev):
-    return torch.cuda.current_stream(dev).cuda_stream
+    return _raw_stream(dev.index) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
 
 
 class _Here(object):
@@ -44,18 +48,20 @@ def _device(dev):
 
 def _matrix(t, what, cols=None, dtype=None):
     """A [..., D] tensor as rows of D consecutive elements (a view where its layout allows it)."""
-    if t.dim() < 1 or t.dtype not in _TYPES:
+    shape = t.shape
+    if len(shape) < 1 or t.dtype not in _TYPES:
         raise _lib.InvalidArgumentError("%s must be a float32, bfloat16 or float16 tensor with at least one dimension" % what)
-    if cols is not None and t.shape[-1] != cols:
-        raise _lib.InvalidArgumentError("%s must have %d columns, not %d" % (what, cols, t.shape[-1]))
+    if cols is not None and shape[-1] != cols:
+        raise _lib.InvalidArgumentError("%s must have %d columns, not %d" % (what, cols, shape[-1]))
     if dtype is not None and t.dtype != dtype:
         raise _lib.InvalidArgumentError("%s is %s where %s is expected" % (what, t.dtype, dtype))
-    if t.shape[-1] == 0:
+    if shape[-1] == 0:
         raise _lib.InvalidArgumentError("%s has rows of no elements" % what)
-    t = t.detach()
-    t = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
-    if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        t = t.contiguous()
+    if len(shape) != 2:
+        t = t.detach().reshape(-1, shape[-1])
+    step, one = t.stride()
+    if one != 1 or (step < t.shape[1] and t.shape[0] > 1):
+        t = t.detach().contiguous()
     return t
 
 
@@ -76,16 +82,16 @@ def _on_device(first, **others):
 def _ids(t, what, shape=None):
     if t.dtype not in (torch.int32, torch.int64):
         raise _lib.InvalidArgumentError("%s must be int32 or int64, not %s" % (what, t.dtype))
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         raise _lib.InvalidArgumentError("%s has shape %s where %s is expected" % (what, tuple(t.shape), tuple(shape)))
-    return t.detach().contiguous()
+    return t.contiguous()
 
 
 def _per_token(t, what, shape):
     """fp32 values of the tokens' shape."""
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise _lib.InvalidArgumentError("%s has shape %s where %s is expected" % (what, tuple(t.shape), tuple(shape)))
-    return t.detach().to(torch.float32).contiguous()
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.detach().to(torch.float32).contiguous()
 
 
 def _workspace(nbytes, device):
@@ -106,7 +112,7 @@ def embed_forward(ids, table, scale=1.0, token_scale=None):
     i = _ids(ids, "ids")
     s = _per_token(token_scale, "token_scale", ids.shape) if token_scale is not None else None
     dev = _on_device(t, ids=i, token_scale=s)
-    y = torch.empty(tuple(ids.shape) + (D,), dtype=t.dtype, device=dev)
+    y = torch.empty(ids.shape + (D,), dtype=t.dtype, device=dev)
     lib = _lib.load()
     with _device(dev):
         _lib.check(lib.gnet_embed_forward(_p(i), int(i.dtype == torch.int64), _p(t), _ld(t), float(scale), _p(s), i.numel(), V, D,
@@ -123,7 +129,7 @@ def embed_backward(ids, dy, table, scale=1.0, token_scale=None, need_dscale=Fals
     t = _matrix(table, "table")
     V, D = t.shape
     i = _ids(ids, "ids")
-    if tuple(dy.shape) != tuple(ids.shape) + (D,):
+    if dy.shape != ids.shape + (D,):
         raise _lib.InvalidArgumentError("dy has shape %s where %s is expected" % (tuple(dy.shape), tuple(ids.shape) + (D,)))
     g = _matrix(dy, "dy", D, t.dtype)
     s = _per_token(token_scale, "token_scale", ids.shape) if token_scale is not None else None
@@ -134,7 +140,7 @@ def embed_backward(ids, dy, table, scale=1.0, token_scale=None, need_dscale=Fals
     dtable = out.detach() if out is not None else torch.empty(V, D, dtype=t.dtype, device=dev)
     M = i.numel()
     lib = _lib.load()
-    dscale = torch.empty(tuple(ids.shape), dtype=torch.float32, device=dev) if need_dscale else None
+    dscale = torch.empty(ids.shape, dtype=torch.float32, device=dev) if need_dscale else None
     with _device(dev):
         nbytes = lib.gnet_embed_workspace_bytes(M, D)
         buf, ws = _workspace(nbytes, dev)
@@ -154,9 +160,9 @@ def _features(x, w):
 def _teacher(top_ids, top_logits, x, temperature):
     if not (temperature > 0 and temperature < float("inf")):
         raise _lib.InvalidArgumentError("temperature must be positive and finite, not %s" % (temperature,))
-    lead = tuple(x.shape[:-1])
-    if top_ids.dim() != len(lead) + 1 or tuple(top_ids.shape[:-1]) != lead or top_ids.shape[-1] < 1:
-        raise _lib.InvalidArgumentError("top_ids must be [*tokens, K] with K >= 1, tokens %s" % (lead,))
+    lead = x.shape[:-1]
+    if top_ids.dim() != len(lead) + 1 or top_ids.shape[:-1] != lead or top_ids.shape[-1] < 1:
+        raise _lib.InvalidArgumentError("top_ids must be [*tokens, K] with K >= 1, tokens %s" % (tuple(lead),))
     return _ids(top_ids, "top_ids"), _per_token(top_logits, "top_logits", top_ids.shape)
 
 
@@ -171,11 +177,12 @@ def xent_forward(x, w, labels):
     """(loss, lse, hit), fp32, of labels' shape: softmax cross entropy of the logits x . w^T (x [*tokens, D], w [V, D]) against
     labels [*tokens], the logits' log-sum-exp and the label's logit.  All three are 0 where the label is outside [0, V)."""
     xm, wm = _features(x, w)
-    lead = tuple(x.shape[:-1])
+    lead = x.shape[:-1]
     i = _ids(labels, "labels", lead)
     dev = _on_device(wm, x=xm, labels=i)
     (M, D), V = xm.shape, wm.shape[0]
-    loss, lse, hit = (torch.empty(lead, dtype=torch.float32, device=dev) for _ in range(3))
+    loss = torch.empty(lead, dtype=torch.float32, device=dev)
+    lse, hit = torch.empty_like(loss), torch.empty_like(loss)
     lib = _lib.load()
     with _device(dev):
         nbytes = lib.gnet_vocab_workspace_bytes(_p(wm), _ld(wm), M, V, D, 0, _TYPES[wm.dtype], 0)
@@ -189,7 +196,7 @@ def xent_backward(x, w, labels, lse, hit, dloss, need_dx=True, need_dw=True):
     """(dx, dw) of xent_forward, of x's and w's shapes and type, from its lse and hit and the losses' gradient dloss (labels' shape,
     or a tensor without dimensions for all tokens).  None for what is not needed."""
     xm, wm = _features(x, w)
-    lead = tuple(x.shape[:-1])
+    lead = x.shape[:-1]
     i = _ids(labels, "labels", lead)
     return _backward(xm, wm, i, None, 1.0, _per_token(lse, "lse", lead), _per_token(hit, "hit", lead), _loss_gradient(dloss, lead), x.shape, 0, need_dx, need_dw)
 
@@ -199,11 +206,12 @@ def distill_forward(x, w, top_ids, top_logits, temperature=1.0):
     logits / temperature (top_ids, top_logits [*tokens, K]), the student's log-sum-exp [*tokens], and its logits / temperature at
     top_ids [*tokens, K].  Slots with an id outside [0, V) or a logit of -inf are left out; a token without slots has loss 0."""
     xm, wm = _features(x, w)
-    lead = tuple(x.shape[:-1])
+    lead = x.shape[:-1]
     i, t = _teacher(top_ids, top_logits, x, temperature)
     dev = _on_device(wm, x=xm, top_ids=i, top_logits=t)
     (M, D), V, K = xm.shape, wm.shape[0], i.shape[-1]
-    loss, lse = (torch.empty(lead, dtype=torch.float32, device=dev) for _ in range(2))
+    loss = torch.empty(lead, dtype=torch.float32, device=dev)
+    lse = torch.empty_like(loss)
     hit = torch.empty(lead + (K,), dtype=torch.float32, device=dev)
     lib = _lib.load()
     with _device(dev):
@@ -218,7 +226,7 @@ def distill_forward(x, w, top_ids, top_logits, temperature=1.0):
 def distill_backward(x, w, top_ids, top_logits, lse, hit, dloss, temperature=1.0, need_dx=True, need_dw=True):
     """(dx, dw) of distill_forward, of x's and w's shapes and type (the teacher's logits get no gradient)."""
     xm, wm = _features(x, w)
-    lead = tuple(x.shape[:-1])
+    lead = x.shape[:-1]
     i, t = _teacher(top_ids, top_logits, x, temperature)
     return _backward(xm, wm, i, t, temperature, _per_token(lse, "lse", lead), _per_token(hit, "hit", i.shape), _loss_gradient(dloss, lead), x.shape, i.shape[-1], need_dx, need_dw)
 
