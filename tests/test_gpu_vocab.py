@@ -376,7 +376,7 @@ def test_gradient_against_differences():
 # ---- embedding rows -----------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("shape,V,D", [((1,), 1, 1), ((3, 5), 7, 3), ((1,), 100, 4096), ((130,), 50, 65), ((4097,), 81, 128), ((2, 700), 3000, 264), ((70000,), 33, 8),
-                                       ((9000,), 100000, 16), ((2000,), 300, 1003), ((5000,), 2 ** 20 - 2, 8), ((5000,), 2 ** 20 - 1, 8), ((300, 300), 2 ** 21, 2)])
+                                       ((9000,), 100000, 16), ((2000,), 300, 1003), ((64,), 5000, 1000), ((65,), 5000, 1000), ((7, 9), 3001, 65), ((40,), 2 ** 21, 3), ((5000,), 2 ** 20 - 2, 8), ((5000,), 2 ** 20 - 1, 8), ((300, 300), 2 ** 21, 2)])
 def test_embed(shape, V, D, dtype):
     from gossipnet_amd import vocab
     t = TYPES[dtype]
@@ -415,7 +415,7 @@ def test_embed(shape, V, D, dtype):
 
 
 @pytest.mark.parametrize("V", [40, 4000])
-@pytest.mark.parametrize("M", [15, 16, 17, 32, 33, 64, 129, 2048, 2049, 4096, 4097, 65537, 70000])
+@pytest.mark.parametrize("M", [15, 16, 17, 32, 33, 63, 64, 65, 129, 2048, 2049, 4096, 4097, 65537, 70000])
 def test_embed_gradient_of_one_row_and_of_runs_around_the_hot_limit(M, V):
     """All tokens the same id; and runs of 15, 16, 17 and more tokens at every place of the sorted order."""
     from gossipnet_amd import vocab
