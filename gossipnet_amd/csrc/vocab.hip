@@ -9,8 +9,7 @@
 //   backward   the first two, then for one piece of the vocabulary after the other
 //              vocab_gemm<EPI_DZ>  dz = g (softmax(z) - label) from recomputed logits       vocab_hits   dz at the teacher's ids
 //              vocab_gemm<EPI_SLAB>  dx += dz . W (fp32)     vocab_gemm<EPI_OUT>  dW = dz^T . x     and at last vocab_finish  dx
-// A token whose targets are all outside [0, V) is left out of everything, whatever its row of x holds: it is not read again after
-// vocab_targets, its dx is zero.
+// A token whose targets are all outside [0, V) is left out of everything, whatever its row of x holds, and its dx is zero.
 // A small vocabulary takes other kernels (vocab_small.hpp), and so do few tokens on a W that would have to be laid out (vocab_few.hpp) or on little of it; few
 // tiles of logits take another softmax (logits_splits).
 #include "vocab_gemm.hpp"

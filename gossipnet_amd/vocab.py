@@ -8,8 +8,8 @@ plain tensors out, forward and backward as two calls (as in fc.py); PyTorch only
     embed_backward(ids, dy, table, scale, out=dw)                 # a table that is also w: its second gradient is added
 
 Tokens may be laid out in any number of leading dimensions ([B, T] or flat); x, w, table, dy are float32, bfloat16 or float16,
-all of a call of one type; ids and labels int32 or int64.  An id or label outside [0, V) means "no token here" (padding): nothing
-is read or added for it.  Every result is reproducible bit for bit.  The calls run on the current stream of the tensors' device and
+all of a call of one type; ids and labels int32 or int64.  An id or label outside [0, V) means "no token here" (padding): it adds
+nothing, whatever its row holds.  Every result is reproducible bit for bit.  The calls run on the current stream of the tensors' device and
 may be captured into a graph; workspaces come from PyTorch's allocator for each call."""
 import torch
 
