@@ -193,8 +193,9 @@ def xent_forward(x, w, labels):
 
 
 def xent_backward(x, w, labels, lse, hit, dloss, need_dx=True, need_dw=True):
-    """(dx, dw) of xent_forward, of x's and w's shapes and type, from its lse and hit and the losses' gradient dloss (labels' shape,
-    or a tensor without dimensions for all tokens).  None for what is not needed."""
+    """(dx, dw) of xent_forward, of x's and w's shapes and type, from its lse and hit (of the same x, w and labels: they are not looked
+    at where a token's whole softmax is formed again) and the losses' gradient dloss (labels' shape, or a tensor without dimensions for
+    all tokens).  None for what is not needed."""
     xm, wm = _features(x, w)
     lead = x.shape[:-1]
     i = _ids(labels, "labels", lead)

@@ -325,8 +325,10 @@ int gnet_embed_backward(const void* ids, int32_t ids64, const void* dy, int64_t 
  * A token whose label is outside [0, V) is left out: loss, lse, hit and its row of dx are 0 and it adds nothing to dw, whatever its row
  * of x holds.  Backward: from the forward pass's lse and hit and the losses' gradients dloss [M],
  *   dz[m,v] = dloss[m] (exp(z[m,v] - lse[m]) - [v = labels[m]])     dx = dz . w     dw = dz^T . x
+ * lse and hit have to be what the forward call gave for the same operands: where a token's whole row of logits is at hand its softmax
+ * is formed again, and they are not looked at.
  * dx [M,D] and dw [V,D] are overwritten; either may be NULL.  The logits are formed again, one piece of the vocabulary at a time;
- * dz is kept in 16 bits (GNET_F32: two fp16 of together 22 bits) for the piece.  w and the rows of x that count must be finite.  Reproducible.
+ * dz is kept in 16 bits (GNET_F32: two fp16 of together 22 bits) for the piece, or in fp32 for few tokens or a small vocabulary.  w and the rows of x that count must be finite.  Reproducible.
  * workspace of all four calls: gnet_vocab_workspace_bytes(w, ldw, M, V, D, K, dtype, backward) (K = 0: cross entropy). */
 size_t gnet_vocab_workspace_bytes(const void* w, int64_t ldw, int64_t M, int64_t V, int64_t D, int64_t K, int32_t dtype,
                                   int32_t backward);
