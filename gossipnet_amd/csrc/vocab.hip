@@ -13,6 +13,7 @@
 // A small vocabulary takes other kernels (vocab_small.hpp), and so do few tokens on a W that would have to be laid out (vocab_few.hpp) or on little of it; few
 // tiles of logits take another softmax (logits_splits).
 #include "vocab_gemm.hpp"
+#include <algorithm>
 
 namespace {
 
@@ -584,18 +585,20 @@ inline int64_t tiles(int64_t v, int64_t a) { return (v + a - 1) / a; }
 
 // Tile shapes of the products.  A contraction step of 64 takes 256 x 256 tiles 1.5 us (one workgroup a CU: 1.4 PFLOP/s) and 128 x 128
 // tiles 0.9 us (two a CU: 1.2), and every tile 6 or 3.5 us before and behind its steps (fitted to 4096 x 131072 x 4096, 833 x 50257 x 1024 and
-// 464 x 65537 x 1536).  128 x 64 and 128 x 32 are for products with that few tokens, which wait for W: they only have to keep
+// 464 x 65537 x 1536).  A last round that fills half of the chip at most is worked on as half tiles (vocab_gemm.hpp).  128 x 64 and 128 x 32 are for products with that few tokens, which wait for W: they only have to keep
 // loads in flight.
 enum Shape { S256, S128, S64, S32 };
 struct ShapeInfo { int bm, bn; };
 constexpr ShapeInfo SHAPE[] = {{256, 256}, {128, 128}, {128, 64}, {128, 32}};
 struct Product { int shape, splits; };
 
-double product_us(int shape, int splits, int64_t rows, int64_t cols, int64_t steps) {
+double product_us(int shape, int splits, int64_t rows, int64_t cols, int64_t steps, bool halves) {
   const int64_t n = tiles(rows, SHAPE[shape].bm) * tiles(cols, SHAPE[shape].bn) * splits;
   const double round = shape == S256 ? tiles(steps, splits) * 1.5 + 6 : tiles(steps, splits) * 0.9 + 3.5;
+  const int64_t at_once = shape == S256 ? 256 : 512, rest = n % at_once;
+  const double rounds = (double)(n / at_once) + (!rest ? 0. : halves && 2 * rest <= at_once ? 0.65 : 1.);
   const double joined = splits > 1 ? 5 + (double)rows * cols * 4 * (2 * splits) / 4e6 : 0;       // partial sums out and in at 4 TB/s
-  return tiles(n, shape == S256 ? 256 : 512) * round + joined;
+  return rounds * round + joined;
 }
 // few_cols: the columns are tokens, for which the narrow shapes exist
 Product pick_product(int64_t rows, int64_t cols, int64_t steps, bool few_cols, bool may_split) {
@@ -604,7 +607,7 @@ Product pick_product(int64_t rows, int64_t cols, int64_t steps, bool few_cols, b
     double least = 1e30;
     for (int shape = S256; shape <= S128; ++shape)
       for (int splits = 1; splits <= (may_split ? 16 : 1) && (splits == 1 || steps / splits >= 4); ++splits) {
-        const double us = product_us(shape, splits, rows, cols, steps);
+        const double us = product_us(shape, splits, rows, cols, steps, shape == S256 || few_cols);
         if (us < least) { least = us; best.shape = shape; best.splits = splits; }
       }
   } else if (may_split) {
@@ -824,7 +827,15 @@ template <int DT> struct Few {
 template <int DT, class T, int PLANES> struct Run {
   template <int BM, int BN, int WM, int WN, int STAGES, bool AS, bool BS, int EPI> static void launch(VocabGemm& g, int64_t rows, int64_t cols, int splits, hipStream_t s) {
     g.row_tiles = (int)tiles(rows, BM); g.col_tiles = (int)tiles(cols, BN); g.splits = splits;
-    vocab_gemm<T, BM, BN, WM, WN, STAGES, AS, BS, EPI, PLANES><<<(unsigned)((int64_t)g.row_tiles * g.col_tiles * splits), 64 * WM * WN, 0, s>>>(g);
+    // half tiles are workgroups of their own; how many columns of tiles there are is known on the device, so the most of all counts
+    const int64_t at_once = vocab_halves<BN, BS>() ? vocab_at_once<BM>() : 1;
+    int64_t groups = 0;
+    for (int64_t c = g.col_tiles; c > 0; --c) {
+      const int64_t share = tiles((int64_t)g.row_tiles * c * splits, 8);
+      for (int64_t k = share; k >= 0 && k >= share - 1; --k) groups = std::max(groups, k + (2 * (k % at_once) <= at_once ? k % at_once : 0));
+      if (!g.cols_from_meta || share + at_once / 2 <= groups) break;
+    }
+    vocab_gemm<T, BM, BN, WM, WN, STAGES, AS, BS, EPI, PLANES><<<(unsigned)(8 * groups), 64 * WM * WN, 0, s>>>(g);
   }
   // columns are tokens (all shapes) or vocabulary (the square ones)
   template <bool AS, bool BS, int EPI> static void gemm(VocabGemm& g, const Product& p, int64_t rows, int64_t cols, hipStream_t s) {
