@@ -30,20 +30,17 @@ def _stream(dev):
     return _raw_stream(dev.index) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
 
 
-class _Here(object):
-    """Nothing to switch: the call's device is the current one (torch.cuda.device costs microseconds that a small call feels)."""
-    def __enter__(self):
-        pass
-
-    def __exit__(self, *_):
-        pass
+_current = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-_HERE = _Here()
-
-
-def _device(dev):
-    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+def _call(dev, f, *args):
+    """The library's f on the stream that is current on device dev (which is made the current one if it is not: torch.cuda.device costs
+    microseconds that a small call feels)."""
+    if _current() == dev.index:
+        _lib.check(f(*args, _stream(dev)), f.__name__)
+    else:
+        with torch.cuda.device(dev):
+            _lib.check(f(*args, _stream(dev)), f.__name__)
 
 
 def _matrix(t, what, cols=None, dtype=None):
@@ -69,13 +66,14 @@ def _ld(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _on_device(first, **others):
-    """The device of a call (after the checks of shapes and types)."""
-    if not first.is_cuda:
+def _on_device(first, *others):
+    """The device of a call (after the checks of shapes and types).  others: tensors or None."""
+    here = first.get_device()
+    if here < 0:
         raise _lib.GnetError("the vocabulary operators have only device kernels: pass CUDA/HIP tensors")
-    for what, t in others.items():
-        if t is not None and t.device != first.device:
-            raise _lib.InvalidArgumentError("%s is on %s where %s is expected" % (what, t.device, first.device))
+    for t in others:
+        if t is not None and t.get_device() != here:
+            raise _lib.InvalidArgumentError("a tensor of shape %s is on %s where %s is expected" % (tuple(t.shape), t.device, first.device))
     return first.device
 
 
@@ -111,12 +109,10 @@ def embed_forward(ids, table, scale=1.0, token_scale=None):
     V, D = t.shape
     i = _ids(ids, "ids")
     s = _per_token(token_scale, "token_scale", ids.shape) if token_scale is not None else None
-    dev = _on_device(t, ids=i, token_scale=s)
-    y = torch.empty(ids.shape + (D,), dtype=t.dtype, device=dev)
-    lib = _lib.load()
-    with _device(dev):
-        _lib.check(lib.gnet_embed_forward(_p(i), int(i.dtype == torch.int64), _p(t), _ld(t), float(scale), _p(s), i.numel(), V, D,
-                                          _TYPES[t.dtype], _p(y), _stream(dev)), "gnet_embed_forward")
+    dev = _on_device(t, i, s)
+    y = t.new_empty(ids.shape + (D,))
+    _call(dev, _lib.load().gnet_embed_forward, _p(i), int(i.dtype == torch.int64), _p(t), _ld(t), float(scale), _p(s), i.numel(), V, D,
+          _TYPES[t.dtype], _p(y))
     return y
 
 
@@ -136,16 +132,15 @@ def embed_backward(ids, dy, table, scale=1.0, token_scale=None, need_dscale=Fals
     if out is not None:
         if tuple(out.shape) != (V, D) or out.dtype != t.dtype or not out.is_contiguous():
             raise _lib.InvalidArgumentError("out must be a contiguous [%d, %d] tensor of type %s" % (V, D, t.dtype))
-    dev = _on_device(t, ids=i, dy=g, token_scale=s, out=out)
-    dtable = out.detach() if out is not None else torch.empty(V, D, dtype=t.dtype, device=dev)
+    dev = _on_device(t, i, g, s, out)
+    dtable = out.detach() if out is not None else t.new_empty(V, D)
     M = i.numel()
     lib = _lib.load()
     dscale = torch.empty(ids.shape, dtype=torch.float32, device=dev) if need_dscale else None
-    with _device(dev):
-        nbytes = lib.gnet_embed_workspace_bytes(M, D)
-        buf, ws = _workspace(nbytes, dev)
-        _lib.check(lib.gnet_embed_backward(_p(i), int(i.dtype == torch.int64), _p(g), _ld(g), float(scale), _p(s), M, V, D, _TYPES[t.dtype],
-                                           _p(dtable), int(out is not None), _p(t), _ld(t), _p(dscale), ws, nbytes, _stream(dev)), "gnet_embed_backward")
+    nbytes = lib.gnet_embed_workspace_bytes(M, D)
+    buf, ws = _workspace(nbytes, dev)
+    _call(dev, lib.gnet_embed_backward, _p(i), int(i.dtype == torch.int64), _p(g), _ld(g), float(scale), _p(s), M, V, D, _TYPES[t.dtype],
+          _p(dtable), int(out is not None), _p(t), _ld(t), _p(dscale), ws, nbytes)
     return (out if out is not None else dtable), dscale
 
 
@@ -179,16 +174,15 @@ def xent_forward(x, w, labels):
     xm, wm = _features(x, w)
     lead = x.shape[:-1]
     i = _ids(labels, "labels", lead)
-    dev = _on_device(wm, x=xm, labels=i)
+    dev = _on_device(wm, xm, i)
     (M, D), V = xm.shape, wm.shape[0]
     loss = torch.empty(lead, dtype=torch.float32, device=dev)
     lse, hit = torch.empty_like(loss), torch.empty_like(loss)
     lib = _lib.load()
-    with _device(dev):
-        nbytes = lib.gnet_vocab_workspace_bytes(_p(wm), _ld(wm), M, V, D, 0, _TYPES[wm.dtype], 0)
-        buf, ws = _workspace(nbytes, dev)
-        _lib.check(lib.gnet_xent_forward(_p(xm), _ld(xm), _p(wm), _ld(wm), _p(i), int(i.dtype == torch.int64), M, V, D, _TYPES[wm.dtype],
-                                         _p(loss), _p(lse), _p(hit), ws, nbytes, _stream(dev)), "gnet_xent_forward")
+    nbytes = lib.gnet_vocab_workspace_bytes(_p(wm), _ld(wm), M, V, D, 0, _TYPES[wm.dtype], 0)
+    buf, ws = _workspace(nbytes, dev)
+    _call(dev, lib.gnet_xent_forward, _p(xm), _ld(xm), _p(wm), _ld(wm), _p(i), int(i.dtype == torch.int64), M, V, D, _TYPES[wm.dtype],
+          _p(loss), _p(lse), _p(hit), ws, nbytes)
     return loss, lse, hit
 
 
@@ -209,18 +203,16 @@ def distill_forward(x, w, top_ids, top_logits, temperature=1.0):
     xm, wm = _features(x, w)
     lead = x.shape[:-1]
     i, t = _teacher(top_ids, top_logits, x, temperature)
-    dev = _on_device(wm, x=xm, top_ids=i, top_logits=t)
+    dev = _on_device(wm, xm, i, t)
     (M, D), V, K = xm.shape, wm.shape[0], i.shape[-1]
     loss = torch.empty(lead, dtype=torch.float32, device=dev)
     lse = torch.empty_like(loss)
     hit = torch.empty(lead + (K,), dtype=torch.float32, device=dev)
     lib = _lib.load()
-    with _device(dev):
-        nbytes = lib.gnet_vocab_workspace_bytes(_p(wm), _ld(wm), M, V, D, K, _TYPES[wm.dtype], 0)
-        buf, ws = _workspace(nbytes, dev)
-        _lib.check(lib.gnet_distill_forward(_p(xm), _ld(xm), _p(wm), _ld(wm), _p(i), int(i.dtype == torch.int64), _p(t), float(temperature),
-                                            M, V, D, K, _TYPES[wm.dtype], _p(loss), _p(lse), _p(hit), ws, nbytes, _stream(dev)),
-                   "gnet_distill_forward")
+    nbytes = lib.gnet_vocab_workspace_bytes(_p(wm), _ld(wm), M, V, D, K, _TYPES[wm.dtype], 0)
+    buf, ws = _workspace(nbytes, dev)
+    _call(dev, lib.gnet_distill_forward, _p(xm), _ld(xm), _p(wm), _ld(wm), _p(i), int(i.dtype == torch.int64), _p(t), float(temperature),
+          M, V, D, K, _TYPES[wm.dtype], _p(loss), _p(lse), _p(hit), ws, nbytes)
     return loss, lse, hit
 
 
@@ -233,22 +225,20 @@ def distill_backward(x, w, top_ids, top_logits, lse, hit, dloss, temperature=1.0
 
 
 def _backward(xm, wm, i, t, temperature, lse, hit, dloss, x_shape, K, need_dx, need_dw):
-    dev = _on_device(wm, x=xm, labels=i, top_logits=t, lse=lse, hit=hit, dloss=dloss)
+    dev = _on_device(wm, xm, i, t, lse, hit, dloss)
     (M, D), V, dt = xm.shape, wm.shape[0], _TYPES[wm.dtype]
-    dx = torch.empty(x_shape, dtype=xm.dtype, device=dev) if need_dx else None
-    dw = torch.empty(V, D, dtype=wm.dtype, device=dev) if need_dw else None
+    dx = xm.new_empty(x_shape) if need_dx else None
+    dw = wm.new_empty(V, D) if need_dw else None
     if not (need_dx or need_dw):
         return dx, dw
     lib = _lib.load()
-    with _device(dev):
-        nbytes = lib.gnet_vocab_workspace_bytes(_p(wm), _ld(wm), M, V, D, K, dt, 1)
-        buf, ws = _workspace(nbytes, dev)
-        ids64 = int(i.dtype == torch.int64)
-        if t is None:
-            _lib.check(lib.gnet_xent_backward(_p(xm), _ld(xm), _p(wm), _ld(wm), _p(i), ids64, _p(lse), _p(hit), _p(dloss), M, V, D, dt,
-                                              _p(dx), _p(dw), ws, nbytes, _stream(dev)), "gnet_xent_backward")
-        else:
-            _lib.check(lib.gnet_distill_backward(_p(xm), _ld(xm), _p(wm), _ld(wm), _p(i), ids64, _p(t), float(temperature), _p(lse), _p(hit),
-                                                 _p(dloss), M, V, D, K, dt, _p(dx), _p(dw), ws, nbytes, _stream(dev)),
-                       "gnet_distill_backward")
+    nbytes = lib.gnet_vocab_workspace_bytes(_p(wm), _ld(wm), M, V, D, K, dt, 1)
+    buf, ws = _workspace(nbytes, dev)
+    ids64 = int(i.dtype == torch.int64)
+    if t is None:
+        _call(dev, lib.gnet_xent_backward, _p(xm), _ld(xm), _p(wm), _ld(wm), _p(i), ids64, _p(lse), _p(hit), _p(dloss), M, V, D, dt,
+              _p(dx), _p(dw), ws, nbytes)
+    else:
+        _call(dev, lib.gnet_distill_backward, _p(xm), _ld(xm), _p(wm), _ld(wm), _p(i), ids64, _p(t), float(temperature), _p(lse), _p(hit),
+              _p(dloss), M, V, D, K, dt, _p(dx), _p(dw), ws, nbytes)
     return dx, dw
