@@ -213,12 +213,11 @@ template <int DT> __device__ __forceinline__ void zero_row(void* out, int64_t fi
   }
 }
 // Rows of W that the matrix products cannot read where they lie (32 bits; widths that are no multiple of 8; alignment).
-struct PackW { const void* w; int64_t ldw, rows, rows_out; u16* dst; RowCopy c; };
-constexpr int PACK_W_ROWS = 16;
+struct PackW { const void* w; int64_t ldw, rows, rows_out; u16* dst; int each; RowCopy c; };      // each: rows of a workgroup, a multiple of 4
 template <int DT> __device__ __forceinline__ void pack_w_rows(const PackW& a, int64_t group, float scale) {
   RowCopy c = a.c;
   c.scale = scale;
-  for (int64_t r = group * PACK_W_ROWS + (threadIdx.x >> 6); r < min(a.rows_out, (group + 1) * PACK_W_ROWS); r += 4)
+  for (int64_t r = group * a.each + (threadIdx.x >> 6); r < min(a.rows_out, (group + 1) * a.each); r += 4)
     copy_row<DT>(a.w, r * a.ldw, r >= a.rows, a.dst + r * c.Dp, c, threadIdx.x & 63, 64);
 }
 template <int DT> __global__ void __launch_bounds__(256) vocab_pack_w(const PackW a, const VocabMeta* meta) {
@@ -471,20 +470,22 @@ template <class T, int PLANES, bool BACKWARD> __global__ void __launch_bounds__(
   const float f = a.t.inv_temp * (a.meta->unscale_x * a.meta->unscale_w);
   auto logit = [&](int64_t v) {                        // of rows v .. v + 3
     f32x4 z = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
     for (int s = 0; s < a.splits; ++s) z += *reinterpret_cast<const f32x4*>(a.slab + s * a.stride + p * a.ld + v);
 #pragma unroll
     for (int i = 0; i < 4; ++i) z[i] = v + i < a.t.V ? z[i] * f : -INFINITY;
     return z;
   };
+  const f32x4 own = threadIdx.x * 4 < a.t.V ? logit(threadIdx.x * 4) : f32x4{0.f, 0.f, 0.f, 0.f};      // the first of the thread's, kept
   float top = -INFINITY, sum = 0.f;
   for (int64_t v = threadIdx.x * 4; v < a.t.V; v += 1024) {
-    const f32x4 z = logit(v);
+    const f32x4 z = v < 1024 ? own : logit(v);
     top = fmaxf(top, fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])));
   }
   top = block_max(top, red);
   if (top == -INFINITY) top = 0.f;
   for (int64_t v = threadIdx.x * 4; v < a.t.V; v += 1024) {
-    const f32x4 z = logit(v);
+    const f32x4 z = v < 1024 ? own : logit(v);
 #pragma unroll
     for (int i = 0; i < 4; ++i) sum += exp2f((z[i] - top) * LOG2E);
   }
@@ -495,7 +496,7 @@ template <class T, int PLANES, bool BACKWARD> __global__ void __launch_bounds__(
     for (int64_t v = threadIdx.x * 4; v < a.ld; v += 1024) {
       u16 hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
       if (v < a.t.V) {
-        const f32x4 z = logit(v);
+        const f32x4 z = v < 1024 ? own : logit(v);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float d = (exp2f((z[i] - top) * LOG2E) * over - (v + i == label ? 1.f : 0.f)) * gs;      // (behind V: exp(-inf) = 0)
@@ -851,6 +852,7 @@ template <int DT, class T, int PLANES> struct Run {
     PackW k = {};
     k.w = (const char*)q.w + v0 * q.ldw * (DT == GNET_F32 ? 4 : 2);
     k.ldw = q.ldw; k.rows = q.t.V - v0; k.rows_out = p.piece; k.dst = (u16*)(ws + p.wp);
+    k.each = p.piece <= 8192 ? 4 : 16;                    // (194 x 3858: 11.5 us, 16 a workgroup 19.8; every one looks at the magnitudes first)
     k.c = RowCopy{q.D, p.Dp, p.piece * p.Dp, 1.f};
     return k;
   }
@@ -883,7 +885,7 @@ template <int DT, class T, int PLANES> struct Run {
     k.lse_c = (float*)(ws + p.lse_c); k.gscale = (float*)(ws + p.gscale);
     k.meta = (VocabMeta*)(ws + p.meta);
     if (dx && p.dx_direct) { k.dx = dx; k.row_of = (int32_t*)(ws + p.row_of); }
-    if (p.pack_w) { k.w = pack_of_w(q, p, ws, 0); k.w_groups = (unsigned)tiles(p.piece, PACK_W_ROWS); }
+    if (p.pack_w) { k.w = pack_of_w(q, p, ws, 0); k.w_groups = (unsigned)tiles(p.piece, k.w.each); }
     unsigned groups = k.token_groups + k.w_groups;
     if (hit && q.t.logits) {
       k.dots = DotArgs{q.x, q.ldx, q.w, q.ldw, q.D, hit, (q.t.K + 3) / 4};
@@ -896,7 +898,8 @@ template <int DT, class T, int PLANES> struct Run {
   static VocabOperand piece_of_w(const Problem& q, const Plan& p, char* ws, int64_t v0, hipStream_t s) {
     VocabOperand o = {};
     if (p.pack_w) {
-      if (v0) vocab_pack_w<DT><<<(unsigned)tiles(p.piece, PACK_W_ROWS), 256, 0, s>>>(pack_of_w(q, p, ws, v0), (const VocabMeta*)(ws + p.meta));
+      const PackW k = pack_of_w(q, p, ws, v0);
+      if (v0) vocab_pack_w<DT><<<(unsigned)tiles(p.piece, k.each), 256, 0, s>>>(k, (const VocabMeta*)(ws + p.meta));
       o.p = (const u16*)(ws + p.wp); o.ld = p.Dp; o.plane = p.piece * p.Dp; o.rows = p.piece;
     } else {
       o.p = (const u16*)q.w + v0 * q.ldw; o.ld = q.ldw; o.plane = 0; o.rows = q.t.V - v0;
