@@ -50,19 +50,10 @@ template <int DT, int NT, bool BACKWARD> __global__ void __launch_bounds__(256) 
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[i][n] = f32x4{0.f, 0.f, 0.f, 0.f};
   auto products = [&](const SmallRaw<DT, N> (&wv)[4], const SmallRaw<DT, N> (&xv)[NT]) {
-    if constexpr (DT == GNET_F32) {
 #pragma unroll
-      for (int c = 0; c < N; ++c)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int n = 0; n < NT; ++n) acc[i][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(wv[i].get(c), xv[n].get(c), acc[i][n], 0, 0, 0);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) acc[i][n] = std::conditional_t<DT == GNET_BF16, Bf16T, F16T>::mma(wv[i].v, xv[n].v, acc[i][n]);
-    }
+      for (int n = 0; n < NT; ++n) small_logits<DT>(acc[i][n], wv[i], xv[n]);
   };
   const int64_t full = a.D / CHUNK;
   int64_t c = wave;

@@ -3,8 +3,8 @@
 //   vocab_small<false>   z = x . W^T of 16 tokens, their softmax, losses
 //   vocab_small<true>    the same z again, dz = g (softmax(z) - weights), dx = dz . W
 //   vocab_small_dw       dW = dz^T . x, a workgroup per 16 x 16 of it
-// Products run on the fp32 matrix pipe (v_mfma_f32_16x16x4_f32) with all operands turned into fp32 on the way from memory: exact for every
-// type.  A contraction's order is free as long as both operands agree: lane group q (16 lanes each) takes elements 4 q .. 4 q + 3 of 16,
+// Products run on the fp32 matrix pipe (v_mfma_f32_16x16x4_f32) with all operands turned into fp32 on the way from memory, exact for every
+// type; 16-bit logits on their own pipe.  A contraction's order is free as long as both operands agree: lane group q (16 lanes each) takes elements 4 q .. 4 q + 3 of 16,
 // one vector load, where the instruction would have it take element q of four.
 // (Included by vocab.hip behind its helpers.)
 //
@@ -58,6 +58,13 @@ template <int DT> __device__ __forceinline__ void small_store(void* p, int64_t i
   if constexpr (DT == GNET_F32) ((float*)p)[i] = v;
   else ((u16*)p)[i] = DT == GNET_BF16 ? Bf16T::enc(v) : F16T::enc(v);
 }
+// 16 rows of W times 16 tokens over one vector of each lane
+template <int DT, int N> __device__ __forceinline__ void small_logits(f32x4& acc, const SmallRaw<DT, N>& w, const SmallRaw<DT, N>& x) {
+  if constexpr (DT == GNET_F32) {
+#pragma unroll
+    for (int c = 0; c < N; ++c) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(w.get(c), x.get(c), acc, 0, 0, 0);
+  } else acc = std::conditional_t<DT == GNET_BF16, Bf16T, F16T>::mma(w.v, x.v, acc);
+}
 __device__ __forceinline__ float half_wave_sum(float v) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor(v, o);
@@ -90,33 +97,29 @@ template <int DT, bool BACKWARD> __global__ void __launch_bounds__(64 * SMALL_WA
   // the logits: rows of the product are the vocabulary, columns the tokens.  Rows and tokens that do not exist repeat the last one, and
   // tokens that are left out are computed like the others: no column looks at another, and theirs are not used.
   {
-    const int64_t m = min(m0 + i16, a.t.M - 1);
-    const int64_t full = a.D / 16 * 16;
+    constexpr int N = DT == GNET_F32 ? 4 : 8, CHUNK = 4 * N;
+    const int64_t m = min(m0 + i16, a.t.M - 1), full = a.D / CHUNK * CHUNK;
     for (int tile = wave; tile < v_tiles; tile += SMALL_WAVES) {
       const int64_t row = (int64_t)min(tile * 16 + i16, V - 1) * a.ldw, x = m * a.ldx;
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-      for (int64_t d0 = 0; d0 < full; d0 += 16 * SMALL_AHEAD) {
-        SmallRaw<DT, 4> wv[SMALL_AHEAD], xv[SMALL_AHEAD];
+      for (int64_t d0 = 0; d0 < full; d0 += CHUNK * SMALL_AHEAD) {
+        SmallRaw<DT, N> wv[SMALL_AHEAD], xv[SMALL_AHEAD];
 #pragma unroll
         for (int u = 0; u < SMALL_AHEAD; ++u) {
-          if (d0 + u * 16 >= full) continue;
-          wv[u].load(a.w, row + d0 + u * 16 + q4 * 4);
-          xv[u].load(a.x, x + d0 + u * 16 + q4 * 4);
+          if (d0 + u * CHUNK >= full) continue;
+          wv[u].load(a.w, row + d0 + u * CHUNK + q4 * N);
+          xv[u].load(a.x, x + d0 + u * CHUNK + q4 * N);
         }
 #pragma unroll
-        for (int u = 0; u < SMALL_AHEAD; ++u) {
-          if (d0 + u * 16 >= full) continue;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(wv[u].get(c), xv[u].get(c), acc, 0, 0, 0);
-        }
+        for (int u = 0; u < SMALL_AHEAD; ++u)
+          if (d0 + u * CHUNK < full) small_logits<DT>(acc, wv[u], xv[u]);
       }
       if (full < a.D) {
-        const int64_t d = full + q4 * 4, left = a.D - d;
-        SmallRaw<DT, 4> wv, xv;
+        const int64_t d = full + q4 * N, left = a.D - d;
+        SmallRaw<DT, N> wv, xv;
         wv.load(a.w, row + d, left);
         xv.load(a.x, x + d, left);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(wv.get(c), xv.get(c), acc, 0, 0, 0);
+        small_logits<DT>(acc, wv, xv);
       }
       *reinterpret_cast<f32x4*>(z + i16 * a.ld_z + tile * 16 + q4 * 4) = acc * a.t.inv_temp;
     }
