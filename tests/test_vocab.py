@@ -126,3 +126,22 @@ def test_workspaces_do_not_grow_with_the_logits():
     assert lib.gnet_vocab_workspace_bytes(p, D, 0, V, D, 0, BF16, 0) == 0
     # a weight matrix that cannot be read where it lies is packed: only then is there room for it
     assert lib.gnet_vocab_workspace_bytes(C.c_void_p((1 << 20) + 2), D, 64, V, D, 0, BF16, 0) > lib.gnet_vocab_workspace_bytes(p, D, 64, V, D, 0, BF16, 0)
+
+
+def test_few_tokens_lay_no_weights_out():
+    """fp32 weights and odd widths are copied for many tokens only; both workspaces are checked."""
+    lib = _lib.load()
+    p = C.c_void_p(1 << 20)
+    V, D = 100000, 2047
+    for dtype, size in ((F32, 4), (BF16, 2)):
+        for backward in (0, 1):
+            few, many = (lib.gnet_vocab_workspace_bytes(p, D, M, V, D, 0, dtype, backward) for M in (32, 33))
+            assert 0 < few < V * D * size // 4 and few < many, (dtype, backward)
+        for M in (32, 33):
+            need = lib.gnet_vocab_workspace_bytes(p, D, M, V, D, 0, dtype, 0)
+            assert lib.gnet_xent_forward(p, D, p, D, p, 1, M, V, D, dtype, p, p, p, p, need - 1, None) == _lib.ERR_WORKSPACE
+            need = lib.gnet_vocab_workspace_bytes(p, D, M, V, D, 5, dtype, 1)
+            assert lib.gnet_distill_backward(p, D, p, D, p, 0, p, 1.0, p, p, p, M, V, D, 5, dtype, p, p, p, need - 1, None) == _lib.ERR_WORKSPACE
+    # (a small vocabulary: what its backward pass keeps fits into what is asked for)
+    for M, V, D in ((1, 1, 1), (8192, 256, 16), (4097, 81, 128)):
+        assert lib.gnet_vocab_workspace_bytes(p, D, M, V, D, 0, F32, 1) >= (M + 15) // 16 * 16 * ((V + 15) // 16 * 16 + 1) * 4
