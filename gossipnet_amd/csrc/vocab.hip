@@ -552,6 +552,7 @@ struct FinishArgs {
   const int32_t* pos;                                // NULL: row r of the slab
   int64_t rows, D; unsigned quads; void* out;                 // quads: groups of four a row
   const VocabMeta* meta; int by_x;
+  SplitFit fit; int64_t out_cols;                    // dx: how often the contraction was split (vocab_gemm)
 };
 template <int DT> __global__ void __launch_bounds__(64) vocab_finish(const FinishArgs a) {
   const float f = a.meta->unscale_g * (a.by_x ? a.meta->unscale_x : a.meta->unscale_w);
@@ -559,10 +560,17 @@ template <int DT> __global__ void __launch_bounds__(64) vocab_finish(const Finis
   const int64_t r = i / a.quads, d = (i - r * a.quads) * 4;
   if (r >= a.rows) return;
   const int64_t p = a.pos ? a.pos[r] : r;
+  int splits = a.splits;
+  int64_t stride = a.stride;
+  if (a.fit.slots) {
+    const Splits f = fit_splits(a.fit, splits, (a.meta->rows + VG_BK - 1) & ~(VG_BK - 1), a.out_cols);
+    splits = f.splits;
+    stride = f.cols * a.ld;
+  }
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
   if (p >= 0) {
 #pragma unroll 8
-    for (int s = 0; s < a.splits; ++s) v += *reinterpret_cast<const f32x4*>(a.slab + s * a.stride + p * a.ld + d);
+    for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const f32x4*>(a.slab + s * stride + p * a.ld + d);
     v *= f;
   }
   const int64_t at = r * a.D + d;
@@ -648,6 +656,7 @@ struct Plan {
   int64_t Mp, Dp, flags_n, piece, pieces, w_tiles;
   int planes, pack_w, direct, dx_direct;
   Product logits, dx, dw;
+  SplitFit dx_fit;
   int64_t flag, q, entropy, row_x, row_g, w_part, meta, pos, label, row_of, hit_c, lse_c, gscale, xp, wp, part, z_slab, dz, dx_slab, dw_slab, bytes;
 };
 
@@ -692,7 +701,16 @@ Plan make_plan(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int distil
     p.dx = pick_product(p.Dp, M, p.piece / VG_BK * segments, true, true);
     p.dx_direct = p.pieces == 1 && p.dx.splits == 1;          // one sum: straight to its rows
     p.row_of = take(p.Mp * 4);
-    if (!p.dx_direct) p.dx_slab = take((int64_t)p.dx.splits * p.Mp * p.Dp * 4);
+    if (!p.dx_direct) {
+      int64_t rows = (int64_t)p.dx.splits * p.Mp;
+      if (p.dx.shape <= S128) {
+        const ShapeInfo t = SHAPE[p.dx.shape];
+        const int64_t steps = p.piece / VG_BK * segments;
+        p.dx_fit = SplitFit{p.dx.shape == S256 ? 256 : 512, (int)std::min<int64_t>(steps / 4, 4 * p.dx.splits), (int)tiles(p.Dp, t.bm), (int)tiles(M, t.bn), t.bn};
+        rows = std::max(rows, (int64_t)(p.dx_fit.slots / p.dx_fit.row_tiles) * t.bn);
+      }
+      p.dx_slab = take(rows * p.Dp * 4);
+    }
     p.dw = pick_product(p.Dp, p.piece, p.Mp / VG_BK * segments, false, true);
     if (p.dw.splits > 1) p.dw_slab = take((int64_t)p.dw.splits * p.piece * p.Dp * 4);
   }
@@ -832,8 +850,9 @@ template <int DT, class T, int PLANES> struct Run {
     const int64_t at_once = vocab_halves<BN, BS>() ? vocab_at_once<BM>() : 1;
     int64_t groups = 0;
     for (int64_t c = g.col_tiles; c > 0; --c) {
-      const int64_t share = tiles((int64_t)g.row_tiles * c * splits, 8);
+      const int64_t share = tiles(std::max((int64_t)g.row_tiles * c * splits, (int64_t)g.fit.slots), 8);
       for (int64_t k = share; k >= 0 && k >= share - 1; --k) groups = std::max(groups, k + (2 * (k % at_once) <= at_once ? k % at_once : 0));
+      if (g.fit.slots) groups = share + at_once / 2;                  // (any share up to this one)
       if (!g.cols_from_meta || share + at_once / 2 <= groups) break;
     }
     vocab_gemm<T, BM, BN, WM, WN, STAGES, AS, BS, EPI, PLANES><<<(unsigned)(8 * groups), 64 * WM * WN, 0, s>>>(g);
@@ -994,7 +1013,7 @@ template <int DT, class T, int PLANES> struct Run {
           d.row_of = (const int32_t*)(ws + p.row_of);
           gemm<true, false, EPI_OUT>(d, p.dx, p.Dp, q.t.M, s);
         } else {
-          d.slab = (float*)(ws + p.dx_slab); d.ld_slab = p.Dp; d.slab_stride = p.Mp * p.Dp; d.accumulate = v0 > 0;
+          d.slab = (float*)(ws + p.dx_slab); d.ld_slab = p.Dp; d.slab_stride = p.Mp * p.Dp; d.accumulate = v0 > 0; d.fit = p.dx_fit;
           gemm<true, false, EPI_SLAB>(d, p.dx, p.Dp, q.t.M, s);
         }
       }
@@ -1018,7 +1037,7 @@ template <int DT, class T, int PLANES> struct Run {
     }
     if (dx && !p.dx_direct) {
       FinishArgs f = {};
-      f.slab = (const float*)(ws + p.dx_slab); f.ld = p.Dp; f.stride = p.Mp * p.Dp; f.splits = p.dx.splits;
+      f.slab = (const float*)(ws + p.dx_slab); f.ld = p.Dp; f.stride = p.Mp * p.Dp; f.splits = p.dx.splits; f.fit = p.dx_fit; f.out_cols = p.Mp;
       f.pos = (const int32_t*)(ws + p.pos); f.rows = q.t.M; f.out = dx; f.meta = meta;
       finish(f, q, s);
     }

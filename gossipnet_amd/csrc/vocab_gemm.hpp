@@ -63,12 +63,29 @@ struct VocabOperand {
   int cols;            // elements of a row that may be read (a multiple of 8): a chunk beyond is replaced by the last (zeros of the other operand)
 };
 
+// A split contraction over columns that are tokens: the host plans for all tokens, the device knows how many count.  With fewer column tiles
+// the contraction is split further, up to `most` ways, so that `slots` workgroups have work: dx of 833 of 1111 tokens x 50257 x 1024 113 us as
+// planned and 99 us so, the sums behind it 7 and 9.
+struct SplitFit { int slots, most, row_tiles, col_tiles, bn; };       // slots = 0: as planned
+struct Splits { int splits, col_tiles; int64_t cols; };                // cols: columns of one split's partial sums
+__host__ __device__ inline Splits fit_splits(const SplitFit& f, int planned, int64_t columns, int64_t out_cols) {
+  Splits s;
+  s.col_tiles = (int)((columns + f.bn - 1) / f.bn);
+  if (s.col_tiles > f.col_tiles) s.col_tiles = f.col_tiles;
+  s.cols = (int64_t)s.col_tiles * f.bn < out_cols ? (int64_t)s.col_tiles * f.bn : out_cols;
+  const int fit = s.col_tiles ? f.slots / (f.row_tiles * s.col_tiles) : planned;
+  s.splits = fit > f.most ? f.most : fit;
+  if (s.splits < planned) s.splits = planned;
+  return s;
+}
+
 struct VocabGemm {
   VocabOperand a, b;
   int64_t k;                   // contraction length, a multiple of VG_BK (k_from_meta: meta->rows rounded up)
   int k_from_meta;
   int cols_from_meta;          // columns are tokens: column tiles behind meta->rows are left out
   int row_tiles, col_tiles, splits;
+  SplitFit fit;
   const VocabMeta* meta;
   // logits
   float inv_temp;
@@ -238,13 +255,13 @@ __device__ __forceinline__ bool tile_of(int id, int row_tiles, int col_tiles, in
 // read from LDS into the other set of registers, and while the following stages are on their way from memory.  One barrier a stage, in its
 // middle: behind it the next stage is there for every wave, and nobody reads this stage any more, whose place is loaded next.
 template <class T, int BM, int BN, int WM, int WN, int STAGES, bool A_STRIDED, bool B_STRIDED, int EPI, int PLANES>
-__device__ __forceinline__ void vocab_tile(const VocabGemm& g, char* const lds, const int rows, const int rt, const int64_t c0, const int split) {
+__device__ __forceinline__ void vocab_tile(const VocabGemm& g, char* const lds, const int rows, const int rt, const int64_t c0, const int split, const int splits, const int64_t slab_stride) {
   constexpr int WAVES = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16, STAGE = (BM + BN) * VG_BK * 2;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
   const int64_t r0 = (int64_t)rt * BM;
   const int64_t k_all = g.k_from_meta ? (int64_t)((rows + VG_BK - 1) / VG_BK) * VG_BK : g.k;
-  const int64_t steps = k_all / VG_BK, k0 = steps * split / g.splits * VG_BK, k1 = steps * (split + 1) / g.splits * VG_BK;
+  const int64_t steps = k_all / VG_BK, k0 = steps * split / splits * VG_BK, k1 = steps * (split + 1) / splits * VG_BK;
   const int per_segment = (int)((k1 - k0) / VG_BK), n = per_segment * (PLANES == 1 ? 1 : 3);
 
   f32x4 acc[FM][FN];
@@ -464,7 +481,7 @@ __device__ __forceinline__ void vocab_tile(const VocabGemm& g, char* const lds, 
         for (int p = 0; p < PLANES; ++p)
           *reinterpret_cast<s16x8*>(g.dz + p * g.plane_dz + (BN + n / (BM / 8)) * g.ld_dz + r0 + n % (BM / 8) * 8) = s16x8{0, 0, 0, 0, 0, 0, 0, 0};
   } else if constexpr (EPI == EPI_SLAB) {
-    float* slab = g.slab + split * g.slab_stride;
+    float* slab = g.slab + split * slab_stride;
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
       const int64_t c = c0 + (wn * FN + j) * 16 + col16;
@@ -520,15 +537,23 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) vocab_gemm(const VocabGemm g)
   __shared__ __attribute__((aligned(16))) char lds[STAGES * (BM + BN) * VG_BK * 2];
   const int rows = g.meta->rows;
   // (the last step of a contraction over tokens reads dz up to the next multiple of its length)
-  const int most = (rows + VG_BK - 1) & ~(VG_BK - 1), col_tiles = g.cols_from_meta ? min(g.col_tiles, (most + BN - 1) / BN) : g.col_tiles;
+  const int most = (rows + VG_BK - 1) & ~(VG_BK - 1);
+  const int col_tiles = g.cols_from_meta ? min(g.col_tiles, (most + BN - 1) / BN) : g.col_tiles;
+  int splits = g.splits;
+  int64_t slab_stride = g.slab_stride;
+  if (EPI == EPI_SLAB && g.fit.slots) {
+    const Splits f = fit_splits(g.fit, splits, most, g.out_cols);
+    splits = f.splits;
+    slab_stride = f.cols * g.ld_slab;
+  }
   constexpr bool HALVES = vocab_halves<BN, B_STRIDED>();
   int rt, ct, split, half;
-  if (!tile_of(blockIdx.x, g.row_tiles, col_tiles, g.splits, HALVES ? vocab_at_once<BM>() : 1, rt, ct, split, half)) return;
+  if (!tile_of(blockIdx.x, g.row_tiles, col_tiles, splits, HALVES ? vocab_at_once<BM>() : 1, rt, ct, split, half)) return;
   if constexpr (HALVES)
     if (half >= 0) {
       const int64_t c0 = (int64_t)ct * BN + half * (BN / 2);
       if (g.cols_from_meta && c0 >= most) return;
-      return vocab_tile<T, BM, BN / 2, 4, WM * WN / 4, STAGES, A_STRIDED, B_STRIDED, EPI, PLANES>(g, lds, rows, rt, c0, split);
+      return vocab_tile<T, BM, BN / 2, 4, WM * WN / 4, STAGES, A_STRIDED, B_STRIDED, EPI, PLANES>(g, lds, rows, rt, c0, split, splits, slab_stride);
     }
-  vocab_tile<T, BM, BN, WM, WN, STAGES, A_STRIDED, B_STRIDED, EPI, PLANES>(g, lds, rows, rt, (int64_t)ct * BN, split);
+  vocab_tile<T, BM, BN, WM, WN, STAGES, A_STRIDED, B_STRIDED, EPI, PLANES>(g, lds, rows, rt, (int64_t)ct * BN, split, splits, slab_stride);
 }
