@@ -520,7 +520,7 @@ extern "C" int gnet_embed_forward(const void* ids, int32_t ids64, const void* ta
 }
 
 extern "C" size_t gnet_embed_workspace_bytes(int64_t M, int64_t D) {
-  if (M <= 0 || D <= 0 || M > (1 << 24) || D > (1 << 16)) return 0;
+  if (M <= WAVE || D <= 0 || M > (1 << 24) || D > (1 << 16)) return 0;
   return 2 * keys_bytes(M) + (size_t)((M + HOT - 1) / HOT) * 2 * ((D + 7) & ~7ll) * 4;
 }
 
@@ -530,7 +530,7 @@ extern "C" int gnet_embed_backward(const void* ids, int32_t ids64, const void* d
   clear_hip_error();
   if (const int e = check(M, V, D, ld_dy, dtype)) return e;
   if (!dtable || (M && (!ids || !dy)) || (dscale && M && (!table || ld_table < D))) return GNET_ERR_INVALID;
-  if (M && (!workspace || workspace_bytes < gnet_embed_workspace_bytes(M, D) || ((uintptr_t)workspace & 255))) return GNET_ERR_WORKSPACE;
+  if (M > WAVE && (!workspace || workspace_bytes < gnet_embed_workspace_bytes(M, D) || ((uintptr_t)workspace & 255))) return GNET_ERR_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
   u64* keys = (u64*)workspace;
   u64* other = (u64*)((char*)workspace + keys_bytes(M));

@@ -715,7 +715,6 @@ Plan make_plan(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int distil
     if (p.dw.splits > 1) p.dw_slab = take((int64_t)p.dw.splits * p.piece * p.Dp * 4);
   }
   p.bytes = o;
-  if (backward && small(M, V, D, K, dtype) && (size_t)p.bytes < small_bytes(M, V)) p.bytes = (int64_t)small_bytes(M, V);
   return p;
 }
 
@@ -1061,13 +1060,13 @@ int run_forward(const Problem& q, float* loss, float* lse, float* hit, void* ws,
     case GNET_BF16: return Few<GNET_BF16>::forward(q, ws, ws_bytes, loss, lse, hit, s);
     default: return Few<GNET_F16>::forward(q, ws, ws_bytes, loss, lse, hit, s);
   }
-  const Plan p = make_plan(q.t.M, q.t.V, q.D, q.t.K, q.dtype, q.t.logits != nullptr, pack_w, 0);
-  if (!ws || ws_bytes < (size_t)p.bytes || ((uintptr_t)ws & 255)) return GNET_ERR_WORKSPACE;
   if (small(q.t.M, q.t.V, q.D, q.t.K, q.dtype)) switch (q.dtype) {
     case GNET_F32: return Small<GNET_F32>::forward(q, loss, lse, hit, s);
     case GNET_BF16: return Small<GNET_BF16>::forward(q, loss, lse, hit, s);
     default: return Small<GNET_F16>::forward(q, loss, lse, hit, s);
   }
+  const Plan p = make_plan(q.t.M, q.t.V, q.D, q.t.K, q.dtype, q.t.logits != nullptr, pack_w, 0);
+  if (!ws || ws_bytes < (size_t)p.bytes || ((uintptr_t)ws & 255)) return GNET_ERR_WORKSPACE;
   switch (q.dtype) {
     case GNET_F32: return Run<GNET_F32, F16T, 2>::forward(q, p, (char*)ws, loss, lse, hit, s);
     case GNET_BF16: return Run<GNET_BF16, Bf16T, 1>::forward(q, p, (char*)ws, loss, lse, hit, s);
@@ -1092,13 +1091,16 @@ int run_backward(const Problem& q, const float* lse, const float* hit, const flo
     case GNET_BF16: return Few<GNET_BF16>::backward(q, ws, ws_bytes, lse, hit, dloss, dx, dw, s);
     default: return Few<GNET_F16>::backward(q, ws, ws_bytes, lse, hit, dloss, dx, dw, s);
   }
+  if (small(q.t.M, q.t.V, q.D, q.t.K, q.dtype)) {
+    if (!ws || ws_bytes < small_bytes(q.t.M, q.t.V) || ((uintptr_t)ws & 255)) return GNET_ERR_WORKSPACE;
+    switch (q.dtype) {
+      case GNET_F32: return Small<GNET_F32>::backward(q, (char*)ws, dloss, dx, dw, s);
+      case GNET_BF16: return Small<GNET_BF16>::backward(q, (char*)ws, dloss, dx, dw, s);
+      default: return Small<GNET_F16>::backward(q, (char*)ws, dloss, dx, dw, s);
+    }
+  }
   const Plan p = make_plan(q.t.M, q.t.V, q.D, q.t.K, q.dtype, q.t.logits != nullptr, pack_w, 1);
   if (!ws || ws_bytes < (size_t)p.bytes || ((uintptr_t)ws & 255)) return GNET_ERR_WORKSPACE;
-  if (small(q.t.M, q.t.V, q.D, q.t.K, q.dtype)) switch (q.dtype) {
-    case GNET_F32: return Small<GNET_F32>::backward(q, (char*)ws, dloss, dx, dw, s);
-    case GNET_BF16: return Small<GNET_BF16>::backward(q, (char*)ws, dloss, dx, dw, s);
-    default: return Small<GNET_F16>::backward(q, (char*)ws, dloss, dx, dw, s);
-  }
   switch (q.dtype) {
     case GNET_F32: return Run<GNET_F32, F16T, 2>::backward(q, p, (char*)ws, lse, hit, dloss, dx, dw, s);
     case GNET_BF16: return Run<GNET_BF16, Bf16T, 1>::backward(q, p, (char*)ws, lse, hit, dloss, dx, dw, s);
@@ -1122,6 +1124,7 @@ extern "C" size_t gnet_vocab_workspace_bytes(const void* w, int64_t ldw, int64_t
   if (M <= 0 || V < 1 || D < 1 || K < 0 || M > (1 << 24) || V > (1ll << 30) || D > (1 << 16) || K > 1024) return 0;
   const int pack_w = needs_pack(w, ldw, D, dtype);
   // K = 0: cross entropy
+  if (small(M, V, D, K, dtype)) return backward ? small_bytes(M, V) : 0;
   if (few_tokens(M, V, D, K, dtype, pack_w)) return (size_t)few_plan(M, V, D, K, K > 0, backward).bytes;
   return (size_t)make_plan(M, V, D, K, dtype, K > 0, pack_w, backward).bytes;
 }

@@ -95,6 +95,8 @@ def _per_token(t, what, shape):
 def _workspace(nbytes, device):
     """256-byte aligned scratch of this call.  From the caching allocator: ordered on the current stream, and part of the graph's own
     memory while one is captured, so that no two calls in flight share it."""
+    if not nbytes:
+        return None, None
     buf = torch.empty(nbytes + 256, dtype=torch.uint8, device=device)
     return buf, (buf.data_ptr() + 255) // 256 * 256
 

@@ -91,10 +91,12 @@ def test_c_entries_refuse_before_they_launch():
         assert xent(**a) == _lib.ERR_INVALID, a
     for a in (dict(M=(1 << 24) + 1), dict(V=(1 << 30) + 1), dict(D=(1 << 16) + 1, ldx=1 << 17, ldw=1 << 17), dict(M=1 << 24, V=1 << 21)):
         assert xent(**a) == _lib.ERR_UNSUPPORTED, a
-    need = lib.gnet_vocab_workspace_bytes(p, 8, 4, 10, 8, 0, F32, 0)
-    assert need > 0
-    for a in (dict(ws=None), dict(n=need - 1), dict(ws=odd)):
-        assert xent(**a) == _lib.ERR_WORKSPACE, a
+    assert lib.gnet_vocab_workspace_bytes(p, 8, 4, 10, 8, 0, F32, 0) == 0           # (a small vocabulary's forward pass keeps nothing)
+    for M, V in ((4, 3000), (100, 3000), (9000, 10)):
+        need = lib.gnet_vocab_workspace_bytes(p, 8, M, V, 8, 0, F32, 0)
+        assert need > 0
+        for a in (dict(ws=None), dict(n=need - 1), dict(ws=odd)):
+            assert xent(M=M, V=V, **a) == _lib.ERR_WORKSPACE, a
     assert xent_back(lse=None) == xent_back(g=None) == _lib.ERR_INVALID
     assert xent_back(n=16) == _lib.ERR_WORKSPACE
     assert xent(M=0, x=None, y=None, loss=None, ws=None, n=0) == _lib.OK
@@ -109,8 +111,9 @@ def test_c_entries_refuse_before_they_launch():
         return lib.gnet_embed_backward(ids, 0, p, ld, 1.0, None, M, V, D, dtype, out, 0, table, ld_table, dscale, ws, n, None)
     for a in (dict(M=-1), dict(V=0), dict(D=0), dict(ld=7), dict(dtype=-1), dict(ids=None), dict(out=None), dict(table=None), dict(ld_table=7)):
         assert embed(**a) == _lib.ERR_INVALID, a
+    assert lib.gnet_embed_workspace_bytes(64, 8) == 0 < lib.gnet_embed_workspace_bytes(65, 8)
     for a in (dict(ws=None), dict(n=8), dict(ws=odd)):
-        assert embed(**a) == _lib.ERR_WORKSPACE, a
+        assert embed(M=65, V=3000, **a) == _lib.ERR_WORKSPACE and embed(M=65, **a) == _lib.ERR_WORKSPACE, a
     assert lib.gnet_embed_forward(p, 0, p, 7, 1.0, None, 4, 10, 8, BF16, p, None) == _lib.ERR_INVALID
     assert lib.gnet_embed_forward(None, 0, p, 8, 1.0, None, 4, 10, 8, BF16, p, None) == _lib.ERR_INVALID
     assert lib.gnet_embed_forward(None, 0, None, 8, 1.0, None, 0, 10, 8, BF16, None, None) == _lib.OK
