@@ -67,7 +67,7 @@ struct ForwardArgs {
 };
 template <int DT, int VEC> __global__ void __launch_bounds__(256) embed_rows_out(const ForwardArgs a) {
   typedef typename Elem<DT>::type E;
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t w = group_id() * 4 + (threadIdx.x >> 6);
   const int64_t m = w / a.blocks, d = ((w % a.blocks) * 64 + (threadIdx.x & 63)) * VEC;
   if (m >= a.M || d >= a.D) return;
   const int64_t id = load_id(a.ids, m, a.ids64);
@@ -186,7 +186,7 @@ struct BackwardArgs {
   const void* dy; int64_t ld; float scale; const float* token_scale;
   void* out; int64_t ld_out; int accumulate;
   float* part; int64_t ld_part;        // [segment][2][D rounded up to 8]
-  unsigned hot_groups, run_groups, scale_groups;     // workgroups of each kind, in this order; the zero rows get the rest
+  unsigned hot_groups, run_groups, scale_groups, fill_groups;     // workgroups of each kind, in this order
   const void* ids; int ids64; const void* table; int64_t ld_table; float* dscale;
 };
 
@@ -324,14 +324,15 @@ template <int DT, int VEC> __device__ __forceinline__ void scale_gradient(const 
 
 template <int DT, int VEC> __global__ void __launch_bounds__(256) embed_sums(const BackwardArgs a) {
   __shared__ int64_t start[FILL_ROWS + 1];
-  unsigned g = blockIdx.x;
+  int64_t g = group_id();
   const int wave = threadIdx.x >> 6;
   if (g < a.hot_groups) return hot_sums<DT, VEC>(a, g);
   g -= a.hot_groups;
-  if (g < a.run_groups) return run_sums<DT, VEC>(a, (int64_t)g * 4 + wave);
+  if (g < a.run_groups) return run_sums<DT, VEC>(a, g * 4 + wave);
   g -= a.run_groups;
-  if (g < a.scale_groups) return scale_gradient<DT, VEC>(a, (int64_t)g * 4 + wave);
-  fill_rows<DT, VEC>(a, g - a.scale_groups, start);
+  if (g < a.scale_groups) return scale_gradient<DT, VEC>(a, g * 4 + wave);
+  g -= a.scale_groups;
+  if (g < a.fill_groups) fill_rows<DT, VEC>(a, g, start);
 }
 
 // The segment in which a hot run starts adds the run's partial sums, a workgroup per column block: each wave a quarter of them in order,
@@ -439,13 +440,13 @@ template <int DT, int VEC> __global__ void __launch_bounds__(256) embed_wave(con
   typedef typename Elem<DT>::type E;
   __shared__ int have[FILL_ROWS];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  unsigned g = blockIdx.x;
-  if (g >= a.run_groups && g - a.run_groups < a.scale_groups) return scale_gradient<DT, VEC>(a, (int64_t)(g - a.run_groups) * 4 + wave);
+  const int64_t g = group_id();
+  if (g >= a.run_groups && g - a.run_groups < a.scale_groups) return scale_gradient<DT, VEC>(a, (g - a.run_groups) * 4 + wave);
   int64_t id = -1;
   if (lane < a.M) id = load_id(a.ids, lane, a.ids64);
   if (id < 0 || id >= a.V) id = -1;
   if (g < a.run_groups) {
-    const int64_t blocks = (a.D + 64 * VEC - 1) / (64 * VEC), w = (int64_t)g * 4 + wave, m = w / blocks, d = (w % blocks * 64 + lane) * VEC;
+    const int64_t blocks = (a.D + 64 * VEC - 1) / (64 * VEC), w = g * 4 + wave, m = w / blocks, d = (w % blocks * 64 + lane) * VEC;
     if (m >= a.M) return;
     const int64_t row = __shfl(id, (int)m);
     const u64 mine = __ballot(id == row);
@@ -458,7 +459,8 @@ template <int DT, int VEC> __global__ void __launch_bounds__(256) embed_wave(con
     if (d < a.D) store_row<DT, VEC>(sum[0], a, row, d);
     return;
   }
-  const int64_t v0 = (int64_t)(g - a.run_groups - a.scale_groups) * FILL_ROWS;
+  const int64_t v0 = (g - a.run_groups - a.scale_groups) * FILL_ROWS;
+  if (v0 >= (int64_t)a.fill_groups * FILL_ROWS) return;
   if (threadIdx.x < FILL_ROWS) have[threadIdx.x] = 0;
   __syncthreads();
   if (wave == 0 && id >= v0 && id < v0 + FILL_ROWS) have[id - v0] = 1;
@@ -499,7 +501,7 @@ KERNEL_OF(GoFew, embed_few, BackwardArgs, 64 * FEW_WAVES);
 int check(int64_t M, int64_t V, int64_t D, int64_t ld, int dtype) {
   if (dtype != GNET_F32 && dtype != GNET_BF16 && dtype != GNET_F16) return GNET_ERR_INVALID;
   if (M < 0 || V < 1 || D < 1 || ld < D) return GNET_ERR_INVALID;
-  if (M > (1 << 24) || V > (1ll << 30) || D > (1 << 16)) return GNET_ERR_UNSUPPORTED;
+  if (M > (1 << 24) || V > (1ll << 30) || D > (1 << 16) || M * D > (1ll << 38) || V * D > (1ll << 38)) return GNET_ERR_UNSUPPORTED;
   return GNET_OK;
 }
 size_t keys_bytes(int64_t M) { return ((size_t)M * 8 + 255) & ~(size_t)255; }
@@ -515,7 +517,7 @@ extern "C" int gnet_embed_forward(const void* ids, int32_t ids64, const void* ta
   ForwardArgs a{ids, ids64, M, V, D, table, ld_table, scale, token_scale, y, 1};
   const int vec = pick_vec(dtype, D);
   a.blocks = (int)((D + 64 * vec - 1) / (64 * vec));
-  launch<GoForward>(dtype, vec, a, (unsigned)((M * a.blocks + 3) / 4), (hipStream_t)stream);
+  launch<GoForward>(dtype, vec, a, grid_of((M * a.blocks + 3) / 4), (hipStream_t)stream);
   return launch_status();
 }
 
@@ -535,7 +537,7 @@ extern "C" int gnet_embed_backward(const void* ids, int32_t ids64, const void* d
   u64* keys = (u64*)workspace;
   u64* other = (u64*)((char*)workspace + keys_bytes(M));
   float* part = (float*)((char*)workspace + 2 * keys_bytes(M));
-  BackwardArgs a{keys, M, V, D, dy, ld_dy, scale, token_scale, dtable, D, accumulate, part, (D + 7) & ~7ll, 0, 0, 0, ids, ids64, table, ld_table, dscale};
+  BackwardArgs a{keys, M, V, D, dy, ld_dy, scale, token_scale, dtable, D, accumulate, part, (D + 7) & ~7ll, 0, 0, 0, 0, ids, ids64, table, ld_table, dscale};
   const int vec = pick_vec(dtype, D);
   const unsigned column_blocks = (unsigned)((D + 64 * vec - 1) / (64 * vec));
   if (M && few(M, V, column_blocks)) {
@@ -543,11 +545,11 @@ extern "C" int gnet_embed_backward(const void* ids, int32_t ids64, const void* d
     launch<GoFew>(dtype, vec, a, dim3(a.scale_groups + (unsigned)V, column_blocks), s);
     return launch_status();
   }
-  const unsigned fill_groups = accumulate ? 0 : (unsigned)((V + FILL_ROWS - 1) / FILL_ROWS);
+  a.fill_groups = accumulate ? 0 : (unsigned)((V + FILL_ROWS - 1) / FILL_ROWS);
   if (M && M <= WAVE) {
     a.run_groups = (unsigned)((M * column_blocks + 3) / 4);
     a.scale_groups = dscale ? (unsigned)((M + 3) / 4) : 0;
-    launch<GoWave>(dtype, vec, a, a.run_groups + a.scale_groups + fill_groups, s);
+    launch<GoWave>(dtype, vec, a, grid_of((int64_t)a.run_groups + a.scale_groups + a.fill_groups), s);
     return launch_status();
   }
   if (M) {
@@ -556,8 +558,10 @@ extern "C" int gnet_embed_backward(const void* ids, int32_t ids64, const void* d
     const unsigned runs = (unsigned)((M + RUN - 1) / RUN);
     if (V < (1 << 20) - 1) embed_sort<unsigned><<<runs, n / 4, 0, s>>>(ids, ids64, M, V, n, keys);
     else embed_sort<u64><<<runs, n / 4, 0, s>>>(ids, ids64, M, V, n, keys);
+    if (const int e = launch_status()) return e;      // (nothing runs on keys that are not there)
     for (int64_t run = RUN; run < M; run *= WAY) {
       embed_merge<<<(unsigned)((M + 256 / WAY - 1) / (256 / WAY)), 256, 0, s>>>(keys, other, M, run);
+      if (const int e = launch_status()) return e;
       u64* t = keys; keys = other; other = t;
     }
   }
@@ -566,8 +570,9 @@ extern "C" int gnet_embed_backward(const void* ids, int32_t ids64, const void* d
   a.hot_groups = M > HOT ? segments : 0;
   a.run_groups = (unsigned)((M + 3) / 4);
   a.scale_groups = dscale ? a.run_groups : 0;
-  const unsigned groups = a.hot_groups + a.run_groups + a.scale_groups + fill_groups;
-  if (groups) launch<GoSums>(dtype, vec, a, groups, s);
+  const int64_t groups = (int64_t)a.hot_groups + a.run_groups + a.scale_groups + a.fill_groups;
+  if (groups) launch<GoSums>(dtype, vec, a, grid_of(groups), s);
+  if (const int e = launch_status()) return e;
   if (M > HOT) launch<GoHotRows>(dtype, vec, a, dim3(segments, column_blocks), s);
   return launch_status();
 }

@@ -309,9 +309,13 @@ template <int DT> __global__ void __launch_bounds__(256) vocab_pack(const PackAr
   __shared__ float fred[3][4];
   __shared__ int place[256];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (blockIdx.x >= a.token_groups + a.w_groups) return target_dots<DT>(a.t, a.dots, (int64_t)(blockIdx.x - a.token_groups - a.w_groups) * 4 + (threadIdx.x >> 6));
-  const bool packs_w = blockIdx.x >= a.token_groups;
-  const int64_t r0 = (int64_t)blockIdx.x * a.rows, M = a.t.M;
+  const int64_t group = group_id();
+  if (group >= a.token_groups + a.w_groups) {
+    if (a.dots.hit) target_dots<DT>(a.t, a.dots, (group - a.token_groups - a.w_groups) * 4 + (threadIdx.x >> 6));
+    return;
+  }
+  const bool packs_w = group >= a.token_groups;
+  const int64_t r0 = group * a.rows, M = a.t.M;
   auto counts = [&](int64_t i) { int64_t id; return a.flag ? a.flag[i] != 0 : target_counts(a.t, i, id); };
   // all that is looked through first, then one exchange between the waves
   int before = 0, all = 0;
@@ -351,12 +355,12 @@ template <int DT> __global__ void __launch_bounds__(256) vocab_pack(const PackAr
   before = all = 0;
   for (int w = 0; w < 4; ++w) { before += ired[0][w]; all += ired[1][w]; mw = fmaxf(mw, fred[0][w]); mx = fmaxf(mx, fred[1][w]); mg = fmaxf(mg, fred[2][w]); }
   const int ew = DT == GNET_F32 ? scale_exponent(mw, 13) : 0;
-  if (packs_w) { pack_w_rows<DT>(a.w, blockIdx.x - a.token_groups, ldexpf(1.f, ew)); return; }
+  if (packs_w) { pack_w_rows<DT>(a.w, group - a.token_groups, ldexpf(1.f, ew)); return; }
   const int ex = DT == GNET_F32 ? scale_exponent(mx, 13) : 0;
   // dz is stored in units of the largest |dloss|, not of a power of two: with one dloss for all tokens what is rounded to 16 bits is
   // softmax - target itself, and the -1 of a label and the rest of its row are not off by different shares (top_g: 2^15 for fp16)
   const float unit_g = mg >= 1.17549435e-38f && mg < INFINITY ? mg : 1.f;
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
+  if (group == 0 && threadIdx.x == 0) {
     a.meta->rows = all;
     a.meta->unscale_x = ldexpf(1.f, -ex);
     a.meta->unscale_w = ldexpf(1.f, -ew);
@@ -534,7 +538,7 @@ struct HitsArgs {
   u16* dz; int64_t ld_dz, plane; int64_t v0, v1;
 };
 template <class T, int PLANES> __global__ void __launch_bounds__(256) vocab_hits(const HitsArgs a) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t i = group_id() * 256 + threadIdx.x;
   if (i >= a.t.M * a.t.K) return;
   const int64_t m = i / a.t.K;
   int64_t id;
@@ -556,7 +560,7 @@ struct FinishArgs {
 };
 template <int DT> __global__ void __launch_bounds__(64) vocab_finish(const FinishArgs a) {
   const float f = a.meta->unscale_g * (a.by_x ? a.meta->unscale_x : a.meta->unscale_w);
-  const int64_t i = (int64_t)blockIdx.x * 64 + threadIdx.x;
+  const int64_t i = group_id() * 64 + threadIdx.x;
   const int64_t r = i / a.quads, d = (i - r * a.quads) * 4;
   if (r >= a.rows) return;
   const int64_t p = a.pos ? a.pos[r] : r;
@@ -652,9 +656,14 @@ bool small(int64_t M, int64_t V, int64_t D, int64_t K, int dtype) {
 }
 size_t small_bytes(int64_t M, int64_t V) { return (size_t)up(M, 16) * (up(V, 16) + 1) * 4; }
 
+// Whether a product's workgroups make one launch (half tiles add 16 or 32 to each XCD's)
+bool launchable(const Product& p, int64_t rows, int64_t cols) {
+  return (tiles(rows, SHAPE[p.shape].bm) * tiles(cols, SHAPE[p.shape].bn) * p.splits + 512) * (p.shape == S256 ? 512 : 256) < 1ll << 32;
+}
+
 struct Plan {
   int64_t Mp, Dp, flags_n, piece, pieces, w_tiles;
-  int planes, pack_w, direct, dx_direct;
+  int planes, pack_w, direct, dx_direct, launchable;
   Product logits, dx, dw;
   SplitFit dx_fit;
   int64_t flag, q, entropy, row_x, row_g, w_part, meta, pos, label, row_of, hit_c, lse_c, gscale, xp, wp, part, z_slab, dz, dx_slab, dw_slab, bytes;
@@ -674,6 +683,8 @@ Plan make_plan(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int distil
   const int64_t Vp = up(V, 256);
   int64_t piece = per_row ? (256ll << 20) / per_row / 256 * 256 : Vp;
   if (piece < 2048) piece = 2048;
+  // and at most 2^20 tiles of logits (2^29 threads): a launch has to have fewer than 2^32
+  piece = std::min(piece, std::max<int64_t>((1 << 20) / tiles(M, 256), 1) * 256);
   p.pieces = tiles(Vp, piece);
   p.piece = up(tiles(Vp, p.pieces), 256);
   p.pieces = tiles(Vp, p.piece);
@@ -681,6 +692,7 @@ Plan make_plan(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int distil
   if (V <= SHAPE[S128].bm && p.logits.shape == S256) p.logits.shape = S128;          // (a vocabulary of one tile: EPI_DZ_ONE)
   if (p.pieces == 1) p.logits.splits = logits_splits(p.logits.shape, V, M, p.Dp / VG_BK * segments, (int64_t)p.Mp * p.piece * 4);
   p.w_tiles = tiles(V, SHAPE[p.logits.shape].bm);
+  p.launchable = launchable(p.logits, p.piece, M);
   int64_t o = 0;
   auto take = [&](int64_t bytes) { const int64_t at = o; o = up(o + bytes, 256); return at; };
   p.meta = take(sizeof(VocabMeta));
@@ -712,6 +724,7 @@ Plan make_plan(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int distil
       p.dx_slab = take(rows * p.Dp * 4);
     }
     p.dw = pick_product(p.Dp, p.piece, p.Mp / VG_BK * segments, false, true);
+    p.launchable &= launchable(p.dx, p.Dp, M) & launchable(p.dw, p.Dp, p.piece);
     if (p.dw.splits > 1) p.dw_slab = take((int64_t)p.dw.splits * p.piece * p.Dp * 4);
   }
   p.bytes = o;
@@ -755,6 +768,7 @@ int check(const Problem& q) {
   if (q.dtype != GNET_F32 && q.dtype != GNET_BF16 && q.dtype != GNET_F16) return GNET_ERR_INVALID;
   if (q.t.M < 0 || q.t.V < 1 || q.D < 1 || q.t.K < 1 || q.ldx < q.D || q.ldw < q.D) return GNET_ERR_INVALID;
   if (q.t.M > (1 << 24) || q.t.V > (1ll << 30) || q.t.M * q.t.V > (1ll << 44) || q.D > (1 << 16) || q.t.K > 1024) return GNET_ERR_UNSUPPORTED;
+  if (q.t.M * q.D > (1ll << 38) || q.t.V * q.D > (1ll << 38)) return GNET_ERR_UNSUPPORTED;
   if (!(q.t.inv_temp > 0.f) || !(q.t.inv_temp < INFINITY)) return GNET_ERR_INVALID;
   if (!q.w || (q.t.M && (!q.x || !q.t.ids))) return GNET_ERR_INVALID;
   return GNET_OK;
@@ -779,6 +793,7 @@ template <int DT> struct Small {
     a.dloss = dloss; a.dx = dx;
     a.dz = (float*)ws; a.ld_dz = up(q.t.V, 16); a.alive = (int*)(a.dz + up(q.t.M, 16) * a.ld_dz);
     vocab_small<DT, true><<<(unsigned)tiles(q.t.M, SMALL_TOKENS), 64 * SMALL_WAVES, SMALL_TOKENS * a.ld_z * 4, s>>>(a);
+    if (const int e = launch_status()) return e;
     if (dw) {
       const SmallDwArgs d{q.x, q.ldx, q.t.M, q.t.V, q.D, a.dz, a.ld_dz, a.alive, dw};
       vocab_small_dw<DT><<<dim3((unsigned)tiles(q.t.V, 16), (unsigned)tiles(q.D, 16)), 64 * SMALL_DW_WAVES, 0, s>>>(d);
@@ -789,12 +804,13 @@ template <int DT> struct Small {
 
 // ---- few tokens ------------------------------------------------------------------------------------------------------
 template <int DT> struct Few {
-  static void targets(const Problem& q, const FewPlan& p, char* ws, const float* dloss, hipStream_t s) {
+  static int targets(const Problem& q, const FewPlan& p, char* ws, const float* dloss, hipStream_t s) {
     TargetsArgs a = {};
     a.t = q.t; a.flags_n = up(q.t.M, 16); a.token_groups = (unsigned)tiles(a.flags_n, 4);
     a.dloss = dloss; a.flag = (uint8_t*)(ws + p.flag); a.q = (float*)(ws + p.q); a.q_sum = a.q + q.t.M * q.t.K;
     if (!dloss) a.entropy = (float*)(ws + p.entropy);
     vocab_targets<<<a.token_groups, 256, 0, s>>>(a);
+    return launch_status();
   }
   static FewArgs args(const Problem& q, const FewPlan& p, char* ws) {
     FewArgs a = {};
@@ -804,24 +820,32 @@ template <int DT> struct Few {
     return a;
   }
   template <int NT> static int forward(const Problem& q, const FewPlan& p, char* ws, float* loss, float* lse, float* hit, hipStream_t s) {
-    if (q.t.logits) targets(q, p, ws, nullptr, s);
+    if (q.t.logits)
+      if (const int e = targets(q, p, ws, nullptr, s)) return e;
     FewArgs a = args(q, p, ws);
     a.part = (float2*)(ws + p.part);
     vocab_few_logits<DT, NT, false><<<(unsigned)(p.ld_z / FEW_ROWS), 256, 0, s>>>(a);
+    if (const int e = launch_status()) return e;
     vocab_few_join<<<(unsigned)q.t.M, 256, 0, s>>>(FewJoinArgs{q.t, a.flag, a.z, p.ld_z, a.part, (const float*)(ws + p.q), (const float*)(ws + p.entropy), loss, lse, hit});
     return launch_status();
   }
   template <int NT> static int backward(const Problem& q, const FewPlan& p, char* ws, const float* lse, const float* hit, const float* dloss, void* dx, void* dw, hipStream_t s) {
-    if (q.t.logits) targets(q, p, ws, dloss, s);
+    if (q.t.logits)
+      if (const int e = targets(q, p, ws, dloss, s)) return e;
     FewArgs a = args(q, p, ws);
     a.lse = lse; a.dloss = dloss;
     vocab_few_logits<DT, NT, true><<<(unsigned)(p.ld_z / FEW_ROWS), 256, 0, s>>>(a);
-    if (q.t.logits)
+    if (const int e = launch_status()) return e;
+    if (q.t.logits) {
       vocab_few_hits<<<(unsigned)tiles(q.t.M * q.t.K, 256), 256, 0, s>>>(q.t, lse, hit, (const float*)(ws + p.q) + q.t.M * q.t.K, dloss, a.z, p.ld_z);
+      if (const int e = launch_status()) return e;
+    }
     if (dx) {
       float* slab = (float*)(ws + p.slab);
       vocab_few_dx<DT, NT><<<(unsigned)(p.ld_slab / 64 * up(p.splits, 8)), 256, 0, s>>>(FewDxArgs{q.w, q.ldw, q.t.V, q.D, a.z, p.ld_z, p.dx_rows, p.splits, slab, p.ld_slab});
+      if (const int e = launch_status()) return e;
       vocab_few_finish<DT><<<dim3((unsigned)tiles(q.D, 256), (unsigned)q.t.M), 256, 0, s>>>(q.t, a.flag, slab, p.ld_slab, p.tokens * p.ld_slab, (int)p.splits, q.D, dx);
+      if (const int e = launch_status()) return e;
     }
     if (dw) {
       const int64_t rows = p.ld_z / FEW_ROWS, most = tiles(q.D, 256), parts = most * rows < 1024 ? most : tiles(1024, rows);
@@ -843,7 +867,7 @@ template <int DT> struct Few {
 };
 
 template <int DT, class T, int PLANES> struct Run {
-  template <int BM, int BN, int WM, int WN, int STAGES, bool AS, bool BS, int EPI> static void launch(VocabGemm& g, int64_t rows, int64_t cols, int splits, hipStream_t s) {
+  template <int BM, int BN, int WM, int WN, int STAGES, bool AS, bool BS, int EPI> static int launch(VocabGemm& g, int64_t rows, int64_t cols, int splits, hipStream_t s) {
     g.row_tiles = (int)tiles(rows, BM); g.col_tiles = (int)tiles(cols, BN); g.splits = splits;
     // half tiles are workgroups of their own; how many columns of tiles there are is known on the device, so the most of all counts
     const int64_t at_once = vocab_halves<BN, BS>() ? vocab_at_once<BM>() : 1;
@@ -855,15 +879,16 @@ template <int DT, class T, int PLANES> struct Run {
       if (!g.cols_from_meta || share + at_once / 2 <= groups) break;
     }
     vocab_gemm<T, BM, BN, WM, WN, STAGES, AS, BS, EPI, PLANES><<<(unsigned)(8 * groups), 64 * WM * WN, 0, s>>>(g);
+    return launch_status();
   }
   // columns are tokens (all shapes) or vocabulary (the square ones)
-  template <bool AS, bool BS, int EPI> static void gemm(VocabGemm& g, const Product& p, int64_t rows, int64_t cols, hipStream_t s) {
+  template <bool AS, bool BS, int EPI> static int gemm(VocabGemm& g, const Product& p, int64_t rows, int64_t cols, hipStream_t s) {
     if constexpr (EPI != EPI_DZ_ONE) { if (p.shape == S256) return launch<256, 256, 2, 4, 2, AS, BS, EPI>(g, rows, cols, p.splits, s); }
     if constexpr (!BS) {
       if (p.shape == S64) return launch<128, 64, 4, 1, 2, AS, BS, EPI>(g, rows, cols, p.splits, s);
       if (p.shape == S32) return launch<128, 32, 4, 1, 2, AS, BS, EPI>(g, rows, cols, p.splits, s);
     }
-    launch<128, 128, 2, 2, 2, AS, BS, EPI>(g, rows, cols, p.splits, s);
+    return launch<128, 128, 2, 2, 2, AS, BS, EPI>(g, rows, cols, p.splits, s);
   }
 
   static PackW pack_of_w(const Problem& q, const Plan& p, char* ws, int64_t v0) {
@@ -875,7 +900,7 @@ template <int DT, class T, int PLANES> struct Run {
     return k;
   }
   // everything in front of the first product, the first piece of W included
-  static void prepare(const Problem& q, const Plan& p, char* ws, const float* dloss, const float* lse, void* dx, float* hit, hipStream_t s) {
+  static int prepare(const Problem& q, const Plan& p, char* ws, const float* dloss, const float* lse, void* dx, float* hit, hipStream_t s) {
     TargetsArgs a = {};
     a.t = q.t; a.flags_n = p.flags_n; a.token_groups = (unsigned)tiles(p.flags_n, 4);
     a.dloss = dloss;
@@ -889,6 +914,7 @@ template <int DT, class T, int PLANES> struct Run {
         a.w = (const float*)q.w; a.ldw = q.ldw; a.w_part = (float*)(ws + p.w_part);
       }
       vocab_targets<<<a.token_groups + (PLANES == 2 ? W_PARTS : 0), 256, 0, s>>>(a);
+      if (const int e = launch_status()) return e;
     }
     PackArgs k = {};
     k.t = q.t; k.flag = a.flag; k.flags_n = p.flags_n; k.Mp = p.Mp;
@@ -904,26 +930,28 @@ template <int DT, class T, int PLANES> struct Run {
     k.meta = (VocabMeta*)(ws + p.meta);
     if (dx && p.dx_direct) { k.dx = dx; k.row_of = (int32_t*)(ws + p.row_of); }
     if (p.pack_w) { k.w = pack_of_w(q, p, ws, 0); k.w_groups = (unsigned)tiles(p.piece, k.w.each); }
-    unsigned groups = k.token_groups + k.w_groups;
+    int64_t groups = k.token_groups + k.w_groups;
     if (hit && q.t.logits) {
       k.dots = DotArgs{q.x, q.ldx, q.w, q.ldw, q.D, hit, (q.t.K + 3) / 4};
-      groups += (unsigned)tiles(q.t.M * k.dots.per_token, 4);
+      groups += tiles(q.t.M * k.dots.per_token, 4);
     }
-    vocab_pack<DT><<<groups, 256, 0, s>>>(k);
+    vocab_pack<DT><<<grid_of(groups), 256, 0, s>>>(k);
+    return launch_status();
   }
 
   // W rows v0 .. of one piece as an operand (packed first where needed)
-  static VocabOperand piece_of_w(const Problem& q, const Plan& p, char* ws, int64_t v0, hipStream_t s) {
-    VocabOperand o = {};
+  static int piece_of_w(const Problem& q, const Plan& p, char* ws, int64_t v0, VocabOperand& o, hipStream_t s) {
+    o = VocabOperand{};
     if (p.pack_w) {
       const PackW k = pack_of_w(q, p, ws, v0);
       if (v0) vocab_pack_w<DT><<<(unsigned)tiles(p.piece, k.each), 256, 0, s>>>(k, (const VocabMeta*)(ws + p.meta));
+      if (const int e = launch_status()) return e;
       o.p = (const u16*)(ws + p.wp); o.ld = p.Dp; o.plane = p.piece * p.Dp; o.rows = p.piece;
     } else {
       o.p = (const u16*)q.w + v0 * q.ldw; o.ld = q.ldw; o.plane = 0; o.rows = q.t.V - v0;
     }
     o.cols = (int)(p.pack_w ? p.Dp : q.D);
-    return o;
+    return GNET_OK;
   }
   static VocabOperand packed_x(const Plan& p, char* ws) {
     VocabOperand o = {};
@@ -941,30 +969,33 @@ template <int DT, class T, int PLANES> struct Run {
   }
 
   // the logits' partial sums, all of them
-  static RowsArgs split_logits(VocabGemm g, const Problem& q, const Plan& p, char* ws, hipStream_t s) {
+  static int split_logits(VocabGemm g, const Problem& q, const Plan& p, char* ws, RowsArgs& r, hipStream_t s) {
     g.slab = (float*)(ws + p.z_slab); g.ld_slab = p.piece; g.slab_stride = p.Mp * p.piece; g.out_cols = p.Mp;
-    gemm<false, false, EPI_SLAB>(g, p.logits, q.t.V, q.t.M, s);
-    RowsArgs r = {};
+    r = RowsArgs{};
     r.t = q.t; r.slab = g.slab; r.ld = p.piece; r.stride = g.slab_stride; r.splits = p.logits.splits; r.meta = g.meta;
-    return r;
+    return gemm<false, false, EPI_SLAB>(g, p.logits, q.t.V, q.t.M, s);
   }
 
   static int forward(const Problem& q, const Plan& p, char* ws, float* loss, float* lse, float* hit, hipStream_t s) {
-    prepare(q, p, ws, nullptr, nullptr, nullptr, hit, s);
+    if (const int e = prepare(q, p, ws, nullptr, nullptr, nullptr, hit, s)) return e;
+    VocabOperand w;
     const int32_t* pos = (const int32_t*)(ws + p.pos);
     const float* weights = (const float*)(ws + p.q);
     const float* entropy = (const float*)(ws + p.entropy);
     if (p.logits.splits > 1) {
-      RowsArgs r = split_logits(logits(q, p, ws, piece_of_w(q, p, ws, 0, s), 0), q, p, ws, s);
+      RowsArgs r;
+      if (const int e = piece_of_w(q, p, ws, 0, w, s)) return e;
+      if (const int e = split_logits(logits(q, p, ws, w, 0), q, p, ws, r, s)) return e;
       r.pos = pos; r.q = weights; r.entropy = entropy; r.loss = loss; r.lse = lse; r.hit = hit;
       vocab_rows<T, PLANES, false><<<(unsigned)q.t.M, 256, 0, s>>>(r);
       return launch_status();
     }
     for (int64_t v0 = 0; v0 < q.t.V; v0 += p.piece) {
-      VocabGemm g = logits(q, p, ws, piece_of_w(q, p, ws, v0, s), v0);
+      if (const int e = piece_of_w(q, p, ws, v0, w, s)) return e;
+      VocabGemm g = logits(q, p, ws, w, v0);
       g.part = (float2*)(ws + p.part); g.hit = (float*)(ws + p.hit_c);
       g.first_row_tile = (int)(v0 / SHAPE[p.logits.shape].bm); g.all_row_tiles = (int)p.w_tiles;
-      gemm<false, false, EPI_PART>(g, p.logits, q.t.V - v0 < p.piece ? q.t.V - v0 : p.piece, q.t.M, s);
+      if (const int e = gemm<false, false, EPI_PART>(g, p.logits, q.t.V - v0 < p.piece ? q.t.V - v0 : p.piece, q.t.M, s)) return e;
     }
     JoinArgs j = {};
     j.t = q.t; j.pos = pos; j.part = (const float2*)(ws + p.part); j.tiles = (int)p.w_tiles; j.hit_c = (const float*)(ws + p.hit_c);
@@ -974,33 +1005,38 @@ template <int DT, class T, int PLANES> struct Run {
     return launch_status();
   }
 
-  static void finish(FinishArgs f, const Problem& q, hipStream_t s) {
+  static int finish(FinishArgs f, const Problem& q, hipStream_t s) {
     f.D = q.D; f.quads = (unsigned)tiles(q.D, 4);
-    vocab_finish<DT><<<(unsigned)tiles(f.rows * f.quads, 64), 64, 0, s>>>(f);
+    vocab_finish<DT><<<grid_of(tiles(f.rows * f.quads, 64)), 64, 0, s>>>(f);
+    return launch_status();
   }
 
   static int backward(const Problem& q, const Plan& p, char* ws, const float* lse, const float* hit, const float* dloss, void* dx, void* dw, hipStream_t s) {
-    prepare(q, p, ws, dloss, lse, dx, nullptr, s);
+    if (const int e = prepare(q, p, ws, dloss, lse, dx, nullptr, s)) return e;
+    VocabOperand w;
     const VocabMeta* meta = (const VocabMeta*)(ws + p.meta);
     const int elem = DT == GNET_F32 ? 4 : 2;
     for (int64_t v0 = 0; v0 < q.t.V; v0 += p.piece) {
       const int64_t rows = q.t.V - v0 < p.piece ? q.t.V - v0 : p.piece, rows64 = up(rows, VG_BK);
-      const VocabOperand w = piece_of_w(q, p, ws, v0, s);
+      if (const int e = piece_of_w(q, p, ws, v0, w, s)) return e;
       VocabGemm g = logits(q, p, ws, w, v0);
       g.lse = (const float*)(ws + p.lse_c); g.gscale = (const float*)(ws + p.gscale);
       g.dz = (u16*)(ws + p.dz); g.ld_dz = p.piece; g.plane_dz = p.Mp * p.piece; g.dz_cols = p.Mp;
       if (p.logits.splits > 1) {
-        RowsArgs r = split_logits(g, q, p, ws, s);
+        RowsArgs r;
+        if (const int e = split_logits(g, q, p, ws, r, s)) return e;
         r.label = g.label; r.gscale = g.gscale; r.dz = g.dz; r.ld_dz = g.ld_dz; r.plane = g.plane_dz;
         vocab_rows<T, PLANES, true><<<(unsigned)p.Mp, 256, 0, s>>>(r);
-      } else if (p.logits.shape != S256 && q.t.V <= SHAPE[p.logits.shape].bm) gemm<false, false, EPI_DZ_ONE>(g, p.logits, rows, q.t.M, s);
-      else gemm<false, false, EPI_DZ>(g, p.logits, rows, q.t.M, s);
+        if (const int e = launch_status()) return e;
+      } else if (const int e = p.logits.shape != S256 && q.t.V <= SHAPE[p.logits.shape].bm ? gemm<false, false, EPI_DZ_ONE>(g, p.logits, rows, q.t.M, s)
+                                                                                           : gemm<false, false, EPI_DZ>(g, p.logits, rows, q.t.M, s)) return e;
       if (q.t.logits) {
         HitsArgs h = {};
         h.t = q.t; h.pos = (const int32_t*)(ws + p.pos); h.lse = lse; h.hit = hit;
         h.q = (const float*)(ws + p.q) + q.t.M * q.t.K;
         h.gscale = g.gscale; h.dz = g.dz; h.ld_dz = g.ld_dz; h.plane = g.plane_dz; h.v0 = v0; h.v1 = v0 + rows;
-        vocab_hits<T, PLANES><<<(unsigned)tiles(q.t.M * q.t.K, 256), 256, 0, s>>>(h);
+        vocab_hits<T, PLANES><<<grid_of(tiles(q.t.M * q.t.K, 256)), 256, 0, s>>>(h);
+        if (const int e = launch_status()) return e;
       }
       VocabOperand dz = {};
       dz.p = g.dz; dz.ld = p.piece; dz.plane = g.plane_dz; dz.rows = p.Mp; dz.cols = (int)p.piece;
@@ -1010,10 +1046,10 @@ template <int DT, class T, int PLANES> struct Run {
         if (p.dx_direct) {
           d.out = dx; d.ld_out = q.D; d.out_rows = q.D;
           d.row_of = (const int32_t*)(ws + p.row_of);
-          gemm<true, false, EPI_OUT>(d, p.dx, p.Dp, q.t.M, s);
+          if (const int e = gemm<true, false, EPI_OUT>(d, p.dx, p.Dp, q.t.M, s)) return e;
         } else {
           d.slab = (float*)(ws + p.dx_slab); d.ld_slab = p.Dp; d.slab_stride = p.Mp * p.Dp; d.accumulate = v0 > 0; d.fit = p.dx_fit;
-          gemm<true, false, EPI_SLAB>(d, p.dx, p.Dp, q.t.M, s);
+          if (const int e = gemm<true, false, EPI_SLAB>(d, p.dx, p.Dp, q.t.M, s)) return e;
         }
       }
       if (dw) {
@@ -1023,14 +1059,14 @@ template <int DT, class T, int PLANES> struct Run {
         void* out = (char*)dw + v0 * q.D * elem;
         if (p.dw.splits == 1) {
           d.out = out; d.ld_out = q.D; d.out_rows = q.D; d.unscale_by_x = 1;
-          gemm<true, true, EPI_OUT>(d, p.dw, p.Dp, rows, s);
+          if (const int e = gemm<true, true, EPI_OUT>(d, p.dw, p.Dp, rows, s)) return e;
         } else {
           d.slab = (float*)(ws + p.dw_slab); d.ld_slab = p.Dp; d.slab_stride = p.piece * p.Dp;
-          gemm<true, true, EPI_SLAB>(d, p.dw, p.Dp, rows, s);
+          if (const int e = gemm<true, true, EPI_SLAB>(d, p.dw, p.Dp, rows, s)) return e;
           FinishArgs f = {};
           f.slab = d.slab; f.ld = p.Dp; f.stride = d.slab_stride; f.splits = p.dw.splits;
           f.rows = rows; f.out = out; f.meta = meta; f.by_x = 1;
-          finish(f, q, s);
+          if (const int e = finish(f, q, s)) return e;
         }
       }
     }
@@ -1038,7 +1074,7 @@ template <int DT, class T, int PLANES> struct Run {
       FinishArgs f = {};
       f.slab = (const float*)(ws + p.dx_slab); f.ld = p.Dp; f.stride = p.Mp * p.Dp; f.splits = p.dx.splits; f.fit = p.dx_fit; f.out_cols = p.Mp;
       f.pos = (const int32_t*)(ws + p.pos); f.rows = q.t.M; f.out = dx; f.meta = meta;
-      finish(f, q, s);
+      if (const int e = finish(f, q, s)) return e;
     }
     return launch_status();
   }
@@ -1066,6 +1102,7 @@ int run_forward(const Problem& q, float* loss, float* lse, float* hit, void* ws,
     default: return Small<GNET_F16>::forward(q, loss, lse, hit, s);
   }
   const Plan p = make_plan(q.t.M, q.t.V, q.D, q.t.K, q.dtype, q.t.logits != nullptr, pack_w, 0);
+  if (!p.launchable) return GNET_ERR_UNSUPPORTED;
   if (!ws || ws_bytes < (size_t)p.bytes || ((uintptr_t)ws & 255)) return GNET_ERR_WORKSPACE;
   switch (q.dtype) {
     case GNET_F32: return Run<GNET_F32, F16T, 2>::forward(q, p, (char*)ws, loss, lse, hit, s);
@@ -1100,6 +1137,7 @@ int run_backward(const Problem& q, const float* lse, const float* hit, const flo
     }
   }
   const Plan p = make_plan(q.t.M, q.t.V, q.D, q.t.K, q.dtype, q.t.logits != nullptr, pack_w, 1);
+  if (!p.launchable) return GNET_ERR_UNSUPPORTED;
   if (!ws || ws_bytes < (size_t)p.bytes || ((uintptr_t)ws & 255)) return GNET_ERR_WORKSPACE;
   switch (q.dtype) {
     case GNET_F32: return Run<GNET_F32, F16T, 2>::backward(q, p, (char*)ws, lse, hit, dloss, dx, dw, s);

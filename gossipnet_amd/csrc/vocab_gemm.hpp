@@ -45,6 +45,14 @@ __device__ __forceinline__ void split_f16(float v, u16& hi, u16& lo) {
 
 constexpr float LOG2E = 1.4426950408889634f;
 
+// A launch has fewer than 2^32 threads along x: workgroups beyond GRID_ROW go to further rows of the grid (GRID_ROW is a multiple of 8: they are
+// dealt to the XCDs as in one row).  The last row may hold workgroups without work.
+constexpr int64_t GRID_ROW = 1 << 20;
+inline dim3 grid_of(int64_t groups) {
+  return groups <= GRID_ROW ? dim3((unsigned)groups) : dim3((unsigned)GRID_ROW, (unsigned)((groups + GRID_ROW - 1) / GRID_ROW));
+}
+__device__ __forceinline__ int64_t group_id() { return (int64_t)blockIdx.y * GRID_ROW + blockIdx.x; }
+
 // What the preparation kernels find out on the device.
 struct VocabMeta {
   int rows;            // tokens that count (compacted)

@@ -303,7 +303,8 @@ int roi_pool_bwd_atomic_f32(const float* top_diff, const int32_t* argmax, const 
  * Ids are int32 or int64 (ids64 != 0) in device memory; an id outside [0, V) means "no token": it is never an error.
  * Matrices are row-major with a row stride (ld, elements) where one is given, dense otherwise; workspaces 256-byte aligned.
  * Two calls in flight at the same time must not share a workspace.  Where 0 bytes are asked for it may be NULL.
- * Limits (GNET_ERR_UNSUPPORTED beyond): M <= 2^24 tokens, V <= 2^30, M V <= 2^44, D <= 2^16, K <= 1024. */
+ * Limits (GNET_ERR_UNSUPPORTED beyond, before anything is launched): M <= 2^24 tokens, V <= 2^30, M V <= 2^44, D <= 2^16, M D and
+ * V D <= 2^38, K <= 1024. */
 #define GNET_F32 0
 #define GNET_BF16 1
 #define GNET_F16 2

@@ -1,0 +1,58 @@
+"""The vocabulary operators at their limits, without a GPU: what is beyond is refused before anything is launched, what is within is taken."""
+import ctypes as C
+import random
+
+import pytest
+
+from gossipnet_amd import _lib
+
+F32, BF16, F16 = 0, 1, 2
+P = C.c_void_p(1 << 20)
+
+
+def xent(M, V, D, dtype=BF16, backward=False, K=0):
+    """Status of a call without a workspace: ERR_WORKSPACE where the sizes are taken."""
+    lib = _lib.load()
+    n = 0
+    if K and backward:
+        return lib.gnet_distill_backward(P, D, P, D, P, 0, P, 1.0, P, P, P, M, V, D, K, dtype, P, P, None, n, None)
+    if K:
+        return lib.gnet_distill_forward(P, D, P, D, P, 0, P, 1.0, M, V, D, K, dtype, P, P, P, None, n, None)
+    if backward:
+        return lib.gnet_xent_backward(P, D, P, D, P, 1, P, P, P, M, V, D, dtype, P, P, None, n, None)
+    return lib.gnet_xent_forward(P, D, P, D, P, 1, M, V, D, dtype, P, P, P, None, n, None)
+
+
+def embed(M, V, D, dtype=BF16):
+    return _lib.load().gnet_embed_backward(P, 0, P, D, 1.0, None, M, V, D, dtype, P, 0, P, D, P, None, 0, None)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_matrices_beyond_the_limit_are_refused(dtype):
+    """Fewer elements than 2^38 are what one launch can deal with; the sizes below pass every other limit."""
+    lib = _lib.load()
+    for backward in (False, True):
+        for K in (0, 3):
+            assert xent(1 << 24, 300, (1 << 14) + 1, dtype, backward, K) == _lib.ERR_UNSUPPORTED
+            assert xent(300, 1 << 30, 257, dtype, backward, K) == _lib.ERR_UNSUPPORTED
+            assert xent(1 << 24, 300, 1 << 14, dtype, backward, K) == _lib.ERR_WORKSPACE
+            assert xent(300, 1 << 30, 256, dtype, backward, K) == _lib.ERR_WORKSPACE
+    assert embed(1 << 24, 300, (1 << 14) + 1, dtype) == embed(300, 1 << 30, 257, dtype) == _lib.ERR_UNSUPPORTED
+    assert embed(1 << 24, 300, 1 << 14, dtype) == embed(300, 1 << 30, 256, dtype) == _lib.ERR_WORKSPACE
+    assert lib.gnet_embed_forward(P, 0, P, 1 << 16, 1.0, None, 1 << 24, 5, 1 << 16, dtype, P, None) == _lib.ERR_UNSUPPORTED
+
+
+def test_what_is_within_the_limits_is_taken():
+    """No size within the stated limits is refused for the size of a launch."""
+    rng = random.Random(7)
+    for n in range(4000):
+        M, V, D = 1 << rng.randint(6, 24), 1 << rng.randint(9, 30), 1 << rng.randint(0, 16)
+        if rng.random() < 0.7:
+            M, V, D = max(65, M - rng.randint(0, M // 2)), max(300, V - rng.randint(0, V // 2)), max(1, D - rng.randint(0, D // 2))
+        while M * V > 1 << 44:
+            V = max(300, V >> 1)
+            M = M >> 1 if V == 300 else M
+        while max(M, V) * D > 1 << 38:
+            D = max(1, D >> 1)
+        case = (M, V, D, rng.choice([F32, BF16, F16]), rng.random() < 0.5, rng.choice([0, 1024]))
+        assert xent(*case) == _lib.ERR_WORKSPACE, case
