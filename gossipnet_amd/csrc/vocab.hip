@@ -471,11 +471,15 @@ template <class T, int PLANES, bool BACKWARD> __global__ void __launch_bounds__(
     }
     return;
   }
-  const float f = a.t.inv_temp * (a.meta->unscale_x * a.meta->unscale_w);
-  auto logit = [&](int64_t v) {                        // of rows v .. v + 3
+  const float f = logit_scale(*a.meta, a.t.inv_temp);
+  auto sums = [&](int64_t v) {                         // of rows v .. v + 3
     f32x4 z = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
     for (int s = 0; s < a.splits; ++s) z += *reinterpret_cast<const f32x4*>(a.slab + s * a.stride + p * a.ld + v);
+    return z;
+  };
+  auto logit = [&](int64_t v) {
+    f32x4 z = sums(v);
 #pragma unroll
     for (int i = 0; i < 4; ++i) z[i] = v + i < a.t.V ? z[i] * f : -INFINITY;
     return z;
@@ -515,7 +519,7 @@ template <class T, int PLANES, bool BACKWARD> __global__ void __launch_bounds__(
     float loss = 0.f;
     if (!a.t.logits) {
       const int64_t label = load_id(a.t.ids, m, a.t.ids64);
-      const float hit = logit(label & ~3ll)[label & 3];
+      const float hit = one_logit(sums(label & ~3ll)[label & 3], *a.meta, a.t.inv_temp);
       loss = (top - hit) + log_sum;
       if (loss < 0.f) loss = 0.f;
       if (threadIdx.x == 0) a.hit[m] = hit;

@@ -61,6 +61,16 @@ struct VocabMeta {
   float unscale_g;     // one unit of the stored dz
 };
 
+// A product's sums times this are the logits.  The two tensors' scales may multiply to less or more than a float holds: kept normal, so that 0
+// stays 0 and the -infinity of a row that does not exist stays that (sums are below 2^53: at the lower end the logits are 0 either way).
+__device__ __forceinline__ float logit_scale(const VocabMeta& m, float inv_temp) {
+  return fminf(fmaxf(inv_temp * (m.unscale_x * m.unscale_w), 1.17549435e-38f), 1.7e38f);
+}
+// one of them exactly scaled (the same value wherever the above is not at an end)
+__device__ __forceinline__ float one_logit(float sum, const VocabMeta& m, float inv_temp) {
+  return (float)((double)(sum * inv_temp) * ((double)m.unscale_x * m.unscale_w));
+}
+
 constexpr int VG_BK = 64;      // contraction elements of a stage; contractions are a multiple of it
 
 struct VocabOperand {
@@ -410,7 +420,7 @@ __device__ __forceinline__ void vocab_tile(const VocabGemm& g, char* const lds, 
     return make_float2(m, l);
   };
   if constexpr (EPI == EPI_PART) {
-    const float f = g.inv_temp * (g.meta->unscale_x * g.meta->unscale_w);
+    const float f = logit_scale(*g.meta, g.inv_temp);
     beyond(-INFINITY);
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
@@ -423,7 +433,7 @@ __device__ __forceinline__ void vocab_tile(const VocabGemm& g, char* const lds, 
         for (int i = 0; i < FM; ++i)
 #pragma unroll
           for (int r = 0; r < 4; ++r) { const bool is = label == i * 16 + r; z = is ? acc[i][j][r] : z; mine |= is; }
-        if (mine) g.hit[c] = z * f;
+        if (mine) g.hit[c] = one_logit(z, *g.meta, g.inv_temp);
       }
       wave_stats(j, f);
     }
@@ -433,7 +443,7 @@ __device__ __forceinline__ void vocab_tile(const VocabGemm& g, char* const lds, 
   } else if constexpr (EPI == EPI_DZ || EPI == EPI_DZ_ONE) {
     // A vocabulary of one tile: the sum is formed here again instead of from lse, whose 32 bits are half a step of its own magnitude off --
     // more than what is left of 1 - p in a confident row.
-    const float f = g.inv_temp * (g.meta->unscale_x * g.meta->unscale_w);
+    const float f = logit_scale(*g.meta, g.inv_temp);
     if constexpr (EPI == EPI_DZ_ONE) {
       beyond(-INFINITY);
 #pragma unroll

@@ -1,0 +1,34 @@
+"""The vocabulary losses on operands and gradients far from 1: what scales the matrix products' operands has to cancel for every magnitude
+(the bounds of test_gpu_vocab.py)."""
+import pytest
+import torch
+
+from test_gpu_vocab import DEV, Exact, check_distill, check_xent, make
+
+pytestmark = pytest.mark.gpu
+
+# (tokens, vocabulary, width) of: tiles of logits, a vocabulary of one tile, a contraction in parts, few tokens, a small vocabulary
+PATHS = [(90, 700, 128), (90, 100, 1024), (150, 900, 2240), (20, 700, 128), (90, 81, 128)]
+
+
+@pytest.mark.parametrize("M,V,D", PATHS)
+def test_operands_whose_scales_multiply_to_less_than_a_float_holds(M, V, D):
+    """x and w around 1e-20 and below: the logits are 0, lse = log V, and no row behind the last one takes part."""
+    x, w, labels, dloss = make(M, V, D, "f32", 21)
+    for a, b in ((1e-20, 1e-20), (1e-30, 1e-12), (1e-12, 1e-30)):
+        e = check_xent(x * a, w * b, labels, dloss)
+        assert bool(((e.lse - float(torch.tensor(float(V)).log())).abs() < 1e-5).all())
+    x, w, ids, dloss, logits = make(M, V, D, "f32", 22, 3)
+    check_distill(x * 1e-20, w * 1e-20, ids, logits, 2.0, dloss)
+
+
+@pytest.mark.parametrize("M,V,D", PATHS)
+def test_a_zero_row_beside_the_largest_values(M, V, D):
+    """x and w around 1e37: other tokens' logits are infinite, a token of zeros has logits 0."""
+    from gossipnet_amd import vocab
+    x, w, labels, dloss = make(M, V, D, "f32", 23)
+    x, w = x.clamp(-4, 4) * 1e37, w.clamp(-4, 4) * 1e37
+    x[3] = 0
+    loss, lse, hit = vocab.xent_forward(x, w, labels)
+    e = Exact(torch.zeros(1, D, device=DEV), w, labels[3:4])
+    assert abs(float(lse[3]) - float(e.lse[0])) < 1e-5 and abs(float(loss[3]) - float(e.lse[0])) < 1e-5 and float(hit[3]) == 0
