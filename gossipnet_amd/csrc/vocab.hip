@@ -297,7 +297,7 @@ struct PackArgs {
   unsigned token_groups;
   const void* x; int64_t ldx; u16* xp; RowCopy c;
   const float* row_x; const float* w_part;
-  const float* row_g; const float* dloss; const float* lse; float top_g;
+  const float* row_g; const float* dloss; const float* lse; int top_exp;       // dz is stored in units of the largest |dloss| / 2^top_exp
   int32_t* pos; int32_t* label; int32_t* row_of; float* lse_c; float* gscale;
   void* dx;                            // its rows of tokens that do not count are zeroed here; NULL: later
   VocabMeta* meta;
@@ -358,13 +358,14 @@ template <int DT> __global__ void __launch_bounds__(256) vocab_pack(const PackAr
   if (packs_w) { pack_w_rows<DT>(a.w, group - a.token_groups, ldexpf(1.f, ew)); return; }
   const int ex = DT == GNET_F32 ? scale_exponent(mx, 13) : 0;
   // dz is stored in units of the largest |dloss|, not of a power of two: with one dloss for all tokens what is rounded to 16 bits is
-  // softmax - target itself, and the -1 of a label and the rest of its row are not off by different shares (top_g: 2^15 for fp16)
+  // softmax - target itself, and the -1 of a label and the rest of its row are not off by different shares (fp16: 2^15 times that)
   const float unit_g = mg >= 1.17549435e-38f && mg < INFINITY ? mg : 1.f;
   if (group == 0 && threadIdx.x == 0) {
     a.meta->rows = all;
     a.meta->unscale_x = ldexpf(1.f, -ex);
     a.meta->unscale_w = ldexpf(1.f, -ew);
-    a.meta->unscale_g = unit_g / a.top_g;
+    a.meta->unit_g = unit_g;
+    a.meta->exp_g = -a.top_exp;
   }
   RowCopy c = a.c;
   c.scale = ldexpf(1.f, ex);
@@ -397,7 +398,7 @@ template <int DT> __global__ void __launch_bounds__(256) vocab_pack(const PackAr
         if (a.row_of) a.row_of[to] = (int32_t)r;
         if (a.dloss) {
           a.lse_c[to] = a.lse[r];
-          a.gscale[to] = a.dloss[r] * a.t.inv_temp / unit_g * a.top_g;
+          a.gscale[to] = ldexpf(a.dloss[r] * a.t.inv_temp / unit_g, a.top_exp);
         }
       }
     }
@@ -563,7 +564,7 @@ struct FinishArgs {
   SplitFit fit; int64_t out_cols;                    // dx: how often the contraction was split (vocab_gemm)
 };
 template <int DT> __global__ void __launch_bounds__(64) vocab_finish(const FinishArgs a) {
-  const float f = a.meta->unscale_g * (a.by_x ? a.meta->unscale_x : a.meta->unscale_w);
+  const GradScale f = grad_scale(*a.meta, a.by_x);
   const int64_t i = group_id() * 64 + threadIdx.x;
   const int64_t r = i / a.quads, d = (i - r * a.quads) * 4;
   if (r >= a.rows) return;
@@ -571,15 +572,16 @@ template <int DT> __global__ void __launch_bounds__(64) vocab_finish(const Finis
   int splits = a.splits;
   int64_t stride = a.stride;
   if (a.fit.slots) {
-    const Splits f = fit_splits(a.fit, splits, (a.meta->rows + VG_BK - 1) & ~(VG_BK - 1), a.out_cols);
-    splits = f.splits;
-    stride = f.cols * a.ld;
+    const Splits n = fit_splits(a.fit, splits, (a.meta->rows + VG_BK - 1) & ~(VG_BK - 1), a.out_cols);
+    splits = n.splits;
+    stride = n.cols * a.ld;
   }
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
   if (p >= 0) {
 #pragma unroll 8
     for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const f32x4*>(a.slab + s * stride + p * a.ld + d);
-    v *= f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = unscale(v[k], f);
   }
   const int64_t at = r * a.D + d;
   if (DT == GNET_F32) {
@@ -928,7 +930,7 @@ template <int DT, class T, int PLANES> struct Run {
     k.x = q.x; k.ldx = q.ldx; k.xp = (u16*)(ws + p.xp);
     k.c = RowCopy{q.D, p.Dp, p.Mp * p.Dp, 1.f};
     k.row_x = a.row_x; k.w_part = a.w_part;
-    k.row_g = a.row_g; k.dloss = dloss; k.lse = lse; k.top_g = DT == GNET_BF16 ? 1.f : 32768.f;
+    k.row_g = a.row_g; k.dloss = dloss; k.lse = lse; k.top_exp = DT == GNET_BF16 ? 0 : 15;
     k.pos = (int32_t*)(ws + p.pos); k.label = q.t.logits ? nullptr : (int32_t*)(ws + p.label);
     k.lse_c = (float*)(ws + p.lse_c); k.gscale = (float*)(ws + p.gscale);
     k.meta = (VocabMeta*)(ws + p.meta);

@@ -58,7 +58,8 @@ struct VocabMeta {
   int rows;            // tokens that count (compacted)
   float unscale_x;     // 1 / scale of the packed x (32-bit operands; else 1)
   float unscale_w;
-  float unscale_g;     // one unit of the stored dz
+  float unit_g;        // the stored dz is in units of unit_g 2^exp_g
+  int exp_g;
 };
 
 // A product's sums times this are the logits.  The two tensors' scales may multiply to less or more than a float holds: kept normal, so that 0
@@ -70,6 +71,16 @@ __device__ __forceinline__ float logit_scale(const VocabMeta& m, float inv_temp)
 __device__ __forceinline__ float one_logit(float sum, const VocabMeta& m, float inv_temp) {
   return (float)((double)(sum * inv_temp) * ((double)m.unscale_x * m.unscale_w));
 }
+
+// A gradient from its sums: times unit_g 2^exp_g and the other operand's scale.  Of the two scales' product only the result's magnitude matters: the
+// powers of two are put together as exponents, where their product may be far outside a float while the result is not.
+struct GradScale { float by; int exp; };
+__device__ __forceinline__ GradScale grad_scale(const VocabMeta& m, bool by_x) {
+  int e;
+  const float f = frexpf(m.unit_g, &e);
+  return GradScale{f, e + m.exp_g + ilogbf(by_x ? m.unscale_x : m.unscale_w)};      // (unscale_x, unscale_w: powers of two)
+}
+__device__ __forceinline__ float unscale(float v, const GradScale& s) { return __builtin_amdgcn_ldexpf(v * s.by, s.exp); }
 
 constexpr int VG_BK = 64;      // contraction elements of a stage; contractions are a multiple of it
 
@@ -515,7 +526,7 @@ __device__ __forceinline__ void vocab_tile(const VocabGemm& g, char* const lds, 
       }
     }
   } else {
-    const float f = g.meta->unscale_g * (g.unscale_by_x ? g.meta->unscale_x : g.meta->unscale_w);
+    const GradScale f = grad_scale(*g.meta, g.unscale_by_x);
     const int64_t cols = g.row_of ? (int64_t)rows : g.out_cols;
     if constexpr (PLANES == 2) {
 #pragma unroll
@@ -526,7 +537,9 @@ __device__ __forceinline__ void vocab_tile(const VocabGemm& g, char* const lds, 
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
           const int64_t row = r0 + (wm * FM + i) * 16 + quad * 4;
-          const f32x4 v = acc[i][j] * f;
+          f32x4 v;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] = unscale(acc[i][j][r], f);
           if (row + 4 <= g.out_rows) *reinterpret_cast<f32x4u*>(out + row) = v;
           else
 #pragma unroll
@@ -534,7 +547,7 @@ __device__ __forceinline__ void vocab_tile(const VocabGemm& g, char* const lds, 
         }
       }
     } else {
-      store_tile<BM, BN, WM, WN>(lds, tid, [&](int i, int j, int r) { return T::enc(acc[i][j][r] * f); }, [&](int v, int d, s16x8 x) {
+      store_tile<BM, BN, WM, WN>(lds, tid, [&](int i, int j, int r) { return T::enc(unscale(acc[i][j][r], f)); }, [&](int v, int d, s16x8 x) {
         const int64_t c = c0 + v, row = r0 + d;
         if (c >= cols) return;
         u16* p = (u16*)g.out + (g.row_of ? g.row_of[c] : c) * g.ld_out + row;

@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from test_gpu_vocab import DEV, Exact, check_distill, check_xent, make
+from test_gpu_vocab import DEV, Exact, check_distill, check_xent, make, near
 
 pytestmark = pytest.mark.gpu
 
@@ -32,3 +32,17 @@ def test_a_zero_row_beside_the_largest_values(M, V, D):
     loss, lse, hit = vocab.xent_forward(x, w, labels)
     e = Exact(torch.zeros(1, D, device=DEV), w, labels[3:4])
     assert abs(float(lse[3]) - float(e.lse[0])) < 1e-5 and abs(float(loss[3]) - float(e.lse[0])) < 1e-5 and float(hit[3]) == 0
+
+
+@pytest.mark.parametrize("M,V,D", PATHS)
+@pytest.mark.parametrize("sx,sw,sg", [(2.0 ** -50, 1.0, 2.0 ** -66), (1.0, 2.0 ** -50, 2.0 ** -66), (2.0 ** -40, 2.0 ** 40, 2.0 ** -75), (2.0 ** 60, 2.0 ** -60, 2.0 ** 60),
+                                      (2.0 ** -60, 2.0 ** 60, 2.0 ** 60)])
+def test_small_and_large_gradients_of_small_and_large_operands(M, V, D, sx, sw, sg):
+    """Powers of two on x, w and the losses' gradient: dx and dw as far off as without them (and as the bounds say), relative to their own size."""
+    from gossipnet_amd import vocab
+    x, w, labels, dloss = make(M, V, D, "f32", 24)
+    x, w, dloss = x * sx, w * sw, dloss * sg
+    e = Exact(x, w, labels)
+    loss, lse, hit = vocab.xent_forward(x, w, labels)
+    for got, (exact, tol), size in zip(vocab.xent_backward(x, w, labels, lse, hit, dloss), e.gradients(dloss), (sw * sg, sx * sg)):
+        near(got.double() / size, exact / size, tol / size, "gradient")
