@@ -49,6 +49,8 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   __syncthreads();
   return (red[0] + red[1]) + (red[2] + red[3]);
 }
+// |v|, or 0 for what is not finite: an infinity in one token's values must not set the scale of all others'
+__device__ __forceinline__ float finite_abs(float v) { return fabsf(v) < INFINITY ? fabsf(v) : 0.f; }
 // the exponent of the power of two that brings a magnitude into [2^top, 2^(top+1)); 0 for 0, infinities and NaN
 __device__ __forceinline__ int scale_exponent(float a, int top) {
   if (!(a > 0.f) || !(a < INFINITY)) return 0;
@@ -84,15 +86,15 @@ struct TargetsArgs {
   const float* dloss; float* row_g;                            // backward only
   const float* w; int64_t ldw; float* w_part;
 };
-// the largest magnitude of a thread's share of n consecutive values
+// the largest finite magnitude of a thread's share of n consecutive values
 __device__ __forceinline__ float magnitude(const float* p, int64_t n, int64_t t, int64_t threads) {
   float mx = 0.f;
 #pragma unroll 4
   for (int64_t i = t; i < n / 4; i += threads) {
     const f32x4 v = *reinterpret_cast<const f32x4u*>(p + i * 4);
-    mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))));
+    mx = fmaxf(mx, fmaxf(fmaxf(finite_abs(v[0]), finite_abs(v[1])), fmaxf(finite_abs(v[2]), finite_abs(v[3]))));
   }
-  for (int64_t i = n / 4 * 4 + t; i < n; i += threads) mx = fmaxf(mx, fabsf(p[i]));
+  for (int64_t i = n / 4 * 4 + t; i < n; i += threads) mx = fmaxf(mx, finite_abs(p[i]));
   return mx;
 }
 __global__ void __launch_bounds__(256) vocab_targets(const TargetsArgs a) {
@@ -166,7 +168,7 @@ __global__ void __launch_bounds__(256) vocab_targets(const TargetsArgs a) {
       mx = wave_max(mx);
       if (lane == 0) a.row_x[m] = mx;
     }
-    if (a.row_g && lane == 0) a.row_g[m] = counts ? fabsf(a.dloss[m] * a.t.inv_temp) : 0.f;
+    if (a.row_g && lane == 0) a.row_g[m] = counts ? finite_abs(a.dloss[m] * a.t.inv_temp) : 0.f;
   }
   if (lane == 0) a.flag[m] = counts;
 }
@@ -342,7 +344,7 @@ template <int DT> __global__ void __launch_bounds__(256) vocab_pack(const PackAr
         const bool c = counts(i);
         all += c;
         if (i < r0) before += c;
-        if (a.dloss && c) mg = fmaxf(mg, fabsf(a.dloss[i] * a.t.inv_temp));
+        if (a.dloss && c) mg = fmaxf(mg, finite_abs(a.dloss[i] * a.t.inv_temp));
       }
     }
   }

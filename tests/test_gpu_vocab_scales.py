@@ -46,3 +46,32 @@ def test_small_and_large_gradients_of_small_and_large_operands(M, V, D, sx, sw, 
     loss, lse, hit = vocab.xent_forward(x, w, labels)
     for got, (exact, tol), size in zip(vocab.xent_backward(x, w, labels, lse, hit, dloss), e.gradients(dloss), (sw * sg, sx * sg)):
         near(got.double() / size, exact / size, tol / size, "gradient")
+
+
+@pytest.mark.parametrize("M,V,D", PATHS)
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_an_infinity_stays_with_its_token(dtype, M, V, D):
+    """A token that counts, with an infinity in its row or in its loss' gradient: every other token's results are what they are without it."""
+    from gossipnet_amd import vocab
+    x, w, labels, dloss = make(M, V, D, dtype, 25)
+    if dtype == "f32":
+        x, w = x * 1e6, w * 1e-6                                       # beyond what 16 bits hold without a scale
+    dloss = dloss.sign() * 5.0
+    others = torch.arange(M, device=DEV) != 7
+    e = Exact(x, w, labels)
+    want = vocab.xent_forward(x, w, labels)
+    g = torch.where(others, dloss, float("inf"))
+    dx, _ = vocab.xent_backward(x, w, labels, want[1], want[2], g)
+    exact, tol = e.gradients(dloss)[0]
+    near(dx[others], exact[others], tol[others], "dx")
+    assert not bool(dx[7].isfinite().any())
+    bad = x.clone()
+    bad[7, 3] = float("inf")
+    loss, lse, hit = vocab.xent_forward(bad, w, labels)
+    near(hit[others], e.hit[others, 0], e.hit_err[others, 0], "hit")
+    near(lse[others], e.lse[others], e.lse_err[others], "lse")
+    near(loss[others], e.loss[others], e.loss_err[others], "loss")
+    assert not bool(loss[7].isfinite())
+    dx, _ = vocab.xent_backward(bad, w, labels, lse, hit, dloss)
+    near(dx[others], exact[others], tol[others], "dx")
+    assert not bool(dx[7].isfinite().any())
