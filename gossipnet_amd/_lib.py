@@ -62,7 +62,7 @@ EXPORTS = ["gnet_param_count", "gnet_graph_count", "gnet_graph_fill", "gnet_grap
            "gnet_profiler_destroy", "gnet_profiler_set_stride", "gnet_profiler_begin", "gnet_profiler_end", "gnet_adam_step", "gnet_momentum_step", "gnet_clip_by_norm",
            "gnet_fc_workspace_bytes", "gnet_fc_forward", "gnet_fc_backward", "gnet_box_iou", "gnet_debug_gemm", "gnet_abi_version", "gnet_abi_sizes",
            "gnet_embed_forward", "gnet_embed_workspace_bytes", "gnet_embed_backward", "gnet_vocab_workspace_bytes",
-           "gnet_xent_forward", "gnet_xent_backward", "gnet_distill_forward", "gnet_distill_backward"]
+           "gnet_xent_forward", "gnet_xent_backward", "gnet_xent_backward_loss", "gnet_distill_forward", "gnet_distill_backward"]
 
 KCLASSES = ["graph", "pack", "pw_fwd", "node_fwd", "edge_fwd", "loss", "head_bwd", "winner_lists", "edge_bwd", "gather_winners",
             "node_bwd", "pw_bwd_main", "pw_w1_nodesums", "pw_w1_classrows", "reduce_partials", "edge_geometry"]
@@ -216,6 +216,8 @@ def _bind(lib):
     lib.gnet_xent_forward.argtypes = [vp, i64, vp, i64, vp, i32, i64, i64, i64, i32, vp, vp, vp, vp, sz, vp]
     lib.gnet_xent_backward.restype = C.c_int
     lib.gnet_xent_backward.argtypes = [vp, i64, vp, i64, vp, i32, vp, vp, vp, i64, i64, i64, i32, vp, vp, vp, sz, vp]
+    lib.gnet_xent_backward_loss.restype = C.c_int
+    lib.gnet_xent_backward_loss.argtypes = [vp, i64, vp, i64, vp, i32, vp, vp, vp, vp, i64, i64, i64, i32, vp, vp, vp, sz, vp]
     lib.gnet_distill_forward.restype = C.c_int
     lib.gnet_distill_forward.argtypes = [vp, i64, vp, i64, vp, i32, vp, f32, i64, i64, i64, i64, i32, vp, vp, vp, vp, sz, vp]
     lib.gnet_distill_backward.restype = C.c_int

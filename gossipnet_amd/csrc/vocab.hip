@@ -299,8 +299,8 @@ struct PackArgs {
   unsigned token_groups;
   const void* x; int64_t ldx; u16* xp; RowCopy c;
   const float* row_x; const float* w_part;
-  const float* row_g; const float* dloss; const float* lse; int top_exp;       // dz is stored in units of the largest |dloss| / 2^top_exp
-  int32_t* pos; int32_t* label; int32_t* row_of; float* lse_c; float* gscale;
+  const float* row_g; const float* dloss; const float* loss; const float* lse; int top_exp;       // dz is stored in units of the largest |dloss| / 2^top_exp
+  int32_t* pos; int32_t* label; int32_t* row_of; float* lse_c; float* gscale; float* label_p;      // label_p: with loss
   void* dx;                            // its rows of tokens that do not count are zeroed here; NULL: later
   VocabMeta* meta;
   PackW w; unsigned w_groups;
@@ -400,6 +400,7 @@ template <int DT> __global__ void __launch_bounds__(256) vocab_pack(const PackAr
         if (a.row_of) a.row_of[to] = (int32_t)r;
         if (a.dloss) {
           a.lse_c[to] = a.lse[r];
+          if (a.loss) a.label_p[to] = expm1f(-a.loss[r]);
           a.gscale[to] = ldexpf(a.dloss[r] * a.t.inv_temp / unit_g, a.top_exp);
         }
       }
@@ -456,7 +457,7 @@ struct RowsArgs {
   const float* slab; int64_t ld, stride; int splits;
   const VocabMeta* meta;
   const int32_t* pos; const float* q; const float* entropy; float* loss; float* lse; float* hit;       // forward
-  const int32_t* label; const float* gscale; u16* dz; int64_t ld_dz, plane;                            // backward
+  const int32_t* label; const float* gscale; const float* label_p; u16* dz; int64_t ld_dz, plane;      // backward
 };
 template <class T, int PLANES, bool BACKWARD> __global__ void __launch_bounds__(256) vocab_rows(const RowsArgs a) {
   __shared__ float red[4];
@@ -510,7 +511,9 @@ template <class T, int PLANES, bool BACKWARD> __global__ void __launch_bounds__(
         const f32x4 z = v < 1024 ? own : logit(v);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float d = (exp2f((z[i] - top) * LOG2E) * over - (v + i == label ? 1.f : 0.f)) * gs;      // (behind V: exp(-inf) = 0)
+          float d = exp2f((z[i] - top) * LOG2E) * over;                      // (behind V: exp(-inf) = 0)
+          if (v + i == label) d = a.label_p ? a.label_p[p] : d - 1.f;
+          d *= gs;
           if (PLANES == 1) hi[i] = T::enc(v + i < a.t.V ? d : 0.f); else split_f16(v + i < a.t.V ? d : 0.f, hi[i], lo[i]);
         }
       }
@@ -674,7 +677,7 @@ struct Plan {
   int planes, pack_w, direct, dx_direct, launchable;
   Product logits, dx, dw;
   SplitFit dx_fit;
-  int64_t flag, q, entropy, row_x, row_g, w_part, meta, pos, label, row_of, hit_c, lse_c, gscale, xp, wp, part, z_slab, dz, dx_slab, dw_slab, bytes;
+  int64_t flag, q, entropy, row_x, row_g, w_part, meta, pos, label, row_of, hit_c, lse_c, gscale, label_p, xp, wp, part, z_slab, dz, dx_slab, dw_slab, bytes;
 };
 
 Plan make_plan(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int distill, int pack_w, int backward) {
@@ -717,6 +720,7 @@ Plan make_plan(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int distil
     if (p.logits.splits == 1) p.part = take(p.Mp * p.w_tiles * 8);
   } else {
     p.row_g = take(M * 4); p.lse_c = take(p.Mp * 4); p.gscale = take(p.Mp * 4);
+    if (!distill) p.label_p = take(p.Mp * 4);
     p.dz = take(p.planes * p.Mp * p.piece * 2);
     p.dx = pick_product(p.Dp, M, p.piece / VG_BK * segments, true, true);
     p.dx_direct = p.pieces == 1 && p.dx.splits == 1;          // one sum: straight to its rows
@@ -770,6 +774,7 @@ int needs_pack(const void* w, int64_t ldw, int64_t D, int dtype) {
 }
 struct Problem {
   const void* x; int64_t ldx; const void* w; int64_t ldw; Targets t; int64_t D; int dtype;
+  const float* loss;                                 // cross entropy's backward pass: the forward's, or NULL
 };
 
 int check(const Problem& q) {
@@ -798,7 +803,7 @@ template <int DT> struct Small {
   }
   static int backward(const Problem& q, char* ws, const float* dloss, void* dx, void* dw, hipStream_t s) {
     SmallArgs a = args(q);
-    a.dloss = dloss; a.dx = dx;
+    a.dloss = dloss; a.known_loss = q.loss; a.dx = dx;
     a.dz = (float*)ws; a.ld_dz = up(q.t.V, 16); a.alive = (int*)(a.dz + up(q.t.M, 16) * a.ld_dz);
     vocab_small<DT, true><<<(unsigned)tiles(q.t.M, SMALL_TOKENS), 64 * SMALL_WAVES, SMALL_TOKENS * a.ld_z * 4, s>>>(a);
     if (const int e = launch_status()) return e;
@@ -841,7 +846,7 @@ template <int DT> struct Few {
     if (q.t.logits)
       if (const int e = targets(q, p, ws, dloss, s)) return e;
     FewArgs a = args(q, p, ws);
-    a.lse = lse; a.dloss = dloss;
+    a.lse = lse; a.dloss = dloss; a.loss = q.loss;
     vocab_few_logits<DT, NT, true><<<(unsigned)(p.ld_z / FEW_ROWS), 256, 0, s>>>(a);
     if (const int e = launch_status()) return e;
     if (q.t.logits) {
@@ -932,9 +937,9 @@ template <int DT, class T, int PLANES> struct Run {
     k.x = q.x; k.ldx = q.ldx; k.xp = (u16*)(ws + p.xp);
     k.c = RowCopy{q.D, p.Dp, p.Mp * p.Dp, 1.f};
     k.row_x = a.row_x; k.w_part = a.w_part;
-    k.row_g = a.row_g; k.dloss = dloss; k.lse = lse; k.top_exp = DT == GNET_BF16 ? 0 : 15;
+    k.row_g = a.row_g; k.dloss = dloss; k.loss = q.loss; k.lse = lse; k.top_exp = DT == GNET_BF16 ? 0 : 15;
     k.pos = (int32_t*)(ws + p.pos); k.label = q.t.logits ? nullptr : (int32_t*)(ws + p.label);
-    k.lse_c = (float*)(ws + p.lse_c); k.gscale = (float*)(ws + p.gscale);
+    k.lse_c = (float*)(ws + p.lse_c); k.gscale = (float*)(ws + p.gscale); k.label_p = (float*)(ws + p.label_p);
     k.meta = (VocabMeta*)(ws + p.meta);
     if (dx && p.dx_direct) { k.dx = dx; k.row_of = (int32_t*)(ws + p.row_of); }
     if (p.pack_w) { k.w = pack_of_w(q, p, ws, 0); k.w_groups = (unsigned)tiles(p.piece, k.w.each); }
@@ -1029,11 +1034,12 @@ template <int DT, class T, int PLANES> struct Run {
       if (const int e = piece_of_w(q, p, ws, v0, w, s)) return e;
       VocabGemm g = logits(q, p, ws, w, v0);
       g.lse = (const float*)(ws + p.lse_c); g.gscale = (const float*)(ws + p.gscale);
+      if (q.loss) g.label_p = (const float*)(ws + p.label_p);
       g.dz = (u16*)(ws + p.dz); g.ld_dz = p.piece; g.plane_dz = p.Mp * p.piece; g.dz_cols = p.Mp;
       if (p.logits.splits > 1) {
         RowsArgs r;
         if (const int e = split_logits(g, q, p, ws, r, s)) return e;
-        r.label = g.label; r.gscale = g.gscale; r.dz = g.dz; r.ld_dz = g.ld_dz; r.plane = g.plane_dz;
+        r.label = g.label; r.gscale = g.gscale; r.label_p = g.label_p; r.dz = g.dz; r.ld_dz = g.ld_dz; r.plane = g.plane_dz;
         vocab_rows<T, PLANES, true><<<(unsigned)p.Mp, 256, 0, s>>>(r);
         if (const int e = launch_status()) return e;
       } else if (const int e = p.logits.shape != S256 && q.t.V <= SHAPE[p.logits.shape].bm ? gemm<false, false, EPI_DZ_ONE>(g, p.logits, rows, q.t.M, s)
@@ -1156,7 +1162,7 @@ int run_backward(const Problem& q, const float* lse, const float* hit, const flo
 
 Problem problem(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* ids, int ids64, const float* logits, float temperature,
                 int64_t M, int64_t V, int64_t D, int64_t K, int dtype) {
-  Problem q;
+  Problem q = {};
   q.x = x; q.ldx = ldx; q.w = w; q.ldw = ldw; q.D = D; q.dtype = dtype;
   q.t.ids = ids; q.t.ids64 = ids64; q.t.logits = logits; q.t.M = M; q.t.K = (int)(K > 1 << 20 ? 1 << 20 : K); q.t.V = V;
   q.t.inv_temp = 1.f / temperature; q.t.to_log2 = LOG2E / temperature;
@@ -1179,6 +1185,15 @@ extern "C" int gnet_xent_forward(const void* x, int64_t ldx, const void* w, int6
                                  int64_t V, int64_t D, int32_t dtype, float* loss, float* lse, float* hit, void* workspace,
                                  size_t workspace_bytes, gnet_stream_t stream) {
   return run_forward(problem(x, ldx, w, ldw, labels, labels64, nullptr, 1.f, M, V, D, 1, dtype), loss, lse, hit, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+extern "C" int gnet_xent_backward_loss(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* labels, int32_t labels64,
+                                       const float* loss, const float* lse, const float* hit, const float* dloss, int64_t M, int64_t V,
+                                       int64_t D, int32_t dtype, void* dx, void* dw, void* workspace, size_t workspace_bytes,
+                                       gnet_stream_t stream) {
+  Problem q = problem(x, ldx, w, ldw, labels, labels64, nullptr, 1.f, M, V, D, 1, dtype);
+  q.loss = loss;
+  return run_backward(q, lse, hit, dloss, dx, dw, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 extern "C" int gnet_xent_backward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* labels, int32_t labels64,

@@ -30,7 +30,7 @@ struct FewArgs {
   const void* x; int64_t ldx; const void* w; int64_t ldw; int64_t D;
   float* z; int64_t ld_z;                          // [16 NT][V rounded up to 64]: logits, or dz
   float2* part;                                    // forward: [token][ld_z / 64]
-  const float* lse; const float* dloss;            // backward
+  const float* lse; const float* dloss; const float* loss;      // backward; loss may be NULL
 };
 // The four waves share the contraction, 64 bytes of a row at a time, and exchange their sums: wave w ends with rows 16 w .. of 64.
 template <int DT, int NT, bool BACKWARD> __global__ void __launch_bounds__(256) vocab_few_logits(const FewArgs a) {
@@ -109,7 +109,8 @@ template <int DT, int NT, bool BACKWARD> __global__ void __launch_bounds__(256) 
       const int64_t label = some && !a.t.logits ? load_id(a.t.ids, m, a.t.ids64) - row : -1;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float p = exp2f((z[r] - lse) * LOG2E) - (label == r ? 1.f : 0.f);
+        float p = exp2f((z[r] - lse) * LOG2E);
+        if (label == r) p = a.loss ? expm1f(-a.loss[m]) : p - 1.f;
         z[r] = some && row + r < a.t.V ? p * g : 0.f;
       }
     } else {

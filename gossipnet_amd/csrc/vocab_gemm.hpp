@@ -125,6 +125,7 @@ struct VocabGemm {
   float2* part;                // [column][all_row_tiles] maximum z and sum of exp(z - maximum) of a row tile
   float* hit;                  // per column: the logit of its label
   const float* lse; const float* gscale;   // per column
+  const float* label_p;        // per column: softmax - 1 of the label (from the loss), or NULL: the difference
   u16* dz; int64_t ld_dz, plane_dz, dz_cols;
   // products
   float* slab; int64_t ld_slab, slab_stride; int accumulate;      // [split][column][ld_slab]
@@ -452,8 +453,8 @@ __device__ __forceinline__ void vocab_tile(const VocabGemm& g, char* const lds, 
     for (int c = tid; c < BN; c += 64 * WAVES)
       if (c0 + c < rows) g.part[(size_t)(c0 + c) * g.all_row_tiles + g.first_row_tile + rt] = tile_stats(c);
   } else if constexpr (EPI == EPI_DZ || EPI == EPI_DZ_ONE) {
-    // A vocabulary of one tile: the sum is formed here again instead of from lse, whose 32 bits are half a step of its own magnitude off --
-    // more than what is left of 1 - p in a confident row.
+    // softmax - 1 of a label: lse is off by half a step of its own magnitude, more than what is left in a confident row.  It comes from the
+    // loss, where the caller has it (label_p), and in a vocabulary of one tile from the sum, which is formed here again.
     const float f = logit_scale(*g.meta, g.inv_temp);
     if constexpr (EPI == EPI_DZ_ONE) {
       beyond(-INFINITY);
@@ -467,7 +468,7 @@ __device__ __forceinline__ void vocab_tile(const VocabGemm& g, char* const lds, 
       const bool some = c < rows;
       float lse = some ? g.lse[c] : 0.f, over = 1.f;
       if constexpr (EPI == EPI_DZ_ONE) { const float2 s = tile_stats((wn * FN + j) * 16 + col16); lse = s.x; over = 1.f / s.y; }
-      const float gs = some ? g.gscale[c] : 0.f;             // a token that does not exist is zero (its logits are finite): it takes part in the products
+      const float gs = some ? g.gscale[c] : 0.f, at_label = some && g.label_p ? g.label_p[c] : 0.f;      // a token that does not exist is zero (its logits are finite): it takes part in the products
       const int64_t label = label_row(c);
       auto column = [&](auto here) {
 #pragma unroll
@@ -476,7 +477,7 @@ __device__ __forceinline__ void vocab_tile(const VocabGemm& g, char* const lds, 
           for (int r = 0; r < 4; ++r) {
             float p = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], f, -lse) * LOG2E);
             if (EPI == EPI_DZ_ONE) p *= over;
-            if (here && label == i * 16 + r) p -= 1.f;
+            if (here && label == i * 16 + r) p = g.label_p ? at_label : p - 1.f;
             acc[i][j][r] = p * gs;
           }
       };

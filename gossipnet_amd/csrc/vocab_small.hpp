@@ -84,7 +84,7 @@ struct SmallArgs {
   const void* x; int64_t ldx; const void* w; int64_t ldw; int64_t D;
   int ld_z;                                            // LDS elements a token's row of z: 4 more than a multiple of 64 (banks)
   float* loss; float* lse; float* hit;                 // forward
-  const float* dloss; float* dz; int64_t ld_dz; int* alive; void* dx;      // backward: dz [M up to 16][V up to 16]
+  const float* dloss; const float* known_loss; float* dz; int64_t ld_dz; int* alive; void* dx;      // backward: dz [M up to 16][V up to 16]; known_loss may be NULL
 };
 
 template <int DT, bool BACKWARD> __global__ void __launch_bounds__(64 * SMALL_WAVES) vocab_small(const SmallArgs a) {
@@ -182,6 +182,7 @@ template <int DT, bool BACKWARD> __global__ void __launch_bounds__(64 * SMALL_WA
       const int j = k >> 5;
       if (sub == (k & 31) && (j ? counts[1] : counts[0])) zt[j ? id[1] : id[0]] -= j ? weight[1] : weight[0];
     }
+    if (a.known_loss && sub == 0 && counts[0]) zt[id[0]] = expm1f(-a.known_loss[m]);      // (cross entropy)
     __threadfence_block();
     for (int v = sub; v < v_tiles * 16; v += 32) {
       const float d = some && v < V ? zt[v] * g : 0.f;

@@ -4,7 +4,7 @@ plain tensors out, forward and backward as two calls (as in fc.py); PyTorch only
 
     y = embed_forward(ids, table, scale)                          # features of the tokens
     loss, lse, hit = xent_forward(x, w, labels)                   # one fp32 loss per token; sum or average as needed
-    dx, dw = xent_backward(x, w, labels, lse, hit, dloss)         # dloss: d(total) / d(loss), per token or one number
+    dx, dw = xent_backward(x, w, labels, lse, hit, dloss, loss=loss)      # dloss: d(total) / d(loss), per token or one number
     embed_backward(ids, dy, table, scale, out=dw)                 # a table that is also w: its second gradient is added
 
 Tokens may be laid out in any number of leading dimensions ([B, T] or flat); x, w, table, dy are float32, bfloat16 or float16,
@@ -188,14 +188,16 @@ def xent_forward(x, w, labels):
     return loss, lse, hit
 
 
-def xent_backward(x, w, labels, lse, hit, dloss, need_dx=True, need_dw=True):
+def xent_backward(x, w, labels, lse, hit, dloss, need_dx=True, need_dw=True, loss=None):
     """(dx, dw) of xent_forward, of x's and w's shapes and type, from its lse and hit (of the same x, w and labels: they are not looked
     at where a token's whole softmax is formed again) and the losses' gradient dloss (labels' shape, or a tensor without dimensions for
-    all tokens).  None for what is not needed."""
+    all tokens).  None for what is not needed.  loss: the forward's too; the gradient at a label is then dloss * expm1(-loss).  Without it, it
+    comes from lse, whose fp32 rounding (2^-24 |lse|) is more than is left of 1 - softmax in a row whose loss is below that."""
     xm, wm = _features(x, w)
     lead = x.shape[:-1]
     i = _ids(labels, "labels", lead)
-    return _backward(xm, wm, i, None, 1.0, _per_token(lse, "lse", lead), _per_token(hit, "hit", lead), _loss_gradient(dloss, lead), x.shape, 0, need_dx, need_dw)
+    known = _per_token(loss, "loss", lead) if loss is not None else None
+    return _backward(xm, wm, i, None, 1.0, _per_token(lse, "lse", lead), _per_token(hit, "hit", lead), _loss_gradient(dloss, lead), x.shape, 0, need_dx, need_dw, known)
 
 
 def distill_forward(x, w, top_ids, top_logits, temperature=1.0):
@@ -226,8 +228,8 @@ def distill_backward(x, w, top_ids, top_logits, lse, hit, dloss, temperature=1.0
     return _backward(xm, wm, i, t, temperature, _per_token(lse, "lse", lead), _per_token(hit, "hit", i.shape), _loss_gradient(dloss, lead), x.shape, i.shape[-1], need_dx, need_dw)
 
 
-def _backward(xm, wm, i, t, temperature, lse, hit, dloss, x_shape, K, need_dx, need_dw):
-    dev = _on_device(wm, xm, i, t, lse, hit, dloss)
+def _backward(xm, wm, i, t, temperature, lse, hit, dloss, x_shape, K, need_dx, need_dw, loss=None):
+    dev = _on_device(wm, xm, i, t, lse, hit, dloss, loss)
     (M, D), V, dt = xm.shape, wm.shape[0], _TYPES[wm.dtype]
     dx = xm.new_empty(x_shape) if need_dx else None
     dw = wm.new_empty(V, D) if need_dw else None
@@ -238,7 +240,7 @@ def _backward(xm, wm, i, t, temperature, lse, hit, dloss, x_shape, K, need_dx, n
     buf, ws = _workspace(nbytes, dev)
     ids64 = int(i.dtype == torch.int64)
     if t is None:
-        _call(dev, lib.gnet_xent_backward, _p(xm), _ld(xm), _p(wm), _ld(wm), _p(i), ids64, _p(lse), _p(hit), _p(dloss), M, V, D, dt,
+        _call(dev, lib.gnet_xent_backward_loss, _p(xm), _ld(xm), _p(wm), _ld(wm), _p(i), ids64, _p(loss), _p(lse), _p(hit), _p(dloss), M, V, D, dt,
               _p(dx), _p(dw), ws, nbytes)
     else:
         _call(dev, lib.gnet_distill_backward, _p(xm), _ld(xm), _p(wm), _ld(wm), _p(i), ids64, _p(t), float(temperature), _p(lse), _p(hit),

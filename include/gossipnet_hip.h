@@ -341,6 +341,11 @@ int gnet_xent_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, co
 int gnet_xent_backward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* labels, int32_t labels64,
                        const float* lse, const float* hit, const float* dloss, int64_t M, int64_t V, int64_t D, int32_t dtype,
                        void* dx, void* dw, void* workspace, size_t workspace_bytes, gnet_stream_t stream);
+/* The same with the forward call's loss [M] too (NULL: as above).  dz of a label is then dloss expm1(-loss), exact to fp32 rounding of the loss;
+ * without it, it is formed from lse, whose rounding is up to 2^-24 |lse| of 1 - softmax: more than is left of it where loss < 2^-24 |lse|. */
+int gnet_xent_backward_loss(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* labels, int32_t labels64,
+                            const float* loss, const float* lse, const float* hit, const float* dloss, int64_t M, int64_t V, int64_t D,
+                            int32_t dtype, void* dx, void* dw, void* workspace, size_t workspace_bytes, gnet_stream_t stream);
 /* Distillation from a teacher's K best logits per token (top_ids, top_logits [M,K]) at a temperature > 0: with
  * z = x . w^T / temperature and q = softmax over the row's slots of top_logits / temperature,
  *   loss[m] = sum_k q_k (log q_k - z[m,id_k] + lse[m])     lse[m] = log sum_v exp z[m,v]     hit[m,k] = z[m,id_k]
