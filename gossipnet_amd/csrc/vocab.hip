@@ -301,6 +301,7 @@ struct PackArgs {
   const float* row_x; const float* w_part;
   const float* row_g; const float* dloss; const float* loss; const float* lse; int top_exp;       // dz is stored in units of the largest |dloss| / 2^top_exp
   int32_t* pos; int32_t* label; int32_t* row_of; float* lse_c; float* gscale; float* label_p;      // label_p: with loss
+  u16* xg; int32_t* exp_c;             // two planes, backward: x as dW's operand, and the tokens' own exponents
   void* dx;                            // its rows of tokens that do not count are zeroed here; NULL: later
   VocabMeta* meta;
   PackW w; unsigned w_groups;
@@ -394,6 +395,19 @@ template <int DT> __global__ void __launch_bounds__(256) vocab_pack(const PackAr
       const bool own = at >= 0;
       const int64_t to = own ? at : all + (r - ~at);           // the others' places behind them are zeroed
       copy_row<DT>(a.x, r * a.ldx, !own, a.xp + to * c.Dp, c, t, wide ? 256 : 64);
+      // Two fp16 end at 2^-40 of the unit: a token whose |dloss| is far below the largest has its dz in a unit 2^e smaller, taken back from
+      // dx's sums and, for dW, from its row of x.  (16-bit operands: one unit for all; x times a power of two would leave fp16's range.)
+      float gs = 0.f;
+      int e = 0;
+      if (a.dloss && own) {
+        gs = a.dloss[r] * a.t.inv_temp / unit_g;
+        if (DT == GNET_F32 && gs != 0.f && fabsf(gs) < INFINITY) e = min(max(-1 - ilogbf(gs), 0), 100);      // (below 2^15, as the largest is: fp16 ends at 65504)
+      }
+      if (DT == GNET_F32 && a.dloss) {
+        RowCopy cg = c;
+        cg.scale = ldexpf(1.f, ex - e);
+        copy_row<DT>(a.x, r * a.ldx, !own, a.xg + to * c.Dp, cg, t, wide ? 256 : 64);
+      }
       if (a.dx && !own && r < M) zero_row<DT>(a.dx, r * c.D, c.D, t, wide ? 256 : 64);
       if (own && t == 0) {
         if (a.label) a.label[to] = (int32_t)load_id(a.t.ids, r, a.t.ids64);
@@ -401,7 +415,8 @@ template <int DT> __global__ void __launch_bounds__(256) vocab_pack(const PackAr
         if (a.dloss) {
           a.lse_c[to] = a.lse[r];
           if (a.loss) a.label_p[to] = expm1f(-a.loss[r]);
-          a.gscale[to] = ldexpf(a.dloss[r] * a.t.inv_temp / unit_g, a.top_exp);
+          a.gscale[to] = ldexpf(gs, a.top_exp + e);
+          if (DT == GNET_F32) a.exp_c[to] = e;
         }
       }
     }
@@ -566,10 +581,11 @@ struct FinishArgs {
   const int32_t* pos;                                // NULL: row r of the slab
   int64_t rows, D; unsigned quads; void* out;                 // quads: groups of four a row
   const VocabMeta* meta; int by_x;
+  const int32_t* exp_c;                              // dx of two planes: by place
   SplitFit fit; int64_t out_cols;                    // dx: how often the contraction was split (vocab_gemm)
 };
 template <int DT> __global__ void __launch_bounds__(64) vocab_finish(const FinishArgs a) {
-  const GradScale f = grad_scale(*a.meta, a.by_x);
+  GradScale f = grad_scale(*a.meta, a.by_x);
   const int64_t i = group_id() * 64 + threadIdx.x;
   const int64_t r = i / a.quads, d = (i - r * a.quads) * 4;
   if (r >= a.rows) return;
@@ -583,6 +599,7 @@ template <int DT> __global__ void __launch_bounds__(64) vocab_finish(const Finis
   }
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
   if (p >= 0) {
+    if (DT == GNET_F32 && a.exp_c) f.exp -= a.exp_c[p];
 #pragma unroll 8
     for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const f32x4*>(a.slab + s * stride + p * a.ld + d);
 #pragma unroll
@@ -677,7 +694,7 @@ struct Plan {
   int planes, pack_w, direct, dx_direct, launchable;
   Product logits, dx, dw;
   SplitFit dx_fit;
-  int64_t flag, q, entropy, row_x, row_g, w_part, meta, pos, label, row_of, hit_c, lse_c, gscale, label_p, xp, wp, part, z_slab, dz, dx_slab, dw_slab, bytes;
+  int64_t flag, q, entropy, row_x, row_g, w_part, meta, pos, label, row_of, hit_c, lse_c, gscale, label_p, exp_c, xp, xg, wp, part, z_slab, dz, dx_slab, dw_slab, bytes;
 };
 
 Plan make_plan(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int distill, int pack_w, int backward) {
@@ -721,6 +738,7 @@ Plan make_plan(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int distil
   } else {
     p.row_g = take(M * 4); p.lse_c = take(p.Mp * 4); p.gscale = take(p.Mp * 4);
     if (!distill) p.label_p = take(p.Mp * 4);
+    if (p.planes == 2) { p.exp_c = take(p.Mp * 4); p.xg = take(p.planes * p.Mp * p.Dp * 2); }
     p.dz = take(p.planes * p.Mp * p.piece * 2);
     p.dx = pick_product(p.Dp, M, p.piece / VG_BK * segments, true, true);
     p.dx_direct = p.pieces == 1 && p.dx.splits == 1;          // one sum: straight to its rows
@@ -940,6 +958,7 @@ template <int DT, class T, int PLANES> struct Run {
     k.row_g = a.row_g; k.dloss = dloss; k.loss = q.loss; k.lse = lse; k.top_exp = DT == GNET_BF16 ? 0 : 15;
     k.pos = (int32_t*)(ws + p.pos); k.label = q.t.logits ? nullptr : (int32_t*)(ws + p.label);
     k.lse_c = (float*)(ws + p.lse_c); k.gscale = (float*)(ws + p.gscale); k.label_p = (float*)(ws + p.label_p);
+    k.xg = (u16*)(ws + p.xg); k.exp_c = (int32_t*)(ws + p.exp_c);
     k.meta = (VocabMeta*)(ws + p.meta);
     if (dx && p.dx_direct) { k.dx = dx; k.row_of = (int32_t*)(ws + p.row_of); }
     if (p.pack_w) { k.w = pack_of_w(q, p, ws, 0); k.w_groups = (unsigned)tiles(p.piece, k.w.each); }
@@ -966,9 +985,9 @@ template <int DT, class T, int PLANES> struct Run {
     o.cols = (int)(p.pack_w ? p.Dp : q.D);
     return GNET_OK;
   }
-  static VocabOperand packed_x(const Plan& p, char* ws) {
+  static VocabOperand packed_x(const Plan& p, char* ws, bool for_dw = false) {
     VocabOperand o = {};
-    o.p = (const u16*)(ws + p.xp); o.ld = p.Dp; o.plane = p.Mp * p.Dp; o.rows = p.Mp; o.cols = (int)p.Dp;
+    o.p = (const u16*)(ws + (for_dw && PLANES == 2 ? p.xg : p.xp)); o.ld = p.Dp; o.plane = p.Mp * p.Dp; o.rows = p.Mp; o.cols = (int)p.Dp;
     return o;
   }
   static VocabGemm logits(const Problem& q, const Plan& p, char* ws, const VocabOperand& w, int64_t v0) {
@@ -1059,7 +1078,7 @@ template <int DT, class T, int PLANES> struct Run {
         d.a = w; d.b = dz; d.k = rows64; d.cols_from_meta = 1; d.meta = meta; d.out_cols = p.Mp;
         if (p.dx_direct) {
           d.out = dx; d.ld_out = q.D; d.out_rows = q.D;
-          d.row_of = (const int32_t*)(ws + p.row_of);
+          d.row_of = (const int32_t*)(ws + p.row_of); d.col_exp = (const int32_t*)(ws + p.exp_c);
           if (const int e = gemm<true, false, EPI_OUT>(d, p.dx, p.Dp, q.t.M, s)) return e;
         } else {
           d.slab = (float*)(ws + p.dx_slab); d.ld_slab = p.Dp; d.slab_stride = p.Mp * p.Dp; d.accumulate = v0 > 0; d.fit = p.dx_fit;
@@ -1068,7 +1087,7 @@ template <int DT, class T, int PLANES> struct Run {
       }
       if (dw) {
         VocabGemm d = {};
-        d.a = packed_x(p, ws); d.b = dz; d.k_from_meta = 1; d.meta = meta;
+        d.a = packed_x(p, ws, true); d.b = dz; d.k_from_meta = 1; d.meta = meta;
         d.out_cols = rows;
         void* out = (char*)dw + v0 * q.D * elem;
         if (p.dw.splits == 1) {
@@ -1087,7 +1106,8 @@ template <int DT, class T, int PLANES> struct Run {
     if (dx && !p.dx_direct) {
       FinishArgs f = {};
       f.slab = (const float*)(ws + p.dx_slab); f.ld = p.Dp; f.stride = p.Mp * p.Dp; f.splits = p.dx.splits; f.fit = p.dx_fit; f.out_cols = p.Mp;
-      f.pos = (const int32_t*)(ws + p.pos); f.rows = q.t.M; f.out = dx; f.meta = meta;
+      f.pos = (const int32_t*)(ws + p.pos); if (PLANES == 2) f.exp_c = (const int32_t*)(ws + p.exp_c);
+      f.rows = q.t.M; f.out = dx; f.meta = meta;
       if (const int e = finish(f, q, s)) return e;
     }
     return launch_status();

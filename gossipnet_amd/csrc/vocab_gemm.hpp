@@ -130,6 +130,7 @@ struct VocabGemm {
   // products
   float* slab; int64_t ld_slab, slab_stride; int accumulate;      // [split][column][ld_slab]
   const int32_t* row_of;       // the output row of a column (tokens that count), or NULL
+  const int32_t* col_exp;      // two planes, with row_of: a column's sums are 2^col_exp times too large
   void* out; int64_t ld_out, out_rows, out_cols; int unscale_by_x;   // [column][row]
 };
 
@@ -535,12 +536,13 @@ __device__ __forceinline__ void vocab_tile(const VocabGemm& g, char* const lds, 
         const int64_t c = c0 + (wn * FN + j) * 16 + col16;
         if (c >= cols) continue;
         float* out = (float*)g.out + (g.row_of ? g.row_of[c] : c) * g.ld_out;
+        const GradScale own = {f.by, f.exp - (g.row_of ? g.col_exp[c] : 0)};
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
           const int64_t row = r0 + (wm * FM + i) * 16 + quad * 4;
           f32x4 v;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = unscale(acc[i][j][r], f);
+          for (int r = 0; r < 4; ++r) v[r] = unscale(acc[i][j][r], own);
           if (row + 4 <= g.out_rows) *reinterpret_cast<f32x4u*>(out + row) = v;
           else
 #pragma unroll

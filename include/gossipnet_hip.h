@@ -329,7 +329,8 @@ int gnet_embed_backward(const void* ids, int32_t ids64, const void* dy, int64_t 
  * lse and hit have to be what the forward call gave for the same operands: where a token's whole row of logits is at hand its softmax
  * is formed again, and they are not looked at.
  * dx [M,D] and dw [V,D] are overwritten; either may be NULL.  The logits are formed again, one piece of the vocabulary at a time;
- * dz is kept in 16 bits (GNET_F32: two fp16 of together 22 bits) for the piece, or in fp32 for few tokens or a small vocabulary.
+ * dz is kept in 16 bits (GNET_F32: two fp16 of together 22 bits) for the piece, or in fp32 for few tokens or a small vocabulary.  In 16 bits
+ * it is off by half a step of itself; fp16 also ends at 2^-40 of the call's largest |dloss|, two fp16 at 2^-39 of the token's own.
  * w must be finite.  A token that counts with a row of x or a dloss that is not finite has such results, and so has dw; other tokens' are
  * what they are without it.  Reproducible.
  * workspace of all four calls: gnet_vocab_workspace_bytes(w, ldw, M, V, D, K, dtype, backward) (K = 0: cross entropy). */
