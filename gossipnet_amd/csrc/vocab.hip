@@ -705,8 +705,10 @@ Plan make_plan(int64_t M, int64_t V, int64_t D, int64_t K, int dtype, int distil
   // cross entropy on 16 bits needs nothing of its tokens but the labels: up to 8192 of them the packing looks at them itself
   p.direct = !distill && p.planes == 1 && M <= 8192;
   p.Mp = up(M, VG_BK); p.Dp = up(D, 64); p.flags_n = up(M, 16);
-  // A piece's dz and packed rows of W take 256 MB at most: that is what the last-level cache holds for the products that read them
+  // A piece's dz and packed rows of W take at most 256 MB: that is what the last-level cache holds for the products that read them
   // again, though larger pieces measured the same (2048 x 100352 x 2048: 2.25 ms; 64 MB 2.22, 512 MB 2.17; 4096 x 131072 x 4096: 9.85, 9.77, 9.79).
+  // But 2048 rows at least, since every piece reads and writes dx's fp32 sums: past 65536 tokens in 16 bits (32768 in 32) dz takes 4 KB (8 KB)
+  // a token.  A floor of 2 D rows: 131072 x 50304 x 256 17.1 and 19.1 ms, 524288 x 8192 x 128 8.5 and 25.2, 131072 x 16384 x 256 fp32 13.9 and 21.0.
   const int64_t per_row = (int64_t)p.planes * 2 * ((backward ? p.Mp : 0) + (pack_w ? p.Dp : 0));
   const int64_t Vp = up(V, 256);
   int64_t piece = per_row ? (256ll << 20) / per_row / 256 * 256 : Vp;

@@ -333,7 +333,9 @@ int gnet_embed_backward(const void* ids, int32_t ids64, const void* dy, int64_t 
  * it is off by half a step of itself; fp16 also ends at 2^-40 of the call's largest |dloss|, two fp16 at 2^-39 of the token's own.
  * w must be finite.  A token that counts with a row of x or a dloss that is not finite has such results, and so has dw; other tokens' are
  * what they are without it.  Reproducible.
- * workspace of all four calls: gnet_vocab_workspace_bytes(w, ldw, M, V, D, K, dtype, backward) (K = 0: cross entropy). */
+ * workspace of all four calls: gnet_vocab_workspace_bytes(w, ldw, M, V, D, K, dtype, backward) (K = 0: cross entropy).  It grows with
+ * the tokens, not with the logits.  Backward: a copy of the rows of x that count (GNET_F32: two), fp32 sums of dx, and dz of one piece of the vocabulary, which with copied
+ * rows of w takes 256 MB, or, for many tokens, 4 KB a token (GNET_F32: 8 KB). */
 size_t gnet_vocab_workspace_bytes(const void* w, int64_t ldw, int64_t M, int64_t V, int64_t D, int64_t K, int32_t dtype,
                                   int32_t backward);
 int gnet_xent_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* labels, int32_t labels64, int64_t M,

@@ -56,3 +56,20 @@ def test_what_is_within_the_limits_is_taken():
             D = max(1, D >> 1)
         case = (M, V, D, rng.choice([F32, BF16, F16]), rng.random() < 0.5, rng.choice([0, 1024]))
         assert xent(*case) == _lib.ERR_WORKSPACE, case
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M", [1 << 12, 1 << 17, 1 << 20, 1 << 24])
+@pytest.mark.parametrize("V,D", [(50304, 1024), (50304, 64), (1 << 18, 8)])
+def test_workspaces_grow_with_the_tokens_as_documented(M, V, D, dtype):
+    """Copies of x, dx's fp32 sums and one piece of dz: 256 MB or 4 KB a token (fp32: 8 KB), and no more for a larger vocabulary but for W's copy."""
+    planes = 2 if dtype == F32 else 1
+    Mp, Dp = (M + 63) // 64 * 64, (D + 63) // 64 * 64
+    lib = _lib.load()
+    small = 64 * Mp + (1 << 20)                                        # per-token values
+    copies = planes * planes * 2 * Mp * Dp                             # fp32: two copies of two planes
+    sums = 16 * 4 * max(Mp * Dp, 512 * 256 * 256)                      # dx's sums, split at most 16 ways; dw's likewise in a small piece
+    piece = max(256 << 20, planes * 2 * 2048 * (Mp + Dp) + (1 << 20))
+    need = lib.gnet_vocab_workspace_bytes(P, D, M, V, D, 0, dtype, 1)
+    assert need < small + copies + piece + (4 * Mp * Dp if M >= 1 << 17 else sums) + (256 << 20), need
+    assert lib.gnet_vocab_workspace_bytes(P, D, M, 4 * V, D, 0, dtype, 1) <= need + (256 << 20)
