@@ -85,6 +85,14 @@ def _ids(t, what, shape=None):
     return t.contiguous()
 
 
+def _overlap(a, b):
+    """Whether two matrices of consecutive row elements share memory."""
+    if not a.numel() or not b.numel():
+        return False
+    ends = [t.data_ptr() + ((t.shape[0] - 1) * _ld(t) + t.shape[1]) * t.element_size() for t in (a, b)]
+    return a.data_ptr() < ends[1] and b.data_ptr() < ends[0]
+
+
 def _per_token(t, what, shape):
     """fp32 values of the tokens' shape."""
     if t.shape != shape:
@@ -121,7 +129,8 @@ def embed_forward(ids, table, scale=1.0, token_scale=None):
 def embed_backward(ids, dy, table, scale=1.0, token_scale=None, need_dscale=False, out=None):
     """(dtable, dscale): gradients of embed_forward.  dtable [V, D] = scale * sum over the tokens of each id, in token order, of
     token_scale * dy.  out: a contiguous [V, D] gradient of table's type that dtable is added to and that is returned (added in fp32,
-    rounded once; rows without a token keep their bits).  dscale (with need_dscale): fp32, of ids' shape, = scale * dy . table[ids]."""
+    rounded once; rows without a token keep their bits); not memory of dy, nor of table with need_dscale, which are read meanwhile.
+    dscale (with need_dscale): fp32, of ids' shape, = scale * dy . table[ids]."""
     if table.dim() != 2 or table.shape[0] < 1:
         raise _lib.InvalidArgumentError("table must be [V, D] with V >= 1")
     t = _matrix(table, "table")
@@ -134,6 +143,8 @@ def embed_backward(ids, dy, table, scale=1.0, token_scale=None, need_dscale=Fals
     if out is not None:
         if tuple(out.shape) != (V, D) or out.dtype != t.dtype or not out.is_contiguous():
             raise _lib.InvalidArgumentError("out must be a contiguous [%d, %d] tensor of type %s" % (V, D, t.dtype))
+        if _overlap(out, g) or (need_dscale and _overlap(out, t)):
+            raise _lib.InvalidArgumentError("out shares memory with %s, which is read while it is written" % ("dy" if _overlap(out, g) else "table"))
     dev = _on_device(t, i, g, s, out)
     dtable = out.detach() if out is not None else t.new_empty(V, D)
     M = i.numel()

@@ -315,7 +315,7 @@ int gnet_embed_forward(const void* ids, int32_t ids64, const void* table, int64_
 /* dtable [V,D] = scale * sum over the tokens with id v, in token order, of token_scale[m] * dy[m]: overwritten (rows without a token
  * are zero), or, with accumulate != 0, added to (the sum is added in fp32 and rounded once; rows without a token are not touched).
  * dscale (NULL: not needed): [M] = scale * dy[m] . table[ids[m]], the gradient of token_scale; zero where the id is outside [0, V); it
- * alone reads table.  Reproducible: no atomics.  workspace: gnet_embed_workspace_bytes(M, D). */
+ * alone reads table.  dtable must not overlap dy, nor table where dscale is asked for.  Reproducible: no atomics.  workspace: gnet_embed_workspace_bytes(M, D). */
 size_t gnet_embed_workspace_bytes(int64_t M, int64_t D);
 int gnet_embed_backward(const void* ids, int32_t ids64, const void* dy, int64_t ld_dy, float scale, const float* token_scale, int64_t M,
                         int64_t V, int64_t D, int32_t dtype, void* dtable, int32_t accumulate, const void* table, int64_t ld_table,

@@ -98,3 +98,16 @@ def test_rows_of_two_to_the_twenty_four_tokens(dtype, D):
     y = vocab.embed_forward(ids, table)
     for a in range(0, M, 2 ** 20):
         assert torch.equal(y[a:a + 2 ** 20], table[ids[a:a + 2 ** 20].long()])
+
+
+@pytest.mark.parametrize("M,V,D", [(30, 5000, 96), (700, 90, 64), (5000, 3000, 72)])
+def test_a_table_that_is_its_own_gradients_sum(M, V, D):
+    """out=table: a step down the gradient in place."""
+    from gossipnet_amd import vocab
+    g = torch.Generator(device=DEV).manual_seed(M)
+    table = torch.randint(-8, 9, (V, D), device=DEV, generator=g).float()
+    ids = torch.randint(-1, V, (M,), device=DEV, generator=g)
+    dy = torch.randint(-8, 9, (M, D), device=DEV, generator=g).float()
+    want = table - 0.5 * vocab.embed_backward(ids, dy, table)[0]       # (sums of small multiples of a half: exact)
+    assert vocab.embed_backward(ids, dy, table, -0.5, out=table)[0] is table
+    assert torch.equal(table, want)

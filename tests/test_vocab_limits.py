@@ -73,3 +73,22 @@ def test_workspaces_grow_with_the_tokens_as_documented(M, V, D, dtype):
     need = lib.gnet_vocab_workspace_bytes(P, D, M, V, D, 0, dtype, 1)
     assert need < small + copies + piece + (4 * Mp * Dp if M >= 1 << 17 else sums) + (256 << 20), need
     assert lib.gnet_vocab_workspace_bytes(P, D, M, 4 * V, D, 0, dtype, 1) <= need + (256 << 20)
+
+
+def test_a_gradient_on_memory_that_is_read_is_refused():
+    import torch
+    from gossipnet_amd import vocab
+    both = torch.zeros(30, 8)
+    table, ids, dy = torch.zeros(10, 8), torch.zeros(4, dtype=torch.int64), torch.zeros(4, 8)
+    for call in (lambda: vocab.embed_backward(ids, both[8:12], table, out=both[:10]),                  # dy begins inside out
+                 lambda: vocab.embed_backward(ids, both[:4], table, out=both[3:13]),
+                 lambda: vocab.embed_backward(ids, dy, table, need_dscale=True, out=table),
+                 lambda: vocab.embed_backward(ids, dy, both[9:19], need_dscale=True, out=both[:10])):
+        with pytest.raises(_lib.InvalidArgumentError, match="shares memory"):
+            call()
+    for call in (lambda: vocab.embed_backward(ids, both[10:14], table, out=both[:10]),                 # side by side
+                 lambda: vocab.embed_backward(ids, both[:4], table, out=both[4:14]),
+                 lambda: vocab.embed_backward(ids, dy, table, -0.1, out=table),                        # table is not read
+                 lambda: vocab.embed_backward(ids[:0], dy[:0], table, out=table)):
+        with pytest.raises(_lib.GnetError, match="device kernels"):
+            call()
