@@ -21,7 +21,7 @@ The JSON line also carries
                 `fp32_equivalent` = FLOPs of the fp32 formulation / time against the fp32 peak; `reference_formulation`
                 = the same with the FLOPs of the reference's dense per-edge formulation, which a kernel can
                 exceed 1.0 on by not executing them; `traffic` = HBM bytes per launch from the separate rocprofv3
-                --pmc passes (profiles/r06_traffic.json), reported only while that file was collected from the same
+                --pmc passes (profiles/step_traffic.json), reported only while that file was collected from the same
                 kernel sources (hash), else null; `mfma_busy` (per MFMA kernel, same file and gate) =
                 SQ_VALU_MFMA_BUSY_CYCLES / (1024 SIMDs x the launch's GRBM_GUI_ACTIVE cycles) of the --pmc pass
   roi_pool      the RoiPool / RoiPoolGrad ops at the reference's shape (R=2000 rois, 38x63x1024 map, 7x7 bins):
@@ -50,17 +50,21 @@ sys.path.insert(0, ROOT)
 FP32_MFMA_PEAK_TFLOPS = 157.3     # MI355X_MICROARCH.md, v_mfma_f32_32x32x2_f32 (64 FLOP / clk / SIMD x 1024 SIMDs x 2.4 GHz)
 BF16_MFMA_PEAK_TFLOPS = 2516.6    # dense v_mfma_f32_32x32x16_bf16: 32768 FLOP in 32 clk per SIMD (the guide's ~2.5 PFLOP/s)
 HBM_PEAK_GBS = 8000.0
-TRAFFIC_FILE = os.path.join(ROOT, "profiles", "r06_traffic.json")
+TRAFFIC_FILE = os.path.join(ROOT, "profiles", "step_traffic.json")
 PW_FP32_PIPE = bool(os.environ.get("GNET_PW_FP32_PIPE"))     # measurement only: round 5's fp32-MFMA pw_fwd2 / pw_bwd_main instead of pw_fwd3 / pw_bwd_bf
 
 
+# the sources of the kernels of a step; the library's other operators (RoI pooling, FC layers, optimizers, the vocabulary's) are not in them
+STEP_SOURCES = ("backward.hip", "backward_edge.hip", "backward_edge.hpp", "common.hpp", "forward.hip", "graph.hip", "loss.hip", "plan.hip")
+
+
 def kernel_source_hash():
-    """Identity of the kernel sources the library was built from (profiles/*_traffic.json carries the same)."""
+    """Identity of the step's kernels: their sources and the flags they are compiled with (profiles/step_traffic.json carries the same)."""
+    from gossipnet_amd import build
     h = hashlib.sha256()
-    d = os.path.join(ROOT, "gossipnet_amd", "csrc")
-    for f in sorted(os.listdir(d)):
-        if f.endswith((".hip", ".hpp")):
-            h.update(f.encode()); h.update(open(os.path.join(d, f), "rb").read())
+    for f in STEP_SOURCES:
+        h.update(f.encode()); h.update(open(os.path.join(ROOT, "gossipnet_amd", "csrc", f), "rb").read())
+    h.update(" ".join(build.FLAGS).encode())
     return h.hexdigest()[:16]
 
 
@@ -477,7 +481,7 @@ def main():
                         traffic = tf["kernels"].get(cls, {}).get("hbm_bytes")
                         pmc = tf["kernels"]
                     else:
-                        note = "profiles/r06_traffic.json was collected from other kernel sources / another workload: not reported"
+                        note = "profiles/step_traffic.json was collected from other kernel sources / another workload: not reported"
                 # `achieved` counts the FLOPs the algorithm needs in this kernel's formulation (= the MFMA FLOPs it issues:
                 # e.g. edge_fwd computes P.Wp + rc[c] + rn[n] per edge, the per-node products r.Wc / r.Wn live in
                 # node_fwd); the reference's dense per-edge formulation is reported beside it -- a kernel
@@ -527,7 +531,7 @@ def main():
             roofline["mfma_kernels"] = mfma_kernels
             roofline["mfma_busy"] = pmc.get(roofline["kernel"], {}).get("mfma_busy")
             roofline["mfma_busy_note"] = ("SQ_VALU_MFMA_BUSY_CYCLES / (1024 SIMDs x GRBM_GUI_ACTIVE) per launch, from the separate rocprofv3 "
-                                          "--pmc pass (profiles/r06_traffic.json, same kernel sources); null = no current counters")
+                                          "--pmc pass (profiles/step_traffic.json, same kernel sources and flags); null = no current counters")
         # whole-step executed MFMA FLOPs
         ex_f32, ex_bf16, eq_total = 0.0, 0.0, 0.0
         for k_, c_ in counts.items():

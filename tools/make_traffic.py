@@ -1,4 +1,4 @@
-"""profiles/<round>_traffic.json from the FETCH_SIZE, WRITE_SIZE and SQ passes of tools/collect_profiles.sh.
+"""profiles/step_traffic.json from the FETCH_SIZE, WRITE_SIZE and SQ passes of tools/collect_profiles.sh.
 usage: make_traffic.py <fetch counter_collection.csv> <write counter_collection.csv> <sq counter_collection.csv> <out.json>"""
 import json
 import os
