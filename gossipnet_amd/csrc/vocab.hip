@@ -173,11 +173,12 @@ __global__ void __launch_bounds__(256) vocab_targets(const TargetsArgs a) {
   if (lane == 0) a.flag[m] = counts;
 }
 
-// Rows copied to the matrix products' layout: Dp elements (a multiple of 64), zeros behind D; 32 bits as two fp16 planes.
+// Rows copied to the matrix products' layout: Dp elements (a multiple of 64), zeros behind D; 32 bits as two fp16 planes, if asked for (dst2)
+// twice, the second time at a scale of its own.
 struct RowCopy { int64_t D, Dp, plane; float scale; };
-template <int DT> __device__ __forceinline__ void copy_row(const void* src, int64_t first, bool zero, u16* dst, const RowCopy& c, int t, int threads) {
+template <int DT> __device__ __forceinline__ void copy_row(const void* src, int64_t first, bool zero, u16* dst, const RowCopy& c, int t, int threads, u16* dst2 = nullptr, float scale2 = 0.f) {
   for (int64_t d = (int64_t)t * 8; d < c.Dp; d += (int64_t)threads * 8) {
-    s16x8 hi = {0, 0, 0, 0, 0, 0, 0, 0}, lo = hi;
+    s16x8 hi = {0, 0, 0, 0, 0, 0, 0, 0}, lo = hi, hi2 = hi, lo2 = hi;
     if (!zero) {
       if (DT == GNET_F32) {
         const float* p = (const float*)src + first + d;
@@ -196,6 +197,13 @@ template <int DT> __device__ __forceinline__ void copy_row(const void* src, int6
           split_f16(v[i] * c.scale, h, l);
           hi[i] = (short)h; lo[i] = (short)l;
         }
+        if (dst2)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            u16 h, l;
+            split_f16(v[i] * scale2, h, l);
+            hi2[i] = (short)h; lo2[i] = (short)l;
+          }
       } else {
         const u16* p = (const u16*)src + first + d;
         if (d + 8 <= c.D) hi = *reinterpret_cast<const s16x8u*>(p);
@@ -206,6 +214,10 @@ template <int DT> __device__ __forceinline__ void copy_row(const void* src, int6
     }
     *reinterpret_cast<s16x8*>(dst + d) = hi;
     if (DT == GNET_F32) *reinterpret_cast<s16x8*>(dst + c.plane + d) = lo;
+    if (DT == GNET_F32 && dst2) {
+      *reinterpret_cast<s16x8*>(dst2 + d) = hi2;
+      *reinterpret_cast<s16x8*>(dst2 + c.plane + d) = lo2;
+    }
   }
 }
 template <int DT> __device__ __forceinline__ void zero_row(void* out, int64_t first, int64_t D, int t, int threads) {
@@ -310,7 +322,7 @@ struct PackArgs {
 template <int DT> __global__ void __launch_bounds__(256) vocab_pack(const PackArgs a) {
   __shared__ int ired[2][4];
   __shared__ float fred[3][4];
-  __shared__ int place[256];
+  __shared__ int place[256], own_exp[DT == GNET_F32 ? 256 : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t group = group_id();
   if (group >= a.token_groups + a.w_groups) {
@@ -386,6 +398,22 @@ template <int DT> __global__ void __launch_bounds__(256) vocab_pack(const PackAr
     for (int w = 0; w < wave; ++w) rank += ired[0][w];
     place[threadIdx.x] = c256 ? rank : ~rank;
     if (mine < M && threadIdx.x < a.rows - j0) a.pos[mine] = c256 ? rank : -1;
+    // Two fp16 end at 2^-40 of the unit: a token whose |dloss| is far below the largest has its dz in a unit 2^e smaller, taken back from
+    // dx's sums and, for dW, from its row of x.  (16-bit operands: one unit for all; x times a power of two would leave fp16's range.)
+    int e = 0;
+    if (c256) {
+      if (a.label) a.label[rank] = (int32_t)load_id(a.t.ids, mine, a.t.ids64);
+      if (a.row_of) a.row_of[rank] = (int32_t)mine;
+      if (a.dloss) {
+        const float gs = a.dloss[mine] * a.t.inv_temp / unit_g;
+        if (DT == GNET_F32 && gs != 0.f && fabsf(gs) < INFINITY) e = min(max(-1 - ilogbf(gs), 0), 100);      // (below 2^15, as the largest is: fp16 ends at 65504)
+        a.lse_c[rank] = a.lse[mine];
+        if (a.loss) a.label_p[rank] = expm1f(-a.loss[mine]);
+        a.gscale[rank] = ldexpf(gs, a.top_exp + e);
+        if (DT == GNET_F32) a.exp_c[rank] = e;
+      }
+    }
+    if (DT == GNET_F32) own_exp[threadIdx.x] = e;
     before += ired[0][0] + ired[0][1] + ired[0][2] + ired[0][3];
     __syncthreads();
     const int n = (int)min((int64_t)min(256, a.rows - j0), a.Mp - base);
@@ -394,31 +422,9 @@ template <int DT> __global__ void __launch_bounds__(256) vocab_pack(const PackAr
       const int at = place[j];
       const bool own = at >= 0;
       const int64_t to = own ? at : all + (r - ~at);           // the others' places behind them are zeroed
-      copy_row<DT>(a.x, r * a.ldx, !own, a.xp + to * c.Dp, c, t, wide ? 256 : 64);
-      // Two fp16 end at 2^-40 of the unit: a token whose |dloss| is far below the largest has its dz in a unit 2^e smaller, taken back from
-      // dx's sums and, for dW, from its row of x.  (16-bit operands: one unit for all; x times a power of two would leave fp16's range.)
-      float gs = 0.f;
-      int e = 0;
-      if (a.dloss && own) {
-        gs = a.dloss[r] * a.t.inv_temp / unit_g;
-        if (DT == GNET_F32 && gs != 0.f && fabsf(gs) < INFINITY) e = min(max(-1 - ilogbf(gs), 0), 100);      // (below 2^15, as the largest is: fp16 ends at 65504)
-      }
-      if (DT == GNET_F32 && a.dloss) {
-        RowCopy cg = c;
-        cg.scale = ldexpf(1.f, ex - e);
-        copy_row<DT>(a.x, r * a.ldx, !own, a.xg + to * c.Dp, cg, t, wide ? 256 : 64);
-      }
+      copy_row<DT>(a.x, r * a.ldx, !own, a.xp + to * c.Dp, c, t, wide ? 256 : 64, DT == GNET_F32 && a.dloss ? a.xg + to * c.Dp : nullptr,
+                   DT == GNET_F32 ? ldexpf(1.f, ex - own_exp[j]) : 0.f);
       if (a.dx && !own && r < M) zero_row<DT>(a.dx, r * c.D, c.D, t, wide ? 256 : 64);
-      if (own && t == 0) {
-        if (a.label) a.label[to] = (int32_t)load_id(a.t.ids, r, a.t.ids64);
-        if (a.row_of) a.row_of[to] = (int32_t)r;
-        if (a.dloss) {
-          a.lse_c[to] = a.lse[r];
-          if (a.loss) a.label_p[to] = expm1f(-a.loss[r]);
-          a.gscale[to] = ldexpf(gs, a.top_exp + e);
-          if (DT == GNET_F32) a.exp_c[to] = e;
-        }
-      }
     }
   }
 }

@@ -107,11 +107,11 @@ template <int DT, int NT, bool BACKWARD> __global__ void __launch_bounds__(256) 
       const bool some = few_counts(a.t, a.flag, m);
       const float g = some ? a.dloss[m] * a.t.inv_temp : 0.f, lse = some ? a.lse[m] : 0.f;
       const int64_t label = some && !a.t.logits ? load_id(a.t.ids, m, a.t.ids64) - row : -1;
+      const float at_label = some && a.loss ? expm1f(-a.loss[m]) : 0.f;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float p = exp2f((z[r] - lse) * LOG2E);
-        if (label == r) p = a.loss ? expm1f(-a.loss[m]) : p - 1.f;
-        z[r] = some && row + r < a.t.V ? p * g : 0.f;
+        const float p = exp2f((z[r] - lse) * LOG2E), q = a.loss ? at_label : p - 1.f;
+        z[r] = some && row + r < a.t.V ? (label == r ? q : p) * g : 0.f;
       }
     } else {
       float top = -INFINITY, sum = 0.f;
