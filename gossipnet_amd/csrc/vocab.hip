@@ -319,14 +319,14 @@ struct PackArgs {
   PackW w; unsigned w_groups;
   DotArgs dots;
 };
-template <int DT> __global__ void __launch_bounds__(256) vocab_pack(const PackArgs a) {
+template <int DT, bool BACKWARD> __global__ void __launch_bounds__(256) vocab_pack(const PackArgs a) {
   __shared__ int ired[2][4];
   __shared__ float fred[3][4];
-  __shared__ int place[256], own_exp[DT == GNET_F32 ? 256 : 1];
+  __shared__ int place[256], own_exp[DT == GNET_F32 && BACKWARD ? 256 : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t group = group_id();
   if (group >= a.token_groups + a.w_groups) {
-    if (a.dots.hit) target_dots<DT>(a.t, a.dots, (group - a.token_groups - a.w_groups) * 4 + (threadIdx.x >> 6));
+    if (!BACKWARD && a.dots.hit) target_dots<DT>(a.t, a.dots, (group - a.token_groups - a.w_groups) * 4 + (threadIdx.x >> 6));
     return;
   }
   const bool packs_w = group >= a.token_groups;
@@ -345,7 +345,7 @@ template <int DT> __global__ void __launch_bounds__(256) vocab_pack(const PackAr
         all += n;
         if (i < r0) before += n;                                                   // r0 is a multiple of 4
       }
-      if (a.dloss)
+      if (BACKWARD)
 #pragma unroll 4
         for (int64_t i = threadIdx.x; i < M; i += 256) mg = fmaxf(mg, a.row_g[i]);
       if (DT == GNET_F32)
@@ -357,14 +357,14 @@ template <int DT> __global__ void __launch_bounds__(256) vocab_pack(const PackAr
         const bool c = counts(i);
         all += c;
         if (i < r0) before += c;
-        if (a.dloss && c) mg = fmaxf(mg, finite_abs(a.dloss[i] * a.t.inv_temp));
+        if (BACKWARD && c) mg = fmaxf(mg, finite_abs(a.dloss[i] * a.t.inv_temp));
       }
     }
   }
   before = wave_isum(before);
   all = wave_isum(all);
   if (DT == GNET_F32) { mw = wave_max(mw); mx = wave_max(mx); }
-  if (a.dloss) mg = wave_max(mg);
+  if (BACKWARD) mg = wave_max(mg);
   if (lane == 0) { ired[0][wave] = before; ired[1][wave] = all; fred[0][wave] = mw; fred[1][wave] = mx; fred[2][wave] = mg; }
   __syncthreads();
   before = all = 0;
@@ -403,8 +403,8 @@ template <int DT> __global__ void __launch_bounds__(256) vocab_pack(const PackAr
     int e = 0;
     if (c256) {
       if (a.label) a.label[rank] = (int32_t)load_id(a.t.ids, mine, a.t.ids64);
-      if (a.row_of) a.row_of[rank] = (int32_t)mine;
-      if (a.dloss) {
+      if (BACKWARD && a.row_of) a.row_of[rank] = (int32_t)mine;
+      if (BACKWARD) {
         const float gs = a.dloss[mine] * a.t.inv_temp / unit_g;
         if (DT == GNET_F32 && gs != 0.f && fabsf(gs) < INFINITY) e = min(max(-1 - ilogbf(gs), 0), 100);      // (below 2^15, as the largest is: fp16 ends at 65504)
         a.lse_c[rank] = a.lse[mine];
@@ -413,7 +413,7 @@ template <int DT> __global__ void __launch_bounds__(256) vocab_pack(const PackAr
         if (DT == GNET_F32) a.exp_c[rank] = e;
       }
     }
-    if (DT == GNET_F32) own_exp[threadIdx.x] = e;
+    if (DT == GNET_F32 && BACKWARD) own_exp[threadIdx.x] = e;
     before += ired[0][0] + ired[0][1] + ired[0][2] + ired[0][3];
     __syncthreads();
     const int n = (int)min((int64_t)min(256, a.rows - j0), a.Mp - base);
@@ -422,9 +422,9 @@ template <int DT> __global__ void __launch_bounds__(256) vocab_pack(const PackAr
       const int at = place[j];
       const bool own = at >= 0;
       const int64_t to = own ? at : all + (r - ~at);           // the others' places behind them are zeroed
-      copy_row<DT>(a.x, r * a.ldx, !own, a.xp + to * c.Dp, c, t, wide ? 256 : 64, DT == GNET_F32 && a.dloss ? a.xg + to * c.Dp : nullptr,
-                   DT == GNET_F32 ? ldexpf(1.f, ex - own_exp[j]) : 0.f);
-      if (a.dx && !own && r < M) zero_row<DT>(a.dx, r * c.D, c.D, t, wide ? 256 : 64);
+      copy_row<DT>(a.x, r * a.ldx, !own, a.xp + to * c.Dp, c, t, wide ? 256 : 64, DT == GNET_F32 && BACKWARD ? a.xg + to * c.Dp : nullptr,
+                   DT == GNET_F32 && BACKWARD ? ldexpf(1.f, ex - own_exp[j]) : 0.f);
+      if (BACKWARD && a.dx && !own && r < M) zero_row<DT>(a.dx, r * c.D, c.D, t, wide ? 256 : 64);
     }
   }
 }
@@ -975,7 +975,8 @@ template <int DT, class T, int PLANES> struct Run {
       k.dots = DotArgs{q.x, q.ldx, q.w, q.ldw, q.D, hit, (q.t.K + 3) / 4};
       groups += tiles(q.t.M * k.dots.per_token, 4);
     }
-    vocab_pack<DT><<<grid_of(groups), 256, 0, s>>>(k);
+    if (dloss) vocab_pack<DT, true><<<grid_of(groups), 256, 0, s>>>(k);
+    else vocab_pack<DT, false><<<grid_of(groups), 256, 0, s>>>(k);
     return launch_status();
   }
 
