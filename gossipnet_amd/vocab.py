@@ -174,8 +174,10 @@ def _teacher(top_ids, top_logits, x, temperature):
     return _ids(top_ids, "top_ids"), _per_token(top_logits, "top_logits", top_ids.shape)
 
 
-def _loss_gradient(dloss, lead):
-    """d(total) / d(loss) per token; one number (a tensor without dimensions) stands for all of them."""
+def _loss_gradient(dloss, lead, device):
+    """d(total) / d(loss) per token; one number (or a tensor without dimensions) stands for all of them."""
+    if isinstance(dloss, (int, float)):
+        return torch.full(lead, float(dloss), dtype=torch.float32, device=device)
     if dloss.dim() == 0:
         dloss = dloss.expand(lead)
     return _per_token(dloss, "dloss", lead)
@@ -201,14 +203,14 @@ def xent_forward(x, w, labels):
 
 def xent_backward(x, w, labels, lse, hit, dloss, need_dx=True, need_dw=True, loss=None):
     """(dx, dw) of xent_forward, of x's and w's shapes and type, from its lse and hit (of the same x, w and labels: they are not looked
-    at where a token's whole softmax is formed again) and the losses' gradient dloss (labels' shape, or a tensor without dimensions for
-    all tokens).  None for what is not needed.  loss: the forward's too; the gradient at a label is then dloss * expm1(-loss).  Without it, it
+    at where a token's whole softmax is formed again) and the losses' gradient dloss (labels' shape, or a number or a tensor without
+    dimensions for all tokens).  None for what is not needed.  loss: the forward's too; the gradient at a label is then dloss * expm1(-loss).  Without it, it
     comes from lse, whose fp32 rounding (2^-24 |lse|) is more than is left of 1 - softmax in a row whose loss is below that."""
     xm, wm = _features(x, w)
     lead = x.shape[:-1]
     i = _ids(labels, "labels", lead)
     known = _per_token(loss, "loss", lead) if loss is not None else None
-    return _backward(xm, wm, i, None, 1.0, _per_token(lse, "lse", lead), _per_token(hit, "hit", lead), _loss_gradient(dloss, lead), x.shape, 0, need_dx, need_dw, known)
+    return _backward(xm, wm, i, None, 1.0, _per_token(lse, "lse", lead), _per_token(hit, "hit", lead), _loss_gradient(dloss, lead, x.device), x.shape, 0, need_dx, need_dw, known)
 
 
 def distill_forward(x, w, top_ids, top_logits, temperature=1.0):
@@ -236,7 +238,7 @@ def distill_backward(x, w, top_ids, top_logits, lse, hit, dloss, temperature=1.0
     xm, wm = _features(x, w)
     lead = x.shape[:-1]
     i, t = _teacher(top_ids, top_logits, x, temperature)
-    return _backward(xm, wm, i, t, temperature, _per_token(lse, "lse", lead), _per_token(hit, "hit", i.shape), _loss_gradient(dloss, lead), x.shape, i.shape[-1], need_dx, need_dw)
+    return _backward(xm, wm, i, t, temperature, _per_token(lse, "lse", lead), _per_token(hit, "hit", i.shape), _loss_gradient(dloss, lead, x.device), x.shape, i.shape[-1], need_dx, need_dw)
 
 
 def _backward(xm, wm, i, t, temperature, lse, hit, dloss, x_shape, K, need_dx, need_dw, loss=None):

@@ -78,3 +78,29 @@ def test_the_loss_is_checked_and_may_be_left_out():
     loss, lse, hit = vocab.xent_forward(x, w, labels)
     dx, _ = vocab.xent_backward(x, w, labels, lse, hit, dloss, loss=loss)
     assert not bool(dx[::3].any()) and bool(dx[1].any())
+
+
+def test_one_number_for_all_tokens():
+    """A number in place of a tensor of the losses' gradients, eagerly and in a captured graph."""
+    from gossipnet_amd import vocab
+    x, w, labels, _ = confident(40, 300, 64, "bf16", 6, 0.0)
+    ids, logits = torch.stack([labels, (labels + 1) % 300], 1), torch.randn(40, 2, device=DEV)
+    loss, lse, hit = vocab.xent_forward(x, w, labels)
+    _, lse2, hit2 = vocab.distill_forward(x, w, ids, logits, 2.0)
+
+    def both(g):
+        return vocab.xent_backward(x, w, labels, lse, hit, g, loss=loss) + vocab.distill_backward(x, w, ids, logits, lse2, hit2, g, 2.0)
+    want = both(torch.full((40,), 0.25, device=DEV))
+    for g in (0.25, torch.tensor(0.25, device=DEV)):
+        for a, b in zip(both(g), want):
+            assert torch.equal(a, b)
+    for a, b in zip(both(1), both(torch.ones(40, device=DEV))):
+        assert torch.equal(a, b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = both(0.25)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)

@@ -92,3 +92,14 @@ def test_a_gradient_on_memory_that_is_read_is_refused():
                  lambda: vocab.embed_backward(ids[:0], dy[:0], table, out=table)):
         with pytest.raises(_lib.GnetError, match="device kernels"):
             call()
+
+
+def test_a_number_is_taken_as_the_losses_gradient():
+    import torch
+    from gossipnet_amd import vocab
+    x, w, y, one = torch.zeros(4, 8), torch.zeros(10, 8), torch.zeros(4, dtype=torch.int64), torch.zeros(4)
+    for g in (1.0, 1, torch.tensor(1.0)):                              # (as far as the check of the device)
+        with pytest.raises(_lib.GnetError, match="device kernels"):
+            vocab.xent_backward(x, w, y, one, one, g)
+        with pytest.raises(_lib.GnetError, match="device kernels"):
+            vocab.distill_backward(x, w, y[:, None], one[:, None], one, one[:, None], g)
