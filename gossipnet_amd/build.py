@@ -12,8 +12,8 @@ LIB = os.path.join(HERE, "libgossipnet_hip_probe.so" if PROBE_BUILD else "libgos
 SOURCES = ["graph.hip", "forward.hip", "loss.hip", "backward.hip", "backward_edge.hip", "roi_pool.hip", "optim.hip", "fc.hip", "plan.hip", "debug.hip", "vocab.hip", "embed.hip"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-fno-fast-math",
          "-Wall", "-Wno-unused-function",
-         # no packed fp32 instructions: some of their forms have given wrong results on this hardware (and the step is 0.5 % faster
-         # without them: 8.44 against 8.48 ms); hipcc's host pass warns that it does not know the feature
+         # no packed fp32 instructions (v_pk_add / mul / fma_f32): the step takes 8.44 ms without and 8.48 with them; hipcc's host pass
+         # warns that it does not know the feature
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 if os.environ.get("GNET_EXTRA_FLAGS"):    # measurement builds only (probe variants of a kernel: tools/); never shipped
     FLAGS = FLAGS + os.environ["GNET_EXTRA_FLAGS"].split()

@@ -454,6 +454,10 @@ __device__ __forceinline__ void vocab_tile(const VocabGemm& g, char* const lds, 
     for (int c = tid; c < BN; c += 64 * WAVES)
       if (c0 + c < rows) g.part[(size_t)(c0 + c) * g.all_row_tiles + g.first_row_tile + rt] = tile_stats(c);
   } else if constexpr (EPI == EPI_DZ || EPI == EPI_DZ_ONE) {
+    // dz is rounded to the operands' 16 bits here (two fp16 for 32-bit ones): the two products behind it run on the 16-bit pipe, a second plane
+    // for it would be two more products of four (4096 x 131072 x 4096: 13 ms would become 20).  It is all that the gradients are off beyond their own rounding:
+    // 833 x 50257 x 1024 bf16 dx 0.00208 of its norm against 0.00166, and 0.00208 with exact products of the rounded dz; 48 x 32000 x 2048 fp16 0.00028
+    // against 0.00021.  A caller who needs more passes fp32.
     // softmax - 1 of a label: lse is off by half a step of its own magnitude, more than what is left in a confident row.  It comes from the
     // loss, where the caller has it (label_p), and in a vocabulary of one tile from the sum, which is formed here again.
     const float f = logit_scale(*g.meta, g.inv_temp);

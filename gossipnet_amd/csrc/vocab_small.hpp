@@ -18,7 +18,7 @@ template <int DT, int N> struct SmallRaw {
   typedef E U __attribute__((ext_vector_type(N), aligned(sizeof(E))));
   V v;
   // (16 bits at an odd address: the dwords that hold them, shifted.  A vector load that starts inside a dword takes 190 cycles a wave, one
-  // at a dword's start 16; what the first and last dword hold besides is not used.)
+  // at a dword's start 16; what the first and last dword hold besides, up to two bytes outside the row, is not used.)
   __device__ __forceinline__ void load(const void* p, int64_t i) {
     if constexpr (DT == GNET_F32 || N < 4) v = *reinterpret_cast<const U*>((const E*)p + i);
     else {

@@ -301,7 +301,8 @@ int roi_pool_bwd_atomic_f32(const float* top_diff, const int32_t* argmax, const 
  * two ends of a model over a large vocabulary; no reference counterpart).  Element types of x, w, table, dy and of the gradients of
  * each: GNET_F32, GNET_BF16 or GNET_F16, one type a call.  Sums, softmax statistics, losses and per-token values are fp32.
  * Ids are int32 or int64 (ids64 != 0) in device memory; an id outside [0, V) means "no token": it is never an error.
- * Matrices are row-major with a row stride (ld, elements) where one is given, dense otherwise; workspaces 256-byte aligned.
+ * Matrices are row-major with a row stride (ld, elements) where one is given, dense otherwise; workspaces 256-byte aligned.  16-bit x and w that
+ * begin inside a dword are read in whole dwords: up to two bytes in front of a row and behind it (never beyond the dword, and not used).
  * Two calls in flight at the same time must not share a workspace.  Where 0 bytes are asked for it may be NULL.
  * Limits (GNET_ERR_UNSUPPORTED beyond, before anything is launched): M <= 2^24 tokens, V <= 2^30, M V <= 2^44, D <= 2^16, M D and
  * V D <= 2^38, K <= 1024. */
