@@ -103,3 +103,21 @@ def test_a_number_is_taken_as_the_losses_gradient():
             vocab.xent_backward(x, w, y, one, one, g)
         with pytest.raises(_lib.GnetError, match="device kernels"):
             vocab.distill_backward(x, w, y[:, None], one[:, None], one, one[:, None], g)
+
+
+def test_the_entry_with_the_loss_refuses_like_the_one_without():
+    lib = _lib.load()
+    odd = C.c_void_p((1 << 20) + 8)
+
+    def back(x=P, ldx=8, w=P, ldw=8, y=P, loss=P, lse=P, hit=P, g=P, M=65, V=3000, D=8, dtype=F32, ws=P, n=1 << 40):
+        return lib.gnet_xent_backward_loss(x, ldx, w, ldw, y, 1, loss, lse, hit, g, M, V, D, dtype, P, P, ws, n, None)
+    for a in (dict(M=-1), dict(V=0), dict(D=0), dict(ldx=7), dict(ldw=7), dict(dtype=3), dict(x=None), dict(w=None), dict(y=None), dict(lse=None), dict(hit=None), dict(g=None)):
+        assert back(**a) == _lib.ERR_INVALID, a
+    for a in (dict(M=(1 << 24) + 1), dict(V=(1 << 30) + 1), dict(D=(1 << 16) + 1, ldx=1 << 17, ldw=1 << 17)):
+        assert back(**a) == _lib.ERR_UNSUPPORTED, a
+    for V in (10, 3000):
+        for M in (20, 65):
+            need = lib.gnet_vocab_workspace_bytes(P, 8, M, V, 8, 0, F32, 1)
+            for loss in (P, None):
+                for a in (dict(ws=None), dict(n=need - 1), dict(ws=odd)):
+                    assert back(M=M, V=V, loss=loss, **a) == _lib.ERR_WORKSPACE, a
